@@ -62,6 +62,7 @@ pub const WH_GEMV_STREAM: c_int = 1;
 
 // --------------------------------------------------------------------- limits
 pub const WH_LLAMA_DECODE_NOALLOC_MAX_BYTES: usize = 16 << 20;
+pub const WH_MAX_TREE_NODES: usize = 128;
 pub const WH_GGUF_MAX_DIMS: usize = 8;
 
 // ------------------------------------------ GGUF metadata value types (metadata.rs:13-42)
@@ -120,6 +121,27 @@ pub struct wh_ffn_weights {
     pub down: *const c_void,
     pub hidden: usize,
     pub n_ff: usize,
+}
+
+/// What is done to logits before a token is chosen (`wh_logits_process`); device arrays.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct wh_logits_rules {
+    pub rows_per_seq: usize,
+    pub history: *const u32,
+    pub history_stride: usize,
+    pub history_len: *const u32,
+    pub tree_tokens: *const u32,
+    pub tree_parents: *const i32,
+    pub repetition_penalty: c_float,
+    pub frequency_penalty: c_float,
+    pub presence_penalty: c_float,
+    pub bias_ids: *const u32,
+    pub bias: *const c_float,
+    pub n_bias: usize,
+    pub bias_stride: usize,
+    pub mask: *const u32,
+    pub mask_stride: usize,
 }
 
 /// Counters of the device copies kept behind the `*_host` variants.
@@ -336,6 +358,27 @@ extern "C" {
                                         logits: *mut c_float, stream: wh_stream_t) -> c_int;
     pub fn wh_embedding_lookup(r#type: c_int, table: *const c_void, vocab: usize, hidden: usize, ids: *const u32,
                                n_tokens: usize, out: *mut c_float, stream: wh_stream_t) -> c_int;
+
+    // a tree of drafted tokens
+    pub fn wh_attention_tree_workspace_bytes(n_seqs: usize, n_tree: usize, n_heads: usize, n_kv_heads: usize,
+                                             head_dim: usize, max_ctx: usize) -> usize;
+    pub fn wh_attention_tree(q: *const c_float, k: *const c_float, v: *const c_float, ldq: usize, ldkv: usize,
+                             parents: *const i32, ctx_len: *const u32, n_seqs: usize, n_tree: usize,
+                             k_cache: *mut c_void, v_cache: *mut c_void, max_ctx: usize, n_heads: usize,
+                             n_kv_heads: usize, head_dim: usize, inv_freq: *const c_float, out: *mut c_float,
+                             workspace: *mut c_void, workspace_bytes: usize, stream: wh_stream_t) -> c_int;
+    pub fn wh_logits_process_workspace_bytes(rules: *const wh_logits_rules, n_rows: usize, vocab: usize) -> usize;
+    pub fn wh_logits_process(rules: *const wh_logits_rules, logits: *const c_float, ld: usize, n_rows: usize,
+                             vocab: usize, out: *mut c_float, ld_out: usize, token: *mut u32,
+                             workspace: *mut c_void, workspace_bytes: usize, stream: wh_stream_t) -> c_int;
+    pub fn wh_tree_accept(tokens: *const u32, parents: *const i32, picked: *const u32, n_seqs: usize, n_tree: usize,
+                          path: *mut u32, n_accepted: *mut u32, next_token: *mut u32, ctx_len: *const u32,
+                          ctx_len_out: *mut u32, history: *mut u32, history_stride: usize,
+                          stream: wh_stream_t) -> c_int;
+    pub fn wh_kv_cache_compact(k_caches: *mut *mut c_void, v_caches: *mut *mut c_void, n_layers: usize,
+                               n_seqs: usize, max_ctx: usize, n_kv_heads: usize, head_dim: usize, path: *const u32,
+                               n_tree: usize, n_accepted: *const u32, ctx_len: *const u32,
+                               stream: wh_stream_t) -> c_int;
 
     // GGUF files (loader.rs:111-295, format.rs, metadata.rs, tensor_info.rs)
     pub fn wh_gguf_open(path: *const c_char, out: *mut *mut wh_gguf) -> c_int;

@@ -477,6 +477,106 @@ WH_API int wh_llama_decode_step_noalloc(const wh_llama_model* model, size_t pos,
 WH_API int wh_embedding_lookup(int type, const void* table, size_t vocab, size_t hidden, const uint32_t* ids,
                                size_t n_tokens, float* out, wh_stream_t stream);
 
+/* ------------------------------------------- a tree of drafted tokens */
+/* Speculative decoding: a drafting program proposes n_tree tokens ("nodes")
+ * as a tree, one step of the model computes all of them, and the path that the
+ * model's own choices agree with is kept.  No counterpart in the reference,
+ * which decodes one token per step (LazyTransformer::forward); the pieces below
+ * stand beside the decode step's.
+ *   parents[t] = -1: node t follows the tokens in the cache; 0 <= parents[t] < t:
+ *   it follows that node; any other value: the node is absent, and so is every
+ *   node below it (a tree with fewer nodes than n_tree, e.g. in a captured
+ *   graph).  At most WH_MAX_TREE_NODES nodes per tree.
+ * n_seqs sequences are stepped together; arrays are [n_seqs][n_tree], and
+ * every sequence has its own caches, [n_seqs][max_ctx][n_kv_heads][head_dim] f16,
+ * of which the first ctx_len[s] rows are filled.  Lengths, parents and tokens
+ * are device memory, read when the call runs: a captured step follows them. */
+#define WH_MAX_TREE_NODES 128
+
+/* Grouped-query attention of every node over its sequence's cache, its
+ * ancestors and itself: wh_attention_decode for a tree.  q, k and v rows are
+ * [n_seqs * n_tree] rows of ldq (q) and ldkv (k, v) elements, q rows n_heads *
+ * head_dim, k and v rows n_kv_heads * head_dim (three matrices, or the parts of
+ * one [q | k | v] row).  A node with a ancestors has position ctx_len + a: q and
+ * k are rotated by it (inv_freq of wh_rope_inv_freq; the angle in 64 bits, where
+ * wh_attention_decode forms it in f32 as the reference does: they differ by at
+ * most pos * 2^-24 radians), k and v rounded to f16 and stored in cache row
+ * ctx_len + t, and
+ *   out[t][h] = softmax(q k^T / sqrt(head_dim)) v
+ * over cache rows 0 .. ctx_len - 1 and the rows of the node's ancestors and its
+ * own.  Nodes that a row does not see never touch it, whatever they hold.  An
+ * absent node's out row is zeros and its cache row stays as it was.  A sequence
+ * with ctx_len + n_tree > max_ctx stores nothing, and its out rows are NaN.
+ * head_dim 64 or 128, n_heads (at most 1024) a multiple of n_kv_heads, at most
+ * 1024 sequences.  Caches and workspace are 16-byte aligned; the workspace holds
+ * wh_attention_tree_workspace_bytes(..), 0 for shapes that are not taken. */
+WH_API size_t wh_attention_tree_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads,
+                                                size_t head_dim, size_t max_ctx);
+WH_API int wh_attention_tree(const float* q, const float* k, const float* v, size_t ldq, size_t ldkv,
+                             const int32_t* parents, const uint32_t* ctx_len, size_t n_seqs, size_t n_tree,
+                             void* k_cache, void* v_cache, size_t max_ctx, size_t n_heads, size_t n_kv_heads,
+                             size_t head_dim, const float* inv_freq, float* out, void* workspace,
+                             size_t workspace_bytes, wh_stream_t stream);
+
+/* What is done to logits before a token is chosen.  All arrays are device
+ * memory; a zero-initialised member is left out, but repetition_penalty is 1
+ * where nothing is wanted. */
+typedef struct wh_logits_rules {
+  size_t rows_per_seq;          /* rows of one sequence (n_tree; 0 counts as 1) */
+  const uint32_t* history;      /* tokens so far, [sequences][history_stride] */
+  size_t history_stride;
+  const uint32_t* history_len;  /* how many of them count (null: all) */
+  const uint32_t* tree_tokens;  /* [rows]: the drafted tokens; a row's path counts as history */
+  const int32_t* tree_parents;  /* [rows] */
+  float repetition_penalty;     /* l > 0: l / penalty, else l * penalty */
+  float frequency_penalty;      /* l - count * penalty */
+  float presence_penalty;       /* l - penalty where count > 0 */
+  const uint32_t* bias_ids;     /* l + bias of its token, [sequences][bias_stride]; the last entry of a token counts */
+  const float* bias;
+  size_t n_bias;
+  size_t bias_stride;           /* 0: the same entries for every sequence */
+  const uint32_t* mask;         /* bit i of a row clear: token i is not allowed, [rows][mask_stride] words */
+  size_t mask_stride;
+} wh_logits_rules;
+
+/* Applies the rules to n_rows rows of vocab logits (row r at logits + r * ld)
+ * in this order: repetition, then count * frequency + presence, then the bias,
+ * each rounded to f32 by itself, then -inf where the mask's bit is clear.  Tokens
+ * are counted in the row's history and, with a tree, on the path from the cache
+ * to the row's node, itself included; ids >= vocab are passed over.
+ * out (may be logits itself, with the same stride, or null) receives the rows,
+ * token (may be null) the lowest token of each row's largest logit: one that is
+ * neither NaN nor -inf, or 0xFFFFFFFF where there is none (an id that
+ * wh_llama_forward_token answers with NaN).  The row of an absent node is left
+ * as it was, its token 0xFFFFFFFF.  The workspace is needed for token only. */
+WH_API size_t wh_logits_process_workspace_bytes(const wh_logits_rules* rules, size_t n_rows, size_t vocab);
+WH_API int wh_logits_process(const wh_logits_rules* rules, const float* logits, size_t ld, size_t n_rows, size_t vocab,
+                             float* out, size_t ld_out, uint32_t* token, void* workspace, size_t workspace_bytes,
+                             wh_stream_t stream);
+
+/* The walk along the chosen tokens: from node 0 (the token that the last step
+ * chose; parents -1) to the lowest child that carries the token picked at the
+ * node (wh_logits_process), and on from there.  path [n_seqs][n_tree] receives
+ * the nodes in order, then 0xFFFFFFFF; n_accepted their number (0 if node 0 is
+ * absent) and next_token the token picked at the last of them (0xFFFFFFFF for
+ * none).  With ctx_len: ctx_len_out (may be null, or ctx_len itself) receives
+ * ctx_len + n_accepted, and history (may be null) the accepted tokens at
+ * ctx_len .. of its sequence's history_stride tokens, those that fit. */
+WH_API int wh_tree_accept(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs,
+                          size_t n_tree, uint32_t* path, uint32_t* n_accepted, uint32_t* next_token,
+                          const uint32_t* ctx_len, uint32_t* ctx_len_out, uint32_t* history, size_t history_stride,
+                          wh_stream_t stream);
+
+/* Moves the accepted nodes' cache rows together in every layer: row first + i
+ * takes row first + path[i] for i < n_accepted, first = ctx_len - n_accepted,
+ * where ctx_len is the length behind the walk (ctx_len_out).  The caches are
+ * host arrays of n_layers distinct device pointers.  Paths ascend, as
+ * wh_tree_accept writes them; entries that do not name a later row of the tree
+ * move nothing, nor does a sequence whose numbers do not fit its cache. */
+WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, size_t n_layers, size_t n_seqs,
+                               size_t max_ctx, size_t n_kv_heads, size_t head_dim, const uint32_t* path, size_t n_tree,
+                               const uint32_t* n_accepted, const uint32_t* ctx_len, wh_stream_t stream);
+
 /* --------------------------------------------------------------- GGUF files */
 /* A parsed GGUF file: header, metadata key/values and the tensor table of
  * woolly-gguf's GGUFLoader (crates/woolly-gguf/src/loader.rs:111-200), over a

@@ -30,6 +30,8 @@ WH_ERR_TYPE_MISMATCH = 13
 
 # WH_LLAMA_DECODE_NOALLOC_MAX_BYTES: the static scratch of wh_llama_decode_step_noalloc
 LLAMA_DECODE_NOALLOC_MAX_BYTES = 16 << 20
+# WH_MAX_TREE_NODES: nodes of one tree of drafted tokens
+MAX_TREE_NODES = 128
 
 STATUS_NAMES = {
     0: "WH_OK",
@@ -131,6 +133,26 @@ class wh_llama_model(C.Structure):
     ]
 
 
+class wh_logits_rules(C.Structure):
+    _fields_ = [
+        ("rows_per_seq", C.c_size_t),
+        ("history", C.c_void_p),
+        ("history_stride", C.c_size_t),
+        ("history_len", C.c_void_p),
+        ("tree_tokens", C.c_void_p),
+        ("tree_parents", C.c_void_p),
+        ("repetition_penalty", C.c_float),
+        ("frequency_penalty", C.c_float),
+        ("presence_penalty", C.c_float),
+        ("bias_ids", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("n_bias", C.c_size_t),
+        ("bias_stride", C.c_size_t),
+        ("mask", C.c_void_p),
+        ("mask_stride", C.c_size_t),
+    ]
+
+
 _sz = C.c_size_t
 _vp = C.c_void_p
 _int = C.c_int
@@ -207,6 +229,13 @@ SIGNATURES = {
     "wh_llama_forward_token": (_int, [C.POINTER(wh_llama_model), _vp, _sz, _f32p, _f32p, _vp, _sz, _vp]),
     "wh_embedding_lookup": (_int, [_int, _vp, _sz, _sz, _vp, _sz, _f32p, _vp]),
     "wh_llama_decode_step_noalloc": (_int, [C.POINTER(wh_llama_model), _sz, _f32p, _f32p, _vp]),
+    "wh_attention_tree_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
+    "wh_attention_tree": (_int, [_f32p, _f32p, _f32p, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz,
+                                 _f32p, _f32p, _vp, _sz, _vp]),
+    "wh_logits_process_workspace_bytes": (_sz, [C.POINTER(wh_logits_rules), _sz, _sz]),
+    "wh_logits_process": (_int, [C.POINTER(wh_logits_rules), _f32p, _sz, _sz, _sz, _f32p, _sz, _vp, _vp, _sz, _vp]),
+    "wh_tree_accept": (_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "wh_kv_cache_compact": (_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp]),
     "wh_gguf_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "wh_gguf_open_buffer": (_int, [_vp, _sz, C.POINTER(_vp)]),
     "wh_gguf_close": (_int, [_vp]),

@@ -1,0 +1,722 @@
+// tree_attention.hip -- grouped-query attention of a tree of drafted tokens
+// over an f16 KV cache, with rotary position embedding, on gfx950.
+//
+// One step verifies n_tree drafted tokens ("nodes") of each of n_seqs
+// sequences.  With A(t) the node t and its ancestors, p_t = ctx_len + |A(t)| - 1
+// its position, and G = n_heads / n_kv_heads:
+//   q, k rotated as in attention.hip: pairs (i, i + d/2) by p_t * inv_freq[i]
+//   cache row ctx_len + t = f16(k), f16(v)
+//   s_j   = (q . k_j) / sqrt(d)   for j < ctx_len and j = ctx_len + a, a in A(t)
+//   out_t = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},  m = max_j s_j
+// Three launches:
+//   1. prepare: one workgroup per node rotates its q heads into f16 hi + lo
+//      limbs, stores its k and v in the cache and writes its ancestor mask; one
+//      more workgroup cuts the sequences into chunks of equal length
+//   2. partial: one workgroup per (chunk, KV head, group of 32 RW query rows)
+//   3. combine: one wave per query row merges its chunks
+//
+// The angle is formed and reduced in 64 bits: in 32 bits p_t * inv_freq is off
+// by up to p_t 2^-24 radians, 0.008 at position 131072.  k is rotated in
+// 64 bits before its two roundings (to f32, to f16), so the stored row is the
+// one the formula gives.
+//
+// Products on the matrix cores (v_mfma_f32_32x32x16_f16).  Rows of the query
+// tile are (node, head of the group): r = t G + g.  S^T = K Q^T has lane l hold
+// row l % 32 and 16 of the tile's 32 keys, so the softmax of a row needs one
+// exchange with lane l ^ 32; the same registers, in the same key order, are
+// the B operand of O^T = V^T P^T, whose A operand comes from the row-major V
+// tile in LDS through transposing reads (ds_read_b64_tr_b16).  q is scaled by a
+// power of two per row and split into f16 hi + lo, and so is P (e^{s - m} 2^6):
+// both products are then as exact as f32 ones (2^-22), with K and V taken from
+// the cache as they are.
+#include "gemm_dev.hpp"
+#include "tree.hpp"
+
+namespace {
+
+constexpr int kPrepThreads = 256;
+constexpr int kAttnWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPScaleLog2 = 6.0f;  // P is held times 2^6 ...
+constexpr float kLazyMax = 8.0f;     // ... and may grow by 2^8 before the running maximum moves: at most 2^14 in f16
+constexpr int kWholeMask = 4;        // mask words per node
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct Params {
+  const float *q, *k, *v;
+  size_t ldq, ldkv;
+  const int32_t* parents;
+  const uint32_t* ctx_len;
+  _Float16 *k_cache, *v_cache;
+  const float* inv_freq;
+  float* out;
+  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target;
+  float scale;
+  // workspace
+  uint32_t* head;       // [0]: chunk length
+  uint2* slots;         // [max_slots] (sequence, chunk of it); sequence n_seqs: none
+  uint32_t* first;      // [n_seqs + 1] first slot
+  uint32_t* total;      // [n_seqs] cache rows of the step, 0: nothing to do
+  uint32_t* mask;       // [n_seqs][n_tree][4]
+  uint32_t* odd;        // [n_seqs][n_kv][n_tree] 1: absent, or v is not finite in f16
+  float* qscale;        // [n_seqs][n_kv][R]
+  _Float16* qlimb;      // [n_seqs][n_kv][R][2][D]
+  float2* ml;           // [max_slots][n_kv][R]
+  float* acc;           // [max_slots][n_kv][R][D]
+};
+
+// ------------------------------------------------------------------ prepare
+// A 64-bit value as the cache holds it: rounded to f32, then to f16.  (The
+// empty statement keeps the compiler from joining the two into one rounding.)
+__device__ __forceinline__ _Float16 stored(double x) {
+  float f = static_cast<float>(x);
+  asm("" : "+v"(f));
+  return static_cast<_Float16>(f);
+}
+
+__device__ __forceinline__ bool seq_fits(const Params& P, uint32_t ctx) {
+  return ctx <= P.max_ctx && P.n_tree <= P.max_ctx - ctx;
+}
+
+// Inclusive prefix sums over the workgroup's 256 threads; red: 4 words of LDS.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const unsigned long long up = __shfl_up(v, off, 64);
+    if (lane >= off) v += up;
+  }
+  __syncthreads();
+  if (lane == 63) red[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; w++) v += red[w];
+  return v;
+}
+
+// Cuts the sequences into chunks: the chunk length is the one (a multiple of
+// 64) that gives about `target` chunks over all sequences, so long and short
+// sequences share the workgroups evenly whatever the lengths on the device.
+// Thread t plans sequences [t per, (t + 1) per); first: LDS [n_seqs + 1].
+__device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long* red) {
+  const uint32_t t = threadIdx.x;
+  const uint32_t per = (P.n_seqs + kPrepThreads - 1) / kPrepThreads;
+  const uint32_t s0 = min(t * per, P.n_seqs), s1 = min(s0 + per, P.n_seqs);
+  auto rows = [&](uint32_t s) -> uint32_t {
+    const uint32_t ctx = P.ctx_len[s];
+    if (!seq_fits(P, ctx)) return 0;
+    for (uint32_t i = 0; i < P.n_tree; i++)
+      if (P.parents[s * P.n_tree + i] == -1) return ctx + P.n_tree;
+    return 0;  // every node is absent
+  };
+  unsigned long long mine = 0;
+  for (uint32_t s = s0; s < s1; s++) {
+    const uint32_t n = rows(s);
+    first[s] = n;
+    P.total[s] = n;
+    mine += n;
+  }
+  mine = block_scan(mine, red);
+  __shared__ unsigned long long total;
+  if (t == kPrepThreads - 1) total = mine;
+  __syncthreads();
+  const unsigned long long even = (total + P.target - 1) / P.target;
+  const uint32_t chunk = static_cast<uint32_t>(max((even + 63) / 64 * 64, 64ull));
+  uint32_t n = 0;
+  for (uint32_t s = s0; s < s1; s++) n += (first[s] + chunk - 1) / chunk;
+  uint32_t at = static_cast<uint32_t>(block_scan(n, red)) - n;
+  for (uint32_t s = s0; s < s1; s++) {
+    const uint32_t c = (first[s] + chunk - 1) / chunk;
+    first[s] = at;
+    P.first[s] = at;
+    at += c;
+  }
+  if (t == kPrepThreads - 1) {
+    first[P.n_seqs] = at;
+    P.first[P.n_seqs] = at;
+    P.head[0] = chunk;
+  }
+  __syncthreads();
+  const uint32_t used = first[P.n_seqs];
+  for (uint32_t y = t; y < P.max_slots; y += kPrepThreads) {
+    uint32_t lo = 0, hi = P.n_seqs;  // the last sequence whose first slot is at most y
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (first[mid] <= y) lo = mid; else hi = mid;
+    }
+    P.slots[y] = y < used ? make_uint2(lo, y - first[lo]) : make_uint2(P.n_seqs, 0);
+  }
+}
+
+// grid: n_seqs * n_tree workgroups for the nodes, then one for the chunks.
+template <int D>
+__global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params P) {
+  __shared__ whd::TreeScratch ts;
+  __shared__ double cosd[D / 2], sind[D / 2];
+  __shared__ uint32_t first[wh::kMaxTreeSeqs + 1];
+  __shared__ unsigned long long red[kPrepThreads / 64];
+  if (blockIdx.x == P.n_seqs * P.n_tree) {
+    plan_chunks(P, first, red);
+    return;
+  }
+  const uint32_t s = blockIdx.x / P.n_tree, t = blockIdx.x % P.n_tree;
+  const uint32_t(*mask)[4] = whd::tree_ancestors(P.parents + static_cast<size_t>(s) * P.n_tree, P.n_tree, ts);
+  const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t ctx = P.ctx_len[s];
+  const bool fits = seq_fits(P, ctx);
+  const uint32_t depth = __popc(mask[t][0]) + __popc(mask[t][1]) + __popc(mask[t][2]) + __popc(mask[t][3]);
+  const bool present = depth > 0 && fits;  // a present node's mask holds the node itself
+  const size_t row = static_cast<size_t>(s) * P.n_tree + t;
+  if (tid < kWholeMask) P.mask[row * kWholeMask + tid] = present ? mask[t][tid] : 0u;
+  if (tid < D / 2) {
+    const double a = static_cast<double>(ctx + depth - 1) * static_cast<double>(P.inv_freq[tid]);
+    sincos(a, &sind[tid], &cosd[tid]);
+  }
+  __syncthreads();
+  // q: one wave per head; lane i rotates pair i (lanes past D/2 repeat a pair)
+  const uint32_t i = lane % (D / 2);
+  const float cs = static_cast<float>(cosd[i]), sn = static_cast<float>(sind[i]);
+  for (uint32_t h = wave; h < P.n_heads; h += kPrepThreads / 64) {
+    const float* q = P.q + row * P.ldq + static_cast<size_t>(h) * D;
+    float a = 0.f, b = 0.f;
+    if (present) {
+      const float x = q[i], y = q[i + D / 2];
+      a = x * cs - y * sn;
+      b = x * sn + y * cs;
+    }
+    float mx = fmaxf(fabsf(a), fabsf(b));
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+    // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element
+    // to 2^-22 of itself or 2^-38 of the largest
+    int e = 0;
+    if (mx > 0.f && mx < INFINITY) e = min(max(13 - ilogbf(mx), -100), 100);
+    a = ldexpf(a, e);
+    b = ldexpf(b, e);
+    const uint32_t kvh = h / P.G, r = t * P.G + h % P.G;
+    const size_t qrow = (static_cast<size_t>(s) * P.n_kv + kvh) * P.R + r;
+    _Float16* o = P.qlimb + qrow * 2 * D;
+    if (lane < D / 2) {
+      const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+      o[i] = ah;
+      o[i + D / 2] = bh;
+      o[D + i] = static_cast<_Float16>(a - static_cast<float>(ah));
+      o[D + i + D / 2] = static_cast<_Float16>(b - static_cast<float>(bh));
+    }
+    if (lane == 0) P.qscale[qrow] = ldexpf(P.scale * kLog2e, -e);
+  }
+  // k and v into the cache row of the node
+  for (uint32_t h = wave; h < P.n_kv; h += kPrepThreads / 64) {
+    uint32_t odd = 1;
+    if (present) {
+      const float* k = P.k + row * P.ldkv + static_cast<size_t>(h) * D;
+      const float* v = P.v + row * P.ldkv + static_cast<size_t>(h) * D;
+      const size_t at = ((static_cast<size_t>(s) * P.max_ctx + ctx + t) * P.n_kv + h) * D;
+      const double x = k[i], y = k[i + D / 2];
+      const _Float16 v0 = static_cast<_Float16>(v[i]), v1 = static_cast<_Float16>(v[i + D / 2]);
+      if (lane < D / 2) {
+        P.k_cache[at + i] = stored(x * cosd[i] - y * sind[i]);
+        P.k_cache[at + i + D / 2] = stored(x * sind[i] + y * cosd[i]);
+        P.v_cache[at + i] = v0;
+        P.v_cache[at + i + D / 2] = v1;
+      }
+      const bool fine = fabsf(static_cast<float>(v0)) < INFINITY && fabsf(static_cast<float>(v1)) < INFINITY;
+      odd = __ballot(!fine) != 0;
+    }
+    if (lane == 0) P.odd[(static_cast<size_t>(s) * P.n_kv + h) * P.n_tree + t] = odd;
+  }
+}
+
+// ------------------------------------------------------------------ partial
+// LDS rows of K and V are D f16 without padding (the copies write 16 lanes'
+// chunks in a row), so the 16-byte chunks of row r are permuted: chunk c lies
+// at c ^ swz(r).  K: a wave's operand read takes one chunk of 32 rows; V: a
+// transposing read takes four chunks of each of 4 rows.  With these every 16
+// (32) lanes reach all 64 banks once.
+template <int D>
+__device__ __forceinline__ int swz_k(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+template <int D>
+__device__ __forceinline__ int swz_v(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+
+__device__ __forceinline__ s16x4 read_tr(uint32_t lds) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds);
+}
+
+__device__ __forceinline__ float swap_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+__device__ __forceinline__ float swap_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+
+// The f16 values of a fragment with infinities and NaN replaced by 0.
+__device__ __forceinline__ half8 finite_only(half8 x) {
+  u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if ((w[i] & 0x7C00u) == 0x7C00u) w[i] &= 0xFFFF0000u;
+    if ((w[i] & 0x7C000000u) == 0x7C000000u) w[i] &= 0x0000FFFFu;
+  }
+  return __builtin_bit_cast(half8, w);
+}
+
+// RW query tiles of 32 rows per workgroup; the 4 waves are RW rows x KW keys.
+template <int D, int RW>
+struct Shape {
+  static constexpr int KW = kAttnWaves / RW;
+  static constexpr int SK = KW == 4 ? 128 : 64;              // keys per stage
+  static constexpr int TILES = SK / 32 / KW;                 // 32-key tiles per wave and stage
+  static constexpr int kTileBytes = SK * D * 2;              // one of K, V
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kMergeBytes = KW > 1 ? kAttnWaves * 32 * (D + 2) * 4 : 0;
+  static constexpr int kLds = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;
+};
+
+// grid: n_kv * n_rg * max_slots, KV head fastest (with 8 KV heads the workgroups
+// of one head run on one XCD and share its L2).
+template <int D, int RW>
+__global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void tree_partial_kernel(const Params P) {
+  using S = Shape<D, RW>;
+  constexpr int KW = S::KW, SK = S::SK, DT = D / 32, KS = D / 16;
+  extern __shared__ __align__(256) unsigned char lds[];
+  const uint32_t kvh = blockIdx.x % P.n_kv, rg = blockIdx.x / P.n_kv % P.n_rg, slot = blockIdx.x / (P.n_kv * P.n_rg);
+  const uint2 sc = P.slots[slot];
+  if (sc.x >= P.n_seqs) return;
+  const uint32_t seq = sc.x, chunk = P.head[0], rows = P.total[seq];
+  const uint32_t ctx = rows - P.n_tree;
+  const uint32_t c0 = sc.y * chunk, c1 = min(c0 + chunk, rows);  // c0 < rows
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = wave / KW, kw = wave % KW;
+  const size_t RS = static_cast<size_t>(P.n_kv) * D * 2;  // bytes between cache rows
+  const size_t head0 = (static_cast<size_t>(seq) * P.max_ctx * P.n_kv + kvh) * D * 2;
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(P.k_cache) + head0;
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(P.v_cache) + head0;
+  const uint32_t lds0 = lds_addr(lds);
+
+  // One stage: rows [k0, k0 + SK) of K and V; a wave copies 1 KB (1024 / (2 D)
+  // rows) at a time.  Rows past the last one repeat it: they are masked.
+  auto issue = [&](uint32_t k0, int buf) {
+    constexpr int kRowsPer = 1024 / (2 * D), kChunks = D / 8;
+    const uint8_t* kb = kbase + k0 * RS;
+    const uint8_t* vb = vbase + k0 * RS;
+    const uint32_t last = rows - 1 - k0;
+#pragma unroll
+    for (int j = 0; j < SK / kRowsPer / kAttnWaves; j++) {
+      const int piece = wave + kAttnWaves * j;
+      const int r = piece * kRowsPer + lane / kChunks, c = lane % kChunks;
+      const uint32_t row = min(static_cast<uint32_t>(r), last) * static_cast<uint32_t>(RS);
+      const uint32_t at = lds0 + buf * S::kStageBytes + piece * 1024;
+      copy16_to_lds(kb, row + 16 * (c ^ swz_k<D>(r)), at);
+      copy16_to_lds(vb, row + 16 * (c ^ swz_v<D>(r)), at + S::kTileBytes);
+    }
+  };
+  issue(c0, 0);
+
+  // this wave's query rows
+  const uint32_t r0 = (rg * RW + rw) * 32 + l32;
+  const uint32_t r = min(r0, P.R - 1);
+  const size_t qrow = (static_cast<size_t>(seq) * P.n_kv + kvh) * P.R + r;
+  half8 qh[KS], ql[KS];
+#pragma unroll
+  for (int j = 0; j < KS; j++) {
+    const _Float16* q = P.qlimb + qrow * 2 * D + 16 * j + 8 * h;
+    qh[j] = *reinterpret_cast<const half8*>(q);
+    ql[j] = *reinterpret_cast<const half8*>(q + D);
+  }
+  const float qs = P.qscale[qrow];
+  uint32_t tm[kWholeMask];
+  {
+    const uint4 w = *reinterpret_cast<const uint4*>(P.mask + (static_cast<size_t>(seq) * P.n_tree + r / P.G) * kWholeMask);
+    tm[0] = w.x, tm[1] = w.y, tm[2] = w.z, tm[3] = w.w;
+  }
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  auto tile = [&](uint32_t base, uint32_t kt, uint32_t vt, int tr) {
+    // kt, vt: LDS addresses of the stage's K and V; tr: the tile's first row there
+    f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KS; j++) {
+      const int rr = tr + l32;
+      const half8 kf = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+          (uintptr_t)(kt + rr * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(rr))));
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[j], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j], s, 0, 0, 0);
+    }
+    uint32_t bits = 0xFFFFFFFFu, odd = 0;
+    const bool tail = base + 32 > ctx;
+    if (tail) {
+      // keys from ctx on are the tree's nodes: bit k of `bits` for key base + k
+      const int off = static_cast<int>(base - ctx);  // > -32
+      if (off < 0) {
+        bits = (tm[0] << -off) | ((1u << -off) - 1u);
+      } else {
+        const int w = off >> 5, sh = off & 31;
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int i = 0; i < kWholeMask; i++) {
+          if (i == w) lo = tm[i];
+          if (i == w + 1) hi = tm[i];
+        }
+        bits = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
+      }
+      const int node = off + l32;
+      const bool is_odd = h == 0 && node >= 0 && node < static_cast<int>(P.n_tree) &&
+                          P.odd[(static_cast<size_t>(seq) * P.n_kv + kvh) * P.n_tree + node] != 0;
+      odd = static_cast<uint32_t>(__ballot(is_odd));
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int key = 8 * (i >> 2) + 4 * h + (i & 3);
+        s[i] = (bits >> key) & 1u ? s[i] : -INFINITY;
+      }
+    }
+    float mt = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) mt = fmaxf(mt, s[i]);
+    mt = swap_max(mt) * qs;
+    if (__ballot(mt > m + kLazyMax)) {
+      const float mn = fmaxf(m, mt);
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] *= al;
+      m = mn;
+    }
+    const float mb = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
+    float p[16], lt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs, mb));
+      lt[i & 3] += p[i];
+    }
+    l += (lt[0] + lt[1]) + (lt[2] + lt[3]);  // one addition to the running sum per tile
+    half8 ph[2], pl[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const _Float16 hi = static_cast<_Float16>(p[8 * ks + i]);
+        ph[ks][i] = hi;
+        pl[ks][i] = static_cast<_Float16>(p[8 * ks + i] - static_cast<float>(hi));
+      }
+    const int i16 = lane & 15, kq = i16 >> 2, dq = i16 & 3, dg = (lane >> 4) & 1;
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        half8 vf;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int rr = tr + 16 * ks + 8 * u + 4 * h + kq;
+          const int c = 4 * d + 2 * dg + (dq >> 1);
+          const s16x4 x = read_tr(vt + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
+          const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
+#pragma unroll
+          for (int i = 0; i < 4; i++) vf[4 * u + i] = y[i];
+        }
+        if (odd) vf = finite_only(vf);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[ks], acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[ks], acc[d], 0, 0, 0);
+      }
+    // nodes whose v holds an infinity or NaN: those elements count for the
+    // rows that see the node, and for no other (0 * inf would spread a NaN)
+    while (odd) {
+      const int key = __builtin_ctz(odd);
+      odd &= odd - 1;
+      float pk = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (8 * (i >> 2) + (i & 3) == (key & ~4)) pk = p[i];
+      pk = __shfl(pk, l32 + 32 * ((key >> 2) & 1), 64);
+      if (!((bits >> key) & 1u)) continue;
+      const int rr = tr + key;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
+          const float x = static_cast<float>(*reinterpret_cast<const __attribute__((address_space(3))) _Float16*>(
+              (uintptr_t)(vt + rr * 2 * D + 16 * ((dim >> 3) ^ swz_v<D>(rr)) + 2 * (dim & 7))));
+          if (!(fabsf(x) < INFINITY)) acc[d][i] += pk * x;
+        }
+    }
+  };
+
+  const uint32_t n_stages = (c1 - c0 + SK - 1) / SK;
+  for (uint32_t st = 0; st < n_stages; st++) {
+    wait_vmcnt<0>();  // this wave's copies of stage st
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // everyone's; and everyone has read stage st - 1
+    asm volatile("" ::: "memory");
+    if (st + 1 < n_stages) issue(c0 + (st + 1) * SK, (st + 1) & 1);
+    const uint32_t kt = lds0 + (st & 1) * S::kStageBytes, vt = kt + S::kTileBytes;
+#pragma unroll 1
+    for (int u = 0; u < S::TILES; u++) {
+      const int tr = 32 * (kw + KW * u);
+      const uint32_t base = c0 + st * SK + tr;
+      if (base < c1) tile(base, kt, vt, tr);
+    }
+  }
+  l = swap_sum(l);
+
+  const size_t prow = (static_cast<size_t>(slot) * P.n_kv + kvh) * P.R;
+  if constexpr (KW == 1) {
+    if (r0 < P.R) {
+      float* o = P.acc + (prow + r0) * D;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          *reinterpret_cast<float4*>(o + 32 * d + 8 * i + 4 * h) =
+              make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+      if (h == 0) P.ml[prow + r0] = make_float2(m, l);
+    }
+  } else {
+    // the KW waves of each query tile join in LDS, in fixed order
+    __syncthreads();
+    float* am = reinterpret_cast<float*>(lds);             // [4][32][D]
+    float* mm = am + kAttnWaves * 32 * D;                  // [4][32][2]
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<float4*>(am + (wave * 32 + l32) * D + 32 * d + 8 * i + 4 * h) =
+            make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+    if (h == 0) {
+      mm[2 * (wave * 32 + l32)] = m;
+      mm[2 * (wave * 32 + l32) + 1] = l;
+    }
+    __syncthreads();
+    for (int e = tid; e < RW * 32 * (D / 4); e += 64 * kAttnWaves) {
+      const int rr = e / (D / 4), d4 = e % (D / 4);
+      const uint32_t rglob = rg * RW * 32 + rr;
+      if (rglob >= P.R) continue;
+      const int w0 = (rr / 32) * KW, lr = rr % 32;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KW; w++) M = fmaxf(M, mm[2 * ((w0 + w) * 32 + lr)]);
+      float L = 0.f;
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < KW; w++) {
+        const float mw = mm[2 * ((w0 + w) * 32 + lr)];
+        const float ew = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
+        L = __builtin_fmaf(mm[2 * ((w0 + w) * 32 + lr) + 1], ew, L);
+        const float4 a = *reinterpret_cast<const float4*>(am + ((w0 + w) * 32 + lr) * D + 4 * d4);
+        A.x = __builtin_fmaf(a.x, ew, A.x);
+        A.y = __builtin_fmaf(a.y, ew, A.y);
+        A.z = __builtin_fmaf(a.z, ew, A.z);
+        A.w = __builtin_fmaf(a.w, ew, A.w);
+      }
+      *reinterpret_cast<float4*>(P.acc + (prow + rglob) * D + 4 * d4) = A;
+      if (d4 == 0) P.ml[prow + rglob] = make_float2(M, L);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ combine
+// One wave per (node, head): out = sum_c acc_c 2^{m_c - M} / sum_c l_c 2^{m_c - M}.
+// Rows of absent nodes are zeros; those of a sequence whose rows do not fit its
+// cache are NaN.
+template <int D>
+__global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
+  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (id >= P.n_seqs * P.n_tree * P.n_heads) return;
+  const uint32_t head = id % P.n_heads, row = id / P.n_heads, seq = row / P.n_tree, t = row % P.n_tree;
+  constexpr int V = D / 64;  // dims per lane
+  float* o = P.out + static_cast<size_t>(row) * P.n_heads * D + static_cast<size_t>(head) * D + V * lane;
+  const uint4 w = *reinterpret_cast<const uint4*>(P.mask + static_cast<size_t>(row) * kWholeMask);
+  if ((w.x | w.y | w.z | w.w) == 0) {
+    const float fill = seq_fits(P, P.ctx_len[seq]) ? 0.f : __builtin_nanf("");
+    for (int i = 0; i < V; i++) o[i] = fill;
+    return;
+  }
+  const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
+  const size_t step = static_cast<size_t>(P.n_kv) * P.R;
+  const size_t at = (static_cast<size_t>(c0) * P.n_kv + head / P.G) * P.R + t * P.G + head % P.G;
+  float M = -INFINITY;
+  for (uint32_t c = lane; c < n; c += 64) M = fmaxf(M, P.ml[at + c * step].x);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  float L = 0.f, A[V] = {};
+#pragma unroll 4
+  for (uint32_t c = 0; c < n; c++) {
+    const float2 ml = P.ml[at + c * step];
+    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+    L = __builtin_fmaf(ml.y, ew, L);
+    const float* a = P.acc + (at + c * step) * D + V * lane;
+#pragma unroll
+    for (int i = 0; i < V; i++) A[i] = __builtin_fmaf(a[i], ew, A[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) o[i] = A[i] / L;
+}
+
+// ------------------------------------------------------------------ launching
+size_t al256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Query tiles per workgroup: as many as the rows of one KV head fill, up to 4
+// (K and V are read once per 128 rows).
+int row_tiles(size_t R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
+
+struct Plan {
+  int rw;
+  size_t G, R, n_rg, target, max_slots;
+};
+Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t max_ctx) {
+  Plan p;
+  p.G = n_heads / n_kv;
+  p.R = n_tree * p.G;
+  p.rw = row_tiles(p.R);
+  p.n_rg = (p.R + 32 * p.rw - 1) / (32 * p.rw);
+  // one workgroup per CU with 128 KB of stages, two with 64 KB
+  const size_t want = static_cast<size_t>(wh::cu_count()) * (p.rw == 1 ? 1 : 2);
+  p.target = (want + n_kv * p.n_rg - 1) / (n_kv * p.n_rg);
+  const size_t most = n_seqs * ((max_ctx + 63) / 64);
+  p.max_slots = p.target + n_seqs < most ? p.target + n_seqs : most;
+  return p;
+}
+
+// Lays the workspace out (offsets only where base is null); returns its size.
+size_t layout(Params& P, size_t D, void* base) {
+  char* b = static_cast<char*>(base);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* r = b ? b + off : nullptr;
+    off += al256(bytes);
+    return r;
+  };
+  const size_t slots = P.max_slots, rows = static_cast<size_t>(P.n_kv) * P.R;
+  P.head = reinterpret_cast<uint32_t*>(take(4));
+  P.slots = reinterpret_cast<uint2*>(take(8 * slots));
+  P.first = reinterpret_cast<uint32_t*>(take(4 * (static_cast<size_t>(P.n_seqs) + 1)));
+  P.total = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(P.n_seqs)));
+  P.mask = reinterpret_cast<uint32_t*>(take(4 * kWholeMask * static_cast<size_t>(P.n_seqs) * P.n_tree));
+  P.odd = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(P.n_seqs) * P.n_kv * P.n_tree));
+  P.qscale = reinterpret_cast<float*>(take(4 * P.n_seqs * rows));
+  P.qlimb = reinterpret_cast<_Float16*>(take(2 * 2 * D * P.n_seqs * rows));
+  P.ml = reinterpret_cast<float2*>(take(8 * slots * rows));
+  P.acc = reinterpret_cast<float*>(take(4 * D * slots * rows));
+  return off;
+}
+
+Params fill(const Plan& p, size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t D, size_t max_ctx) {
+  Params P{};
+  P.n_seqs = static_cast<uint32_t>(n_seqs);
+  P.n_tree = static_cast<uint32_t>(n_tree);
+  P.max_ctx = static_cast<uint32_t>(max_ctx);
+  P.n_heads = static_cast<uint32_t>(n_heads);
+  P.n_kv = static_cast<uint32_t>(n_kv);
+  P.G = static_cast<uint32_t>(p.G);
+  P.R = static_cast<uint32_t>(p.R);
+  P.n_rg = static_cast<uint32_t>(p.n_rg);
+  P.max_slots = static_cast<uint32_t>(p.max_slots);
+  P.target = static_cast<uint32_t>(p.target);
+  P.scale = 1.0f / sqrtf(static_cast<float>(D));
+  return P;
+}
+
+template <int D, int RW>
+int launch_partial(const Params& P, hipStream_t s) {
+  WH_ENSURE_LDS(static_cast<size_t>(Shape<D, RW>::kLds), &tree_partial_kernel<D, RW>);
+  tree_partial_kernel<D, RW><<<P.n_kv * P.n_rg * P.max_slots, 64 * kAttnWaves, Shape<D, RW>::kLds, s>>>(P);
+  WH_LAUNCH_CHECK("tree attention kernel launch");
+  return WH_OK;
+}
+
+template <int D>
+int launch_all(const Params& P, int rw, hipStream_t s) {
+  tree_prepare_kernel<D><<<P.n_seqs * P.n_tree + 1, kPrepThreads, 0, s>>>(P);
+  WH_LAUNCH_CHECK("tree attention prepare launch");
+  int st = rw == 1 ? launch_partial<D, 1>(P, s) : rw == 2 ? launch_partial<D, 2>(P, s) : launch_partial<D, 4>(P, s);
+  if (st) return st;
+  const size_t out_rows = static_cast<size_t>(P.n_seqs) * P.n_tree * P.n_heads;
+  tree_combine_kernel<D><<<static_cast<unsigned>((out_rows + 3) / 4), 256, 0, s>>>(P);
+  WH_LAUNCH_CHECK("tree attention combine launch");
+  return WH_OK;
+}
+
+}  // namespace
+
+namespace wh {
+
+bool tree_attention_shape_ok(size_t n_heads, size_t n_kv_heads, size_t head_dim) {
+  return (head_dim == 64 || head_dim == 128) && n_kv_heads > 0 && n_heads > 0 && n_heads <= 1024 && n_heads % n_kv_heads == 0;
+}
+
+size_t tree_attention_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                                      size_t max_ctx) {
+  const Plan p = make_plan(n_seqs, n_tree, n_heads, n_kv_heads, max_ctx);
+  Params P = fill(p, n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx);
+  return layout(P, head_dim, nullptr);
+}
+
+int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t s) {
+  const Plan p = make_plan(a.n_seqs, a.n_tree, a.n_heads, a.n_kv_heads, a.max_ctx);
+  Params P = fill(p, a.n_seqs, a.n_tree, a.n_heads, a.n_kv_heads, a.head_dim, a.max_ctx);
+  layout(P, a.head_dim, workspace);
+  P.q = a.q, P.k = a.k, P.v = a.v;
+  P.ldq = a.ldq, P.ldkv = a.ldkv;
+  P.parents = a.parents;
+  P.ctx_len = a.ctx_len;
+  P.k_cache = static_cast<_Float16*>(a.k_cache);
+  P.v_cache = static_cast<_Float16*>(a.v_cache);
+  P.inv_freq = a.inv_freq;
+  P.out = a.out;
+  return a.head_dim == 128 ? launch_all<128>(P, p.rw, s) : launch_all<64>(P, p.rw, s);
+}
+
+}  // namespace wh
+
+WH_API size_t wh_attention_tree_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads,
+                                                size_t head_dim, size_t max_ctx) {
+  if (n_seqs == 0 || n_tree == 0 || n_seqs > wh::kMaxTreeSeqs || n_tree > wh::kMaxTreeNodes || max_ctx >> 31 ||
+      !wh::tree_attention_shape_ok(n_heads, n_kv_heads, head_dim))
+    return 0;
+  return wh::tree_attention_workspace_bytes(n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx);
+}
+
+WH_API int wh_attention_tree(const float* q, const float* k, const float* v, size_t ldq, size_t ldkv,
+                             const int32_t* parents, const uint32_t* ctx_len, size_t n_seqs, size_t n_tree,
+                             void* k_cache, void* v_cache, size_t max_ctx, size_t n_heads, size_t n_kv_heads,
+                             size_t head_dim, const float* inv_freq, float* out, void* workspace,
+                             size_t workspace_bytes, wh_stream_t stream) {
+  if (!wh::tree_attention_shape_ok(n_heads, n_kv_heads, head_dim))
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: head_dim %zu, %zu heads, %zu KV heads not supported",
+                         head_dim, n_heads, n_kv_heads);
+  if (n_tree > wh::kMaxTreeNodes || n_seqs > wh::kMaxTreeSeqs)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: %zu nodes of %zu sequences (at most %zu of %zu)", n_tree,
+                         n_seqs, wh::kMaxTreeNodes, wh::kMaxTreeSeqs);
+  if (max_ctx == 0 || max_ctx >> 31)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: max_ctx = %zu out of range", max_ctx);
+  if (ldq < n_heads * head_dim || ldkv < n_kv_heads * head_dim)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: row strides %zu, %zu below the rows' %zu, %zu elements",
+                         ldq, ldkv, n_heads * head_dim, n_kv_heads * head_dim);
+  if (n_seqs == 0 || n_tree == 0) return WH_OK;
+  if (!q || !k || !v || !parents || !ctx_len || !k_cache || !v_cache || !inv_freq || !out || !workspace)
+    return wh::set_error(WH_ERR_INVALID_ARGUMENT, "attention_tree: null pointer");
+  if (!wh::aligned(k_cache, 16) || !wh::aligned(v_cache, 16) || !wh::aligned(workspace, 16))
+    return wh::set_error(WH_ERR_INVALID_ARGUMENT, "attention_tree: caches and workspace must be 16-byte aligned");
+  if (!wh::aligned(q, 4) || !wh::aligned(k, 4) || !wh::aligned(v, 4) || !wh::aligned(parents, 4) ||
+      !wh::aligned(ctx_len, 4) || !wh::aligned(inv_freq, 4) || !wh::aligned(out, 4))
+    return wh::set_error(WH_ERR_INVALID_ARGUMENT, "attention_tree: arrays must be 4-byte aligned");
+  const size_t need = wh::tree_attention_workspace_bytes(n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx);
+  if (workspace_bytes < need)
+    return wh::set_error(WH_ERR_BUFFER_TOO_SMALL, "attention_tree: workspace too small: needed %zu bytes, available %zu",
+                         need, workspace_bytes);
+  const wh::TreeAttnArgs a{q,       k,       v,       ldq,       ldkv,     parents,    ctx_len,  n_seqs, n_tree,
+                           k_cache, v_cache, max_ctx, n_heads, n_kv_heads, head_dim, inv_freq, out};
+  return wh::launch_tree_attention(a, workspace, reinterpret_cast<hipStream_t>(stream));
+}

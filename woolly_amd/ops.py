@@ -244,6 +244,89 @@ def embedding_lookup(ggml_type: int, table, vocab: int, hidden: int, input_ids, 
     return idb
 
 
+# --------------------------------------------- a tree of drafted tokens
+MAX_TREE_NODES = _lib.MAX_TREE_NODES
+NO_TOKEN = 0xFFFFFFFF
+
+
+def attention_tree_workspace_bytes(n_seqs: int, n_tree: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                                   max_ctx: int) -> int:
+    return int(_lib.load().wh_attention_tree_workspace_bytes(n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx))
+
+
+def attention_tree(q, k, v, ldq: int, ldkv: int, parents, ctx_len, n_seqs: int, n_tree: int, k_cache, v_cache,
+                   max_ctx: int, n_heads: int, n_kv_heads: int, head_dim: int, inv_freq, out, workspace,
+                   workspace_bytes: int, stream: Stream | None = None) -> None:
+    """Attention of every node of n_seqs trees of drafted tokens over its
+    sequence's cache and its own ancestors; the nodes' k and v go to cache rows
+    ctx_len .. (wh_attention_tree)."""
+    _lib.check(_lib.load().wh_attention_tree(_p(q), _p(k), _p(v), ldq, ldkv, _p(parents), _p(ctx_len), n_seqs, n_tree,
+                                             _p(k_cache), _p(v_cache), max_ctx, n_heads, n_kv_heads, head_dim,
+                                             _p(inv_freq), _p(out), _p(workspace), workspace_bytes, _s(stream)))
+
+
+class LogitsRules:
+    """What logits_process does to logits before a token is chosen: the members
+    of wh_logits_rules by name (device buffers or addresses, sizes, penalties).
+    Keeps the buffers that it is given."""
+
+    def __init__(self, rows_per_seq: int = 1, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
+                 presence_penalty: float = 0.0, **members) -> None:
+        r = _lib.wh_logits_rules()
+        r.rows_per_seq = rows_per_seq
+        r.repetition_penalty = repetition_penalty
+        r.frequency_penalty = frequency_penalty
+        r.presence_penalty = presence_penalty
+        known = {n: t for n, t in _lib.wh_logits_rules._fields_}
+        for name, value in members.items():
+            if name not in known:
+                raise TypeError(f"LogitsRules has no member {name!r}")
+            setattr(r, name, (_p(value) or None) if known[name] is C.c_void_p else int(value))
+        self._keep = members
+        self.rules = r
+        self._ref = C.byref(r)
+
+
+def logits_process_workspace_bytes(rules: LogitsRules, n_rows: int, vocab: int) -> int:
+    return int(_lib.load().wh_logits_process_workspace_bytes(rules._ref, n_rows, vocab))
+
+
+def logits_process(rules: LogitsRules, logits, ld: int, n_rows: int, vocab: int, out, ld_out: int, token,
+                   workspace=None, workspace_bytes: int = 0, stream: Stream | None = None) -> None:
+    """Penalties, biases and the grammar's mask on rows of logits, and each row's
+    highest token (wh_logits_process); out and token may each be None."""
+    _lib.check(_lib.load().wh_logits_process(rules._ref, _p(logits), ld, n_rows, vocab, _p(out) or None, ld_out,
+                                             _p(token) or None, _p(workspace) or None, workspace_bytes, _s(stream)))
+
+
+def tree_accept(tokens, parents, picked, n_seqs: int, n_tree: int, path, n_accepted, next_token, ctx_len=None,
+                ctx_len_out=None, history=None, history_stride: int = 0, stream: Stream | None = None) -> None:
+    """The walk from node 0 along the picked tokens (wh_tree_accept)."""
+    _lib.check(_lib.load().wh_tree_accept(_p(tokens), _p(parents), _p(picked), n_seqs, n_tree, _p(path), _p(n_accepted),
+                                          _p(next_token), _p(ctx_len) or None, _p(ctx_len_out) or None,
+                                          _p(history) or None, history_stride, _s(stream)))
+
+
+class KvCaches:
+    """The layers' K and V caches as kv_cache_compact takes them."""
+
+    def __init__(self, k_caches, v_caches) -> None:
+        if len(k_caches) != len(v_caches):
+            raise ValueError(f"{len(k_caches)} K caches and {len(v_caches)} V caches")
+        self._keep = (k_caches, v_caches)
+        self.n_layers = len(k_caches)
+        self.k = (C.c_void_p * self.n_layers)(*[_p(b) or None for b in k_caches])
+        self.v = (C.c_void_p * self.n_layers)(*[_p(b) or None for b in v_caches])
+
+
+def kv_cache_compact(caches: KvCaches, n_seqs: int, max_ctx: int, n_kv_heads: int, head_dim: int, path, n_tree: int,
+                     n_accepted, ctx_len, stream: Stream | None = None) -> None:
+    """The accepted nodes' cache rows moved together in every layer (wh_kv_cache_compact)."""
+    _lib.check(_lib.load().wh_kv_cache_compact(C.addressof(caches.k), C.addressof(caches.v), caches.n_layers, n_seqs,
+                                               max_ctx, n_kv_heads, head_dim, _p(path), n_tree, _p(n_accepted),
+                                               _p(ctx_len), _s(stream)))
+
+
 class LlamaModel:
     """A Llama-shaped model on the device for the decode step: `layers` is a
     list of dicts of device buffers (attn_norm, wq, wk, wv, wo, ffn_norm,
