@@ -67,7 +67,6 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const Params P) {
 #pragma clang fp contract(off)
   __shared__ uint32_t count[kChunk];
   __shared__ int entry[kChunk];
-  __shared__ whd::TreeScratch ts;
   __shared__ unsigned long long red[kThreads / 64];
   const uint32_t row = blockIdx.y, seq = row / P.rows_per_seq, node = row % P.rows_per_seq;
   const uint32_t i0 = blockIdx.x * kChunk, n = min(P.vocab - i0, static_cast<uint32_t>(kChunk));
@@ -80,10 +79,10 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const Params P) {
   __syncthreads();
   bool present = true;
   if (P.tree_parents) {
-    const uint32_t(*mask)[4] =
-        whd::tree_ancestors(P.tree_parents + static_cast<size_t>(seq) * P.rows_per_seq, P.rows_per_seq, ts);
-    present = (mask[node][0] | mask[node][1] | mask[node][2] | mask[node][3]) != 0;
-    if (t < P.rows_per_seq && (mask[node][t >> 5] >> (t & 31)) & 1u) {
+    const whd::TreePath path =
+        whd::tree_path(P.tree_parents + static_cast<size_t>(seq) * P.rows_per_seq, P.rows_per_seq, node);
+    present = path.present();
+    if (t < P.rows_per_seq && path.has(t)) {
       const uint32_t c = P.tree_tokens[static_cast<size_t>(seq) * P.rows_per_seq + t] - i0;
       if (c < n) atomicAdd(&count[c], 1u);
     }

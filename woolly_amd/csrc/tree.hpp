@@ -34,46 +34,33 @@ int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t st
 
 namespace whd {
 
-// Ancestors of every node of one tree in LDS, by pointer doubling: bit a of
-// mask[t] is set where a is t itself or an ancestor of t; depth[t] counts the
-// ancestors.  A node whose parent is neither -1 nor an earlier node is absent,
-// and so are all below it: their masks are 0.  Every thread of the workgroup
-// calls it (thread i < 128 keeps node i); 7 rounds join 2^7 = 128 levels.
-struct TreeScratch {
-  uint32_t mask[2][128][4];
-  int jump[2][128];
+// The path from the cache to node t of one tree: bit a is set where a is t itself
+// or an ancestor of t; depth counts its ancestors.  A node whose parent is
+// neither -1 nor an earlier node is absent, and so are all below it: no bits.
+// One wave walks by itself, without LDS or barriers: its lanes hold the parents
+// and every step reads one of them as a scalar (some 20 cycles; a path has as
+// many steps as nodes, at most 128).
+struct TreePath {
+  unsigned long long lo, hi;  // nodes 0..63, 64..127
+  int depth;
+  __device__ __forceinline__ bool present() const { return (lo | hi) != 0; }
+  __device__ __forceinline__ bool has(int a) const { return ((a < 64 ? lo : hi) >> (a & 63)) & 1u; }
 };
-__device__ __forceinline__ const uint32_t (*tree_ancestors(const int32_t* __restrict__ parents, int n_tree,
-                                                           TreeScratch& ts))[4] {
-  constexpr int kCache = -1, kAbsent = -2;
-  const int t = threadIdx.x;
-  if (t < 128) {
-    int p = kAbsent;
-    if (t < n_tree) {
-      const int g = parents[t];
-      p = g == -1 ? kCache : (g >= 0 && g < t ? g : kAbsent);
-    }
-    for (int w = 0; w < 4; w++) ts.mask[0][t][w] = (t >> 5) == w ? 1u << (t & 31) : 0u;
-    ts.jump[0][t] = p;
+__device__ __forceinline__ TreePath tree_path(const int32_t* __restrict__ parents, int n_tree, int t) {
+  const int lane = threadIdx.x & 63;
+  // a parent that is no earlier node ends the walk below -1
+  const int g0 = lane < n_tree ? parents[lane] : -2, g1 = lane + 64 < n_tree ? parents[lane + 64] : -2;
+  const int p0 = g0 >= lane ? -2 : g0, p1 = g1 >= lane + 64 ? -2 : g1;
+  TreePath p{0, 0, -1};
+  int at = t;
+  while (at >= 0) {  // falls with every step
+    if (at < 64) p.lo |= 1ull << at; else p.hi |= 1ull << (at - 64);
+    p.depth++;
+    const int a = __builtin_amdgcn_readlane(p0, at & 63), b = __builtin_amdgcn_readlane(p1, at & 63);
+    at = at < 64 ? a : b;
   }
-  int cur = 0;
-  for (int round = 0; round < 7; round++) {
-    __syncthreads();
-    if (t < 128) {
-      const int j = ts.jump[cur][t];
-      uint32_t m[4];
-      for (int w = 0; w < 4; w++) m[w] = ts.mask[cur][t][w] | (j >= 0 ? ts.mask[cur][j][w] : 0u);
-      for (int w = 0; w < 4; w++) ts.mask[cur ^ 1][t][w] = m[w];
-      ts.jump[cur ^ 1][t] = j >= 0 ? ts.jump[cur][j] : j;
-    }
-    cur ^= 1;
-  }
-  __syncthreads();
-  if (t < 128 && ts.jump[cur][t] != kCache) {
-    for (int w = 0; w < 4; w++) ts.mask[cur][t][w] = 0u;
-  }
-  __syncthreads();
-  return ts.mask[cur];
+  if (at != -1) p = TreePath{0, 0, 0};
+  return p;
 }
 
 }  // namespace whd

@@ -29,6 +29,8 @@
 // power of two per row and split into f16 hi + lo, and so is P (e^{s - m} 2^6):
 // both products are then as exact as f32 ones (2^-22), with K and V taken from
 // the cache as they are.
+#include <type_traits>
+
 #include "gemm_dev.hpp"
 #include "tree.hpp"
 
@@ -60,7 +62,6 @@ struct Params {
   uint32_t* first;      // [n_seqs + 1] first slot
   uint32_t* total;      // [n_seqs] cache rows of the step, 0: nothing to do
   uint32_t* mask;       // [n_seqs][n_tree][4]
-  uint32_t* odd;        // [n_seqs][n_kv][n_tree] 1: absent, or v is not finite in f16
   float* qscale;        // [n_seqs][n_kv][R]
   _Float16* qlimb;      // [n_seqs][n_kv][R][2][D]
   float2* ml;           // [max_slots][n_kv][R]
@@ -149,82 +150,89 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long
   }
 }
 
-// grid: n_seqs * n_tree workgroups for the nodes, then one for the chunks.
+// grid: (n_seqs * n_tree) nodes x n_groups groups of 8 heads (the q heads, then
+// the KV heads), then one workgroup for the chunks.  A wave takes two heads and
+// asks for their rows before it looks at the tree: the launch is as long as its
+// dependent loads.
+constexpr int kPrepHeads = 2 * kPrepThreads / 64;
 template <int D>
-__global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params P) {
-  __shared__ whd::TreeScratch ts;
-  __shared__ double cosd[D / 2], sind[D / 2];
+__global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params P, uint32_t n_groups) {
   __shared__ uint32_t first[wh::kMaxTreeSeqs + 1];
   __shared__ unsigned long long red[kPrepThreads / 64];
-  if (blockIdx.x == P.n_seqs * P.n_tree) {
+  if (blockIdx.x == P.n_seqs * P.n_tree * n_groups) {
     plan_chunks(P, first, red);
     return;
   }
-  const uint32_t s = blockIdx.x / P.n_tree, t = blockIdx.x % P.n_tree;
-  const uint32_t(*mask)[4] = whd::tree_ancestors(P.parents + static_cast<size_t>(s) * P.n_tree, P.n_tree, ts);
-  const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint32_t ctx = P.ctx_len[s];
-  const bool fits = seq_fits(P, ctx);
-  const uint32_t depth = __popc(mask[t][0]) + __popc(mask[t][1]) + __popc(mask[t][2]) + __popc(mask[t][3]);
-  const bool present = depth > 0 && fits;  // a present node's mask holds the node itself
-  const size_t row = static_cast<size_t>(s) * P.n_tree + t;
-  if (tid < kWholeMask) P.mask[row * kWholeMask + tid] = present ? mask[t][tid] : 0u;
-  if (tid < D / 2) {
-    const double a = static_cast<double>(ctx + depth - 1) * static_cast<double>(P.inv_freq[tid]);
-    sincos(a, &sind[tid], &cosd[tid]);
-  }
-  __syncthreads();
-  // q: one wave per head; lane i rotates pair i (lanes past D/2 repeat a pair)
+  const uint32_t group = blockIdx.x % n_groups, row_id = blockIdx.x / n_groups;
+  const uint32_t s = row_id / P.n_tree, t = row_id % P.n_tree;
+  const size_t row = row_id;
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t i = lane % (D / 2);
-  const float cs = static_cast<float>(cosd[i]), sn = static_cast<float>(sind[i]);
-  for (uint32_t h = wave; h < P.n_heads; h += kPrepThreads / 64) {
-    const float* q = P.q + row * P.ldq + static_cast<size_t>(h) * D;
-    float a = 0.f, b = 0.f;
-    if (present) {
-      const float x = q[i], y = q[i + D / 2];
-      a = x * cs - y * sn;
-      b = x * sn + y * cs;
-    }
-    float mx = fmaxf(fabsf(a), fabsf(b));
+  const uint32_t h0 = group * kPrepHeads + 2 * wave, n_slots = P.n_heads + P.n_kv;
+  float x[2], y[2], vx[2] = {}, vy[2] = {};
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-    // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element
-    // to 2^-22 of itself or 2^-38 of the largest
-    int e = 0;
-    if (mx > 0.f && mx < INFINITY) e = min(max(13 - ilogbf(mx), -100), 100);
-    a = ldexpf(a, e);
-    b = ldexpf(b, e);
-    const uint32_t kvh = h / P.G, r = t * P.G + h % P.G;
-    const size_t qrow = (static_cast<size_t>(s) * P.n_kv + kvh) * P.R + r;
-    _Float16* o = P.qlimb + qrow * 2 * D;
-    if (lane < D / 2) {
-      const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
-      o[i] = ah;
-      o[i + D / 2] = bh;
-      o[D + i] = static_cast<_Float16>(a - static_cast<float>(ah));
-      o[D + i + D / 2] = static_cast<_Float16>(b - static_cast<float>(bh));
+  for (int u = 0; u < 2; u++) {
+    const uint32_t hh = min(h0 + u, n_slots - 1);
+    const bool is_q = hh < P.n_heads;
+    const float* src = is_q ? P.q + row * P.ldq + static_cast<size_t>(hh) * D
+                            : P.k + row * P.ldkv + static_cast<size_t>(hh - P.n_heads) * D;
+    x[u] = src[i];
+    y[u] = src[i + D / 2];
+    if (!is_q) {
+      const float* v = P.v + row * P.ldkv + static_cast<size_t>(hh - P.n_heads) * D;
+      vx[u] = v[i];
+      vy[u] = v[i + D / 2];
     }
-    if (lane == 0) P.qscale[qrow] = ldexpf(P.scale * kLog2e, -e);
   }
-  // k and v into the cache row of the node
-  for (uint32_t h = wave; h < P.n_kv; h += kPrepThreads / 64) {
-    uint32_t odd = 1;
-    if (present) {
-      const float* k = P.k + row * P.ldkv + static_cast<size_t>(h) * D;
-      const float* v = P.v + row * P.ldkv + static_cast<size_t>(h) * D;
-      const size_t at = ((static_cast<size_t>(s) * P.max_ctx + ctx + t) * P.n_kv + h) * D;
-      const double x = k[i], y = k[i + D / 2];
-      const _Float16 v0 = static_cast<_Float16>(v[i]), v1 = static_cast<_Float16>(v[i + D / 2]);
+  const float inv = P.inv_freq[i];
+  const uint32_t ctx = P.ctx_len[s];
+  const whd::TreePath path = whd::tree_path(P.parents + static_cast<size_t>(s) * P.n_tree, P.n_tree, t);
+  const bool present = path.present() && seq_fits(P, ctx);
+  if (group == 0 && tid < kWholeMask) {
+    const unsigned long long w = (tid < 2 ? path.lo : path.hi) >> (32 * (tid & 1));
+    P.mask[row * kWholeMask + tid] = present ? static_cast<uint32_t>(w) : 0u;
+  }
+  const double angle = static_cast<double>(ctx + path.depth) * static_cast<double>(inv);
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const uint32_t hh = h0 + u;
+    if (hh >= n_slots) break;
+    if (hh < P.n_heads) {
+      // q: the angle in turns, whole turns dropped in 64 bits
+      const double turns = angle * 0.15915494309189535;
+      float sn, cs;
+      sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+      float a = present ? x[u] * cs - y[u] * sn : 0.f, b = present ? x[u] * sn + y[u] * cs : 0.f;
+      float mx = fmaxf(fabsf(a), fabsf(b));
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+      // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element
+      // to 2^-22 of itself or 2^-38 of the largest
+      int e = 0;
+      if (mx > 0.f && mx < INFINITY) e = min(max(13 - ilogbf(mx), -100), 100);
+      a = ldexpf(a, e);
+      b = ldexpf(b, e);
+      const size_t qrow = (static_cast<size_t>(s) * P.n_kv + hh / P.G) * P.R + t * P.G + hh % P.G;
+      _Float16* o = P.qlimb + qrow * 2 * D;
       if (lane < D / 2) {
-        P.k_cache[at + i] = stored(x * cosd[i] - y * sind[i]);
-        P.k_cache[at + i + D / 2] = stored(x * sind[i] + y * cosd[i]);
-        P.v_cache[at + i] = v0;
-        P.v_cache[at + i + D / 2] = v1;
+        const _Float16 ah = static_cast<_Float16>(a), bh = static_cast<_Float16>(b);
+        o[i] = ah;
+        o[i + D / 2] = bh;
+        o[D + i] = static_cast<_Float16>(a - static_cast<float>(ah));
+        o[D + i + D / 2] = static_cast<_Float16>(b - static_cast<float>(bh));
       }
-      const bool fine = fabsf(static_cast<float>(v0)) < INFINITY && fabsf(static_cast<float>(v1)) < INFINITY;
-      odd = __ballot(!fine) != 0;
+      if (lane == 0) P.qscale[qrow] = ldexpf(P.scale * kLog2e, -e);
+    } else if (present && lane < D / 2) {
+      // k and v into the cache row of the node
+      const size_t at = ((static_cast<size_t>(s) * P.max_ctx + ctx + t) * P.n_kv + (hh - P.n_heads)) * D;
+      double sn, cs;
+      sincos(angle, &sn, &cs);
+      P.k_cache[at + i] = stored(x[u] * cs - y[u] * sn);
+      P.k_cache[at + i + D / 2] = stored(x[u] * sn + y[u] * cs);
+      P.v_cache[at + i] = static_cast<_Float16>(vx[u]);
+      P.v_cache[at + i + D / 2] = static_cast<_Float16>(vy[u]);
     }
-    if (lane == 0) P.odd[(static_cast<size_t>(s) * P.n_kv + h) * P.n_tree + t] = odd;
   }
 }
 
@@ -263,6 +271,41 @@ __device__ __forceinline__ half8 finite_only(half8 x) {
   return __builtin_bit_cast(half8, w);
 }
 
+// The rows of a 32-row V tile in LDS that hold an infinity or NaN, as a bit
+// mask: lane l looks through half of row l / 2 (in any order of its chunks).
+template <int D>
+__device__ __forceinline__ uint32_t odd_rows(uint32_t vt, int lane) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int j = 0; j < D / 16; j++) {
+    const u32x4 w = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + lane * D + 16 * j));
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      bad |= static_cast<uint32_t>((w[i] & 0x7C00u) == 0x7C00u) | static_cast<uint32_t>((w[i] & 0x7C000000u) == 0x7C000000u);
+  }
+  unsigned long long b = __ballot(bad != 0);
+  b = (b | b >> 1) & 0x5555555555555555ull;  // rows at the even bits, drawn together
+  b = (b | b >> 1) & 0x3333333333333333ull;
+  b = (b | b >> 2) & 0x0F0F0F0F0F0F0F0Full;
+  b = (b | b >> 4) & 0x00FF00FF00FF00FFull;
+  b = (b | b >> 8) & 0x0000FFFF0000FFFFull;
+  return static_cast<uint32_t>(b | b >> 16);
+}
+
+// Two weights as f16 hi + lo: elements i and i + 1 of the fragments.  hi is
+// rounded to nearest, lo is what it leaves (one v_fma_mix each).
+__device__ __forceinline__ void split2(float a, float b, half8& hi, half8& lo, int i) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const half2v h = __builtin_convertvector((f32x2{a, b}), half2v);
+  const uint32_t hw = __builtin_bit_cast(uint32_t, h);
+  float ra, rb;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hw), "v"(a));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hw), "v"(b));
+  const half2v r = __builtin_convertvector((f32x2{ra, rb}), half2v);
+  hi[i] = h[0], hi[i + 1] = h[1];
+  lo[i] = r[0], lo[i + 1] = r[1];
+}
+
 // RW query tiles of 32 rows per workgroup; the 4 waves are RW rows x KW keys.
 template <int D, int RW>
 struct Shape {
@@ -298,20 +341,35 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
   const uint32_t lds0 = lds_addr(lds);
 
   // One stage: rows [k0, k0 + SK) of K and V; a wave copies 1 KB (1024 / (2 D)
-  // rows) at a time.  Rows past the last one repeat it: they are masked.
+  // rows) of each at a time, the workgroup kRowsAll rows.  The chunks'
+  // permutation repeats within kRowsAll rows, so a lane's offset is the same
+  // each time.  Rows past the last one repeat it: they are masked.
+  constexpr int kRowsPer = 1024 / (2 * D), kRowsAll = kRowsPer * kAttnWaves, kChunks = D / 8;
+  const int crow = wave * kRowsPer + lane / kChunks, cchunk = lane % kChunks;
+  const uint32_t ck = 16 * (cchunk ^ swz_k<D>(crow)), cv = 16 * (cchunk ^ swz_v<D>(crow));
+  const uint32_t crs = crow * static_cast<uint32_t>(RS);
   auto issue = [&](uint32_t k0, int buf) {
-    constexpr int kRowsPer = 1024 / (2 * D), kChunks = D / 8;
     const uint8_t* kb = kbase + k0 * RS;
     const uint8_t* vb = vbase + k0 * RS;
-    const uint32_t last = rows - 1 - k0;
+    uint32_t at = lds0 + buf * S::kStageBytes + wave * 1024;
+    if (k0 + SK <= rows) {
 #pragma unroll
-    for (int j = 0; j < SK / kRowsPer / kAttnWaves; j++) {
-      const int piece = wave + kAttnWaves * j;
-      const int r = piece * kRowsPer + lane / kChunks, c = lane % kChunks;
-      const uint32_t row = min(static_cast<uint32_t>(r), last) * static_cast<uint32_t>(RS);
-      const uint32_t at = lds0 + buf * S::kStageBytes + piece * 1024;
-      copy16_to_lds(kb, row + 16 * (c ^ swz_k<D>(r)), at);
-      copy16_to_lds(vb, row + 16 * (c ^ swz_v<D>(r)), at + S::kTileBytes);
+      for (int j = 0; j < SK / kRowsAll; j++) {
+        copy16_to_lds(kb, crs + ck, at);
+        copy16_to_lds(vb, crs + cv, at + S::kTileBytes);
+        kb += kRowsAll * RS;
+        vb += kRowsAll * RS;
+        at += kAttnWaves * 1024;
+      }
+    } else {
+      const uint32_t last = rows - 1 - k0;
+#pragma unroll
+      for (int j = 0; j < SK / kRowsAll; j++) {
+        const uint32_t row = min(static_cast<uint32_t>(crow + kRowsAll * j), last) * static_cast<uint32_t>(RS);
+        copy16_to_lds(kb, row + ck, at);
+        copy16_to_lds(vb, row + cv, at + S::kTileBytes);
+        at += kAttnWaves * 1024;
+      }
     }
   };
   issue(c0, 0);
@@ -328,11 +386,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     ql[j] = *reinterpret_cast<const half8*>(q + D);
   }
   const float qs = P.qscale[qrow];
-  uint32_t tm[kWholeMask];
-  {
-    const uint4 w = *reinterpret_cast<const uint4*>(P.mask + (static_cast<size_t>(seq) * P.n_tree + r / P.G) * kWholeMask);
-    tm[0] = w.x, tm[1] = w.y, tm[2] = w.z, tm[3] = w.w;
-  }
+  uint32_t tm[kWholeMask] = {};
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; d++)
@@ -340,25 +394,27 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  auto tile = [&](uint32_t base, uint32_t kt, uint32_t vt, int tr) {
-    // kt, vt: LDS addresses of the stage's K and V; tr: the tile's first row there
+  // One 32-key tile.  kt, vt: LDS addresses of its first K and V row.  Edge: the
+  // tile may reach beyond the cache into the nodes' rows or past the last one.
+  auto tile = [&](uint32_t base, uint32_t kt, uint32_t vt, auto edge) {
+    constexpr bool kEdge = decltype(edge)::value;
     f32x16 s;
 #pragma unroll
     for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < KS; j++) {
-      const int rr = tr + l32;
       const half8 kf = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-          (uintptr_t)(kt + rr * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(rr))));
+          (uintptr_t)(kt + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[j], s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j], s, 0, 0, 0);
     }
-    uint32_t bits = 0xFFFFFFFFu, odd = 0;
-    const bool tail = base + 32 > ctx;
-    if (tail) {
+    [[maybe_unused]] uint32_t bits = 0xFFFFFFFFu, odd = 0;
+    if constexpr (kEdge) {
       // keys from ctx on are the tree's nodes: bit k of `bits` for key base + k
-      const int off = static_cast<int>(base - ctx);  // > -32
-      if (off < 0) {
+      const int off = static_cast<int>(base) - static_cast<int>(ctx);
+      if (off <= -32) {
+        bits = 0xFFFFFFFFu;
+      } else if (off < 0) {
         bits = (tm[0] << -off) | ((1u << -off) - 1u);
       } else {
         const int w = off >> 5, sh = off & 31;
@@ -370,10 +426,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         }
         bits = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
       }
-      const int node = off + l32;
-      const bool is_odd = h == 0 && node >= 0 && node < static_cast<int>(P.n_tree) &&
-                          P.odd[(static_cast<size_t>(seq) * P.n_kv + kvh) * P.n_tree + node] != 0;
-      odd = static_cast<uint32_t>(__ballot(is_odd));
+      odd = odd_rows<D>(vt, lane);
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int key = 8 * (i >> 2) + 4 * h + (i & 3);
@@ -402,71 +455,87 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       lt[i & 3] += p[i];
     }
     l += (lt[0] + lt[1]) + (lt[2] + lt[3]);  // one addition to the running sum per tile
-    half8 ph[2], pl[2];
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const _Float16 hi = static_cast<_Float16>(p[8 * ks + i]);
-        ph[ks][i] = hi;
-        pl[ks][i] = static_cast<_Float16>(p[8 * ks + i] - static_cast<float>(hi));
-      }
     const int i16 = lane & 15, kq = i16 >> 2, dq = i16 & 3, dg = (lane >> 4) & 1;
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++)
+    for (int ks = 0; ks < 2; ks++) {
+      half8 ph, pl;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) split2(p[8 * ks + i], p[8 * ks + i + 1], ph, pl, i);
 #pragma unroll
       for (int d = 0; d < DT; d++) {
         half8 vf;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const int rr = tr + 16 * ks + 8 * u + 4 * h + kq;
+          const int rr = 16 * ks + 8 * u + 4 * h + kq;
           const int c = 4 * d + 2 * dg + (dq >> 1);
           const s16x4 x = read_tr(vt + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
           const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
 #pragma unroll
           for (int i = 0; i < 4; i++) vf[4 * u + i] = y[i];
         }
-        if (odd) vf = finite_only(vf);
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[ks], acc[d], 0, 0, 0);
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[ks], acc[d], 0, 0, 0);
+        if constexpr (kEdge) vf = finite_only(vf);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, acc[d], 0, 0, 0);
       }
-    // nodes whose v holds an infinity or NaN: those elements count for the
-    // rows that see the node, and for no other (0 * inf would spread a NaN)
-    while (odd) {
-      const int key = __builtin_ctz(odd);
-      odd &= odd - 1;
-      float pk = 0.f;
+    }
+    if constexpr (kEdge) {
+      // rows of V with infinities or NaN: those elements are 0 in the products
+      // above and are added here to the query rows that see them, and to no
+      // other (0 * inf would spread a NaN)
+      while (odd) {
+        const int key = __builtin_ctz(odd);
+        odd &= odd - 1;
+        if (!__ballot((bits >> key) & 1u)) continue;
+        float pk = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; i++)
-        if (8 * (i >> 2) + (i & 3) == (key & ~4)) pk = p[i];
-      pk = __shfl(pk, l32 + 32 * ((key >> 2) & 1), 64);
-      if (!((bits >> key) & 1u)) continue;
-      const int rr = tr + key;
+        for (int i = 0; i < 16; i++)
+          if (8 * (i >> 2) + (i & 3) == (key & ~4)) pk = p[i];
+        pk = __shfl(pk, l32 + 32 * ((key >> 2) & 1), 64);
+        if (!((bits >> key) & 1u)) continue;
 #pragma unroll
-      for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
-          const float x = static_cast<float>(*reinterpret_cast<const __attribute__((address_space(3))) _Float16*>(
-              (uintptr_t)(vt + rr * 2 * D + 16 * ((dim >> 3) ^ swz_v<D>(rr)) + 2 * (dim & 7))));
-          if (!(fabsf(x) < INFINITY)) acc[d][i] += pk * x;
-        }
+          for (int i = 0; i < 16; i++) {
+            const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
+            const float x = static_cast<float>(*reinterpret_cast<const __attribute__((address_space(3))) _Float16*>(
+                (uintptr_t)(vt + key * 2 * D + 16 * ((dim >> 3) ^ swz_v<D>(key)) + 2 * (dim & 7))));
+            if (!(fabsf(x) < INFINITY)) acc[d][i] += pk * x;
+          }
+      }
     }
   };
 
+  // stages of cache rows only, then those that reach the nodes' rows or the chunk's end
   const uint32_t n_stages = (c1 - c0 + SK - 1) / SK;
-  for (uint32_t st = 0; st < n_stages; st++) {
+  const uint32_t inner = min(c1, ctx), n_inner = inner > c0 ? (inner - c0) / SK : 0;
+  auto turn = [&](uint32_t st) {
     wait_vmcnt<0>();  // this wave's copies of stage st
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // everyone's; and everyone has read stage st - 1
     asm volatile("" ::: "memory");
     if (st + 1 < n_stages) issue(c0 + (st + 1) * SK, (st + 1) & 1);
-    const uint32_t kt = lds0 + (st & 1) * S::kStageBytes, vt = kt + S::kTileBytes;
+    return lds0 + (st & 1) * S::kStageBytes;
+  };
+  uint32_t st = 0;
+  for (; st < n_inner; st++) {
+    const uint32_t kt = turn(st);
+#pragma unroll
+    for (int u = 0; u < S::TILES; u++) {
+      const uint32_t to = 32 * (kw + KW * u) * 2 * D;
+      tile(0, kt + to, kt + S::kTileBytes + to, std::false_type{});
+    }
+  }
+  if (st < n_stages) {
+    const uint4 w = *reinterpret_cast<const uint4*>(P.mask + (static_cast<size_t>(seq) * P.n_tree + r / P.G) * kWholeMask);
+    tm[0] = w.x, tm[1] = w.y, tm[2] = w.z, tm[3] = w.w;
+  }
+#pragma unroll 1
+  for (; st < n_stages; st++) {
+    const uint32_t kt = turn(st);
 #pragma unroll 1
     for (int u = 0; u < S::TILES; u++) {
-      const int tr = 32 * (kw + KW * u);
-      const uint32_t base = c0 + st * SK + tr;
-      if (base < c1) tile(base, kt, vt, tr);
+      const uint32_t base = c0 + st * SK + 32 * (kw + KW * u), to = 32 * (kw + KW * u) * 2 * D;
+      if (base < c1) tile(base, kt + to, kt + S::kTileBytes + to, std::true_type{});
     }
   }
   l = swap_sum(l);
@@ -527,23 +596,26 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 }
 
 // ------------------------------------------------------------------ combine
-// One wave per (node, head): out = sum_c acc_c 2^{m_c - M} / sum_c l_c 2^{m_c - M}.
-// Rows of absent nodes are zeros; those of a sequence whose rows do not fit its
-// cache are NaN.
+// One workgroup per (node, head): out = sum_c acc_c 2^{m_c - M} / sum_c l_c 2^{m_c - M}.
+// Every wave forms the weights of 64 chunks at a time, one per lane, and adds a
+// quarter of their accumulators, 8 loads in flight; the waves' sums add in fixed
+// order.  Rows of absent nodes are zeros; those of a sequence whose rows do not
+// fit its cache are NaN.
 template <int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
-  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (id >= P.n_seqs * P.n_tree * P.n_heads) return;
-  const uint32_t head = id % P.n_heads, row = id / P.n_heads, seq = row / P.n_tree, t = row % P.n_tree;
   constexpr int V = D / 64;  // dims per lane
-  float* o = P.out + static_cast<size_t>(row) * P.n_heads * D + static_cast<size_t>(head) * D + V * lane;
+  constexpr int kPer = 8;
+  __shared__ float part[4][D];
+  const uint32_t head = blockIdx.x % P.n_heads, row = blockIdx.x / P.n_heads, seq = row / P.n_tree, t = row % P.n_tree;
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float* o = P.out + static_cast<size_t>(row) * P.n_heads * D + static_cast<size_t>(head) * D;
   const uint4 w = *reinterpret_cast<const uint4*>(P.mask + static_cast<size_t>(row) * kWholeMask);
+  const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
   if ((w.x | w.y | w.z | w.w) == 0) {
-    const float fill = seq_fits(P, P.ctx_len[seq]) ? 0.f : __builtin_nanf("");
-    for (int i = 0; i < V; i++) o[i] = fill;
+    if (threadIdx.x < D) o[threadIdx.x] = seq_fits(P, P.ctx_len[seq]) ? 0.f : __builtin_nanf("");
     return;
   }
-  const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
   const size_t step = static_cast<size_t>(P.n_kv) * P.R;
   const size_t at = (static_cast<size_t>(c0) * P.n_kv + head / P.G) * P.R + t * P.G + head % P.G;
   float M = -INFINITY;
@@ -551,17 +623,36 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
   float L = 0.f, A[V] = {};
-#pragma unroll 4
-  for (uint32_t c = 0; c < n; c++) {
-    const float2 ml = P.ml[at + c * step];
-    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+  for (uint32_t b = 0; b < n; b += 64) {
+    const float2 ml = b + lane < n ? P.ml[at + (b + lane) * step] : make_float2(-INFINITY, 0.f);
+    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);  // 0 past the last chunk
     L = __builtin_fmaf(ml.y, ew, L);
-    const float* a = P.acc + (at + c * step) * D + V * lane;
+    const uint32_t end = min(n - b, 64u);
+    for (uint32_t c = wave; c < end; c += 4 * kPer) {
+      float a[kPer][V];
 #pragma unroll
-    for (int i = 0; i < V; i++) A[i] = __builtin_fmaf(a[i], ew, A[i]);
+      for (int j = 0; j < kPer; j++) {
+        const float* src = P.acc + (at + (b + min(c + 4 * j, end - 1)) * step) * D + V * lane;
+#pragma unroll
+        for (int i = 0; i < V; i++) a[j][i] = src[i];
+      }
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        const uint32_t cj = c + 4 * j;
+        const float wj = cj < end ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ew), cj & 63)) : 0.f;
+        if (cj < end) {
+#pragma unroll
+          for (int i = 0; i < V; i++) A[i] = __builtin_fmaf(a[j][i], wj, A[i]);
+        }
+      }
+    }
   }
 #pragma unroll
-  for (int i = 0; i < V; i++) o[i] = A[i] / L;
+  for (int i = 0; i < V; i++) part[wave][V * lane + i] = A[i];
+  L = whd::wave_sum(L);
+  __syncthreads();
+  const uint32_t d = threadIdx.x;
+  if (d < D) o[d] = ((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) / L;
 }
 
 // ------------------------------------------------------------------ launching
@@ -604,7 +695,6 @@ size_t layout(Params& P, size_t D, void* base) {
   P.first = reinterpret_cast<uint32_t*>(take(4 * (static_cast<size_t>(P.n_seqs) + 1)));
   P.total = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(P.n_seqs)));
   P.mask = reinterpret_cast<uint32_t*>(take(4 * kWholeMask * static_cast<size_t>(P.n_seqs) * P.n_tree));
-  P.odd = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(P.n_seqs) * P.n_kv * P.n_tree));
   P.qscale = reinterpret_cast<float*>(take(4 * P.n_seqs * rows));
   P.qlimb = reinterpret_cast<_Float16*>(take(2 * 2 * D * P.n_seqs * rows));
   P.ml = reinterpret_cast<float2*>(take(8 * slots * rows));
@@ -638,12 +728,12 @@ int launch_partial(const Params& P, hipStream_t s) {
 
 template <int D>
 int launch_all(const Params& P, int rw, hipStream_t s) {
-  tree_prepare_kernel<D><<<P.n_seqs * P.n_tree + 1, kPrepThreads, 0, s>>>(P);
+  const uint32_t n_groups = (P.n_heads + P.n_kv + kPrepHeads - 1) / kPrepHeads;
+  tree_prepare_kernel<D><<<P.n_seqs * P.n_tree * n_groups + 1, kPrepThreads, 0, s>>>(P, n_groups);
   WH_LAUNCH_CHECK("tree attention prepare launch");
   int st = rw == 1 ? launch_partial<D, 1>(P, s) : rw == 2 ? launch_partial<D, 2>(P, s) : launch_partial<D, 4>(P, s);
   if (st) return st;
-  const size_t out_rows = static_cast<size_t>(P.n_seqs) * P.n_tree * P.n_heads;
-  tree_combine_kernel<D><<<static_cast<unsigned>((out_rows + 3) / 4), 256, 0, s>>>(P);
+  tree_combine_kernel<D><<<P.n_seqs * P.n_tree * P.n_heads, 256, 0, s>>>(P);
   WH_LAUNCH_CHECK("tree attention combine launch");
   return WH_OK;
 }
