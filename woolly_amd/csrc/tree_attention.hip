@@ -54,13 +54,11 @@ struct Params {
   _Float16 *k_cache, *v_cache;
   const float* inv_freq;
   float* out;
-  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target;
+  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, unit;
   float scale;
   // workspace
-  uint32_t* head;       // [0]: chunk length
-  uint2* slots;         // [max_slots] (sequence, chunk of it); sequence n_seqs: none
+  uint4* slots;         // [max_slots] (sequence, first key, key behind the last, cache rows of the step); sequence n_seqs: none
   uint32_t* first;      // [n_seqs + 1] first slot
-  uint32_t* total;      // [n_seqs] cache rows of the step, 0: nothing to do
   uint32_t* mask;       // [n_seqs][n_tree][4]
   float* qscale;        // [n_seqs][n_kv][R]
   _Float16* qlimb;      // [n_seqs][n_kv][R][2][D]
@@ -96,10 +94,14 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
   return v;
 }
 
-// Cuts the sequences into chunks: the chunk length is the one (a multiple of
-// 64) that gives about `target` chunks over all sequences, so long and short
-// sequences share the workgroups evenly whatever the lengths on the device.
+// Cuts the sequences into chunks of one length, a multiple of a stage of the
+// partial kernel, so long and short sequences share the workgroups evenly
+// whatever the lengths on the device.  About `target` chunks over all sequences
+// give every CU two workgroups, whose matrix and vector work overlap; while the
+// chunks would be shorter than kDeepChunk, `sparse` chunks, one workgroup per CU,
+// do: half the partial results to write and to join.
 // Thread t plans sequences [t per, (t + 1) per); first: LDS [n_seqs + 1].
+constexpr uint32_t kDeepChunk = 512;
 __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long* red) {
   const uint32_t t = threadIdx.x;
   const uint32_t per = (P.n_seqs + kPrepThreads - 1) / kPrepThreads;
@@ -115,15 +117,15 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long
   for (uint32_t s = s0; s < s1; s++) {
     const uint32_t n = rows(s);
     first[s] = n;
-    P.total[s] = n;
     mine += n;
   }
   mine = block_scan(mine, red);
   __shared__ unsigned long long total;
   if (t == kPrepThreads - 1) total = mine;
   __syncthreads();
-  const unsigned long long even = (total + P.target - 1) / P.target;
-  const uint32_t chunk = static_cast<uint32_t>(max((even + 63) / 64 * 64, 64ull));
+  unsigned long long even = (total + P.target - 1) / P.target;
+  if (even < kDeepChunk) even = min<unsigned long long>((total + P.sparse - 1) / P.sparse, kDeepChunk);
+  const uint32_t chunk = max(static_cast<uint32_t>((even + P.unit - 1) / P.unit), 1u) * P.unit;
   uint32_t n = 0;
   for (uint32_t s = s0; s < s1; s++) n += (first[s] + chunk - 1) / chunk;
   uint32_t at = static_cast<uint32_t>(block_scan(n, red)) - n;
@@ -136,7 +138,6 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long
   if (t == kPrepThreads - 1) {
     first[P.n_seqs] = at;
     P.first[P.n_seqs] = at;
-    P.head[0] = chunk;
   }
   __syncthreads();
   const uint32_t used = first[P.n_seqs];
@@ -146,7 +147,12 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long
       const uint32_t mid = (lo + hi) / 2;
       if (first[mid] <= y) lo = mid; else hi = mid;
     }
-    P.slots[y] = y < used ? make_uint2(lo, y - first[lo]) : make_uint2(P.n_seqs, 0);
+    uint4 slot = make_uint4(P.n_seqs, 0, 0, 0);
+    if (y < used) {
+      const uint32_t n = P.ctx_len[lo] + P.n_tree, c0 = (y - first[lo]) * chunk;
+      slot = make_uint4(lo, c0, min(c0 + chunk, n), n);
+    }
+    P.slots[y] = slot;
   }
 }
 
@@ -271,25 +277,26 @@ __device__ __forceinline__ half8 finite_only(half8 x) {
   return __builtin_bit_cast(half8, w);
 }
 
-// The rows of a 32-row V tile in LDS that hold an infinity or NaN, as a bit
-// mask: lane l looks through half of row l / 2 (in any order of its chunks).
+// Replaces the infinities and NaN of a 32-row V tile in LDS by 0 and tells
+// whether there were any: lane l looks through half of row l / 2 (the order of
+// its chunks does not matter).  Waves that share a tile may do so at the same
+// time: they store the same values, each before it reads the tile itself.
 template <int D>
-__device__ __forceinline__ uint32_t odd_rows(uint32_t vt, int lane) {
-  uint32_t bad = 0;
+__device__ __forceinline__ bool clean_tile(uint32_t vt, int lane) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  auto at = [&](int j) { return reinterpret_cast<__attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + lane * D + 16 * j)); };
+  u16x2 top = {0, 0};  // the largest exponent of the even and of the odd elements
 #pragma unroll
   for (int j = 0; j < D / 16; j++) {
-    const u32x4 w = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + lane * D + 16 * j));
+    const u32x4 w = *at(j);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      bad |= static_cast<uint32_t>((w[i] & 0x7C00u) == 0x7C00u) | static_cast<uint32_t>((w[i] & 0x7C000000u) == 0x7C000000u);
+    for (int i = 0; i < 4; i++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7C007C00u));
   }
-  unsigned long long b = __ballot(bad != 0);
-  b = (b | b >> 1) & 0x5555555555555555ull;  // rows at the even bits, drawn together
-  b = (b | b >> 1) & 0x3333333333333333ull;
-  b = (b | b >> 2) & 0x0F0F0F0F0F0F0F0Full;
-  b = (b | b >> 4) & 0x00FF00FF00FF00FFull;
-  b = (b | b >> 8) & 0x0000FFFF0000FFFFull;
-  return static_cast<uint32_t>(b | b >> 16);
+  const bool bad = top[0] == 0x7C00 || top[1] == 0x7C00;
+  if (!__ballot(bad)) return false;
+#pragma unroll 1
+  for (int j = 0; j < D / 16; j++) *at(j) = __builtin_bit_cast(u32x4, finite_only(__builtin_bit_cast(half8, *at(j))));
+  return true;
 }
 
 // Two weights as f16 hi + lo: elements i and i + 1 of the fragments.  hi is
@@ -326,11 +333,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
   constexpr int KW = S::KW, SK = S::SK, DT = D / 32, KS = D / 16;
   extern __shared__ __align__(256) unsigned char lds[];
   const uint32_t kvh = blockIdx.x % P.n_kv, rg = blockIdx.x / P.n_kv % P.n_rg, slot = blockIdx.x / (P.n_kv * P.n_rg);
-  const uint2 sc = P.slots[slot];
+  const uint4 sc = P.slots[slot];
   if (sc.x >= P.n_seqs) return;
-  const uint32_t seq = sc.x, chunk = P.head[0], rows = P.total[seq];
+  const uint32_t seq = sc.x, c0 = sc.y, c1 = sc.z, rows = sc.w;  // c0 < c1 <= rows
   const uint32_t ctx = rows - P.n_tree;
-  const uint32_t c0 = sc.y * chunk, c1 = min(c0 + chunk, rows);  // c0 < rows
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave / KW, kw = wave % KW;
@@ -393,6 +399,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
   float m = -INFINITY, l = 0.f;
+  bool odd = false;  // an edge tile of this wave held infinities or NaN in V
 
   // One 32-key tile.  kt, vt: LDS addresses of its first K and V row.  Edge: the
   // tile may reach beyond the cache into the nodes' rows or past the last one.
@@ -408,8 +415,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[j], s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j], s, 0, 0, 0);
     }
-    [[maybe_unused]] uint32_t bits = 0xFFFFFFFFu, odd = 0;
     if constexpr (kEdge) {
+      uint32_t bits;
       // keys from ctx on are the tree's nodes: bit k of `bits` for key base + k
       const int off = static_cast<int>(base) - static_cast<int>(ctx);
       if (off <= -32) {
@@ -426,7 +433,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         }
         bits = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
       }
-      odd = odd_rows<D>(vt, lane);
+      odd |= clean_tile<D>(vt, lane);
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int key = 8 * (i >> 2) + 4 * h + (i & 3);
@@ -473,34 +480,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 #pragma unroll
           for (int i = 0; i < 4; i++) vf[4 * u + i] = y[i];
         }
-        if constexpr (kEdge) vf = finite_only(vf);
         acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, acc[d], 0, 0, 0);
         acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, acc[d], 0, 0, 0);
-      }
-    }
-    if constexpr (kEdge) {
-      // rows of V with infinities or NaN: those elements are 0 in the products
-      // above and are added here to the query rows that see them, and to no
-      // other (0 * inf would spread a NaN)
-      while (odd) {
-        const int key = __builtin_ctz(odd);
-        odd &= odd - 1;
-        if (!__ballot((bits >> key) & 1u)) continue;
-        float pk = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (8 * (i >> 2) + (i & 3) == (key & ~4)) pk = p[i];
-        pk = __shfl(pk, l32 + 32 * ((key >> 2) & 1), 64);
-        if (!((bits >> key) & 1u)) continue;
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
-            const float x = static_cast<float>(*reinterpret_cast<const __attribute__((address_space(3))) _Float16*>(
-                (uintptr_t)(vt + key * 2 * D + 16 * ((dim >> 3) ^ swz_v<D>(key)) + 2 * (dim & 7))));
-            if (!(fabsf(x) < INFINITY)) acc[d][i] += pk * x;
-          }
       }
     }
   };
@@ -539,6 +520,28 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
   }
   l = swap_sum(l);
+  if (odd) {
+    // infinities and NaN of V count for the query rows that see them, and for no
+    // other (0 * inf in the products would have spread a NaN): every weight is
+    // above 0, so an element becomes what their sum is.  The rows are read again.
+    for (uint32_t key = c0 + n_inner * SK; key < c1; key++) {
+      if ((key - c0) / 32 % KW != static_cast<uint32_t>(kw)) continue;
+      const uint32_t node = key - ctx;  // wraps for the cache's rows
+      uint32_t w = tm[0];
+#pragma unroll
+      for (int i = 1; i < kWholeMask; i++)
+        if (node >> 5 == static_cast<uint32_t>(i)) w = tm[i];
+      if (key >= ctx && !((w >> (node & 31)) & 1u)) continue;
+      const _Float16* v = reinterpret_cast<const _Float16*>(vbase + key * RS);
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float x = static_cast<float>(v[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
+          if (!(fabsf(x) < INFINITY)) acc[d][i] += x;
+        }
+    }
+  }
 
   const size_t prow = (static_cast<size_t>(slot) * P.n_kv + kvh) * P.R;
   if constexpr (KW == 1) {
@@ -568,29 +571,34 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       mm[2 * (wave * 32 + l32) + 1] = l;
     }
     __syncthreads();
-    for (int e = tid; e < RW * 32 * (D / 4); e += 64 * kAttnWaves) {
-      const int rr = e / (D / 4), d4 = e % (D / 4);
+#pragma unroll
+    for (int it = 0; it < RW * 32 * (D / 4) / (64 * kAttnWaves); it++) {
+      const int e = tid + it * 64 * kAttnWaves, rr = e / (D / 4), d4 = e % (D / 4);
       const uint32_t rglob = rg * RW * 32 + rr;
-      if (rglob >= P.R) continue;
       const int w0 = (rr / 32) * KW, lr = rr % 32;
       float M = -INFINITY;
+      float2 ml[KW];
 #pragma unroll
-      for (int w = 0; w < KW; w++) M = fmaxf(M, mm[2 * ((w0 + w) * 32 + lr)]);
+      for (int w = 0; w < KW; w++) {
+        ml[w] = *reinterpret_cast<const float2*>(mm + 2 * ((w0 + w) * 32 + lr));
+        M = fmaxf(M, ml[w].x);
+      }
       float L = 0.f;
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < KW; w++) {
-        const float mw = mm[2 * ((w0 + w) * 32 + lr)];
-        const float ew = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-        L = __builtin_fmaf(mm[2 * ((w0 + w) * 32 + lr) + 1], ew, L);
+        const float ew = ml[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w].x - M);
+        L = __builtin_fmaf(ml[w].y, ew, L);
         const float4 a = *reinterpret_cast<const float4*>(am + ((w0 + w) * 32 + lr) * D + 4 * d4);
         A.x = __builtin_fmaf(a.x, ew, A.x);
         A.y = __builtin_fmaf(a.y, ew, A.y);
         A.z = __builtin_fmaf(a.z, ew, A.z);
         A.w = __builtin_fmaf(a.w, ew, A.w);
       }
-      *reinterpret_cast<float4*>(P.acc + (prow + rglob) * D + 4 * d4) = A;
-      if (d4 == 0) P.ml[prow + rglob] = make_float2(M, L);
+      if (rglob < P.R) {
+        *reinterpret_cast<float4*>(P.acc + (prow + rglob) * D + 4 * d4) = A;
+        if (d4 == 0) P.ml[prow + rglob] = make_float2(M, L);
+      }
     }
   }
 }
@@ -606,7 +614,10 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
   constexpr int V = D / 64;  // dims per lane
   constexpr int kPer = 8;
   __shared__ float part[4][D];
-  const uint32_t head = blockIdx.x % P.n_heads, row = blockIdx.x / P.n_heads, seq = row / P.n_tree, t = row % P.n_tree;
+  // KV head fastest, as the partial kernel's workgroups: with 8 KV heads a head's
+  // chunks are joined on the XCD whose L2 they were written through
+  const uint32_t kvh = blockIdx.x % P.n_kv, g = blockIdx.x / P.n_kv % P.G, row = blockIdx.x / P.n_heads;
+  const uint32_t seq = row / P.n_tree, t = row % P.n_tree, head = kvh * P.G + g;
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float* o = P.out + static_cast<size_t>(row) * P.n_heads * D + static_cast<size_t>(head) * D;
@@ -617,7 +628,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
     return;
   }
   const size_t step = static_cast<size_t>(P.n_kv) * P.R;
-  const size_t at = (static_cast<size_t>(c0) * P.n_kv + head / P.G) * P.R + t * P.G + head % P.G;
+  const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.R + t * P.G + g;
   float M = -INFINITY;
   for (uint32_t c = lane; c < n; c += 64) M = fmaxf(M, P.ml[at + c * step].x);
 #pragma unroll
@@ -664,7 +675,7 @@ int row_tiles(size_t R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
 
 struct Plan {
   int rw;
-  size_t G, R, n_rg, target, max_slots;
+  size_t G, R, n_rg, target, sparse, unit, max_slots;
 };
 Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t max_ctx) {
   Plan p;
@@ -672,10 +683,12 @@ Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t
   p.R = n_tree * p.G;
   p.rw = row_tiles(p.R);
   p.n_rg = (p.R + 32 * p.rw - 1) / (32 * p.rw);
+  p.unit = p.rw == 1 ? 128 : 64;
   // one workgroup per CU with 128 KB of stages, two with 64 KB
-  const size_t want = static_cast<size_t>(wh::cu_count()) * (p.rw == 1 ? 1 : 2);
-  p.target = (want + n_kv * p.n_rg - 1) / (n_kv * p.n_rg);
-  const size_t most = n_seqs * ((max_ctx + 63) / 64);
+  const size_t per = n_kv * p.n_rg, cus = static_cast<size_t>(wh::cu_count());
+  p.sparse = (cus + per - 1) / per;
+  p.target = ((p.rw == 1 ? 1 : 2) * cus + per - 1) / per;
+  const size_t most = n_seqs * ((max_ctx + p.unit - 1) / p.unit);
   p.max_slots = p.target + n_seqs < most ? p.target + n_seqs : most;
   return p;
 }
@@ -690,10 +703,8 @@ size_t layout(Params& P, size_t D, void* base) {
     return r;
   };
   const size_t slots = P.max_slots, rows = static_cast<size_t>(P.n_kv) * P.R;
-  P.head = reinterpret_cast<uint32_t*>(take(4));
-  P.slots = reinterpret_cast<uint2*>(take(8 * slots));
+  P.slots = reinterpret_cast<uint4*>(take(16 * slots));
   P.first = reinterpret_cast<uint32_t*>(take(4 * (static_cast<size_t>(P.n_seqs) + 1)));
-  P.total = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(P.n_seqs)));
   P.mask = reinterpret_cast<uint32_t*>(take(4 * kWholeMask * static_cast<size_t>(P.n_seqs) * P.n_tree));
   P.qscale = reinterpret_cast<float*>(take(4 * P.n_seqs * rows));
   P.qlimb = reinterpret_cast<_Float16*>(take(2 * 2 * D * P.n_seqs * rows));
@@ -714,6 +725,8 @@ Params fill(const Plan& p, size_t n_seqs, size_t n_tree, size_t n_heads, size_t 
   P.n_rg = static_cast<uint32_t>(p.n_rg);
   P.max_slots = static_cast<uint32_t>(p.max_slots);
   P.target = static_cast<uint32_t>(p.target);
+  P.sparse = static_cast<uint32_t>(p.sparse);
+  P.unit = static_cast<uint32_t>(p.unit);
   P.scale = 1.0f / sqrtf(static_cast<float>(D));
   return P;
 }
