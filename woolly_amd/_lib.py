@@ -268,6 +268,8 @@ _lib: C.CDLL | None = None
 def load() -> C.CDLL:
     """Loads libwoolly_hip.so (raises if it has not been built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

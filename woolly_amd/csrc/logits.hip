@@ -12,24 +12,27 @@
 // Every operation is rounded by itself, in this order (no fused multiply-add),
 // so the values do not depend on how the row is cut up.
 //
-// One pass over the logits: a workgroup takes kChunk tokens of a row, counts
-// the history's tokens that fall into them in LDS, applies everything and
-// reduces its highest token; a second small launch joins the chunks of a row.
-// Counting and the choice of a bias entry use integer LDS atomics (add, max):
-// their order does not change the result.
+// One pass over the logits: a workgroup takes kChunk tokens of some rows of one
+// sequence, counts the history's tokens that fall into them in LDS once, and per
+// row adds the path's tokens, applies everything and reduces the highest token;
+// a second small launch joins the chunks of a row.  Counting and the choice of a
+// bias entry use integer LDS atomics (add, max): their order does not change the
+// result.  The rows are bound by memory; long histories, which every chunk reads,
+// by L2: large chunks read them less often.
 #include "tree.hpp"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kChunk = 2048;  // tokens of a row per workgroup
+constexpr int kThreads = 1024;
+constexpr int kChunk = 8192;  // tokens of a row per workgroup
+constexpr int kPer = kChunk / kThreads;
 constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 
 struct Params {
   const float* logits;
   float* out;
   size_t ld, ldo;
-  uint32_t vocab, rows_per_seq, n_chunks;
+  uint32_t vocab, rows_per_seq, rows_per_wg, n_chunks;
   const uint32_t* history;
   size_t history_stride;
   const uint32_t* history_len;
@@ -42,113 +45,231 @@ struct Params {
   size_t bias_stride;
   const uint32_t* mask;
   size_t mask_stride;
-  unsigned long long* best;  // [n_rows][n_chunks], null: no token wanted
+  float2* best;         // [n_rows][n_chunks] (logit, token's bits), null: no token wanted
   uint32_t* token;
 };
 
-// Orders floats as unsigned integers (-0 as +0); NaN and -inf give 0: no candidate.
-__device__ __forceinline__ uint32_t order_key(float v) {
-  if (!(v > -INFINITY)) return 0u;
-  const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+// The highest token of some, as (logit, token): logit -inf and no token where
+// there is none.
+struct Best {
+  float top;
+  uint32_t at;
+};
+__device__ __forceinline__ Best wave_best(Best b) {
+  const float m = whd::wave_max(b.top);
+  return Best{m, whd::wave_min(b.top == m && m > -INFINITY ? b.at : kNoToken)};
 }
 
-__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const unsigned long long o = __shfl_xor(v, off, 64);
-    v = o > v ? o : v;
-  }
-  return v;
-}
-
-// grid: (n_chunks, n_rows)
-__global__ __launch_bounds__(kThreads) void logits_kernel(const Params P) {
+// grid: (n_chunks, sequences * groups of rows_per_wg rows).  Thread t holds
+// tokens 4 t .. 4 t + 3 and those 4096 behind them (VEC: rows 16-byte aligned), or
+// tokens t, t + 1024, ...; `at` is the place of its j-th token in the chunk.
+template <bool VEC>
+__global__ __launch_bounds__(kThreads, 8) void logits_kernel(const Params P) {
 #pragma clang fp contract(off)
-  __shared__ uint32_t count[kChunk];
-  __shared__ int entry[kChunk];
-  __shared__ unsigned long long red[kThreads / 64];
-  const uint32_t row = blockIdx.y, seq = row / P.rows_per_seq, node = row % P.rows_per_seq;
+  extern __shared__ __align__(16) uint32_t lds[];
+  uint32_t* count = lds;                                   // [kChunk]
+  int* entry = reinterpret_cast<int*>(lds + kChunk);       // [kChunk], with biases only
+  __shared__ Best red[kThreads / 64];
+  const uint32_t groups = (P.rows_per_seq + P.rows_per_wg - 1) / P.rows_per_wg;
+  const uint32_t seq = blockIdx.y / groups, node0 = blockIdx.y % groups * P.rows_per_wg;
+  const uint32_t nodes = min(P.rows_per_wg, P.rows_per_seq - node0);
   const uint32_t i0 = blockIdx.x * kChunk, n = min(P.vocab - i0, static_cast<uint32_t>(kChunk));
   const uint32_t t = threadIdx.x;
-  const bool said = P.history || P.tree_tokens;
-  for (int i = t; i < kChunk; i += kThreads) {
-    count[i] = 0;
-    entry[i] = -1;
-  }
-  __syncthreads();
-  bool present = true;
-  if (P.tree_parents) {
-    const whd::TreePath path =
-        whd::tree_path(P.tree_parents + static_cast<size_t>(seq) * P.rows_per_seq, P.rows_per_seq, node);
-    present = path.present();
-    if (t < P.rows_per_seq && path.has(t)) {
-      const uint32_t c = P.tree_tokens[static_cast<size_t>(seq) * P.rows_per_seq + t] - i0;
-      if (c < n) atomicAdd(&count[c], 1u);
+  auto at = [&](int j) -> uint32_t { return VEC ? 4 * t + (j & 3) + 4096 * (j >> 2) : t + kThreads * j; };
+  float next[kPer];
+  uint32_t next_open[kPer / 4];  // bit k: token at(4 q + k) exists and is allowed
+  auto load = [&](size_t row) {
+    const uint32_t* m = P.mask ? P.mask + row * P.mask_stride + i0 / 32 : nullptr;
+#pragma unroll
+    for (int q = 0; q < kPer / 4; q++) {
+      if constexpr (VEC) {
+        const uint32_t a = at(4 * q), left = a < n ? n - a : 0u;
+        next_open[q] = (m && left ? m[a >> 5] >> (a & 31) : 15u) & (left < 4 ? (1u << left) - 1u : 15u);
+      } else {
+        next_open[q] = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t a = at(4 * q + k);
+          if (a < n) next_open[q] |= (m ? m[a >> 5] >> (a & 31) & 1u : 1u) << k;
+        }
+      }
     }
+    const float* p = P.logits + row * P.ld + i0;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < kPer; j += 4) {
+        const uint32_t a = at(j);
+        if (a + 4 <= n) {
+          const float4 v = *reinterpret_cast<const float4*>(p + a);
+          next[j] = v.x, next[j + 1] = v.y, next[j + 2] = v.z, next[j + 3] = v.w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++) next[j + k] = a + k < n ? p[a + k] : 0.f;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; j++) next[j] = at(j) < n ? p[at(j)] : 0.f;
+    }
+  };
+  const size_t row0 = static_cast<size_t>(seq) * P.rows_per_seq + node0;
+  load(row0);
+  whd::TreeLanes tree{};
+  uint32_t node_token = 0;
+  if (P.tree_parents) {
+    tree = whd::tree_lanes(P.tree_parents + static_cast<size_t>(seq) * P.rows_per_seq, P.rows_per_seq);
+    if (t < P.rows_per_seq) node_token = P.tree_tokens[static_cast<size_t>(seq) * P.rows_per_seq + t];
   }
-  if (!present) {
-    if (t == 0 && P.best) P.best[static_cast<size_t>(row) * P.n_chunks + blockIdx.x] = 0;
-    return;
+  const bool said = P.history || P.tree_tokens;
+#pragma unroll
+  for (int j = 0; j < kChunk / 4 / kThreads; j++) {
+    reinterpret_cast<uint4*>(count)[t + kThreads * j] = make_uint4(0, 0, 0, 0);
+    if (P.n_bias) reinterpret_cast<int4*>(entry)[t + kThreads * j] = make_int4(-1, -1, -1, -1);
   }
+  whd::lds_barrier();
+  auto add = [&](uint32_t id) {
+    if (id - i0 < n) atomicAdd(&count[id - i0], 1u);
+  };
   if (P.history) {
     const uint32_t* h = P.history + seq * P.history_stride;
-    size_t len = P.history_stride;
+    // 16-byte loads from the first aligned entry on; the first ones do not wait for the length
+    const size_t cap = P.history_stride, head = min(cap, (16 - (reinterpret_cast<uintptr_t>(h) & 15)) / 4 & 3);
+    const size_t body = (cap - head) / 4, tail = head + 4 * body;
+    const uint4* h4 = reinterpret_cast<const uint4*>(h + head);
+    uint4 a = make_uint4(kNoToken, kNoToken, kNoToken, kNoToken), b = a;
+    uint32_t c = kNoToken, d = kNoToken;
+    if (t < body) a = h4[t];
+    if (t + kThreads < body) b = h4[t + kThreads];
+    if (t < head) c = h[t];
+    if (tail + t < cap) d = h[tail + t];
+    size_t len = cap;
     if (P.history_len && P.history_len[seq] < len) len = P.history_len[seq];
-    for (size_t i = t; i < len; i += kThreads) {
-      const uint32_t c = h[i] - i0;
-      if (c < n) atomicAdd(&count[c], 1u);
+    auto add4 = [&](const uint4& v, size_t i) {
+      if (i < len) add(v.x);
+      if (i + 1 < len) add(v.y);
+      if (i + 2 < len) add(v.z);
+      if (i + 3 < len) add(v.w);
+    };
+    if (t < len) add(c);
+    if (tail + t < len) add(d);
+    for (size_t i = t;; i += 2 * kThreads) {
+      const size_t next = i + 2 * kThreads;
+      const uint4 u = a, v = b;
+      if (head + 4 * next < len && next < body) a = h4[next];
+      if (head + 4 * (next + kThreads) < len && next + kThreads < body) b = h4[next + kThreads];
+      if (i < body) add4(u, head + 4 * i);
+      if (i + kThreads < body) add4(v, head + 4 * (i + kThreads));
+      if (next >= body || head + 4 * next >= len) break;
     }
   }
   for (uint32_t i = t; i < P.n_bias; i += kThreads) {
     const uint32_t c = P.bias_ids[seq * P.bias_stride + i] - i0;
     if (c < n) atomicMax(&entry[c], static_cast<int>(i));
   }
-  __syncthreads();
-  const float* x = P.logits + row * P.ld + i0;
-  float* o = P.out ? P.out + row * P.ldo + i0 : nullptr;
-  const uint32_t* mask = P.mask ? P.mask + row * P.mask_stride + i0 / 32 : nullptr;
-  unsigned long long best = 0;
-  for (uint32_t i = t; i < n; i += kThreads) {
-    float l = x[i];
-    if (said) {
-      const uint32_t c = count[i];
-      if (c) {
-        l = l > 0.f ? l / P.repetition : l * P.repetition;
-        const float f = static_cast<float>(c) * P.frequency;
-        l = l - (f + P.presence);
+  const float* bias = P.bias + seq * P.bias_stride;
+  for (uint32_t r = 0; r < nodes; r++) {
+    const size_t row = row0 + r;
+    bool present = true, mine = false;
+    if (P.tree_parents) {
+      const whd::TreePath path = whd::tree_path(tree, node0 + r);
+      present = path.present();
+      mine = t < P.rows_per_seq && path.has(t) && node_token - i0 < n;
+      if (mine) atomicAdd(&count[node_token - i0], 1u);
+    }
+    whd::lds_barrier();  // the counts of this row
+    Best best{-INFINITY, kNoToken};
+    float x[kPer];
+    uint32_t open[kPer / 4];
+#pragma unroll
+    for (int j = 0; j < kPer; j++) x[j] = next[j];
+#pragma unroll
+    for (int q = 0; q < kPer / 4; q++) open[q] = next_open[q];
+    if (r + 1 < nodes) load(row + 1);
+    if (present) {
+      float* o = P.out ? P.out + row * P.ldo + i0 : nullptr;
+#pragma unroll
+      for (int q = 0; q < kPer / 4; q++) {
+        float* l = x + 4 * q;
+        if (said) {
+          uint32_t c[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) c[k] = count[at(4 * q + k)];
+          if (c[0] | c[1] | c[2] | c[3]) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const float p = l[k] > 0.f ? l[k] / P.repetition : l[k] * P.repetition;
+              const float f = static_cast<float>(c[k]) * P.frequency;
+              l[k] = c[k] ? p - (f + P.presence) : l[k];
+            }
+          }
+        }
+        if (P.n_bias) {
+          int e[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) e[k] = entry[at(4 * q + k)];
+          if ((e[0] & e[1] & e[2] & e[3]) >= 0) {  // an entry's index is no negative number
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              if (e[k] >= 0) l[k] = l[k] + bias[e[k]];
+          }
+        }
+        if (open[q] != 15u) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) l[k] = open[q] >> k & 1u ? l[k] : -INFINITY;
+        }
+        const float m = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));  // passes NaN over
+        if (m > best.top) {  // at() grows with q and k: the lowest of equal ones
+          best.top = m;
+          best.at = i0 + at(4 * q + (l[0] == m ? 0 : l[1] == m ? 1 : l[2] == m ? 2 : 3));
+        }
+      }
+      if (o) {
+        if constexpr (VEC) {
+#pragma unroll
+          for (int j = 0; j < kPer; j += 4) {
+            const uint32_t a = at(j);
+            if (a + 4 <= n) {
+              *reinterpret_cast<float4*>(o + a) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                if (a + k < n) o[a + k] = x[j + k];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPer; j++)
+            if (at(j) < n) o[at(j)] = x[j];
+        }
       }
     }
-    if (P.n_bias) {
-      const int e = entry[i];
-      if (e >= 0) l = l + P.bias[seq * P.bias_stride + e];
+    if (P.best) {
+      best = wave_best(best);
+      if ((t & 63) == 0) red[t >> 6] = best;
     }
-    if (mask && !((mask[i >> 5] >> (i & 31)) & 1u)) l = -INFINITY;
-    if (o) o[i] = l;
-    const uint32_t key = order_key(l);
-    const unsigned long long b = static_cast<unsigned long long>(key) << 32 | (kNoToken - (i0 + i));
-    if (key && b > best) best = b;
-  }
-  if (!P.best) return;
-  best = wave_max(best);
-  if ((t & 63) == 0) red[t >> 6] = best;
-  __syncthreads();
-  if (t == 0) {
-    for (int w = 1; w < kThreads / 64; w++) best = red[w] > best ? red[w] : best;
-    P.best[static_cast<size_t>(row) * P.n_chunks + blockIdx.x] = best;
+    if (P.best || P.tree_parents) whd::lds_barrier();  // red, and every thread is done with the counts
+    if (mine) atomicSub(&count[node_token - i0], 1u);
+    if (P.best && t < 64) {
+      best = wave_best(t < kThreads / 64 ? red[t] : Best{-INFINITY, kNoToken});
+      if (t == 0) {
+        if (P.n_chunks == 1) P.token[row] = best.at;
+        else P.best[row * P.n_chunks + blockIdx.x] = make_float2(best.top, __builtin_bit_cast(float, best.at));
+      }
+    }
+    whd::lds_barrier();  // red is free; the counts are the history's again
   }
 }
 
 // One wave per row.
-__global__ __launch_bounds__(64) void logits_pick_kernel(const unsigned long long* __restrict__ best, uint32_t n_chunks,
+__global__ __launch_bounds__(64) void logits_pick_kernel(const float2* __restrict__ best, uint32_t n_chunks,
                                                          uint32_t* __restrict__ token) {
-  unsigned long long b = 0;
+  Best b{-INFINITY, kNoToken};
   for (uint32_t c = threadIdx.x; c < n_chunks; c += 64) {
-    const unsigned long long v = best[static_cast<size_t>(blockIdx.x) * n_chunks + c];
-    b = v > b ? v : b;
+    const float2 v = best[static_cast<size_t>(blockIdx.x) * n_chunks + c];
+    if (v.x > b.top) b = Best{v.x, __builtin_bit_cast(uint32_t, v.y)};  // chunks ascend: so do their tokens
   }
-  b = wave_max(b);
-  if (threadIdx.x == 0) token[blockIdx.x] = b ? kNoToken - static_cast<uint32_t>(b) : kNoToken;
+  b = wave_best(b);
+  if (threadIdx.x == 0) token[blockIdx.x] = b.at;
 }
 
 size_t chunks_of(size_t vocab) { return (vocab + kChunk - 1) / kChunk; }
@@ -157,7 +278,7 @@ size_t chunks_of(size_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 WH_API size_t wh_logits_process_workspace_bytes(const wh_logits_rules* rules, size_t n_rows, size_t vocab) {
   if (!rules) return 0;
-  return n_rows * chunks_of(vocab) * sizeof(unsigned long long);
+  return n_rows * chunks_of(vocab) * sizeof(float2);
 }
 
 WH_API int wh_logits_process(const wh_logits_rules* rules, const float* logits, size_t ld, size_t n_rows, size_t vocab,
@@ -223,12 +344,25 @@ WH_API int wh_logits_process(const wh_logits_rules* rules, const float* logits, 
   }
   P.mask = r.mask;
   P.mask_stride = r.mask_stride;
-  P.best = token ? static_cast<unsigned long long*>(workspace) : nullptr;
+  P.best = token ? static_cast<float2*>(workspace) : nullptr;
   P.token = token;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  logits_kernel<<<dim3(P.n_chunks, static_cast<unsigned>(n_rows)), kThreads, 0, s>>>(P);
+  // rows of one sequence share the counts of a workgroup: as many as leave two workgroups per CU
+  const size_t wgs = P.n_chunks * n_rows, most = 2 * static_cast<size_t>(wh::cu_count());
+  P.rows_per_wg = static_cast<uint32_t>(wgs / most < 1 ? 1 : wgs / most < per ? wgs / most : per);
+  const size_t groups = (per + P.rows_per_wg - 1) / P.rows_per_wg;
+  const dim3 grid(P.n_chunks, static_cast<unsigned>(n_rows / per * groups));
+  const size_t lds = kChunk * 4 * (P.n_bias ? 2 : 1);
+  const bool vec = wh::aligned(logits, 16) && ld % 4 == 0 && (!out || (wh::aligned(out, 16) && ld_out % 4 == 0));
+  if (vec) {
+    WH_ENSURE_LDS(lds, &logits_kernel<true>);
+    logits_kernel<true><<<grid, kThreads, lds, s>>>(P);
+  } else {
+    WH_ENSURE_LDS(lds, &logits_kernel<false>);
+    logits_kernel<false><<<grid, kThreads, lds, s>>>(P);
+  }
   WH_LAUNCH_CHECK("logits kernel launch");
-  if (token) {
+  if (token && P.n_chunks > 1) {
     logits_pick_kernel<<<static_cast<unsigned>(n_rows), 64, 0, s>>>(P.best, P.n_chunks, token);
     WH_LAUNCH_CHECK("logits pick launch");
   }

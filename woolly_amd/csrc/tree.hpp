@@ -34,6 +34,38 @@ int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t st
 
 namespace whd {
 
+// Largest float (NaN passed over) and smallest number over the wave's 64 lanes, in
+// every lane: swaps within rows of 16 lanes (DPP), then of rows and halves
+// (v_permlane16_swap, v_permlane32_swap).  No LDS round trips, as __shfl_xor
+// would take: some 60 cycles instead of 700.
+template <typename Op>
+__device__ __forceinline__ uint32_t wave_join(uint32_t v, Op op) {
+  v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xF, 0xF, false)));
+  v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, false)));
+  v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x141, 0xF, 0xF, false)));
+  v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x140, 0xF, 0xF, false)));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = op(static_cast<uint32_t>(a[0]), static_cast<uint32_t>(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return op(static_cast<uint32_t>(b[0]), static_cast<uint32_t>(b[1]));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return __builtin_bit_cast(float, wave_join(__builtin_bit_cast(uint32_t, v), [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+  }));
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+  return wave_join(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
+// A barrier for what goes through LDS only: __syncthreads() would also wait for
+// the global loads and stores in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // The path from the cache to node t of one tree: bit a is set where a is t itself
 // or an ancestor of t; depth counts its ancestors.  A node whose parent is
 // neither -1 nor an earlier node is absent, and so are all below it: no bits.
@@ -46,17 +78,23 @@ struct TreePath {
   __device__ __forceinline__ bool present() const { return (lo | hi) != 0; }
   __device__ __forceinline__ bool has(int a) const { return ((a < 64 ? lo : hi) >> (a & 63)) & 1u; }
 };
-__device__ __forceinline__ TreePath tree_path(const int32_t* __restrict__ parents, int n_tree, int t) {
+// A tree's parents over the lanes of a wave (lane l: nodes l and l + 64); one
+// that is no earlier node, but not -1 either, is -2.
+struct TreeLanes {
+  int p0, p1;
+};
+__device__ __forceinline__ TreeLanes tree_lanes(const int32_t* __restrict__ parents, int n_tree) {
   const int lane = threadIdx.x & 63;
-  // a parent that is no earlier node ends the walk below -1
-  const int g0 = lane < n_tree ? parents[lane] : -2, g1 = lane + 64 < n_tree ? parents[lane + 64] : -2;
-  const int p0 = g0 >= lane ? -2 : g0, p1 = g1 >= lane + 64 ? -2 : g1;
+  const int a = lane < n_tree ? parents[lane] : -2, b = lane + 64 < n_tree ? parents[lane + 64] : -2;
+  return TreeLanes{a >= lane ? -2 : a, b >= lane + 64 ? -2 : b};
+}
+__device__ __forceinline__ TreePath tree_path(const TreeLanes& tree, int t) {
   TreePath p{0, 0, -1};
   int at = t;
   while (at >= 0) {  // falls with every step
     if (at < 64) p.lo |= 1ull << at; else p.hi |= 1ull << (at - 64);
     p.depth++;
-    const int a = __builtin_amdgcn_readlane(p0, at & 63), b = __builtin_amdgcn_readlane(p1, at & 63);
+    const int a = __builtin_amdgcn_readlane(tree.p0, at & 63), b = __builtin_amdgcn_readlane(tree.p1, at & 63);
     at = at < 64 ? a : b;
   }
   if (at != -1) p = TreePath{0, 0, 0};

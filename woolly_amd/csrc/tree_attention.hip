@@ -191,9 +191,10 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
       vy[u] = v[i + D / 2];
     }
   }
+  const whd::TreeLanes tree = whd::tree_lanes(P.parents + static_cast<size_t>(s) * P.n_tree, P.n_tree);
   const float inv = P.inv_freq[i];
   const uint32_t ctx = P.ctx_len[s];
-  const whd::TreePath path = whd::tree_path(P.parents + static_cast<size_t>(s) * P.n_tree, P.n_tree, t);
+  const whd::TreePath path = whd::tree_path(tree, t);
   const bool present = path.present() && seq_fits(P, ctx);
   if (group == 0 && tid < kWholeMask) {
     const unsigned long long w = (tid < 2 ? path.lo : path.hi) >> (32 * (tid & 1));
@@ -210,9 +211,7 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
       float sn, cs;
       sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
       float a = present ? x[u] * cs - y[u] * sn : 0.f, b = present ? x[u] * sn + y[u] * cs : 0.f;
-      float mx = fmaxf(fabsf(a), fabsf(b));
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+      const float mx = whd::wave_max(fmaxf(fabsf(a), fabsf(b)));
       // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element
       // to 2^-22 of itself or 2^-38 of the largest
       int e = 0;
@@ -631,8 +630,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
   const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.R + t * P.G + g;
   float M = -INFINITY;
   for (uint32_t c = lane; c < n; c += 64) M = fmaxf(M, P.ml[at + c * step].x);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  M = whd::wave_max(M);
   float L = 0.f, A[V] = {};
   for (uint32_t b = 0; b < n; b += 64) {
     const float2 ml = b + lane < n ? P.ml[at + (b + lane) * step] : make_float2(-INFINITY, 0.f);

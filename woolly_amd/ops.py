@@ -21,6 +21,8 @@ def _s(stream: Stream | None):
 
 def _p(buf) -> int:
     """Device address of a DeviceBuffer, a Weight handle or a plain integer."""
+    if type(buf) is int:
+        return buf
     if buf is None:
         return 0
     ptr = getattr(buf, "ptr", None)
