@@ -54,7 +54,7 @@ struct Params {
   _Float16 *k_cache, *v_cache;
   const float* inv_freq;
   float* out;
-  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, unit;
+  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, unit, tiles;
   float scale;
   // workspace
   uint4* slots;         // [max_slots] (sequence, first key, key behind the last, cache rows of the step); sequence n_seqs: none
@@ -62,8 +62,9 @@ struct Params {
   uint32_t* mask;       // [n_seqs][n_tree][4]
   float* qscale;        // [n_seqs][n_kv][R]
   _Float16* qlimb;      // [n_seqs][n_kv][R][2][D]
-  float2* ml;           // [max_slots][n_kv][R]
-  float* acc;           // [max_slots][n_kv][R][D]
+  // partial results of a slot, KV head and tile of 32 query rows
+  float2* ml;           // [max_slots][n_kv][tiles][32] (maximum in powers of 2, sum)
+  float4* acc;          // [max_slots][n_kv][tiles][D / 8][64]: the registers of the lanes, as in the product
 };
 
 // ------------------------------------------------------------------ prepare
@@ -320,7 +321,7 @@ struct Shape {
   static constexpr int TILES = SK / 32 / KW;                 // 32-key tiles per wave and stage
   static constexpr int kTileBytes = SK * D * 2;              // one of K, V
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kMergeBytes = KW > 1 ? kAttnWaves * 32 * (D + 2) * 4 : 0;
+  static constexpr int kMergeBytes = KW > 1 ? kAttnWaves * 32 * (D + 2) * 4 : 0;  // all waves' sums, maxima and totals
   static constexpr int kLds = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;
 };
 
@@ -542,126 +543,153 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
   }
 
-  const size_t prow = (static_cast<size_t>(slot) * P.n_kv + kvh) * P.R;
+  // Results go out in the lanes' own order: a wave stores 1 KB in a row, and the
+  // combine kernel reads it back the same way.
+  constexpr int kQuads = D / 8;  // float4 per lane
+  const size_t tile0 = (static_cast<size_t>(slot) * P.n_kv + kvh) * P.n_rg * RW + rg * RW;
   if constexpr (KW == 1) {
     if (r0 < P.R) {
-      float* o = P.acc + (prow + r0) * D;
+      float4* o = P.acc + (tile0 + rw) * kQuads * 64 + lane;
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          *reinterpret_cast<float4*>(o + 32 * d + 8 * i + 4 * h) =
-              make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
-      if (h == 0) P.ml[prow + r0] = make_float2(m, l);
+          o[(4 * d + i) * 64] = make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+      if (h == 0) P.ml[(tile0 + rw) * 32 + l32] = make_float2(m, l);
     }
   } else {
     // the KW waves of each query tile join in LDS, in fixed order
-    __syncthreads();
-    float* am = reinterpret_cast<float*>(lds);             // [4][32][D]
-    float* mm = am + kAttnWaves * 32 * D;                  // [4][32][2]
+    whd::lds_barrier();
+    float4* am = reinterpret_cast<float4*>(lds);                       // [4][D / 8][64]
+    float2* mm = reinterpret_cast<float2*>(am + kAttnWaves * kQuads * 64);  // [4][32]
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        *reinterpret_cast<float4*>(am + (wave * 32 + l32) * D + 32 * d + 8 * i + 4 * h) =
+        am[(wave * kQuads + 4 * d + i) * 64 + lane] =
             make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
-    if (h == 0) {
-      mm[2 * (wave * 32 + l32)] = m;
-      mm[2 * (wave * 32 + l32) + 1] = l;
+    if (h == 0) mm[wave * 32 + l32] = make_float2(m, l);
+    whd::lds_barrier();
+    // wave -> its query tile's quads kw, kw + KW, ...
+    float M = -INFINITY, L = 0.f, ew[KW];
+    float2 ml[KW];
+#pragma unroll
+    for (int w = 0; w < KW; w++) {
+      ml[w] = mm[(rw * KW + w) * 32 + l32];
+      M = fmaxf(M, ml[w].x);
     }
-    __syncthreads();
 #pragma unroll
-    for (int it = 0; it < RW * 32 * (D / 4) / (64 * kAttnWaves); it++) {
-      const int e = tid + it * 64 * kAttnWaves, rr = e / (D / 4), d4 = e % (D / 4);
-      const uint32_t rglob = rg * RW * 32 + rr;
-      const int w0 = (rr / 32) * KW, lr = rr % 32;
-      float M = -INFINITY;
-      float2 ml[KW];
+    for (int w = 0; w < KW; w++) {
+      ew[w] = ml[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w].x - M);
+      L = __builtin_fmaf(ml[w].y, ew[w], L);
+    }
+    if (r0 < P.R) {
 #pragma unroll
-      for (int w = 0; w < KW; w++) {
-        ml[w] = *reinterpret_cast<const float2*>(mm + 2 * ((w0 + w) * 32 + lr));
-        M = fmaxf(M, ml[w].x);
-      }
-      float L = 0.f;
-      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < kQuads / KW; q++) {
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < KW; w++) {
-        const float ew = ml[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w].x - M);
-        L = __builtin_fmaf(ml[w].y, ew, L);
-        const float4 a = *reinterpret_cast<const float4*>(am + ((w0 + w) * 32 + lr) * D + 4 * d4);
-        A.x = __builtin_fmaf(a.x, ew, A.x);
-        A.y = __builtin_fmaf(a.y, ew, A.y);
-        A.z = __builtin_fmaf(a.z, ew, A.z);
-        A.w = __builtin_fmaf(a.w, ew, A.w);
+        for (int w = 0; w < KW; w++) {
+          const float4 a = am[((rw * KW + w) * kQuads + kw + KW * q) * 64 + lane];
+          A.x = __builtin_fmaf(a.x, ew[w], A.x);
+          A.y = __builtin_fmaf(a.y, ew[w], A.y);
+          A.z = __builtin_fmaf(a.z, ew[w], A.z);
+          A.w = __builtin_fmaf(a.w, ew[w], A.w);
+        }
+        P.acc[((tile0 + rw) * kQuads + kw + KW * q) * 64 + lane] = A;
       }
-      if (rglob < P.R) {
-        *reinterpret_cast<float4*>(P.acc + (prow + rglob) * D + 4 * d4) = A;
-        if (d4 == 0) P.ml[prow + rglob] = make_float2(M, L);
-      }
+      if (kw == 0 && h == 0) P.ml[(tile0 + rw) * 32 + l32] = make_float2(M, L);
     }
   }
 }
 
 // ------------------------------------------------------------------ combine
-// One workgroup per (node, head): out = sum_c acc_c 2^{m_c - M} / sum_c l_c 2^{m_c - M}.
-// Every wave forms the weights of 64 chunks at a time, one per lane, and adds a
-// quarter of their accumulators, 8 loads in flight; the waves' sums add in fixed
-// order.  Rows of absent nodes are zeros; those of a sequence whose rows do not
-// fit its cache are NaN.
+// out = sum_c acc_c 2^{m_c - M} / sum_c l_c 2^{m_c - M}.  A workgroup takes one
+// register quad of a tile of 32 query rows: lane l has four dims of row l % 32,
+// so every row's maximum and sums stay in its lane, and a load is 1 KB in a row.
+// Wave w joins chunks w, w + 4, .., 8 loads in flight, then the four waves join
+// in fixed order.  Rows of absent nodes are zeros; those of a sequence whose
+// rows do not fit its cache are NaN.
+// grid: n_kv x D / 8 quads x tiles x sequences, KV head fastest, as the partial
+// kernel's workgroups: with 8 KV heads a head's chunks are joined on the XCD
+// whose L2 they were written through.
 template <int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const Params P) {
-  constexpr int V = D / 64;  // dims per lane
-  constexpr int kPer = 8;
-  __shared__ float part[4][D];
-  // KV head fastest, as the partial kernel's workgroups: with 8 KV heads a head's
-  // chunks are joined on the XCD whose L2 they were written through
-  const uint32_t kvh = blockIdx.x % P.n_kv, g = blockIdx.x / P.n_kv % P.G, row = blockIdx.x / P.n_heads;
-  const uint32_t seq = row / P.n_tree, t = row % P.n_tree, head = kvh * P.G + g;
-  const uint32_t lane = threadIdx.x & 63;
+__global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint32_t n_tiles) {
+  constexpr int kQuads = D / 8, kPer = 8;
+  typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+  __shared__ float4 pa[4][64];
+  __shared__ float2 pm[4][64];
+  uint32_t b = blockIdx.x;
+  const uint32_t kvh = b % P.n_kv;
+  b /= P.n_kv;
+  const uint32_t quad = b % kQuads;
+  b /= kQuads;
+  const uint32_t tile = b % n_tiles, seq = b / n_tiles;
+  const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float* o = P.out + static_cast<size_t>(row) * P.n_heads * D + static_cast<size_t>(head) * D;
-  const uint4 w = *reinterpret_cast<const uint4*>(P.mask + static_cast<size_t>(row) * kWholeMask);
+  const uint32_t row = tile * 32 + (lane & 31);
   const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
-  if ((w.x | w.y | w.z | w.w) == 0) {
-    if (threadIdx.x < D) o[threadIdx.x] = seq_fits(P, P.ctx_len[seq]) ? 0.f : __builtin_nanf("");
-    return;
-  }
-  const size_t step = static_cast<size_t>(P.n_kv) * P.R;
-  const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.R + t * P.G + g;
-  float M = -INFINITY;
-  for (uint32_t c = lane; c < n; c += 64) M = fmaxf(M, P.ml[at + c * step].x);
-  M = whd::wave_max(M);
-  float L = 0.f, A[V] = {};
-  for (uint32_t b = 0; b < n; b += 64) {
-    const float2 ml = b + lane < n ? P.ml[at + (b + lane) * step] : make_float2(-INFINITY, 0.f);
-    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);  // 0 past the last chunk
-    L = __builtin_fmaf(ml.y, ew, L);
-    const uint32_t end = min(n - b, 64u);
-    for (uint32_t c = wave; c < end; c += 4 * kPer) {
-      float a[kPer][V];
+  const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
+  const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.tiles + tile;
+  float M = -INFINITY, L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t c = wave; c < n; c += 4 * kPer) {
+    float2 ml[kPer];
+    float4 a[kPer];
+    float mx = M;
 #pragma unroll
-      for (int j = 0; j < kPer; j++) {
-        const float* src = P.acc + (at + (b + min(c + 4 * j, end - 1)) * step) * D + V * lane;
+    for (int j = 0; j < kPer; j++) {
+      const size_t s = at + min(c + 4 * j, n - 1) * step;  // a chunk past the last has no weight
+      ml[j] = P.ml[s * 32 + (lane & 31)];
+      a[j] = P.acc[(s * kQuads + quad) * 64 + lane];
+    }
 #pragma unroll
-        for (int i = 0; i < V; i++) a[j][i] = src[i];
-      }
+    for (int j = 0; j < kPer; j++) {
+      if (c + 4 * j >= n) ml[j].x = -INFINITY;
+      mx = fmaxf(mx, ml[j].x);
+    }
+    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mx);
+    M = mx;
+    if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
 #pragma unroll
-      for (int j = 0; j < kPer; j++) {
-        const uint32_t cj = c + 4 * j;
-        const float wj = cj < end ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ew), cj & 63)) : 0.f;
-        if (cj < end) {
-#pragma unroll
-          for (int i = 0; i < V; i++) A[i] = __builtin_fmaf(a[j][i], wj, A[i]);
-        }
-      }
+    for (int j = 0; j < kPer; j++) {
+      if (ml[j].x == -INFINITY) continue;
+      const float ew = __builtin_amdgcn_exp2f(ml[j].x - M);
+      L = __builtin_fmaf(ml[j].y, ew, L);
+      A.x = __builtin_fmaf(a[j].x, ew, A.x);
+      A.y = __builtin_fmaf(a[j].y, ew, A.y);
+      A.z = __builtin_fmaf(a[j].z, ew, A.z);
+      A.w = __builtin_fmaf(a[j].w, ew, A.w);
     }
   }
-#pragma unroll
-  for (int i = 0; i < V; i++) part[wave][V * lane + i] = A[i];
-  L = whd::wave_sum(L);
-  __syncthreads();
-  const uint32_t d = threadIdx.x;
-  if (d < D) o[d] = ((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) / L;
+  pa[wave][lane] = A;
+  pm[wave][lane] = make_float2(M, L);
+  whd::lds_barrier();
+  if (wave != 0 || row >= P.R) return;
+  const uint32_t t = row / P.G, g = row % P.G;
+  const size_t node = static_cast<size_t>(seq) * P.n_tree + t;
+  const uint4 w4 = *reinterpret_cast<const uint4*>(P.mask + node * kWholeMask);
+  float4u o;
+  if ((w4.x | w4.y | w4.z | w4.w) == 0) {
+    o = seq_fits(P, P.ctx_len[seq]) ? 0.f : __builtin_nanf("");
+  } else {
+    for (int w = 1; w < 4; w++) M = fmaxf(M, pm[w][lane].x);
+    L = 0.f;
+    o = 0.f;
+    for (int w = 0; w < 4; w++) {
+      const float2 ml = pm[w][lane];
+      if (ml.x == -INFINITY) continue;
+      const float ew = __builtin_amdgcn_exp2f(ml.x - M);
+      const float4 a = pa[w][lane];
+      L = __builtin_fmaf(ml.y, ew, L);
+      o[0] = __builtin_fmaf(a.x, ew, o[0]);
+      o[1] = __builtin_fmaf(a.y, ew, o[1]);
+      o[2] = __builtin_fmaf(a.z, ew, o[2]);
+      o[3] = __builtin_fmaf(a.w, ew, o[3]);
+    }
+    o = o / L;  // no key's score above -inf: 0 / 0, as the formula
+  }
+  *reinterpret_cast<float4u*>(P.out + node * P.n_heads * D + static_cast<size_t>(kvh * P.G + g) * D + 32 * (quad >> 2) +
+                              8 * (quad & 3) + 4 * h) = o;
 }
 
 // ------------------------------------------------------------------ launching
@@ -706,8 +734,9 @@ size_t layout(Params& P, size_t D, void* base) {
   P.mask = reinterpret_cast<uint32_t*>(take(4 * kWholeMask * static_cast<size_t>(P.n_seqs) * P.n_tree));
   P.qscale = reinterpret_cast<float*>(take(4 * P.n_seqs * rows));
   P.qlimb = reinterpret_cast<_Float16*>(take(2 * 2 * D * P.n_seqs * rows));
-  P.ml = reinterpret_cast<float2*>(take(8 * slots * rows));
-  P.acc = reinterpret_cast<float*>(take(4 * D * slots * rows));
+  const size_t all_tiles = slots * P.n_kv * P.tiles;
+  P.ml = reinterpret_cast<float2*>(take(8 * 32 * all_tiles));
+  P.acc = reinterpret_cast<float4*>(take(4 * D * 32 * all_tiles));
   return off;
 }
 
@@ -725,6 +754,7 @@ Params fill(const Plan& p, size_t n_seqs, size_t n_tree, size_t n_heads, size_t 
   P.target = static_cast<uint32_t>(p.target);
   P.sparse = static_cast<uint32_t>(p.sparse);
   P.unit = static_cast<uint32_t>(p.unit);
+  P.tiles = static_cast<uint32_t>(p.n_rg * p.rw);
   P.scale = 1.0f / sqrtf(static_cast<float>(D));
   return P;
 }
@@ -744,7 +774,8 @@ int launch_all(const Params& P, int rw, hipStream_t s) {
   WH_LAUNCH_CHECK("tree attention prepare launch");
   int st = rw == 1 ? launch_partial<D, 1>(P, s) : rw == 2 ? launch_partial<D, 2>(P, s) : launch_partial<D, 4>(P, s);
   if (st) return st;
-  tree_combine_kernel<D><<<P.n_seqs * P.n_tree * P.n_heads, 256, 0, s>>>(P);
+  const uint32_t n_tiles = (P.R + 31) / 32;
+  tree_combine_kernel<D><<<P.n_kv * (D / 8) * n_tiles * P.n_seqs, 256, 0, s>>>(P, n_tiles);
   WH_LAUNCH_CHECK("tree attention combine launch");
   return WH_OK;
 }
