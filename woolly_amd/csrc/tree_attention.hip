@@ -401,21 +401,28 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
   float m = -INFINITY, l = 0.f;
   bool odd = false;  // an edge tile of this wave held infinities or NaN in V
 
-  // One 32-key tile.  kt, vt: LDS addresses of its first K and V row.  Edge: the
-  // tile may reach beyond the cache into the nodes' rows or past the last one.
-  auto tile = [&](uint32_t base, uint32_t kt, uint32_t vt, auto edge) {
+  // N 32-key tiles, KW tiles apart.  kt, vt: LDS addresses of the first one's first
+  // K and V row.  Edge (N = 1): the tile may reach beyond the cache into the nodes'
+  // rows or past the last one.
+  auto tiles = [&](uint32_t base, uint32_t kt, uint32_t vt, auto edge, auto count) {
     constexpr bool kEdge = decltype(edge)::value;
-    f32x16 s;
+    constexpr int N = decltype(count)::value, kStep = KW * 32 * 2 * D;
+    f32x16 s[N];
 #pragma unroll
-    for (int i = 0; i < 16; i++) s[i] = 0.f;
+    for (int n = 0; n < N; n++)
 #pragma unroll
-    for (int j = 0; j < KS; j++) {
-      const half8 kf = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-          (uintptr_t)(kt + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[j], s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j], s, 0, 0, 0);
-    }
+      for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        const half8 kf = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+            (uintptr_t)(kt + n * kStep + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
+        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[j], s[n], 0, 0, 0);
+        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j], s[n], 0, 0, 0);
+      }
     if constexpr (kEdge) {
+      static_assert(N == 1, "one tile at a time");
       uint32_t bits;
       // keys from ctx on are the tree's nodes: bit k of `bits` for key base + k
       const int off = static_cast<int>(base) - static_cast<int>(ctx);
@@ -437,12 +444,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int key = 8 * (i >> 2) + 4 * h + (i & 3);
-        s[i] = (bits >> key) & 1u ? s[i] : -INFINITY;
+        s[0][i] = (bits >> key) & 1u ? s[0][i] : -INFINITY;
       }
     }
-    float mt = s[0];
+    float mt = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; i++) mt = fmaxf(mt, s[i]);
+    for (int i = 1; i < 16 * N; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
     mt = swap_max(mt) * qs;
     if (__ballot(mt > m + kLazyMax)) {
       const float mn = fmaxf(m, mt);
@@ -455,27 +462,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       m = mn;
     }
     const float mb = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
-    float p[16], lt[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs, mb));
-      lt[i & 3] += p[i];
-    }
-    l += (lt[0] + lt[1]) + (lt[2] + lt[3]);  // one addition to the running sum per tile
+    float lt[4] = {0.f, 0.f, 0.f, 0.f};
     const int i16 = lane & 15, kq = i16 >> 2, dq = i16 & 3, dg = (lane >> 4) & 1;
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
+    for (int ks = 0; ks < 2 * N; ks++) {
       half8 ph, pl;
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) split2(p[8 * ks + i], p[8 * ks + i + 1], ph, pl, i);
+      for (int i = 0; i < 8; i += 2) {
+        float p[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][8 * (ks % 2) + i + k], qs, mb));
+          lt[(i + k) & 3] += p[k];
+        }
+        split2(p[0], p[1], ph, pl, i);
+      }
 #pragma unroll
       for (int d = 0; d < DT; d++) {
         half8 vf;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const int rr = 16 * ks + 8 * u + 4 * h + kq;
+          const int rr = 16 * (ks % 2) + 8 * u + 4 * h + kq;
           const int c = 4 * d + 2 * dg + (dq >> 1);
-          const s16x4 x = read_tr(vt + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
+          const s16x4 x = read_tr(vt + ks / 2 * kStep + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
           const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
 #pragma unroll
           for (int i = 0; i < 4; i++) vf[4 * u + i] = y[i];
@@ -484,6 +493,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, acc[d], 0, 0, 0);
       }
     }
+    l += (lt[0] + lt[1]) + (lt[2] + lt[3]);  // one addition to the running sum
   };
 
   // stages of cache rows only, then those that reach the nodes' rows or the chunk's end
@@ -499,12 +509,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
   };
   uint32_t st = 0;
   for (; st < n_inner; st++) {
-    const uint32_t kt = turn(st);
-#pragma unroll
-    for (int u = 0; u < S::TILES; u++) {
-      const uint32_t to = 32 * (kw + KW * u) * 2 * D;
-      tile(0, kt + to, kt + S::kTileBytes + to, std::false_type{});
-    }
+    const uint32_t kt = turn(st), to = 32 * kw * 2 * D;
+    tiles(0, kt + to, kt + S::kTileBytes + to, std::false_type{}, std::integral_constant<int, S::TILES>{});
   }
   if (st < n_stages) {
     const uint4 w = *reinterpret_cast<const uint4*>(P.mask + (static_cast<size_t>(seq) * P.n_tree + r / P.G) * kWholeMask);
@@ -516,7 +522,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 #pragma unroll 1
     for (int u = 0; u < S::TILES; u++) {
       const uint32_t base = c0 + st * SK + 32 * (kw + KW * u), to = 32 * (kw + KW * u) * 2 * D;
-      if (base < c1) tile(base, kt + to, kt + S::kTileBytes + to, std::true_type{});
+      if (base < c1) tiles(base, kt + to, kt + S::kTileBytes + to, std::true_type{}, std::integral_constant<int, 1>{});
     }
   }
   l = swap_sum(l);
