@@ -412,15 +412,26 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     for (int n = 0; n < N; n++)
 #pragma unroll
       for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+    // LDS reads run one step ahead of the matrix products that take them: kNoLds
+    // lets the compiler move anything but them across
+    constexpr int kNoLds = 0x47F;
+    half8 kf[2][N];
+    auto read_k = [&](int j) {
 #pragma unroll
-    for (int j = 0; j < KS; j++)
-#pragma unroll
-      for (int n = 0; n < N; n++) {
-        const half8 kf = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+      for (int n = 0; n < N; n++)
+        kf[j & 1][n] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
             (uintptr_t)(kt + n * kStep + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
-        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[j], s[n], 0, 0, 0);
-        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[j], s[n], 0, 0, 0);
-      }
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    read_k(0);
+#pragma unroll
+    for (int j = 0; j < KS; j++) {
+      if (j + 1 < KS) read_k(j + 1);
+#pragma unroll
+      for (int n = 0; n < N; n++) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j & 1][n], qh[j], s[n], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < N; n++) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j & 1][n], ql[j], s[n], 0, 0, 0);
+    }
     if constexpr (kEdge) {
       static_assert(N == 1, "one tile at a time");
       uint32_t bits;
@@ -447,6 +458,23 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         s[0][i] = (bits >> key) & 1u ? s[0][i] : -INFINITY;
       }
     }
+    half8 vf[2][DT];
+    auto read_v = [&](int ks) {
+      const int i16 = lane & 15, kq = i16 >> 2, dq = i16 & 3, dg = (lane >> 4) & 1;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int rr = 16 * (ks % 2) + 8 * u + 4 * h + kq;
+          const int c = 4 * d + 2 * dg + (dq >> 1);
+          const s16x4 x = read_tr(vt + ks / 2 * kStep + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
+          const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
+#pragma unroll
+          for (int i = 0; i < 4; i++) vf[ks & 1][d][4 * u + i] = y[i];
+        }
+      __builtin_amdgcn_sched_barrier(kNoLds);
+    };
+    read_v(0);
     float mt = s[0][0];
 #pragma unroll
     for (int i = 1; i < 16 * N; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
@@ -463,7 +491,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
     const float mb = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
     float lt[4] = {0.f, 0.f, 0.f, 0.f};
-    const int i16 = lane & 15, kq = i16 >> 2, dq = i16 & 3, dg = (lane >> 4) & 1;
 #pragma unroll
     for (int ks = 0; ks < 2 * N; ks++) {
       half8 ph, pl;
@@ -477,21 +504,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         }
         split2(p[0], p[1], ph, pl, i);
       }
+      if (ks + 1 < 2 * N) read_v(ks + 1);
 #pragma unroll
-      for (int d = 0; d < DT; d++) {
-        half8 vf;
+      for (int d = 0; d < DT; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[ks & 1][d], ph, acc[d], 0, 0, 0);
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int rr = 16 * (ks % 2) + 8 * u + 4 * h + kq;
-          const int c = 4 * d + 2 * dg + (dq >> 1);
-          const s16x4 x = read_tr(vt + ks / 2 * kStep + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
-          const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
-#pragma unroll
-          for (int i = 0; i < 4; i++) vf[4 * u + i] = y[i];
-        }
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, acc[d], 0, 0, 0);
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, acc[d], 0, 0, 0);
-      }
+      for (int d = 0; d < DT; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[ks & 1][d], pl, acc[d], 0, 0, 0);
     }
     l += (lt[0] + lt[1]) + (lt[2] + lt[3]);  // one addition to the running sum
   };
