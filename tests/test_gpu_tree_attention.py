@@ -118,6 +118,14 @@ def test_ragged_batches(gpu, heads, kv, d, n_tree, shape):
     run(Case(len(lens), n_tree, heads, kv, d, lens, shape=shape, seed=d), f"ragged {heads}/{kv}x{d} tree {n_tree} {shape}")
 
 
+@pytest.mark.parametrize("heads,kv,d,n_tree", [(8, 2, 128, 5), (8, 2, 128, 12), (8, 2, 64, 30)])
+@pytest.mark.parametrize("room", [0, 100, 400, 5000])
+def test_room_behind_the_rows(gpu, heads, kv, d, n_tree, room):
+    """The cache's size decides how the rows are cut up, not what comes out."""
+    run(Case(3, n_tree, heads, kv, d, [100 - n_tree, 0, 17], room=room, shape="padded", seed=room),
+        f"{heads}/{kv}x{d} tree {n_tree} room {room}")
+
+
 def test_many_sequences(gpu):
     rng = np.random.default_rng(3)
     lens = [int(v) for v in rng.integers(0, 90, 300)]
@@ -157,7 +165,7 @@ def test_scores_beyond_f16(gpu):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("n_tree,ctx", [(12, 37), (70, 37), (6, 0)])
+@pytest.mark.parametrize("n_tree,ctx", [(12, 37), (70, 37), (6, 0), (12, 700), (6, 900), (100, 640)])
 def test_what_a_row_does_not_see(gpu, d, n_tree, ctx):
     """NaN and infinities in stale cache rows, in absent nodes and in nodes off a
     row's path must not reach it; on its path they must."""

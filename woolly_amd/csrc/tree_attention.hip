@@ -44,6 +44,7 @@ constexpr float kLazyMax = 8.0f;     // ... and may grow by 2^8 before the runni
 constexpr int kWholeMask = 4;        // mask words per node
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // four floats of the caller's output
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 struct Params {
@@ -54,7 +55,7 @@ struct Params {
   _Float16 *k_cache, *v_cache;
   const float* inv_freq;
   float* out;
-  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, unit, tiles;
+  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, unit, least, tiles;
   float scale;
   // workspace
   uint4* slots;         // [max_slots] (sequence, first key, key behind the last, cache rows of the step); sequence n_seqs: none
@@ -126,7 +127,7 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long
   __syncthreads();
   unsigned long long even = (total + P.target - 1) / P.target;
   if (even < kDeepChunk) even = min<unsigned long long>((total + P.sparse - 1) / P.sparse, kDeepChunk);
-  const uint32_t chunk = max(static_cast<uint32_t>((even + P.unit - 1) / P.unit), 1u) * P.unit;
+  const uint32_t chunk = max(static_cast<uint32_t>((even + P.unit - 1) / P.unit) * P.unit, P.least);
   uint32_t n = 0;
   for (uint32_t s = s0; s < s1; s++) n += (first[s] + chunk - 1) / chunk;
   uint32_t at = static_cast<uint32_t>(block_scan(n, red)) - n;
@@ -207,6 +208,13 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
     const uint32_t hh = h0 + u;
     if (hh >= n_slots) break;
     if (hh < P.n_heads) {
+      if (!present && lane < D / 2) {
+        // an absent node's rows are zeros; those of a sequence that does not fit its cache are NaN
+        const float fill = seq_fits(P, ctx) ? 0.f : __builtin_nanf("");
+        float* o = P.out + row * P.n_heads * D + static_cast<size_t>(hh) * D;
+        o[i] = fill;
+        o[i + D / 2] = fill;
+      }
       // q: the angle in turns, whole turns dropped in 64 bits
       const double turns = angle * 0.15915494309189535;
       float sn, cs;
@@ -566,19 +574,30 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
   }
 
-  // Results go out in the lanes' own order: a wave stores 1 KB in a row, and the
+  // A sequence in one chunk is done: its rows go to the caller's output.  Else
+  // results go out in the lanes' own order: a wave stores 1 KB in a row, and the
   // combine kernel reads it back the same way.
   constexpr int kQuads = D / 8;  // float4 per lane
+  const bool whole = c0 == 0 && c1 == rows;
   const size_t tile0 = (static_cast<size_t>(slot) * P.n_kv + kvh) * P.n_rg * RW + rg * RW;
+  const uint32_t node = r / P.G;
+  float* const orow = P.out + (static_cast<size_t>(seq) * P.n_tree + node) * P.n_heads * D +
+                      static_cast<size_t>(kvh * P.G + r % P.G) * D + 4 * h;
+  // a row to store: not one of the padding, nor, in the output, an absent node's
+  const bool mine = r0 < P.R && (!whole || (tm[0] | tm[1] | tm[2] | tm[3]) != 0);
+  auto put = [&](int q, float4 a, float total) {
+    if (whole) *reinterpret_cast<f32x4u*>(orow + 32 * (q >> 2) + 8 * (q & 3)) = f32x4u{a.x, a.y, a.z, a.w} / total;
+    else P.acc[((tile0 + rw) * kQuads + q) * 64 + lane] = a;
+  };
   if constexpr (KW == 1) {
-    if (r0 < P.R) {
-      float4* o = P.acc + (tile0 + rw) * kQuads * 64 + lane;
+    if (mine) {
 #pragma unroll
-      for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          o[(4 * d + i) * 64] = make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
-      if (h == 0) P.ml[(tile0 + rw) * 32 + l32] = make_float2(m, l);
+      for (int q = 0; q < kQuads; q++) {
+        const f32x16& v = acc[q / 4];
+        const int i = 4 * (q % 4);
+        put(q, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), l);
+      }
+      if (h == 0 && !whole) P.ml[(tile0 + rw) * 32 + l32] = make_float2(m, l);
     }
   } else {
     // the KW waves of each query tile join in LDS, in fixed order
@@ -606,7 +625,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       ew[w] = ml[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w].x - M);
       L = __builtin_fmaf(ml[w].y, ew[w], L);
     }
-    if (r0 < P.R) {
+    if (mine) {
 #pragma unroll
       for (int q = 0; q < kQuads / KW; q++) {
         float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -618,9 +637,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
           A.z = __builtin_fmaf(a.z, ew[w], A.z);
           A.w = __builtin_fmaf(a.w, ew[w], A.w);
         }
-        P.acc[((tile0 + rw) * kQuads + kw + KW * q) * 64 + lane] = A;
+        put(kw + KW * q, A, L);
       }
-      if (kw == 0 && h == 0) P.ml[(tile0 + rw) * 32 + l32] = make_float2(M, L);
+      if (kw == 0 && h == 0 && !whole) P.ml[(tile0 + rw) * 32 + l32] = make_float2(M, L);
     }
   }
 }
@@ -630,15 +649,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 // register quad of a tile of 32 query rows: lane l has four dims of row l % 32,
 // so every row's maximum and sums stay in its lane, and a load is 1 KB in a row.
 // Wave w joins chunks w, w + 4, .., 8 loads in flight, then the four waves join
-// in fixed order.  Rows of absent nodes are zeros; those of a sequence whose
-// rows do not fit its cache are NaN.
+// in fixed order.  Sequences in one chunk, and absent nodes, have their output.
 // grid: n_kv x D / 8 quads x tiles x sequences, KV head fastest, as the partial
 // kernel's workgroups: with 8 KV heads a head's chunks are joined on the XCD
 // whose L2 they were written through.
 template <int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint32_t n_tiles) {
   constexpr int kQuads = D / 8, kPer = 8;
-  typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ float4 pa[4][64];
   __shared__ float2 pm[4][64];
   uint32_t b = blockIdx.x;
@@ -651,6 +668,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t row = tile * 32 + (lane & 31);
   const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
+  if (n <= 1) return;
   const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
   const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.tiles + tile;
   float M = -INFINITY, L = 0.f;
@@ -691,28 +709,24 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
   const uint32_t t = row / P.G, g = row % P.G;
   const size_t node = static_cast<size_t>(seq) * P.n_tree + t;
   const uint4 w4 = *reinterpret_cast<const uint4*>(P.mask + node * kWholeMask);
-  float4u o;
-  if ((w4.x | w4.y | w4.z | w4.w) == 0) {
-    o = seq_fits(P, P.ctx_len[seq]) ? 0.f : __builtin_nanf("");
-  } else {
-    for (int w = 1; w < 4; w++) M = fmaxf(M, pm[w][lane].x);
-    L = 0.f;
-    o = 0.f;
-    for (int w = 0; w < 4; w++) {
-      const float2 ml = pm[w][lane];
-      if (ml.x == -INFINITY) continue;
-      const float ew = __builtin_amdgcn_exp2f(ml.x - M);
-      const float4 a = pa[w][lane];
-      L = __builtin_fmaf(ml.y, ew, L);
-      o[0] = __builtin_fmaf(a.x, ew, o[0]);
-      o[1] = __builtin_fmaf(a.y, ew, o[1]);
-      o[2] = __builtin_fmaf(a.z, ew, o[2]);
-      o[3] = __builtin_fmaf(a.w, ew, o[3]);
-    }
-    o = o / L;  // no key's score above -inf: 0 / 0, as the formula
+  if ((w4.x | w4.y | w4.z | w4.w) == 0) return;
+  for (int w = 1; w < 4; w++) M = fmaxf(M, pm[w][lane].x);
+  L = 0.f;
+  f32x4u o = 0.f;
+  for (int w = 0; w < 4; w++) {
+    const float2 ml = pm[w][lane];
+    if (ml.x == -INFINITY) continue;
+    const float ew = __builtin_amdgcn_exp2f(ml.x - M);
+    const float4 a = pa[w][lane];
+    L = __builtin_fmaf(ml.y, ew, L);
+    o[0] = __builtin_fmaf(a.x, ew, o[0]);
+    o[1] = __builtin_fmaf(a.y, ew, o[1]);
+    o[2] = __builtin_fmaf(a.z, ew, o[2]);
+    o[3] = __builtin_fmaf(a.w, ew, o[3]);
   }
-  *reinterpret_cast<float4u*>(P.out + node * P.n_heads * D + static_cast<size_t>(kvh * P.G + g) * D + 32 * (quad >> 2) +
-                              8 * (quad & 3) + 4 * h) = o;
+  // no key's score above -inf: 0 / 0, as the formula
+  *reinterpret_cast<f32x4u*>(P.out + node * P.n_heads * D + static_cast<size_t>(kvh * P.G + g) * D + 32 * (quad >> 2) +
+                             8 * (quad & 3) + 4 * h) = o / L;
 }
 
 // ------------------------------------------------------------------ launching
@@ -722,9 +736,16 @@ size_t al256(size_t v) { return (v + 255) / 256 * 256; }
 // (K and V are read once per 128 rows).
 int row_tiles(size_t R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
 
+// A cache of up to so many rows is one chunk: no partial results to join, no third
+// launch.  A call on 32 / 8 heads of 128, one chunk against several: 5 nodes (20
+// query rows a KV head, stages of 128 keys) 13.1 against 15.4 us at 300
+// positions, 14.6 against 15.5 at 480; 26 nodes (104 rows, stages of 64) 16.4
+// against 15.4 at 120, 20.7 against 15.7 at 300.
+size_t single_rows(int rw) { return rw == 1 ? 512 : 128; }
 struct Plan {
   int rw;
-  size_t G, R, n_rg, target, sparse, unit, max_slots;
+  size_t G, R, n_rg, target, sparse, unit, least, max_slots;
+  bool single;  // every sequence is one chunk
 };
 Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t max_ctx) {
   Plan p;
@@ -737,7 +758,9 @@ Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t
   const size_t per = n_kv * p.n_rg, cus = static_cast<size_t>(wh::cu_count());
   p.sparse = (cus + per - 1) / per;
   p.target = ((p.rw == 1 ? 1 : 2) * cus + per - 1) / per;
-  const size_t most = n_seqs * ((max_ctx + p.unit - 1) / p.unit);
+  p.single = max_ctx <= single_rows(p.rw);
+  p.least = p.single ? (max_ctx + p.unit - 1) / p.unit * p.unit : p.unit;
+  const size_t most = n_seqs * ((max_ctx + p.least - 1) / p.least);
   p.max_slots = p.target + n_seqs < most ? p.target + n_seqs : most;
   return p;
 }
@@ -777,6 +800,7 @@ Params fill(const Plan& p, size_t n_seqs, size_t n_tree, size_t n_heads, size_t 
   P.target = static_cast<uint32_t>(p.target);
   P.sparse = static_cast<uint32_t>(p.sparse);
   P.unit = static_cast<uint32_t>(p.unit);
+  P.least = static_cast<uint32_t>(p.least);
   P.tiles = static_cast<uint32_t>(p.n_rg * p.rw);
   P.scale = 1.0f / sqrtf(static_cast<float>(D));
   return P;
@@ -791,12 +815,12 @@ int launch_partial(const Params& P, hipStream_t s) {
 }
 
 template <int D>
-int launch_all(const Params& P, int rw, hipStream_t s) {
+int launch_all(const Params& P, const Plan& p, hipStream_t s) {
   const uint32_t n_groups = (P.n_heads + P.n_kv + kPrepHeads - 1) / kPrepHeads;
   tree_prepare_kernel<D><<<P.n_seqs * P.n_tree * n_groups + 1, kPrepThreads, 0, s>>>(P, n_groups);
   WH_LAUNCH_CHECK("tree attention prepare launch");
-  int st = rw == 1 ? launch_partial<D, 1>(P, s) : rw == 2 ? launch_partial<D, 2>(P, s) : launch_partial<D, 4>(P, s);
-  if (st) return st;
+  int st = p.rw == 1 ? launch_partial<D, 1>(P, s) : p.rw == 2 ? launch_partial<D, 2>(P, s) : launch_partial<D, 4>(P, s);
+  if (st || p.single) return st;
   const uint32_t n_tiles = (P.R + 31) / 32;
   tree_combine_kernel<D><<<P.n_kv * (D / 8) * n_tiles * P.n_seqs, 256, 0, s>>>(P, n_tiles);
   WH_LAUNCH_CHECK("tree attention combine launch");
@@ -830,7 +854,7 @@ int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t s)
   P.v_cache = static_cast<_Float16*>(a.v_cache);
   P.inv_freq = a.inv_freq;
   P.out = a.out;
-  return a.head_dim == 128 ? launch_all<128>(P, p.rw, s) : launch_all<64>(P, p.rw, s);
+  return a.head_dim == 128 ? launch_all<128>(P, p, s) : launch_all<64>(P, p, s);
 }
 
 }  // namespace wh
