@@ -493,7 +493,7 @@ KERNEL_SOURCE_GROUPS = {
 KERNEL_SOURCE_GROUPS["decode"] = tuple(sorted(set(sum(KERNEL_SOURCE_GROUPS.values(), ())) |
                                               {_C + "decode.hip", _C + "embed.hip"}))
 # verifying a tree of drafted tokens: attention, logits, acceptance and cache rows
-KERNEL_SOURCE_GROUPS["tree"] = (_C + "tree_attention.hip", _C + "tree.hip", _C + "logits.hip", _C + "tree.hpp",
+KERNEL_SOURCE_GROUPS["tree"] = (_C + "tree_attention.hip", _C + "tree_step.hip", _C + "tree.hip", _C + "logits.hip", _C + "tree.hpp",
                                 _C + "gemm_dev.hpp") + _COMMON
 GEMV_KERNEL_SOURCES = KERNEL_SOURCE_GROUPS["gemv"]
 PMC_PROFILE = ROOT / "profiles" / "gemv_q4_0_14336x4096_pmc.txt"

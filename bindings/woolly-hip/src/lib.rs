@@ -367,6 +367,10 @@ extern "C" {
                              k_cache: *mut c_void, v_cache: *mut c_void, max_ctx: usize, n_heads: usize,
                              n_kv_heads: usize, head_dim: usize, inv_freq: *const c_float, out: *mut c_float,
                              workspace: *mut c_void, workspace_bytes: usize, stream: wh_stream_t) -> c_int;
+    pub fn wh_llama_forward_tree_workspace_bytes(model: *const wh_llama_model, n_tree: usize) -> usize;
+    pub fn wh_llama_forward_tree(model: *const wh_llama_model, tokens: *const u32, parents: *const i32, n_tree: usize,
+                                 ctx_len: *const u32, x: *mut c_float, logits: *mut c_float, workspace: *mut c_void,
+                                 workspace_bytes: usize, stream: wh_stream_t) -> c_int;
     pub fn wh_logits_process_workspace_bytes(rules: *const wh_logits_rules, n_rows: usize, vocab: usize) -> usize;
     pub fn wh_logits_process(rules: *const wh_logits_rules, logits: *const c_float, ld: usize, n_rows: usize,
                              vocab: usize, out: *mut c_float, ld_out: usize, token: *mut u32,

@@ -518,6 +518,19 @@ WH_API int wh_attention_tree(const float* q, const float* k, const float* v, siz
                              size_t head_dim, const float* inv_freq, float* out, void* workspace,
                              size_t workspace_bytes, wh_stream_t stream);
 
+/* One step of the model for all nodes of one tree: x [n_tree][hidden] receives
+ * the nodes' last hidden states (x = the embedding rows of tokens, then every
+ * layer with wh_attention_tree), logits [n_tree][vocab] (may be null) the head's
+ * rows, the model's caches the nodes' k and v at rows *ctx_len .. .  tokens,
+ * parents and ctx_len (one number) are device memory, x is 16-byte aligned, the
+ * model has a token_embd table; rows of absent nodes are without meaning.  The
+ * workspace (256-byte aligned) holds wh_llama_forward_tree_workspace_bytes(..), 0
+ * for a model or tree that is not taken.  Launches only, as the decode step. */
+WH_API size_t wh_llama_forward_tree_workspace_bytes(const wh_llama_model* model, size_t n_tree);
+WH_API int wh_llama_forward_tree(const wh_llama_model* model, const uint32_t* tokens, const int32_t* parents,
+                                 size_t n_tree, const uint32_t* ctx_len, float* x, float* logits, void* workspace,
+                                 size_t workspace_bytes, wh_stream_t stream);
+
 /* What is done to logits before a token is chosen.  All arrays are device
  * memory; a zero-initialised member is left out, but repetition_penalty is 1
  * where nothing is wanted. */

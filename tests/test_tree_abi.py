@@ -143,3 +143,65 @@ def test_compact_refusals():
     assert compact(n_seqs=0, path=None) == _lib.WH_OK
     with pytest.raises(ValueError, match="2 K caches and 1 V caches"):
         ops.KvCaches([P, P], [P])
+
+
+def fake_model(**over):
+    layers = (_lib.wh_llama_layer * 2)()
+    for L in layers:
+        for name, _ in _lib.wh_llama_layer._fields_:
+            if not name.endswith("_type"):
+                setattr(L, name, P)
+    m = _lib.wh_llama_model()
+    m.type = 2
+    m.n_layers, m.hidden, m.n_heads, m.n_kv_heads, m.head_dim = 2, 256, 4, 2, 64
+    m.n_ff, m.max_ctx, m.vocab, m.eps = 512, 16, 300, 1e-5
+    m.rope_inv_freq, m.output_norm, m.output, m.output_type = P, P, P, 8
+    m.token_embd, m.token_embd_type = P, 1
+    m.layers = C.cast(layers, C.POINTER(_lib.wh_llama_layer))
+    for k, v in over.items():
+        if k.startswith("layer_"):
+            setattr(layers[1], k[6:], v)
+        else:
+            setattr(m, k, v)
+    return m, layers
+
+
+def forward(model, **over):
+    a = dict(tokens=P, parents=P, n_tree=26, ctx_len=P, x=P, logits=P, workspace=P, workspace_bytes=HUGE)
+    a.update(over)
+    return _lib.load().wh_llama_forward_tree(C.byref(model[0]), *a.values(), None)
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(head_dim=96), 2), (dict(n_heads=3), 2), (dict(hidden=0), 2), (dict(n_ff=0), 2), (dict(max_ctx=0), 2),
+    (dict(max_ctx=1 << 31), 2), (dict(hidden=272), 2), (dict(vocab=0), 2), (dict(vocab=1 << 30), 2), (dict(type=6), 1),
+    (dict(type=12, n_ff=544), 2), (dict(output_type=1), 1), (dict(output=None), 4), (dict(output_norm=None), 4),
+    (dict(token_embd=None), 4), (dict(token_embd_type=10), 1), (dict(rope_inv_freq=None), 4), (dict(layer_wv=None), 4),
+    (dict(layer_w_down=None), 4), (dict(layer_w_up_type=7), 1), (dict(layer_k_cache=P + 8), 4), (dict(layer_v_cache=None), 4),
+    (dict(layer_ffn_norm=None), 4), (dict(layer_attn_norm=P + 2), 4)])
+def test_forward_tree_models(over, status):
+    m = fake_model(**over)
+    assert forward(m) == status
+    assert b"llama_forward_tree" in _lib.load().wh_last_error()
+
+
+def test_forward_tree_arguments():
+    lib, m = _lib.load(), fake_model()
+    assert forward(m, n_tree=129) == _lib.WH_ERR_INVALID_SHAPE
+    assert forward(m, n_tree=0, tokens=None) == _lib.WH_OK
+    for name in ("tokens", "parents", "ctx_len", "x"):
+        assert forward(m, **{name: None}) == _lib.WH_ERR_INVALID_ARGUMENT, name
+        assert forward(m, **{name: P + 2}) == _lib.WH_ERR_INVALID_ARGUMENT, name
+    assert forward(m, x=P + 8) == _lib.WH_ERR_INVALID_ARGUMENT
+    assert forward(m, workspace=P + 128) == _lib.WH_ERR_INVALID_ARGUMENT
+    need = lib.wh_llama_forward_tree_workspace_bytes(C.byref(m[0]), 26)
+    assert need > ops.attention_tree_workspace_bytes(1, 26, 4, 2, 64, 16)
+    assert forward(m, workspace_bytes=need - 1) == _lib.WH_ERR_BUFFER_TOO_SMALL
+    assert f"needed {need} bytes".encode() in lib.wh_last_error()
+    assert forward(m, workspace=None) == _lib.WH_ERR_BUFFER_TOO_SMALL
+    assert lib.wh_llama_forward_tree_workspace_bytes(C.byref(m[0]), 0) == 0
+    assert lib.wh_llama_forward_tree_workspace_bytes(C.byref(m[0]), 129) == 0
+    assert lib.wh_llama_forward_tree_workspace_bytes(None, 5) == 0
+    assert lib.wh_llama_forward_tree(None, P, P, 5, P, P, P, P, HUGE, None) == _lib.WH_ERR_INVALID_ARGUMENT
+    # without logits the head is not looked at
+    assert forward(fake_model(output=None), logits=None, workspace_bytes=0) == _lib.WH_ERR_BUFFER_TOO_SMALL

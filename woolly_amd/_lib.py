@@ -232,6 +232,8 @@ SIGNATURES = {
     "wh_attention_tree_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
     "wh_attention_tree": (_int, [_f32p, _f32p, _f32p, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz,
                                  _f32p, _f32p, _vp, _sz, _vp]),
+    "wh_llama_forward_tree_workspace_bytes": (_sz, [C.POINTER(wh_llama_model), _sz]),
+    "wh_llama_forward_tree": (_int, [C.POINTER(wh_llama_model), _vp, _vp, _sz, _vp, _f32p, _f32p, _vp, _sz, _vp]),
     "wh_logits_process_workspace_bytes": (_sz, [C.POINTER(wh_logits_rules), _sz, _sz]),
     "wh_logits_process": (_int, [C.POINTER(wh_logits_rules), _f32p, _sz, _sz, _sz, _f32p, _sz, _vp, _vp, _sz, _vp]),
     "wh_tree_accept": (_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

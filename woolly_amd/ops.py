@@ -508,3 +508,20 @@ class LlamaModel:
         _lib.check(_lib.load().wh_llama_decode_step(C.byref(self.model), pos, _p(x),
                                                     _p(logits) or None, _p(workspace), workspace_bytes,
                                                     _s(stream)))
+
+    def tree_workspace_bytes(self, n_tree: int) -> int:
+        return int(_lib.load().wh_llama_forward_tree_workspace_bytes(C.byref(self.model), n_tree))
+
+    def forward_tree(self, tokens, parents, n_tree: int, ctx_len, x, logits, workspace, workspace_bytes: int,
+                     stream: Stream | None = None) -> None:
+        """One step for all nodes of a tree of drafted tokens (wh_llama_forward_tree):
+        x [n_tree][hidden] and logits [n_tree][vocab] (may be None); the caches take
+        the nodes' rows behind the first *ctx_len."""
+        _lib.check(_lib.load().wh_llama_forward_tree(C.byref(self.model), _p(tokens), _p(parents), n_tree, _p(ctx_len),
+                                                     _p(x), _p(logits) or None, _p(workspace), workspace_bytes,
+                                                     _s(stream)))
+
+    def kv_caches(self) -> KvCaches:
+        """The layers' caches for kv_cache_compact."""
+        layers = self._keep[0]
+        return KvCaches([L["k_cache"] for L in layers], [L["v_cache"] for L in layers])
