@@ -508,7 +508,7 @@ WH_API int wh_embedding_lookup(int type, const void* table, size_t vocab, size_t
  * absent node's out row is zeros and its cache row stays as it was.  A sequence
  * with ctx_len + n_tree > max_ctx stores nothing, and its out rows are NaN.
  * head_dim 64 or 128, n_heads (at most 1024) a multiple of n_kv_heads, at most
- * 1024 sequences.  Caches and workspace are 16-byte aligned; the workspace holds
+ * 1024 sequences and 2^32 - 1 cache rows in all.  Caches and workspace are 16-byte aligned; the workspace holds
  * wh_attention_tree_workspace_bytes(..), 0 for shapes that are not taken. */
 WH_API size_t wh_attention_tree_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads,
                                                 size_t head_dim, size_t max_ctx);

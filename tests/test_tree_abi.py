@@ -18,7 +18,7 @@ def attention(**over):
 
 @pytest.mark.parametrize("over", [dict(head_dim=96), dict(head_dim=0), dict(n_kv_heads=0), dict(n_heads=30), dict(n_heads=0),
                                   dict(n_heads=1032, ldq=HUGE), dict(n_tree=129), dict(n_seqs=1025), dict(max_ctx=0),
-                                  dict(max_ctx=1 << 31), dict(ldq=4095), dict(ldkv=1023)])
+                                  dict(max_ctx=1 << 31), dict(max_ctx=1 << 30, n_seqs=4), dict(ldq=4095), dict(ldkv=1023)])
 def test_attention_shapes(over):
     assert attention(**over) == _lib.WH_ERR_INVALID_SHAPE
     assert b"attention_tree" in _lib.load().wh_last_error()
@@ -41,7 +41,7 @@ def test_attention_workspace_and_empty_calls():
     assert attention(n_seqs=0, q=None) == _lib.WH_OK
     assert attention(n_tree=0, q=None) == _lib.WH_OK
     for bad in ((0, 26, 32, 8, 128, 4096), (2, 0, 32, 8, 128, 4096), (2, 129, 32, 8, 128, 4096), (1025, 1, 32, 8, 128, 4096),
-                (2, 26, 32, 8, 80, 4096), (2, 26, 30, 8, 128, 4096), (2, 26, 32, 8, 128, 1 << 31)):
+                (2, 26, 32, 8, 80, 4096), (2, 26, 30, 8, 128, 4096), (2, 26, 32, 8, 128, 1 << 31), (4, 26, 32, 8, 128, 1 << 30)):
         assert ops.attention_tree_workspace_bytes(*bad) == 0
     # more room, more nodes or more sequences never need less
     assert ops.attention_tree_workspace_bytes(2, 26, 32, 8, 128, 64) <= need

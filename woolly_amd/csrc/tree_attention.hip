@@ -81,19 +81,21 @@ __device__ __forceinline__ bool seq_fits(const Params& P, uint32_t ctx) {
   return ctx <= P.max_ctx && P.n_tree <= P.max_ctx - ctx;
 }
 
-// Inclusive prefix sums over the workgroup's 256 threads; red: 4 words of LDS.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* red) {
+// Inclusive prefix sum over the workgroup's 256 threads, and their total; red: 4
+// words of LDS.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const unsigned long long up = __shfl_up(v, off, 64);
+    const uint32_t up = __shfl_up(v, off, 64);
     if (lane >= off) v += up;
   }
-  __syncthreads();
+  whd::lds_barrier();
   if (lane == 63) red[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; w++) v += red[w];
-  return v;
+  whd::lds_barrier();
+  const uint32_t a = red[0], b = red[1], c = red[2], d = red[3];
+  total = a + b + c + d;
+  return v + (wave > 0 ? a : 0) + (wave > 1 ? b : 0) + (wave > 2 ? c : 0);
 }
 
 // Cuts the sequences into chunks of one length, a multiple of a stage of the
@@ -102,47 +104,39 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
 // give every CU two workgroups, whose matrix and vector work overlap; while the
 // chunks would be shorter than kDeepChunk, `sparse` chunks, one workgroup per CU,
 // do: half the partial results to write and to join.
-// Thread t plans sequences [t per, (t + 1) per); first: LDS [n_seqs + 1].
+// Thread t plans sequences [t per, (t + 1) per); first: LDS [n_seqs + 1].  All rows
+// together number less than 2^32 (checked by the host).
 constexpr uint32_t kDeepChunk = 512;
-__device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long* red) {
+__device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
   const uint32_t t = threadIdx.x;
   const uint32_t per = (P.n_seqs + kPrepThreads - 1) / kPrepThreads;
   const uint32_t s0 = min(t * per, P.n_seqs), s1 = min(s0 + per, P.n_seqs);
-  auto rows = [&](uint32_t s) -> uint32_t {
-    const uint32_t ctx = P.ctx_len[s];
-    if (!seq_fits(P, ctx)) return 0;
-    for (uint32_t i = 0; i < P.n_tree; i++)
-      if (P.parents[s * P.n_tree + i] == -1) return ctx + P.n_tree;
-    return 0;  // every node is absent
-  };
-  unsigned long long mine = 0;
+  uint32_t mine = 0;
   for (uint32_t s = s0; s < s1; s++) {
-    const uint32_t n = rows(s);
+    const uint32_t ctx = P.ctx_len[s];
+    const int32_t* parents = P.parents + static_cast<size_t>(s) * P.n_tree;
+    bool any = parents[0] == -1;  // a sequence whose nodes are all absent has nothing to do
+    for (uint32_t i = 1; i < P.n_tree && !any; i++) any = parents[i] == -1;
+    const uint32_t n = any && seq_fits(P, ctx) ? ctx + P.n_tree : 0;
     first[s] = n;
     mine += n;
   }
-  mine = block_scan(mine, red);
-  __shared__ unsigned long long total;
-  if (t == kPrepThreads - 1) total = mine;
-  __syncthreads();
-  unsigned long long even = (total + P.target - 1) / P.target;
-  if (even < kDeepChunk) even = min<unsigned long long>((total + P.sparse - 1) / P.sparse, kDeepChunk);
-  const uint32_t chunk = max(static_cast<uint32_t>((even + P.unit - 1) / P.unit) * P.unit, P.least);
+  uint32_t total, used;
+  block_scan(mine, red, total);
+  uint32_t even = (total + P.target - 1) / P.target;
+  if (even < kDeepChunk) even = min((total + P.sparse - 1) / P.sparse, kDeepChunk);
+  const uint32_t chunk = max((even + P.unit - 1) / P.unit * P.unit, P.least);
   uint32_t n = 0;
   for (uint32_t s = s0; s < s1; s++) n += (first[s] + chunk - 1) / chunk;
-  uint32_t at = static_cast<uint32_t>(block_scan(n, red)) - n;
+  uint32_t at = block_scan(n, red, used) - n;
   for (uint32_t s = s0; s < s1; s++) {
     const uint32_t c = (first[s] + chunk - 1) / chunk;
     first[s] = at;
     P.first[s] = at;
     at += c;
   }
-  if (t == kPrepThreads - 1) {
-    first[P.n_seqs] = at;
-    P.first[P.n_seqs] = at;
-  }
-  __syncthreads();
-  const uint32_t used = first[P.n_seqs];
+  if (t == 0) P.first[P.n_seqs] = used;
+  whd::lds_barrier();
   for (uint32_t y = t; y < P.max_slots; y += kPrepThreads) {
     uint32_t lo = 0, hi = P.n_seqs;  // the last sequence whose first slot is at most y
     while (hi - lo > 1) {
@@ -151,8 +145,8 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, unsigned long long
     }
     uint4 slot = make_uint4(P.n_seqs, 0, 0, 0);
     if (y < used) {
-      const uint32_t n = P.ctx_len[lo] + P.n_tree, c0 = (y - first[lo]) * chunk;
-      slot = make_uint4(lo, c0, min(c0 + chunk, n), n);
+      const uint32_t rows = P.ctx_len[lo] + P.n_tree, c0 = (y - first[lo]) * chunk;
+      slot = make_uint4(lo, c0, min(c0 + chunk, rows), rows);
     }
     P.slots[y] = slot;
   }
@@ -166,7 +160,7 @@ constexpr int kPrepHeads = 2 * kPrepThreads / 64;
 template <int D>
 __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params P, uint32_t n_groups) {
   __shared__ uint32_t first[wh::kMaxTreeSeqs + 1];
-  __shared__ unsigned long long red[kPrepThreads / 64];
+  __shared__ uint32_t red[kPrepThreads / 64];
   if (blockIdx.x == P.n_seqs * P.n_tree * n_groups) {
     plan_chunks(P, first, red);
     return;
@@ -862,6 +856,7 @@ int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t s)
 WH_API size_t wh_attention_tree_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads,
                                                 size_t head_dim, size_t max_ctx) {
   if (n_seqs == 0 || n_tree == 0 || n_seqs > wh::kMaxTreeSeqs || n_tree > wh::kMaxTreeNodes || max_ctx >> 31 ||
+      n_seqs * max_ctx >> 32 ||
       !wh::tree_attention_shape_ok(n_heads, n_kv_heads, head_dim))
     return 0;
   return wh::tree_attention_workspace_bytes(n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx);
@@ -880,6 +875,9 @@ WH_API int wh_attention_tree(const float* q, const float* k, const float* v, siz
                          n_seqs, wh::kMaxTreeNodes, wh::kMaxTreeSeqs);
   if (max_ctx == 0 || max_ctx >> 31)
     return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: max_ctx = %zu out of range", max_ctx);
+  if (n_seqs * max_ctx >> 32)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: %zu sequences of %zu rows (together less than 2^32)", n_seqs,
+                         max_ctx);
   if (ldq < n_heads * head_dim || ldkv < n_kv_heads * head_dim)
     return wh::set_error(WH_ERR_INVALID_SHAPE, "attention_tree: row strides %zu, %zu below the rows' %zu, %zu elements",
                          ldq, ldkv, n_heads * head_dim, n_kv_heads * head_dim);
