@@ -185,6 +185,35 @@ def test_what_a_row_does_not_see(gpu, d, n_tree, ctx):
     run(c, f"unseen rows d {d} tree {n_tree} ctx {ctx}")
 
 
+@pytest.mark.parametrize("n_tree", [5, 12, 30, 64])
+@pytest.mark.parametrize("room", [0, 4000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinities_in_the_cache_count(gpu, n_tree, room, d):
+    """Infinities and NaN that the cache itself holds are seen by every row: a dim with infinities of one sign is that
+    infinity, of both NaN; a NaN in k makes every row of its KV head NaN."""
+    ctx = 900 if room else 100
+    c = Case(1, n_tree, 8, 2, d, [ctx], room=room, seed=d + n_tree)
+    c.vc[0, 3, 0, 5] = np.inf
+    c.vc[0, 40, 0, 9] = -np.inf
+    c.vc[0, 41, 0, 9] = -np.inf
+    c.vc[0, ctx - 1, 0, 11] = np.inf
+    c.vc[0, ctx - 70, 0, 11] = -np.inf
+    c.vc[0, ctx - 3, 0, 20] = np.nan
+    c.vc[0, 17, 0, d - 1] = np.nan
+    c.kc[0, 64, 1, 2] = np.nan
+    want, _, _, _ = c.expect()
+    assert np.isposinf(want[0, :, 0, 5]).all() and np.isneginf(want[0, :, 1, 9]).all() and np.isnan(want[0, :, 2, 11]).all()
+    run(c, f"infinities d {d} tree {n_tree} room {room}")
+
+
+def test_largest_queries(gpu):
+    """Queries of 1e36 over keys of 1e-4: the scale of a row has the whole range of f32's exponents."""
+    c = Case(1, 6, 4, 2, 128, [90], seed=3, qscale=1e36)
+    c.kc *= np.float16(1e-4)
+    c.k *= np.float32(1e-4)
+    run(c, "q times 1e36")
+
+
 def test_sequence_that_does_not_fit(gpu):
     """ctx_len + n_tree > max_ctx: NaN for that sequence, nothing stored, the others as ever."""
     c = Case(4, 8, 4, 2, 128, [20, 60, 61, 30], room=0, seed=2)

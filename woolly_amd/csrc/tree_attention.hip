@@ -64,7 +64,7 @@ struct Params {
   float* qscale;        // [n_seqs][n_kv][R]
   _Float16* qlimb;      // [n_seqs][n_kv][R][2][D]
   // partial results of a slot, KV head and tile of 32 query rows
-  float2* ml;           // [max_slots][n_kv][tiles][32] (maximum in powers of 2, sum)
+  float2* ml;           // [max_slots][n_kv][tiles][32] (maximum, sum)
   float4* acc;          // [max_slots][n_kv][tiles][D / 8][64]: the registers of the lanes, as in the product
 };
 
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
       // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element
       // to 2^-22 of itself or 2^-38 of the largest
       int e = 0;
-      if (mx > 0.f && mx < INFINITY) e = min(max(13 - ilogbf(mx), -100), 100);
+      if (mx > 0.f && mx < INFINITY) e = min(13 - ilogbf(mx), 100);
       a = ldexpf(a, e);
       b = ldexpf(b, e);
       const size_t qrow = (static_cast<size_t>(s) * P.n_kv + hh / P.G) * P.R + t * P.G + hh % P.G;
@@ -393,7 +393,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     qh[j] = *reinterpret_cast<const half8*>(q);
     ql[j] = *reinterpret_cast<const half8*>(q + D);
   }
-  const float qs = P.qscale[qrow];
+  // scores are qs times s, in powers of 2; maxima are kept as s, so that the
+  // largest of a row is exactly 0 however large it is
+  const float qs = P.qscale[qrow], lazy = kLazyMax / qs;
   uint32_t tm[kWholeMask] = {};
   f32x16 acc[DT];
 #pragma unroll
@@ -401,7 +403,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
   float m = -INFINITY, l = 0.f;
-  bool odd = false;  // an edge tile of this wave held infinities or NaN in V
+  bool odd = false;  // V holds infinities or NaN
 
   // N 32-key tiles, KW tiles apart.  kt, vt: LDS addresses of the first one's first
   // K and V row.  Edge (N = 1): the tile may reach beyond the cache into the nodes'
@@ -480,10 +482,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     float mt = s[0][0];
 #pragma unroll
     for (int i = 1; i < 16 * N; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
-    mt = swap_max(mt) * qs;
-    if (__ballot(mt > m + kLazyMax)) {
+    mt = swap_max(mt);
+    if (__ballot(mt > m + lazy)) {
       const float mn = fmaxf(m, mt);
-      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * qs);
       l *= al;
 #pragma unroll
       for (int d = 0; d < DT; d++)
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         for (int i = 0; i < 16; i++) acc[d][i] *= al;
       m = mn;
     }
-    const float mb = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
+    const float mb = m == -INFINITY ? 0.f : m;
     float lt[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < 2 * N; ks++) {
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         float p[2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][8 * (ks % 2) + i + k], qs, mb));
+          p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][8 * (ks % 2) + i + k] - mb, qs, kPScaleLog2));
           lt[(i + k) & 3] += p[k];
         }
         split2(p[0], p[1], ph, pl, i);
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     const uint32_t kt = turn(st), to = 32 * kw * 2 * D;
     tiles(0, kt + to, kt + S::kTileBytes + to, std::false_type{}, std::integral_constant<int, S::TILES>{});
   }
-  if (st < n_stages) {
+  {
     const uint4 w = *reinterpret_cast<const uint4*>(P.mask + (static_cast<size_t>(seq) * P.n_tree + r / P.G) * kWholeMask);
     tm[0] = w.x, tm[1] = w.y, tm[2] = w.z, tm[3] = w.w;
   }
@@ -545,26 +547,55 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
   }
   l = swap_sum(l);
+  // Infinities and NaN of V count for the query rows that see them, and for no
+  // other.  The edge tiles took them out (0 * inf would have spread a NaN), in the
+  // others they made infinities and NaN of these sums, of either kind (the lo limb
+  // of a weight may be below 0).  Every weight is above 0, so such an element's
+  // sum is that of the infinities and NaN alone: the rows are read again for them.
+  {
+    float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) zero[i & 3] = __builtin_fmaf(acc[d][i], 0.f, zero[i & 3]);
+    odd |= __ballot(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.f)) != 0;
+  }
   if (odd) {
-    // infinities and NaN of V count for the query rows that see them, and for no
-    // other (0 * inf in the products would have spread a NaN): every weight is
-    // above 0, so an element becomes what their sum is.  The rows are read again.
-    for (uint32_t key = c0 + n_inner * SK; key < c1; key++) {
-      if ((key - c0) / 32 % KW != static_cast<uint32_t>(kw)) continue;
-      const uint32_t node = key - ctx;  // wraps for the cache's rows
-      uint32_t w = tm[0];
 #pragma unroll
-      for (int i = 1; i < kWholeMask; i++)
-        if (node >> 5 == static_cast<uint32_t>(i)) w = tm[i];
-      if (key >= ctx && !((w >> (node & 31)) & 1u)) continue;
-      const _Float16* v = reinterpret_cast<const _Float16*>(vbase + key * RS);
+    for (int d = 0; d < DT; d++)
 #pragma unroll
-      for (int d = 0; d < DT; d++)
+      for (int i = 0; i < 16; i++)
+        if (!(fabsf(acc[d][i]) < INFINITY)) acc[d][i] = 0.f;
+    for (uint32_t base = c0 + 32 * kw; base < c1; base += 32 * KW) {
+      // lane l looks through half of row l / 2
+      const uint32_t look = min(base + lane / 2, c1 - 1);
+      const uint4* half = reinterpret_cast<const uint4*>(vbase + look * RS + (lane & 1) * D);
+      bool bad = false;
+      for (int j = 0; j < D / 16; j++) {
+        const uint4 w = half[j];
+        for (const uint32_t x : {w.x, w.y, w.z, w.w}) bad |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
+      }
+      unsigned long long rows_bad = __ballot(bad);
+      rows_bad = (rows_bad | rows_bad >> 1) & 0x5555555555555555ull;  // bit 2 k: row k
+      while (rows_bad) {
+        const uint32_t key = base + __builtin_ctzll(rows_bad) / 2;
+        rows_bad &= rows_bad - 1;
+        if (key >= c1) break;  // the last row, looked at again
+        const uint32_t node = key - ctx;  // wraps for the cache's rows
+        uint32_t w = tm[0];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float x = static_cast<float>(v[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
-          if (!(fabsf(x) < INFINITY)) acc[d][i] += x;
-        }
+        for (int i = 1; i < kWholeMask; i++)
+          if (node >> 5 == static_cast<uint32_t>(i)) w = tm[i];
+        if (key >= ctx && !((w >> (node & 31)) & 1u)) continue;
+        const _Float16* v = reinterpret_cast<const _Float16*>(vbase + key * RS);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float x = static_cast<float>(v[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
+            if (!(fabsf(x) < INFINITY)) acc[d][i] += x;
+          }
+      }
     }
   }
 
@@ -616,7 +647,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
 #pragma unroll
     for (int w = 0; w < KW; w++) {
-      ew[w] = ml[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w].x - M);
+      ew[w] = ml[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[w].x - M) * qs);
       L = __builtin_fmaf(ml[w].y, ew[w], L);
     }
     if (mine) {
@@ -639,7 +670,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 }
 
 // ------------------------------------------------------------------ combine
-// out = sum_c acc_c 2^{m_c - M} / sum_c l_c 2^{m_c - M}.  A workgroup takes one
+// out = sum_c acc_c w_c / sum_c l_c w_c, w_c = 2^{(m_c - M) qs}.  A workgroup takes one
 // register quad of a tile of 32 query rows: lane l has four dims of row l % 32,
 // so every row's maximum and sums stay in its lane, and a load is 1 KB in a row.
 // Wave w joins chunks w, w + 4, .., 8 loads in flight, then the four waves join
@@ -661,6 +692,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
   const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t row = tile * 32 + (lane & 31);
+  const float qs = P.qscale[(static_cast<size_t>(seq) * P.n_kv + kvh) * P.R + min(row, P.R - 1)];
   const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
   if (n <= 1) return;
   const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
@@ -682,13 +714,13 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
       if (c + 4 * j >= n) ml[j].x = -INFINITY;
       mx = fmaxf(mx, ml[j].x);
     }
-    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mx);
+    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mx) * qs);
     M = mx;
     if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
 #pragma unroll
     for (int j = 0; j < kPer; j++) {
       if (ml[j].x == -INFINITY) continue;
-      const float ew = __builtin_amdgcn_exp2f(ml[j].x - M);
+      const float ew = __builtin_amdgcn_exp2f((ml[j].x - M) * qs);
       L = __builtin_fmaf(ml[j].y, ew, L);
       A.x = __builtin_fmaf(a[j].x, ew, A.x);
       A.y = __builtin_fmaf(a[j].y, ew, A.y);
@@ -710,7 +742,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
   for (int w = 0; w < 4; w++) {
     const float2 ml = pm[w][lane];
     if (ml.x == -INFINITY) continue;
-    const float ew = __builtin_amdgcn_exp2f(ml.x - M);
+    const float ew = __builtin_amdgcn_exp2f((ml.x - M) * qs);
     const float4 a = pa[w][lane];
     L = __builtin_fmaf(ml.y, ew, L);
     o[0] = __builtin_fmaf(a.x, ew, o[0]);
