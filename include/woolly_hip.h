@@ -509,7 +509,8 @@ WH_API int wh_embedding_lookup(int type, const void* table, size_t vocab, size_t
  * with ctx_len + n_tree > max_ctx stores nothing, and its out rows are NaN.
  * head_dim 64 or 128, n_heads (at most 1024) a multiple of n_kv_heads, at most
  * 1024 sequences and 2^32 - 1 cache rows in all.  Caches and workspace are 16-byte aligned; the workspace holds
- * wh_attention_tree_workspace_bytes(..), 0 for shapes that are not taken. */
+ * wh_attention_tree_workspace_bytes(..), 0 for shapes that are not taken; calls
+ * that overlap on one workspace race. */
 WH_API size_t wh_attention_tree_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads,
                                                 size_t head_dim, size_t max_ctx);
 WH_API int wh_attention_tree(const float* q, const float* k, const float* v, size_t ldq, size_t ldkv,
@@ -525,7 +526,8 @@ WH_API int wh_attention_tree(const float* q, const float* k, const float* v, siz
  * parents and ctx_len (one number) are device memory, x is 16-byte aligned, the
  * model has a token_embd table; rows of absent nodes are without meaning.  The
  * workspace (256-byte aligned) holds wh_llama_forward_tree_workspace_bytes(..), 0
- * for a model or tree that is not taken.  Launches only, as the decode step. */
+ * for a model or tree that is not taken; calls that overlap on one workspace
+ * race.  Launches only, as the decode step. */
 WH_API size_t wh_llama_forward_tree_workspace_bytes(const wh_llama_model* model, size_t n_tree);
 WH_API int wh_llama_forward_tree(const wh_llama_model* model, const uint32_t* tokens, const int32_t* parents,
                                  size_t n_tree, const uint32_t* ctx_len, float* x, float* logits, void* workspace,
@@ -557,11 +559,12 @@ typedef struct wh_logits_rules {
  * each rounded to f32 by itself, then -inf where the mask's bit is clear.  Tokens
  * are counted in the row's history and, with a tree, on the path from the cache
  * to the row's node, itself included; ids >= vocab are passed over.
- * out (may be logits itself, with the same stride, or null) receives the rows,
+ * out (logits itself, with the same stride, or memory apart from it, or null) receives the rows,
  * token (may be null) the lowest token of each row's largest logit: one that is
  * neither NaN nor -inf, or 0xFFFFFFFF where there is none (an id that
  * wh_llama_forward_token answers with NaN).  The row of an absent node is left
- * as it was, its token 0xFFFFFFFF.  The workspace is needed for token only. */
+ * as it was, its token 0xFFFFFFFF.  The workspace (8-byte aligned) is needed for
+ * token only; calls that overlap on one workspace race. */
 WH_API size_t wh_logits_process_workspace_bytes(const wh_logits_rules* rules, size_t n_rows, size_t vocab);
 WH_API int wh_logits_process(const wh_logits_rules* rules, const float* logits, size_t ld, size_t n_rows, size_t vocab,
                              float* out, size_t ld_out, uint32_t* token, void* workspace, size_t workspace_bytes,

@@ -206,6 +206,19 @@ def test_infinities_in_the_cache_count(gpu, n_tree, room, d):
     run(c, f"infinities d {d} tree {n_tree} room {room}")
 
 
+@pytest.mark.parametrize("heads,kv,d,n_tree", [(8, 2, 128, 6), (8, 2, 64, 20), (8, 1, 128, 30)])
+def test_a_chunk_of_nothing_but_nan(gpu, heads, kv, d, n_tree):
+    """The nodes lie in a chunk of their own (the cache is whole chunks), in which node 0 sees itself alone: its k is
+    NaN, so are its row and every row below it, and a sibling's row is not."""
+    c = Case(1, n_tree, heads, kv, d, [1024], room=3000, shape="star", seed=d)
+    c.parents[0, 1] = -1  # a second root, and a node below it
+    c.parents[0, 2] = 1
+    c.views()[1][0, 0, :, 3] = np.nan
+    want, _, _, _ = c.expect()
+    assert np.isnan(want[0, 0]).all() and np.isfinite(want[0, 1:3]).all() and np.isnan(want[0, 3:]).all()
+    run(c, f"chunk of NaN {heads}/{kv}x{d} tree {n_tree}")
+
+
 def test_largest_queries(gpu):
     """Queries of 1e36 over keys of 1e-4: the scale of a row has the whole range of f32's exponents."""
     c = Case(1, 6, 4, 2, 128, [90], seed=3, qscale=1e36)
@@ -361,3 +374,19 @@ def test_same_bits_again(gpu):
         c.dev["ws"].fill(0x55)
         c.launch()
         assert np.array_equal(c.results()[0].view(np.uint32), first.view(np.uint32))
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams with workspaces of their own, several in flight on each, do not disturb each other."""
+    streams = [Stream(), Stream()]
+    cases = [Case(2, 13, 8, 2, 128, [1500, 200], seed=40).upload(), Case(1, 64, 16, 4, 64, [3000], seed=41).upload()]
+    synchronize()
+    for _ in range(5):
+        for c, s in zip(cases, streams):
+            c.launch(s)
+    for s in streams:
+        s.synchronize()
+    for i, c in enumerate(cases):
+        c.check(f"stream {i}")
+    for s in streams:
+        s.destroy()

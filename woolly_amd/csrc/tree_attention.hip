@@ -8,12 +8,22 @@
 //   cache row ctx_len + t = f16(k), f16(v)
 //   s_j   = (q . k_j) / sqrt(d)   for j < ctx_len and j = ctx_len + a, a in A(t)
 //   out_t = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},  m = max_j s_j
-// Three launches:
-//   1. prepare: one workgroup per node rotates its q heads into f16 hi + lo
-//      limbs, stores its k and v in the cache and writes its ancestor mask; one
-//      more workgroup cuts the sequences into chunks of equal length
+// Three launches (two where the caches are short):
+//   1. prepare: a wave per two heads of a node rotates q into f16 hi + lo limbs,
+//      stores k and v in the cache and writes the node's ancestor mask; one more
+//      workgroup cuts the sequences into chunks of equal length
 //   2. partial: one workgroup per (chunk, KV head, group of 32 RW query rows)
-//   3. combine: one wave per query row merges its chunks
+//   3. combine: one workgroup per 32 query rows and 8 dims joins their chunks
+//
+// What bounds it.  Short and middle contexts: the three launches' dependent loads
+// and their ends.  26 nodes at 4070 positions, 32 / 8 heads of 128 (17.8 MB: 3.7 us
+// at the 4.8 TB/s of a large copy): 4.4 + 13.9 + 4.8 us, of the partial kernel's
+// 13.9 some 3 until the first data is there, 6 for 4 tiles a wave, 3 for writing
+// 13.6 MB of partial results.  8 sequences of 16 nodes up to 8100, 32 / 4 heads of
+// 64: 5.3 + 13.2 + 4.3.  5 nodes at 300 of 312 rows: 3.7 + 10.0.  Long contexts: the
+// matrix cores.  64 nodes at 131000: 275 GFLOP of limb products in 250 us, 1.1
+// PFLOP/s; a large f16 library product reaches 1.15 on this card, where the clock
+// falls under such work (440 k cycles, 60 % of them with a product under way).
 //
 // The angle is formed and reduced in 64 bits: in 32 bits p_t * inv_freq is off
 // by up to p_t 2^-24 radians, 0.008 at position 131072.  k is rotated in
@@ -710,17 +720,16 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
       a[j] = P.acc[(s * kQuads + quad) * 64 + lane];
     }
 #pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      if (c + 4 * j >= n) ml[j].x = -INFINITY;
-      mx = fmaxf(mx, ml[j].x);
-    }
+    for (int j = 0; j < kPer; j++)
+      if (c + 4 * j < n) mx = fmaxf(mx, ml[j].x);
     const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mx) * qs);
     M = mx;
     if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
 #pragma unroll
     for (int j = 0; j < kPer; j++) {
-      if (ml[j].x == -INFINITY) continue;
-      const float ew = __builtin_amdgcn_exp2f((ml[j].x - M) * qs);
+      if (c + 4 * j >= n) break;
+      // a chunk without a maximum has no weight, but NaN of its scores stay
+      const float ew = ml[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[j].x - M) * qs);
       L = __builtin_fmaf(ml[j].y, ew, L);
       A.x = __builtin_fmaf(a[j].x, ew, A.x);
       A.y = __builtin_fmaf(a[j].y, ew, A.y);
@@ -741,8 +750,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
   f32x4u o = 0.f;
   for (int w = 0; w < 4; w++) {
     const float2 ml = pm[w][lane];
-    if (ml.x == -INFINITY) continue;
-    const float ew = __builtin_amdgcn_exp2f((ml.x - M) * qs);
+    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * qs);
     const float4 a = pa[w][lane];
     L = __builtin_fmaf(ml.y, ew, L);
     o[0] = __builtin_fmaf(a.x, ew, o[0]);
@@ -759,7 +767,9 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
 size_t al256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Query tiles per workgroup: as many as the rows of one KV head fill, up to 4
-// (K and V are read once per 128 rows).
+// (K and V are read once per 128 rows).  On the 104 rows of 26 nodes at 4070
+// positions 1, 2 and 4 tiles take 15.9, 15.7 and 16.0 us; on the 128 rows of 8
+// ragged sequences 19.0, 18.0 and 16.0.
 int row_tiles(size_t R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
 
 // A cache of up to so many rows is one chunk: no partial results to join, no third
