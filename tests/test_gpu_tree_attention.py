@@ -132,6 +132,13 @@ def test_many_sequences(gpu):
     run(Case(300, 3, 4, 2, 64, lens, seed=5), "300 sequences")
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_batches(gpu, d):
+    """Enough nodes, heads and tiles that waves take more of them each; sequences of one chunk and of several."""
+    lens = [0, 3, 40, 1500, 64, 700, 17, 130, 1, 90, 400, 33]
+    run(Case(12, 81, 30, 6, d, lens, room=60, shape="padded", seed=d), f"large batch d {d}")
+
+
 @pytest.mark.parametrize("pad", [1, 4, 64])
 def test_row_strides(gpu, pad):
     run(Case(2, 9, 6, 2, 64, [50, 200], pad=pad, seed=pad), f"rows padded by {pad}")

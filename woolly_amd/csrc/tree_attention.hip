@@ -162,12 +162,12 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
   }
 }
 
-// grid: (n_seqs * n_tree) nodes x n_groups groups of 8 heads (the q heads, then
-// the KV heads), then one workgroup for the chunks.  A wave takes two heads and
-// asks for their rows before it looks at the tree: the launch is as long as its
-// dependent loads.
-constexpr int kPrepHeads = 2 * kPrepThreads / 64;
-template <int D>
+// grid: (n_seqs * n_tree) nodes x n_groups groups of 4 N heads (the q heads, then
+// the KV heads), then one workgroup for the chunks.  A wave takes N heads and asks
+// for their rows before it looks at the tree.  With few nodes N = 2: the launch is
+// as long as its dependent loads; with many N = 8, which share the walk and the
+// angles (22 sequences of 81 nodes, 80 + 16 heads: 68 -> 37 us).
+template <int D, int N>
 __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params P, uint32_t n_groups) {
   __shared__ uint32_t first[wh::kMaxTreeSeqs + 1];
   __shared__ uint32_t red[kPrepThreads / 64];
@@ -181,10 +181,10 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
   const uint32_t tid = threadIdx.x, lane = tid & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t i = lane % (D / 2);
-  const uint32_t h0 = group * kPrepHeads + 2 * wave, n_slots = P.n_heads + P.n_kv;
-  float x[2], y[2], vx[2] = {}, vy[2] = {};
+  const uint32_t h0 = (group * (kPrepThreads / 64) + wave) * N, n_slots = P.n_heads + P.n_kv;
+  float x[N], y[N], vx[N] = {}, vy[N] = {};
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
+  for (int u = 0; u < N; u++) {
     const uint32_t hh = min(h0 + u, n_slots - 1);
     const bool is_q = hh < P.n_heads;
     const float* src = is_q ? P.q + row * P.ldq + static_cast<size_t>(hh) * D
@@ -207,8 +207,14 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
     P.mask[row * kWholeMask + tid] = present ? static_cast<uint32_t>(w) : 0u;
   }
   const double angle = static_cast<double>(ctx + path.depth) * static_cast<double>(inv);
+  // q: the angle in turns, whole turns dropped in 64 bits
+  const double turns = angle * 0.15915494309189535;
+  float qsn, qcs;
+  sincospif(2.0f * static_cast<float>(turns - rint(turns)), &qsn, &qcs);
+  double sn = 0, cs = 0;
+  if (h0 + N > P.n_heads) sincos(angle, &sn, &cs);
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
+  for (int u = 0; u < N; u++) {
     const uint32_t hh = h0 + u;
     if (hh >= n_slots) break;
     if (hh < P.n_heads) {
@@ -219,11 +225,7 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
         o[i] = fill;
         o[i + D / 2] = fill;
       }
-      // q: the angle in turns, whole turns dropped in 64 bits
-      const double turns = angle * 0.15915494309189535;
-      float sn, cs;
-      sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-      float a = present ? x[u] * cs - y[u] * sn : 0.f, b = present ? x[u] * sn + y[u] * cs : 0.f;
+      float a = present ? x[u] * qcs - y[u] * qsn : 0.f, b = present ? x[u] * qsn + y[u] * qcs : 0.f;
       const float mx = whd::wave_max(fmaxf(fabsf(a), fabsf(b)));
       // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element
       // to 2^-22 of itself or 2^-38 of the largest
@@ -244,8 +246,6 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
     } else if (present && lane < D / 2) {
       // k and v into the cache row of the node
       const size_t at = ((static_cast<size_t>(s) * P.max_ctx + ctx + t) * P.n_kv + (hh - P.n_heads)) * D;
-      double sn, cs;
-      sincos(angle, &sn, &cs);
       P.k_cache[at + i] = stored(x[u] * cs - y[u] * sn);
       P.k_cache[at + i + D / 2] = stored(x[u] * sn + y[u] * cs);
       P.v_cache[at + i] = static_cast<_Float16>(vx[u]);
@@ -680,87 +680,95 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
 }
 
 // ------------------------------------------------------------------ combine
-// out = sum_c acc_c w_c / sum_c l_c w_c, w_c = 2^{(m_c - M) qs}.  A workgroup takes one
-// register quad of a tile of 32 query rows: lane l has four dims of row l % 32,
-// so every row's maximum and sums stay in its lane, and a load is 1 KB in a row.
-// Wave w joins chunks w, w + 4, .., 8 loads in flight, then the four waves join
-// in fixed order.  Sequences in one chunk, and absent nodes, have their output.
-// grid: n_kv x D / 8 quads x tiles x sequences, KV head fastest, as the partial
+// out = sum_c acc_c w_c / sum_c l_c w_c, w_c = 2^{(m_c - M) qs}.  An item is one register
+// quad of a tile of 32 query rows: lane l has four dims of row l % 32, so every
+// row's maximum and sums stay in its lane, and a load is 1 KB in a row.  Wave w
+// joins chunks w, w + W, .., 8 loads in flight, then the W waves join in fixed
+// order.  Sequences in one chunk, and absent nodes, have their output.
+// With few items W = 4 waves take one, with many W = 1 (a wave joins all chunks of
+// its quad, and the workgroups stride over the items: 22 sequences
+// of 81 nodes and 80 heads, most in one chunk: 28 -> 12 us).
+// Items: n_kv x D / 8 quads x tiles x sequences, KV head fastest, as the partial
 // kernel's workgroups: with 8 KV heads a head's chunks are joined on the XCD
 // whose L2 they were written through.
-template <int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint32_t n_tiles) {
-  constexpr int kQuads = D / 8, kPer = 8;
-  __shared__ float4 pa[4][64];
-  __shared__ float2 pm[4][64];
-  uint32_t b = blockIdx.x;
-  const uint32_t kvh = b % P.n_kv;
-  b /= P.n_kv;
-  const uint32_t quad = b % kQuads;
-  b /= kQuads;
-  const uint32_t tile = b % n_tiles, seq = b / n_tiles;
+template <int D, int W>
+__global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint32_t n_tiles, uint32_t n_items) {
+  constexpr int kQuads = D / 8, kPer = 8, kGroup = 4 / W;  // quads per workgroup
+  __shared__ float4 pa[W > 1 ? W : 1][64];
+  __shared__ float2 pm[W > 1 ? W : 1][64];
   const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t row = tile * 32 + (lane & 31);
-  const float qs = P.qscale[(static_cast<size_t>(seq) * P.n_kv + kvh) * P.R + min(row, P.R - 1)];
-  const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
-  if (n <= 1) return;
   const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
-  const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.tiles + tile;
-  float M = -INFINITY, L = 0.f;
-  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t c = wave; c < n; c += 4 * kPer) {
-    float2 ml[kPer];
-    float4 a[kPer];
-    float mx = M;
-#pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      const size_t s = at + min(c + 4 * j, n - 1) * step;  // a chunk past the last has no weight
-      ml[j] = P.ml[s * 32 + (lane & 31)];
-      a[j] = P.acc[(s * kQuads + quad) * 64 + lane];
+  for (uint32_t item = blockIdx.x; item < n_items; item += gridDim.x) {
+    uint32_t b = item;
+    const uint32_t kvh = b % P.n_kv;
+    b /= P.n_kv;
+    const uint32_t quad = b % (kQuads / kGroup) * kGroup + wave / W;
+    b /= kQuads / kGroup;
+    const uint32_t tile = b % n_tiles, seq = b / n_tiles;
+    const uint32_t row = tile * 32 + (lane & 31);
+    const float qs = P.qscale[(static_cast<size_t>(seq) * P.n_kv + kvh) * P.R + min(row, P.R - 1)];
+    const uint32_t c0 = P.first[seq], n = P.first[seq + 1] - c0;
+    if (n <= 1) {
+      if constexpr (W > 1) return;
+      continue;
     }
+    const size_t at = (static_cast<size_t>(c0) * P.n_kv + kvh) * P.tiles + tile;
+    float M = -INFINITY, L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto join = [&](float2 ml, float4 a) {
+      // a part without a maximum has no weight, but NaN of its scores stay
+      const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * qs);
+      L = __builtin_fmaf(ml.y, ew, L);
+      A.x = __builtin_fmaf(a.x, ew, A.x);
+      A.y = __builtin_fmaf(a.y, ew, A.y);
+      A.z = __builtin_fmaf(a.z, ew, A.z);
+      A.w = __builtin_fmaf(a.w, ew, A.w);
+    };
+    for (uint32_t c = wave % W; c < n; c += W * kPer) {
+      float2 ml[kPer];
+      float4 a[kPer];
+      float mx = M;
 #pragma unroll
-    for (int j = 0; j < kPer; j++)
-      if (c + 4 * j < n) mx = fmaxf(mx, ml[j].x);
-    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mx) * qs);
-    M = mx;
-    if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
+      for (int j = 0; j < kPer; j++) {
+        const size_t s = at + min(c + W * j, n - 1) * step;
+        ml[j] = P.ml[s * 32 + (lane & 31)];
+        a[j] = P.acc[(s * kQuads + quad) * 64 + lane];
+      }
 #pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      if (c + 4 * j >= n) break;
-      // a chunk without a maximum has no weight, but NaN of its scores stay
-      const float ew = ml[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[j].x - M) * qs);
-      L = __builtin_fmaf(ml[j].y, ew, L);
-      A.x = __builtin_fmaf(a[j].x, ew, A.x);
-      A.y = __builtin_fmaf(a[j].y, ew, A.y);
-      A.z = __builtin_fmaf(a[j].z, ew, A.z);
-      A.w = __builtin_fmaf(a[j].w, ew, A.w);
+      for (int j = 0; j < kPer; j++)
+        if (c + W * j < n) mx = fmaxf(mx, ml[j].x);
+      const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mx) * qs);
+      M = mx;
+      if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        if (c + W * j >= n) break;
+        join(ml[j], a[j]);
+      }
     }
+    if constexpr (W > 1) {
+      pa[wave][lane] = A;
+      pm[wave][lane] = make_float2(M, L);
+      whd::lds_barrier();
+      if (wave == 0) {
+        for (int w = 1; w < W; w++) M = fmaxf(M, pm[w][lane].x);
+        L = 0.f;
+        A = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < W; w++) join(pm[w][lane], pa[w][lane]);
+      }
+    }
+    if ((W == 1 || wave == 0) && row < P.R) {
+      const uint32_t t = row / P.G, g = row % P.G;
+      const size_t node = static_cast<size_t>(seq) * P.n_tree + t;
+      const uint4 w4 = *reinterpret_cast<const uint4*>(P.mask + node * kWholeMask);
+      // no key's score above -inf: 0 / 0, as the formula
+      if ((w4.x | w4.y | w4.z | w4.w) != 0)
+        *reinterpret_cast<f32x4u*>(P.out + node * P.n_heads * D + static_cast<size_t>(kvh * P.G + g) * D +
+                                   32 * (quad >> 2) + 8 * (quad & 3) + 4 * h) = f32x4u{A.x, A.y, A.z, A.w} / L;
+    }
+    if constexpr (W > 1) return;  // one item per workgroup
   }
-  pa[wave][lane] = A;
-  pm[wave][lane] = make_float2(M, L);
-  whd::lds_barrier();
-  if (wave != 0 || row >= P.R) return;
-  const uint32_t t = row / P.G, g = row % P.G;
-  const size_t node = static_cast<size_t>(seq) * P.n_tree + t;
-  const uint4 w4 = *reinterpret_cast<const uint4*>(P.mask + node * kWholeMask);
-  if ((w4.x | w4.y | w4.z | w4.w) == 0) return;
-  for (int w = 1; w < 4; w++) M = fmaxf(M, pm[w][lane].x);
-  L = 0.f;
-  f32x4u o = 0.f;
-  for (int w = 0; w < 4; w++) {
-    const float2 ml = pm[w][lane];
-    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * qs);
-    const float4 a = pa[w][lane];
-    L = __builtin_fmaf(ml.y, ew, L);
-    o[0] = __builtin_fmaf(a.x, ew, o[0]);
-    o[1] = __builtin_fmaf(a.y, ew, o[1]);
-    o[2] = __builtin_fmaf(a.z, ew, o[2]);
-    o[3] = __builtin_fmaf(a.w, ew, o[3]);
-  }
-  // no key's score above -inf: 0 / 0, as the formula
-  *reinterpret_cast<f32x4u*>(P.out + node * P.n_heads * D + static_cast<size_t>(kvh * P.G + g) * D + 32 * (quad >> 2) +
-                             8 * (quad & 3) + 4 * h) = o / L;
 }
 
 // ------------------------------------------------------------------ launching
@@ -850,15 +858,30 @@ int launch_partial(const Params& P, hipStream_t s) {
   return WH_OK;
 }
 
+// Workgroups of 8 heads from which on 32 heads take one.
+constexpr size_t kManyHeads = 4096;
+
 template <int D>
 int launch_all(const Params& P, const Plan& p, hipStream_t s) {
-  const uint32_t n_groups = (P.n_heads + P.n_kv + kPrepHeads - 1) / kPrepHeads;
-  tree_prepare_kernel<D><<<P.n_seqs * P.n_tree * n_groups + 1, kPrepThreads, 0, s>>>(P, n_groups);
+  const uint32_t nodes = P.n_seqs * P.n_tree, heads = P.n_heads + P.n_kv;
+  if (static_cast<size_t>(nodes) * heads < 8 * kManyHeads) {
+    const uint32_t n_groups = (heads + 7) / 8;
+    tree_prepare_kernel<D, 2><<<nodes * n_groups + 1, kPrepThreads, 0, s>>>(P, n_groups);
+  } else {
+    const uint32_t n_groups = (heads + 31) / 32;
+    tree_prepare_kernel<D, 8><<<nodes * n_groups + 1, kPrepThreads, 0, s>>>(P, n_groups);
+  }
   WH_LAUNCH_CHECK("tree attention prepare launch");
   int st = p.rw == 1 ? launch_partial<D, 1>(P, s) : p.rw == 2 ? launch_partial<D, 2>(P, s) : launch_partial<D, 4>(P, s);
   if (st || p.single) return st;
   const uint32_t n_tiles = (P.R + 31) / 32;
-  tree_combine_kernel<D><<<P.n_kv * (D / 8) * n_tiles * P.n_seqs, 256, 0, s>>>(P, n_tiles);
+  const size_t cus = static_cast<size_t>(wh::cu_count()), items = static_cast<size_t>(P.n_kv) * (D / 8) * n_tiles * P.n_seqs;
+  if (items <= 8 * cus) {
+    tree_combine_kernel<D, 4><<<static_cast<unsigned>(items), 256, 0, s>>>(P, n_tiles, static_cast<uint32_t>(items));
+  } else {
+    const size_t grid = items / 4 < 8 * cus ? items / 4 : 8 * cus;
+    tree_combine_kernel<D, 1><<<static_cast<unsigned>(grid), 256, 0, s>>>(P, n_tiles, static_cast<uint32_t>(items / 4));
+  }
   WH_LAUNCH_CHECK("tree attention combine launch");
   return WH_OK;
 }
