@@ -90,6 +90,10 @@ def test_tree_logits_are_the_paths_logits(gpu, name):
     for i, tok in enumerate(prompt):
         want = m.step(tok, i)
         assert rel_l2(got[i], want) <= 1e-4, (i, rel_l2(got[i], want))
+    # the decode step goes on from rows that a tree step stored
+    x1, lg1 = DeviceBuffer(4 * m.hidden), DeviceBuffer(4 * m.vocab)
+    m.tree.forward_token(up(np.array([33], np.uint32))[0], t, x1, lg1, m.ws, m.wsz)
+    assert rel_l2(down(lg1, np.float32, m.vocab), m.step(33, t)) <= 1e-4
     parents = np.array([-1, 0, 0, 1, 1, 2, 3, 3, -2, 8, 6, 5], np.int32)
     n = len(parents)
     tokens = rng.integers(0, 400, n)
