@@ -111,14 +111,16 @@ class Case:
     def run(self, write=True, pick=True):
         rules = self.rules()
         xb = up(self.x)[0]
-        ob = DeviceBuffer(4 * self.rows * self.ldo) if write else None
-        tb = DeviceBuffer(4 * self.rows) if pick else None
-        if write:
-            ob.fill(0xEE)
+        ob = DeviceBuffer(4 * self.rows * self.ldo + 256) if write else None
+        tb = DeviceBuffer(4 * self.rows + 256) if pick else None
         wsz = ops.logits_process_workspace_bytes(rules, self.rows, self.v) if pick else 0
-        ws = DeviceBuffer(max(wsz, 8))
-        ws.fill(0xFF)
+        ws = DeviceBuffer(wsz + 256)
+        for b in (ob, tb, ws):
+            if b:
+                b.fill(0xEE)
         self.launch(rules, xb, ob, tb, ws, wsz)
+        for b, size in ((ob, 4 * self.rows * self.ldo), (tb, 4 * self.rows), (ws, wsz)):
+            assert not b or (down(b, np.uint8, 256, offset=size) == 0xEE).all(), "behind a buffer"
         out = down(ob, np.float32, self.rows * self.ldo).reshape(self.rows, self.ldo) if write else None
         token = down(tb, np.uint32, self.rows) if pick else None
         assert np.array_equal(down(xb, np.uint32, self.x.size), self.x.view(np.uint32).ravel()), "the input changed"
@@ -160,10 +162,10 @@ def test_penalties_that_do_nothing_or_reward(gpu, rep, freq, pres):
 
 
 def test_long_history(gpu):
-    """A token that occurs tens of thousands of times, in a history of 200000."""
+    """A token that occurs tens of thousands of times, in a history of 200000; a length beyond the row is the row."""
     c = Case(1, 0, 40000, 200_000, 0, False, seed=6, freq=0.001)
     c.hist[0, ::3] = 12345
-    c.hist_len[:] = 200_000
+    c.hist_len[:] = 200_050
     c.run()
 
 

@@ -44,11 +44,12 @@ class Case:
         self.dev = dict(q=up(self.q)[0], k=up(self.k)[0], v=up(self.v)[0], parents=up(self.parents)[0],
                         ctx=up(np.array(self.lens, np.uint32))[0], kc=up(flat(self.kc))[0], vc=up(flat(self.vc))[0],
                         inv=up(self.inv)[0])
-        self.dev["out"] = DeviceBuffer(4 * self.n * self.t * self.h * self.d)
+        self.dev["out"] = DeviceBuffer(4 * self.n * self.t * self.h * self.d + 256)  # and a guard
         self.dev["out"].fill(0xEE)
         self.wsz = ops.attention_tree_workspace_bytes(self.n, self.t, self.h, self.kv, self.d, self.max_ctx)
-        self.dev["ws"] = DeviceBuffer(self.wsz)
-        self.dev["ws"].fill(0xFF)  # NaN
+        self.dev["ws"] = DeviceBuffer(self.wsz + 256)
+        self.dev["ws"].fill(0xFF)  # NaN, and a guard
+        self.guard = self.dev["ws"]
         return self
 
     def launch(self, stream=None):
@@ -59,6 +60,9 @@ class Case:
 
     def results(self):
         out = down(self.dev["out"], np.float32, self.n * self.t * self.h * self.d).reshape(self.n, self.t, self.h, self.d)
+        assert (down(self.dev["out"], np.uint8, 256, offset=out.nbytes) == 0xEE).all(), "behind the output"
+        if self.dev["ws"] is self.guard:
+            assert (down(self.guard, np.uint8, 256, offset=self.wsz) == 0xFF).all(), "behind the workspace"
         caches = []
         for name in ("kc", "vc"):
             c = down(self.dev[name], np.float16, (self.n * self.max_ctx + 1) * self.kv * self.d).reshape(-1, self.kv, self.d)
@@ -126,10 +130,11 @@ def test_room_behind_the_rows(gpu, heads, kv, d, n_tree, room):
         f"{heads}/{kv}x{d} tree {n_tree} room {room}")
 
 
-def test_many_sequences(gpu):
+@pytest.mark.parametrize("n,n_tree", [(300, 3), (1024, 1)])
+def test_many_sequences(gpu, n, n_tree):
     rng = np.random.default_rng(3)
-    lens = [int(v) for v in rng.integers(0, 90, 300)]
-    run(Case(300, 3, 4, 2, 64, lens, seed=5), "300 sequences")
+    lens = [int(v) for v in rng.integers(0, 90, n)]
+    run(Case(n, n_tree, 4, 2, 64, lens, seed=5), f"{n} sequences")
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -379,6 +384,7 @@ def test_same_bits_again(gpu):
     first = c.results()[0]
     for _ in range(3):
         c.dev["ws"].fill(0x55)
+        c.guard = None
         c.launch()
         assert np.array_equal(c.results()[0].view(np.uint32), first.view(np.uint32))
 

@@ -5,7 +5,7 @@
 // Neither moves enough to be bound by memory: a walk reads 1.5 KB at most and a
 // step keeps a few rows of each layer.  Both are one launch whose latency is
 // that of its dependent loads: 1.6 us for one walk over 26 nodes, 3.6 for 256
-// over 64; 4.8 us for 7 rows in 32 layers, 5.8 for 16 sequences in 24.
+// over 64; 3.8 us for 7 rows in 32 layers, 4.0 for 16 sequences in 24.
 #include "tree.hpp"
 
 namespace {
@@ -75,8 +75,9 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(const AcceptParams P) {
 // Layers of one launch: their cache pointers are kernel arguments.
 constexpr int kCompactLayers = 64;
 constexpr int kCompactBatch = 8;
+typedef uint32_t piece16 __attribute__((ext_vector_type(4)));  // arrays of HIP's uint4 end up in scratch memory here
 struct CompactParams {
-  uint4* cache[2 * kCompactLayers];
+  piece16* cache[2 * kCompactLayers];
   const uint32_t* path;
   const uint32_t* n_accepted;
   const uint32_t* ctx_len;
@@ -95,22 +96,22 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(const CompactParams P) 
   if (n > P.n_tree || n > after || after > P.max_ctx) return;
   const uint32_t first = after - n;
   if (c >= P.row16) return;
-  uint4* base = P.cache[blockIdx.x] + (static_cast<size_t>(s) * P.max_ctx + first) * P.row16 + c;
+  piece16* base = P.cache[blockIdx.x] + (static_cast<size_t>(s) * P.max_ctx + first) * P.row16 + c;
   const uint32_t* path = P.path + static_cast<size_t>(s) * P.n_tree;
   for (uint32_t i0 = 0; i0 < n; i0 += kCompactBatch) {
-    uint32_t from[kCompactBatch];
-    uint4 v[kCompactBatch];
+    piece16 v[kCompactBatch];
+    bool moved[kCompactBatch];
 #pragma unroll
     for (int j = 0; j < kCompactBatch; j++) {
       const uint32_t i = i0 + j;
-      const uint32_t p = i < n ? path[i] : i;
-      // a row that stays, or that the cache does not hold, is not moved
-      from[j] = p > i && p < P.n_tree && static_cast<size_t>(first) + p < P.max_ctx ? p : i;
-      if (from[j] != i) v[j] = base[static_cast<size_t>(from[j]) * P.row16];
+      const uint32_t p = i < n ? path[i] : 0;
+      // a row that stays, or that the cache does not hold, is not moved: its load takes row 0
+      moved[j] = p > i && p < P.n_tree && static_cast<size_t>(first) + p < P.max_ctx;
+      v[j] = base[static_cast<size_t>(moved[j] ? p : 0) * P.row16];
     }
 #pragma unroll
     for (int j = 0; j < kCompactBatch; j++)
-      if (from[j] != i0 + j) base[static_cast<size_t>(i0 + j) * P.row16] = v[j];
+      if (moved[j]) base[static_cast<size_t>(i0 + j) * P.row16] = v[j];
   }
 }
 
@@ -168,8 +169,8 @@ WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, siz
   for (size_t l0 = 0; l0 < n_layers; l0 += kCompactLayers) {
     const size_t n = n_layers - l0 < kCompactLayers ? n_layers - l0 : kCompactLayers;
     for (size_t l = 0; l < n; l++) {
-      P.cache[2 * l] = static_cast<uint4*>(k_caches[l0 + l]);
-      P.cache[2 * l + 1] = static_cast<uint4*>(v_caches[l0 + l]);
+      P.cache[2 * l] = static_cast<piece16*>(k_caches[l0 + l]);
+      P.cache[2 * l + 1] = static_cast<piece16*>(v_caches[l0 + l]);
     }
     const dim3 grid(static_cast<unsigned>(2 * n), static_cast<unsigned>(n_seqs), (P.row16 + 255) / 256);
     kv_compact_kernel<<<grid, 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(P);
