@@ -123,6 +123,13 @@ def compact(k=(P, P), v=(P, P), **over):
     return _lib.load().wh_kv_cache_compact(*a.values(), None)
 
 
+@pytest.mark.parametrize("k, v", [((P, P + 64), (P + 128, P)), ((P, P + 64), (P + 128, P + 128)), ((P, P), (P + 64, P + 128)),
+                                  ((P, P + 64), (P, P + 128)), ((P, P + 64), (P + 64, P + 128))])
+def test_compact_refuses_a_cache_named_twice(k, v):
+    assert compact(k=k, v=v) == _lib.WH_ERR_INVALID_ARGUMENT
+    assert b"named twice" in _lib.load().wh_last_error()
+
+
 def test_compact_refusals():
     for over in (dict(n_kv_heads=1, head_dim=4), dict(head_dim=0), dict(n_tree=129), dict(n_seqs=65536), dict(max_ctx=0),
                  dict(max_ctx=1 << 31), dict(n_kv_heads=1 << 20, head_dim=1 << 12)):

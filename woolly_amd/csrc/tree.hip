@@ -159,6 +159,14 @@ WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, siz
     if (!k_caches[l] || !v_caches[l] || !wh::aligned(k_caches[l], 16) || !wh::aligned(v_caches[l], 16))
       return wh::set_error(WH_ERR_INVALID_ARGUMENT,
                            "kv_cache_compact: layer %zu caches must be non-null and 16-byte aligned", l);
+  // rows of a cache named twice would be moved twice at once
+  for (size_t l = 0; l < n_layers; l++) {
+    bool twice = k_caches[l] == v_caches[l];
+    for (size_t i = 0; i < l; i++)
+      twice |= k_caches[i] == k_caches[l] || k_caches[i] == v_caches[l] || v_caches[i] == k_caches[l] ||
+               v_caches[i] == v_caches[l];
+    if (twice) return wh::set_error(WH_ERR_INVALID_ARGUMENT, "kv_cache_compact: a cache of layer %zu is named twice", l);
+  }
   CompactParams P{};
   P.path = path;
   P.n_accepted = n_accepted;
