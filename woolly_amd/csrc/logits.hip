@@ -17,12 +17,15 @@
 // row adds the path's tokens, applies everything and reduces the highest token;
 // a second small launch joins the chunks of a row.  Counting and the choice of a
 // bias entry use integer LDS atomics (add, max): their order does not change the
-// result.  Many rows are bound by memory: 64 nodes x 128256 (66.7 MB) take 19.5 us,
+// result.  Many rows are bound by memory: 64 nodes x 128256 (66.7 MB) take 19.3 us,
 // 3.9 TB/s once the launch is under way, whether a workgroup takes 2048, 4096 or
-// 8192 tokens (20.0, 19.3, 19.6 us; 2 rows of them: one row 22, four 22, eight 37).
+// 8192 tokens (before the next: 20.0, 19.3, 19.6 us); 2 rows of them each (call
+// 20.3 us; one row 22.6, four 23.4).  The rows go out past the L2, which holds
+// nothing of them for anyone else and had them to write back when the kernel ended
+// (21.0 us; 16 x 128256 10.6 against 9.5); loads past it gain nothing (20.4).
 // Long histories, which every chunk reads, favour large chunks: 16 x 128256 with
-// up to 20000 tokens each 14.2, 11.2 and 10.0 us.  One row of 32000 is the launch's
-// latency: 5.8 us.
+// up to 20000 tokens each 14.2, 11.2 and 10.0 us, now 9.5.  One row of 32000 is the
+// launch's latency: 5.8 us.
 #include "tree.hpp"
 
 namespace {
@@ -31,6 +34,7 @@ constexpr int kThreads = 1024;
 constexpr int kChunk = 8192;  // tokens of a row per workgroup
 constexpr int kPer = kChunk / kThreads;
 constexpr uint32_t kNoToken = 0xFFFFFFFFu;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct Params {
   const float* logits;
@@ -233,7 +237,7 @@ __global__ __launch_bounds__(kThreads, 8) void logits_kernel(const Params P) {
           for (int j = 0; j < kPer; j += 4) {
             const uint32_t a = at(j);
             if (a + 4 <= n) {
-              *reinterpret_cast<float4*>(o + a) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+              __builtin_nontemporal_store(f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]}, reinterpret_cast<f32x4*>(o + a));
             } else {
 #pragma unroll
               for (int k = 0; k < 4; k++)
