@@ -774,11 +774,20 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
 // ------------------------------------------------------------------ launching
 size_t al256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Query tiles per workgroup: as many as the rows of one KV head fill, up to 4
-// (K and V are read once per 128 rows).  On the 104 rows of 26 nodes at 4070
-// positions 1, 2 and 4 tiles take 15.9, 15.7 and 16.0 us; on the 128 rows of 8
-// ragged sequences 19.0, 18.0 and 16.0.
-int row_tiles(size_t R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
+// Query tiles per workgroup: as many as the rows of one KV head fill, up to 2 or 4.
+// With 4, K and V are read once per 128 rows; with 2, the workgroups that fill the
+// CUs are half as many chunks, so half the partial results.  2 are taken where all
+// rows the caches hold make chunks of up to kDeepChunk keys, one workgroup per CU.
+// A call with 32 / 8 heads of 128, 2 against 4: 26 nodes (104 query rows) at 2000,
+// 4070, 8100 positions 18.3 / 20.0, 20.3 / 22.1, 24.6 / 25.1 us (there 2 are taken),
+// at 16000 32.6 / 32.0; 64 nodes at 1000, 4070 20.2 / 21.3, 27.2 / 28.4, at 16000,
+// 131000 49.1 / 48.3, 292 / 276; 128 nodes at 1000 25.4 / 29.0, at 4070 37.4 / 36.4;
+// 8 sequences of 16 nodes up to 8100, 32 / 4 heads of 64 23.0 / 22.2.
+int row_tiles(size_t R, size_t n_kv, size_t cache_rows) {
+  if (R <= 64) return R <= 32 ? 1 : 2;
+  const size_t per = n_kv * ((R + 63) / 64), chunks = (static_cast<size_t>(wh::cu_count()) + per - 1) / per;
+  return cache_rows <= kDeepChunk * chunks ? 2 : 4;
+}
 
 // A cache of up to so many rows is one chunk: no partial results to join, no third
 // launch.  A call on 32 / 8 heads of 128, one chunk against several: 5 nodes (20
@@ -795,7 +804,7 @@ Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t
   Plan p;
   p.G = n_heads / n_kv;
   p.R = n_tree * p.G;
-  p.rw = row_tiles(p.R);
+  p.rw = row_tiles(p.R, n_kv, n_seqs * max_ctx);
   p.n_rg = (p.R + 32 * p.rw - 1) / (32 * p.rw);
   p.unit = p.rw == 1 ? 128 : 64;
   // one workgroup per CU with 128 KB of stages, two with 64 KB
