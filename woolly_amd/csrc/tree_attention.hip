@@ -774,44 +774,57 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
 // ------------------------------------------------------------------ launching
 size_t al256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Query tiles per workgroup: as many as the rows of one KV head fill, up to 2 or 4.
-// With 4, K and V are read once per 128 rows; with 2, the workgroups that fill the
-// CUs are half as many chunks, so half the partial results.  2 are taken where all
-// rows the caches hold make chunks of up to kDeepChunk keys, one workgroup per CU.
-// A call with 32 / 8 heads of 128, 2 against 4: 26 nodes (104 query rows) at 2000,
-// 4070, 8100 positions 18.3 / 20.0, 20.3 / 22.1, 24.6 / 25.1 us (there 2 are taken),
-// at 16000 32.6 / 32.0; 64 nodes at 1000, 4070 20.2 / 21.3, 27.2 / 28.4, at 16000,
-// 131000 49.1 / 48.3, 292 / 276; 128 nodes at 1000 25.4 / 29.0, at 4070 37.4 / 36.4;
-// 8 sequences of 16 nodes up to 8100, 32 / 4 heads of 64 23.0 / 22.2.
-int row_tiles(size_t R, size_t n_kv, size_t cache_rows) {
-  if (R <= 64) return R <= 32 ? 1 : 2;
-  const size_t per = n_kv * ((R + 63) / 64), chunks = (static_cast<size_t>(wh::cu_count()) + per - 1) / per;
-  return cache_rows <= kDeepChunk * chunks ? 2 : 4;
+// A cache of up to so many rows is one chunk: no partial results to join, no third
+// launch.  A call, one chunk against several: 32 / 8 heads of 128, 5 nodes (20 query
+// rows a KV head) at 300, 480 positions 13.2 / 15.4, 14.7 / 15.2 us, 100 sequences of
+// them at 480 36.6 / 40.9; 26 nodes (104 rows) at 200, 360 13.1 / 15.3, 16.1 / 15.5; 32
+// / 4 heads of 64, 10 nodes at 700 13.0 / 15.1, 64 nodes 15.6 / 15.8.  Workgroups of two
+// or four tiles, whose waves have all keys to go through: 26 nodes at 120, 300 16.4 /
+// 15.4, 20.7 / 15.7.
+size_t single_rows(int rw, size_t R, size_t D) { return rw > 1 ? 128 : D == 64 ? 768 : R <= 32 ? 512 : 384; }
+
+// Query tiles per workgroup: 1, 2 or 4.  With 4, K and V are read once per 128 rows;
+// with fewer, the waves share the keys, and the workgroups that fill the CUs are a
+// half or a quarter as many chunks, with as many fewer partial results.  So fewer are
+// taken where the caches are short: one chunk a sequence with a tile per workgroup, or
+// chunks of up to 384 (1 tile) or 512 keys (2 tiles), fill the CUs at most once.  A call with
+// 32 / 8 heads of 128, fewer against 4 tiles: 26 nodes (104 query rows) at 200, 1000
+// positions (1 tile) 13.1 / 16.2, 17.0 / 17.4 us, at 4070, 8100 (2) 20.3 / 22.1, 24.6 /
+// 25.1, beyond at 16000 (2) 32.6 / 32.0; 64 nodes at 60 (1) 12.8 / 18.5, at 1000 (2)
+// 20.2 / 21.3, beyond at 16000 (2) 49.1 / 48.3 and at 131000 292 / 276; 4 sequences of
+// 40 nodes at 200, 4070 (1, 2) 16.2 / 19.6, 28.8 / 31.7.
+int row_tiles(size_t R, size_t D, size_t n_kv, size_t n_seqs, size_t max_ctx) {
+  auto fits = [&](size_t rows, size_t keys) {
+    const size_t chunks = n_seqs * ((max_ctx + keys - 1) / keys);
+    return R <= rows || chunks * n_kv * ((R + rows - 1) / rows) <= static_cast<size_t>(wh::cu_count());
+  };
+  const size_t one = single_rows(1, R, D);
+  return fits(32, 384) || (max_ctx <= one && fits(32, one)) ? 1 : fits(64, kDeepChunk) ? 2 : 4;
 }
 
-// A cache of up to so many rows is one chunk: no partial results to join, no third
-// launch.  A call on 32 / 8 heads of 128, one chunk against several: 5 nodes (20
-// query rows a KV head, stages of 128 keys) 13.1 against 15.4 us at 300
-// positions, 14.6 against 15.5 at 480; 26 nodes (104 rows, stages of 64) 16.4
-// against 15.4 at 120, 20.7 against 15.7 at 300.
-size_t single_rows(int rw) { return rw == 1 ? 512 : 128; }
 struct Plan {
   int rw;
   size_t G, R, n_rg, target, sparse, unit, least, max_slots;
   bool single;  // every sequence is one chunk
 };
-Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t max_ctx) {
+Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t D, size_t max_ctx) {
   Plan p;
   p.G = n_heads / n_kv;
   p.R = n_tree * p.G;
-  p.rw = row_tiles(p.R, n_kv, n_seqs * max_ctx);
+  p.rw = row_tiles(p.R, D, n_kv, n_seqs, max_ctx);
   p.n_rg = (p.R + 32 * p.rw - 1) / (32 * p.rw);
   p.unit = p.rw == 1 ? 128 : 64;
-  // one workgroup per CU with 128 KB of stages, two with 64 KB
+  // one workgroup per CU with 128 KB of stages, two with 64 KB; every sequence but
+  // one may add a chunk by its rounding, and one workgroup too many is a second turn
+  // (32 / 8 heads of 128, 4 sequences of 5 nodes at 20000 positions: 32.9 -> 29.4 us)
   const size_t per = n_kv * p.n_rg, cus = static_cast<size_t>(wh::cu_count());
-  p.sparse = (cus + per - 1) / per;
-  p.target = ((p.rw == 1 ? 1 : 2) * cus + per - 1) / per;
-  p.single = max_ctx <= single_rows(p.rw);
+  auto spread = [&](size_t wgs) {
+    const size_t n = wgs / per ? wgs / per : 1;
+    return n >= 4 * n_seqs ? n - (n_seqs - 1) : n;
+  };
+  p.sparse = spread(cus);
+  p.target = spread((p.rw == 1 ? 1 : 2) * cus);
+  p.single = max_ctx <= single_rows(p.rw, p.R, D);
   p.least = p.single ? (max_ctx + p.unit - 1) / p.unit * p.unit : p.unit;
   const size_t most = n_seqs * ((max_ctx + p.least - 1) / p.least);
   p.max_slots = p.target + n_seqs < most ? p.target + n_seqs : most;
@@ -905,13 +918,13 @@ bool tree_attention_shape_ok(size_t n_heads, size_t n_kv_heads, size_t head_dim)
 
 size_t tree_attention_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                                       size_t max_ctx) {
-  const Plan p = make_plan(n_seqs, n_tree, n_heads, n_kv_heads, max_ctx);
+  const Plan p = make_plan(n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx);
   Params P = fill(p, n_seqs, n_tree, n_heads, n_kv_heads, head_dim, max_ctx);
   return layout(P, head_dim, nullptr);
 }
 
 int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t s) {
-  const Plan p = make_plan(a.n_seqs, a.n_tree, a.n_heads, a.n_kv_heads, a.max_ctx);
+  const Plan p = make_plan(a.n_seqs, a.n_tree, a.n_heads, a.n_kv_heads, a.head_dim, a.max_ctx);
   Params P = fill(p, a.n_seqs, a.n_tree, a.n_heads, a.n_kv_heads, a.head_dim, a.max_ctx);
   layout(P, a.head_dim, workspace);
   P.q = a.q, P.k = a.k, P.v = a.v;
