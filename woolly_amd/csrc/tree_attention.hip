@@ -65,7 +65,7 @@ struct Params {
   _Float16 *k_cache, *v_cache;
   const float* inv_freq;
   float* out;
-  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, unit, least, tiles;
+  uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, lone, unit, least, tiles;
   float scale;
   // workspace
   uint4* slots;         // [max_slots] (sequence, first key, key behind the last, cache rows of the step); sequence n_seqs: none
@@ -111,9 +111,11 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32
 // Cuts the sequences into chunks of one length, a multiple of a stage of the
 // partial kernel, so long and short sequences share the workgroups evenly
 // whatever the lengths on the device.  About `target` chunks over all sequences
-// give every CU two workgroups, whose matrix and vector work overlap; while the
-// chunks would be shorter than kDeepChunk, `sparse` chunks, one workgroup per CU,
-// do: half the partial results to write and to join.
+// give every CU two workgroups, whose matrix and vector work overlap; while theirs
+// would have up to `lone` keys, `sparse` chunks, one workgroup per CU, do: half the
+// partial results to write and to join.  (32 / 8 heads of 128, 26 nodes at 18000
+// and 25000 positions, lone = 1024 against 512 and then chunks of 512: 34.3 / 40.5,
+// 41.0 / 46.0 us; at 31000 53.0 / 53.1.)
 // Thread t plans sequences [t per, (t + 1) per); first: LDS [n_seqs + 1].  All rows
 // together number less than 2^32 (checked by the host).
 constexpr uint32_t kDeepChunk = 512;
@@ -134,7 +136,8 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
   uint32_t total, used;
   block_scan(mine, red, total);
   uint32_t even = (total + P.target - 1) / P.target;
-  if (even < kDeepChunk) even = min((total + P.sparse - 1) / P.sparse, kDeepChunk);
+  const uint32_t lone = (total + P.sparse - 1) / P.sparse;
+  even = lone <= P.lone ? lone : max(even, kDeepChunk);
   const uint32_t chunk = max((even + P.unit - 1) / P.unit * P.unit, P.least);
   uint32_t n = 0;
   for (uint32_t s = s0; s < s1; s++) n += (first[s] + chunk - 1) / chunk;
@@ -804,7 +807,7 @@ int row_tiles(size_t R, size_t D, size_t n_kv, size_t n_seqs, size_t max_ctx) {
 
 struct Plan {
   int rw;
-  size_t G, R, n_rg, target, sparse, unit, least, max_slots;
+  size_t G, R, n_rg, target, sparse, lone, unit, least, max_slots;
   bool single;  // every sequence is one chunk
 };
 Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t D, size_t max_ctx) {
@@ -823,6 +826,9 @@ Plan make_plan(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv, size_t
     return n >= 4 * n_seqs ? n - (n_seqs - 1) : n;
   };
   p.sparse = spread(cus);
+  // sequences that are many against the chunks leave CUs with one more or one less: 16
+  // sequences of 16 nodes, 15000 positions in all, 33.7 us with 512, 35.4 with 1024
+  p.lone = cus / per >= 4 * n_seqs ? 2 * kDeepChunk : kDeepChunk;
   p.target = spread((p.rw == 1 ? 1 : 2) * cus);
   p.single = max_ctx <= single_rows(p.rw, p.R, D);
   p.least = p.single ? (max_ctx + p.unit - 1) / p.unit * p.unit : p.unit;
@@ -865,6 +871,7 @@ Params fill(const Plan& p, size_t n_seqs, size_t n_tree, size_t n_heads, size_t 
   P.max_slots = static_cast<uint32_t>(p.max_slots);
   P.target = static_cast<uint32_t>(p.target);
   P.sparse = static_cast<uint32_t>(p.sparse);
+  P.lone = static_cast<uint32_t>(p.lone);
   P.unit = static_cast<uint32_t>(p.unit);
   P.least = static_cast<uint32_t>(p.least);
   P.tiles = static_cast<uint32_t>(p.n_rg * p.rw);
