@@ -231,6 +231,49 @@ def test_a_chunk_of_nothing_but_nan(gpu, heads, kv, d, n_tree):
     run(c, f"chunk of NaN {heads}/{kv}x{d} tree {n_tree}")
 
 
+# Caches of so many rows have their query rows cut into tiles that workgroups take by 1, 2 and 4: on 32 KV heads up to
+# 70 nodes by 1 up to 768 rows, by 2 up to 2048, then by 4; on 8 KV heads 27 nodes of 3 heads by 1 up to 3840, by 2 up
+# to 8192 (two sequences: half as many each).
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ctx", [0, 1, 31, 64, 129, 600])
+@pytest.mark.parametrize("heads,kv,n_tree,rows", [(32, 32, 70, 700), (32, 32, 70, 1500), (32, 32, 70, 2200),
+                                                  (24, 8, 27, 8500)])
+def test_tiles_of_a_workgroup(gpu, heads, kv, n_tree, rows, ctx, d):
+    run(Case(1, n_tree, heads, kv, d, [ctx], room=rows - ctx - n_tree, shape="padded", seed=ctx + d),
+        f"{heads}/{kv}x{d} tree {n_tree} ctx {ctx} of {rows}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1000, 2500, 4500])
+@pytest.mark.parametrize("ctx", [0, 37, 640])
+def test_unseen_rows_and_infinities_in_every_tiling(gpu, rows, ctx, d):
+    c = Case(2, 27, 24, 8, d, [ctx, ctx + 5], room=rows - ctx - 32, shape="padded", seed=rows)
+    for s, n in enumerate(c.lens):
+        c.kc[s, n:] = np.nan
+        c.vc[s, n:] = -np.inf
+    q, k, v = c.views()
+    for s in range(2):
+        absent = [t for t, p in enumerate(_tree.paths(c.parents[s])) if p is None]
+        q[s, absent] = k[s, absent] = np.nan
+        v[s, absent] = np.inf
+    k[0, 1, 0, 3] = np.nan
+    v[0, 2, :, 5] = np.inf
+    if ctx:
+        c.vc[1, 3, 7, 9] = np.inf
+        c.vc[1, ctx - 1, 7, 11] = -np.inf
+        c.vc[1, 30, 6, d - 1] = np.nan
+        c.kc[0, 20, 5, 2] = np.nan
+    run(c, f"unseen rows d {d} ctx {ctx} of {rows}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunks_of_one_and_of_two_workgroups_per_cu(gpu, d):
+    """Chunks grow with the rows up to 1024 keys, are halved beyond, and grow again."""
+    for ctx in (9000, 17500, 36000):
+        run(Case(1, 2, 32, 8, d, [ctx], seed=ctx), f"2 nodes at {ctx}, d {d}")
+        run(Case(1, 30, 6, 6, d, [ctx], seed=ctx), f"30 nodes at {ctx}, d {d}")
+
+
 def test_largest_queries(gpu):
     """Queries of 1e36 over keys of 1e-4: the scale of a row has the whole range of f32's exponents."""
     c = Case(1, 6, 4, 2, 128, [90], seed=3, qscale=1e36)
