@@ -18,14 +18,13 @@
 // a second small launch joins the chunks of a row.  Counting and the choice of a
 // bias entry use integer LDS atomics (add, max): their order does not change the
 // result.  Many rows are bound by memory: 64 nodes x 128256 (66.7 MB) take 19.3 us,
-// 3.9 TB/s once the launch is under way, whether a workgroup takes 2048, 4096 or
-// 8192 tokens (before the next: 20.0, 19.3, 19.6 us); 2 rows of them each (call
-// 20.3 us; one row 22.6, four 23.4).  The rows go out past the L2, which holds
-// nothing of them for anyone else and had them to write back when the kernel ended
-// (21.0 us; 16 x 128256 10.6 against 9.5); loads past it gain nothing (20.4).
-// Long histories, which every chunk reads, favour large chunks: 16 x 128256 with
-// up to 20000 tokens each 14.2, 11.2 and 10.0 us, now 9.5.  One row of 32000 is the
-// launch's latency: 5.8 us.
+// 3.9 TB/s once the launch is under way.  With 2 rows per workgroup a call takes
+// 20.3 us, with one 22.6, with four 23.4.  The rows go out past the L2, which would
+// have them to write back when the kernel ends (21.0 us; 16 x 128256 10.6 against
+// 9.5); loads past it gain nothing (20.4).  Workgroups of 2048, 4096 and 8192
+// tokens, before that: 20.0, 19.3 and 19.6 us, but long histories, which every
+// workgroup reads, favour large ones: 16 x 128256 with up to 20000 tokens each
+// 14.2, 11.2 and 10.0.  One row of 32000 is the launch's latency: 5.8 us.
 #include "tree.hpp"
 
 namespace {

@@ -4,8 +4,8 @@
 //
 // Neither moves enough to be bound by memory: a walk reads 1.5 KB at most and a
 // step keeps a few rows of each layer.  Both are one launch whose latency is
-// that of its dependent loads: 1.6 us for one walk over 26 nodes, 3.6 for 256
-// over 64; 3.8 us for 7 rows in 32 layers, 4.0 for 16 sequences in 24.
+// that of its dependent loads: 2.3 us for one walk over 26 nodes, 3.8 for 256
+// over 64; 4.1 us for 7 rows in 32 layers, 4.2 for 16 sequences in 24.
 #include "tree.hpp"
 
 namespace {

@@ -15,15 +15,15 @@
 //   2. partial: one workgroup per (chunk, KV head, group of 32 RW query rows)
 //   3. combine: one workgroup per 32 query rows and 8 dims joins their chunks
 //
-// What bounds it.  Short and middle contexts: the three launches' dependent loads
-// and their ends.  26 nodes at 4070 positions, 32 / 8 heads of 128 (17.8 MB: 3.7 us
-// at the 4.8 TB/s of a large copy): 4.4 + 13.9 + 4.8 us, of the partial kernel's
-// 13.9 some 3 until the first data is there, 6 for 4 tiles a wave, 3 for writing
-// 13.6 MB of partial results.  8 sequences of 16 nodes up to 8100, 32 / 4 heads of
-// 64: 5.3 + 13.2 + 4.3.  5 nodes at 300 of 312 rows: 3.7 + 10.0.  Long contexts: the
-// matrix cores.  64 nodes at 131000: 275 GFLOP of limb products in 250 us, 1.1
-// PFLOP/s; a large f16 library product reaches 1.15 on this card, where the clock
-// falls under such work (440 k cycles, 60 % of them with a product under way).
+// What bounds it.  Short and middle contexts: the launches' dependent loads and
+// their ends.  26 nodes at 4070 positions, 32 / 8 heads of 128 (17.8 MB: 3.7 us at
+// the 4.8 TB/s of a large copy): 4.3 + 14.2 + 4.1 us, of the partial kernel's 14.2
+// some 3 until the first data is there, 6 for 4 tiles a wave, 2 for writing 6.9 MB of
+// partial results.  8 sequences of 16 nodes up to 8100, 32 / 4 heads of 64: 5.0 + 13.1
+// + 4.3.  5 nodes at 300 of 312 rows: 3.6 + 10.4.  Long contexts: the matrix cores.  64
+// nodes at 131000: 275 GFLOP of limb products in 250 us, 1.1 PFLOP/s; a large f16
+// library product reaches 1.15 on this card, where the clock falls under such work
+// (460 k cycles, 57 % of them with a product under way).
 //
 // The angle is formed and reduced in 64 bits: in 32 bits p_t * inv_freq is off
 // by up to p_t 2^-24 radians, 0.008 at position 131072.  k is rotated in
