@@ -295,7 +295,9 @@ __device__ __forceinline__ half8 finite_only(half8 x) {
 // Replaces the infinities and NaN of a 32-row V tile in LDS by 0 and tells
 // whether there were any: lane l looks through half of row l / 2 (the order of
 // its chunks does not matter).  Waves that share a tile may do so at the same
-// time: they store the same values, each before it reads the tile itself.
+// time: they store the same values, each before it reads the tile itself.  But
+// one that looks after another has stored finds nothing: only all of them
+// together know what the tile held.
 template <int D>
 __device__ __forceinline__ bool clean_tile(uint32_t vt, int lane) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -337,7 +339,8 @@ struct Shape {
   static constexpr int kTileBytes = SK * D * 2;              // one of K, V
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kMergeBytes = KW > 1 ? kAttnWaves * 32 * (D + 2) * 4 : 0;  // all waves' sums, maxima and totals
-  static constexpr int kLds = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;
+  static constexpr int kFlag = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;  // a word: a tile was cleaned
+  static constexpr int kLds = kFlag + 16;
 };
 
 // grid: n_kv * n_rg * max_slots, KV head fastest (with 8 KV heads the workgroups
@@ -417,6 +420,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   bool odd = false;  // V holds infinities or NaN
+  uint32_t* const cleaned = reinterpret_cast<uint32_t*>(lds + S::kFlag);
+  if (RW > 1 && tid == 0) *cleaned = 0;  // seen by all from the first stage's barrier on
 
   // N 32-key tiles, KW tiles apart.  kt, vt: LDS addresses of the first one's first
   // K and V row.  Edge (N = 1): the tile may reach beyond the cache into the nodes'
@@ -468,7 +473,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         }
         bits = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
       }
-      odd |= clean_tile<D>(vt, lane);
+      if (clean_tile<D>(vt, lane)) {
+        odd = true;
+        if (RW > 1) *cleaned = 1;
+      }
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int key = 8 * (i >> 2) + 4 * h + (i & 3);
@@ -560,6 +568,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
   }
   l = swap_sum(l);
+  if constexpr (RW > 1) {
+    whd::lds_barrier();
+    odd = *cleaned != 0;  // waves of different rows share their tiles: one of them found what there was
+  }
   // Infinities and NaN of V count for the query rows that see them, and for no
   // other.  The edge tiles took them out (0 * inf would have spread a NaN), in the
   // others they made infinities and NaN of these sums, of either kind (the lo limb
