@@ -272,9 +272,15 @@ __device__ __forceinline__ s16x4 read_tr(uint32_t lds) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds);
 }
 
+// The largest of this lane's and lane ^ 32's value: NaN passed over, or kept.
 __device__ __forceinline__ float swap_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
   return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+__device__ __forceinline__ float swap_max_nan(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  return __builtin_elementwise_maximum(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
+                                       __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 __device__ __forceinline__ float swap_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
@@ -438,11 +444,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     // lets the compiler move anything but them across
     constexpr int kNoLds = 0x47F;
     half8 kf[2][N];
+    auto k_at = [&](int j, int n) {
+      return *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
+          (uintptr_t)(kt + n * kStep + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
+    };
     auto read_k = [&](int j) {
 #pragma unroll
-      for (int n = 0; n < N; n++)
-        kf[j & 1][n] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-            (uintptr_t)(kt + n * kStep + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
+      for (int n = 0; n < N; n++) kf[j & 1][n] = k_at(j, n);
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     read_k(0);
@@ -502,8 +510,35 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     read_v(0);
     float mt = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16 * N; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
-    mt = swap_max(mt);
+    for (int i = 1; i < 16 * N; i++) mt = __builtin_elementwise_maximum(mt, s[i / 16][i % 16]);
+    mt = swap_max_nan(mt);
+    if (__ballot(mt != mt)) {
+      // A score is NaN: the formula's, or made of an infinity in K that q's limbs meet
+      // with both signs or as 0.  q's sign and size are the hi limb's: its product alone
+      // says what an infinity makes of the score (an element of q below 2^-38 of its
+      // row's largest counts as 0 here).
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        f32x16 x;
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = 0.f;
+#pragma unroll 1
+        for (int j = 0; j < KS; j++) {
+          half8 q = qh[0];
+#pragma unroll
+          for (int u = 1; u < KS; u++) q = j == u ? qh[u] : q;
+          x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(j, n), q, x, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (s[n][i] != s[n][i]) s[n][i] = x[i];
+      }
+      mt = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 16 * N; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
+      mt = swap_max(mt);
+      read_v(0);  // so that its registers are free above
+    }
     if (__ballot(mt > m + lazy)) {
       const float mn = fmaxf(m, mt);
       const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * qs);
