@@ -3,7 +3,10 @@ import numpy as np
 import pytest
 
 from tests import _tree
+from tests._gpu import down, up
 from tests.test_gpu_tree_attention import Case
+from woolly_amd import ops
+from woolly_amd.device import DeviceBuffer
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +105,94 @@ def test_infinite_keys(gpu, d, heads, kv, rows, ctx):
     err = np.where(fine, np.abs(np.where(fine, out - want, 0)), 0)
     print(f"[case] infinite keys d {d} {heads}/{kv} ctx {ctx} of {rows}: {err.max():.2e}, {fine.mean():.2f} finite", flush=True)
     assert (err <= bound).all(), float(err.max())
+
+
+def weights_case(n_tree, heads, kv, d, ctx, room, share, sink, seed=0, spread=1.0):
+    """One sequence without rotation (inv_freq 0) in which every query row of a KV head is the same, so that one key holds
+    `share` of every row's weight, with a v of 0; sink: its cache row, or -1 for node 0, which all nodes see."""
+    c = Case(1, n_tree, heads, kv, d, [ctx], room=room, shape="star", seed=seed)
+    c.inv[:] = 0
+    q, k, v = c.views()
+    u = (c.rng.standard_normal((kv, d)) * spread).astype(np.float32)
+    q[0] = np.repeat(u, heads // kv, 0)
+    k[0, 1:] *= 0.5
+    for h in range(kv):
+        keys = c.kc[0, :ctx, h].astype(np.float64) if sink < 0 else np.delete(c.kc[0, :ctx, h], sink, 0).astype(np.float64)
+        rest = np.exp(keys @ u[h].astype(np.float64) / np.sqrt(d)).sum()
+        if share:
+            key = u[h] * (np.log(rest * share / (1 - share)) * np.sqrt(d) / float((u[h].astype(np.float64) ** 2).sum()))
+            (k[0, 0] if sink < 0 else c.kc[0, sink])[h] = key
+            (v[0, 0] if sink < 0 else c.vc[0, sink])[h] = 0
+    return c
+
+
+def weights_exact(c, nodes):
+    """(out [node][kv][d] in 64 bits, largest |score|) of a weights_case; the query heads of a KV head are alike."""
+    q, k, v = c.views()
+    g, ctx, top = c.h // c.kv, c.lens[0], 0.0
+    out = np.zeros((len(nodes), c.kv, c.d))
+    for h in range(c.kv):
+        kk, vv = c.kc[0, :ctx, h].astype(np.float64), c.vc[0, :ctx, h].astype(np.float64)
+        u = q[0, 0, h * g].astype(np.float64) / np.sqrt(c.d)
+        s = kk @ u
+        for i, t in enumerate(nodes):
+            path = _tree.paths(c.parents[0])[t]
+            own = _tree.stored(k[0, path, h].astype(np.float64)).astype(np.float64) @ u
+            w = np.exp(np.concatenate([s, own]) - max(s.max(initial=-np.inf), own.max()))
+            vals = np.concatenate([vv, v[0, path, h].astype(np.float16).astype(np.float64)])
+            out[i, h] = w @ vals / w.sum()
+            top = max(top, float(np.abs(s).max(initial=0)), float(np.abs(own).max()))
+    return out, top
+
+
+def weights_bar(top):
+    """Relative L2: the keys' v are independent, so errors of the weights, each relative to its weight, move the output by
+    no more than their size.  A score is a sum in f32 of magnitude <= top in steps of 16 products (2 d / 16 of them, each
+    off by 2^-24 of it, of random signs: under 4 * 2^-24 top), of limbs that hold q to 2^-22 (2^-22 top); the exponent's
+    argument, in powers of two, and the exponential add 1.45 * 2^-24 * 2 top + 2^-22; the limbs of the weights 2^-20; the sums of weights
+    and products 300 additions of random signs, 2^-20 again."""
+    return 2.0 ** -22 * (4 * top + 16)
+
+
+# query rows in tiles of a workgroup: one (20 rows), two, four; a chunk of thousands of keys (32 groups of 128 rows)
+@pytest.mark.parametrize("share", [0, 0.9, 0.99, 0.999, 0.9999, 0.999999])
+@pytest.mark.parametrize("n_tree,heads,kv,d,ctx,room", [(1, 8, 2, 64, 4000, 50), (1, 8, 2, 128, 500, 0), (5, 8, 2, 128, 300, 20),
+                                                        (5, 8, 2, 64, 130000, 20), (26, 32, 8, 128, 4070, 7),
+                                                        (64, 8, 1, 128, 20000, 5000), (128, 32, 1, 64, 60000, 0),
+                                                        (128, 32, 1, 128, 40000, 0)])
+def test_one_key_with_nearly_all_the_weight(gpu, n_tree, heads, kv, d, ctx, room, share):
+    """The others carry the output, and keep the precision that f32 weights have."""
+    nodes = sorted({0, n_tree // 2, n_tree - 1})
+    for sink in (0, ctx // 2 + 3, ctx - 1, -1)[:4 if share else 1]:
+        c = weights_case(n_tree, heads, kv, d, ctx, room, share, sink, seed=ctx)
+        want, top = weights_exact(c, nodes)
+        c.upload().launch()
+        got = c.results()[0][0, nodes].reshape(len(nodes), kv, heads // kv, d).astype(np.float64)
+        rel = float(np.linalg.norm(got - want[:, :, None]) / np.linalg.norm(np.broadcast_to(want[:, :, None], got.shape)))
+        bar = weights_bar(top)
+        print(f"[result] {share} of the weight on key {sink}, {n_tree} nodes {heads}/{kv}x{d} at {ctx}: {rel:.2e}, bar {bar:.2e}",
+              flush=True)
+        assert rel <= bar
+        if n_tree == 1:
+            qkv = up(np.concatenate([c.q, c.k, c.v], 1))[0]
+            k0, v0, out = up(c.kc.view(np.uint16))[0], up(c.vc.view(np.uint16))[0], DeviceBuffer(4 * heads * d)
+            wsz = ops.attention_workspace_bytes(heads, kv, d, ctx + 1)
+            ops.attention_decode(qkv, k0, v0, ctx, heads, kv, d, c.dev["inv"], out, DeviceBuffer(wsz), wsz)
+            one = down(out, np.float32, heads * d).reshape(1, kv, -1, d)
+            rel = float(np.linalg.norm(one - want[:, :, None]) / np.linalg.norm(np.broadcast_to(want[:, :, None], one.shape)))
+            print(f"[result] the decode step: {rel:.2e}", flush=True)
+            assert rel <= bar
+
+
+@pytest.mark.parametrize("spread", [3.0, 8.0])
+@pytest.mark.parametrize("n_tree,heads,kv,d,ctx", [(5, 8, 2, 128, 3000), (64, 8, 1, 64, 20000), (128, 32, 1, 128, 9000)])
+def test_scores_far_apart(gpu, n_tree, heads, kv, d, ctx, spread):
+    """Scores whose standard deviation is 3 and 8: tiles with weights of every size, references that move up and down."""
+    c = weights_case(n_tree, heads, kv, d, ctx, 20, 0, 0, seed=7, spread=spread)
+    nodes = [0, n_tree - 1]
+    want, top = weights_exact(c, nodes)
+    c.upload().launch()
+    got = c.results()[0][0, nodes].reshape(2, kv, heads // kv, d)
+    err, size = np.linalg.norm(got - want[:, :, None]), np.linalg.norm(np.broadcast_to(want[:, :, None], got.shape))
+    print(f"[result] scores of spread {spread}: {err / size:.2e}, bar {weights_bar(top):.2e}", flush=True)
+    assert err <= weights_bar(top) * size

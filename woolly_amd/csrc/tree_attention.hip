@@ -36,9 +36,15 @@
 // exchange with lane l ^ 32; the same registers, in the same key order, are
 // the B operand of O^T = V^T P^T, whose A operand comes from the row-major V
 // tile in LDS through transposing reads (ds_read_b64_tr_b16).  q is scaled by a
-// power of two per row and split into f16 hi + lo, and so is P (e^{s - m} 2^6):
-// both products are then as exact as f32 ones (2^-22), with K and V taken from
-// the cache as they are.
+// power of two per row and split into f16 hi + lo, and so is P (e^{s - m} 2^12),
+// with K and V taken from the cache as they are.  An element of q keeps 2^-22 of
+// itself or 2^-38 of its row's largest.  P ends at 2^-25, so m follows the tiles'
+// maxima, up and down: a weight keeps 2^-22 of itself or 2^-24 of its tile's largest.
+// Beside one key with nearly all the weight (often the first, whose v is small, so
+// that the others make the output) they keep what f32 would leave them; in that key's own
+// tile they take a turn of their own.  Relative L2 with 90 to 99.9999 % of the weight on
+// one key, up to 130000 positions: 4e-7 to 4e-6, the decode step's 5e-7 to 4e-6 (with m
+// the running maximum alone 1e-5 to 4e-2).
 #include <type_traits>
 
 #include "gemm_dev.hpp"
@@ -49,8 +55,17 @@ namespace {
 constexpr int kPrepThreads = 256;
 constexpr int kAttnWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPScaleLog2 = 6.0f;  // P is held times 2^6 ...
-constexpr float kLazyMax = 8.0f;     // ... and may grow by 2^8 before the running maximum moves: at most 2^14 in f16
+// Weights are held in f16 as 2^12 e^{s - m}, hi + lo.  The reference m of a row stays
+// where it is while the weight of a tile's largest score is within [2^-13, 2^3] of it (at
+// most 2^15 in f16), else it moves there, up or down, but never 2^48 below its highest.
+// Scores of deviation 1.3 and 3 move some row's in 3 % and 8 % of the tiles.
+constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f, kMoveDown = -13.0f, kLowest = 48.0f;
+// A row's keys in a tile are four groups, by their parity and by the lane that holds
+// them.  Where the largest weight of a group is below 2^-22 of the reference's (2^-10 in
+// f16: off by 2^-15 of itself), the row moves to the tile's maximum, and where it is so
+// against that too, the tile takes two turns: the keys down to 2^-9 of its largest weight,
+// then the others.  Scores of deviation 5 do so in 3 % of the tiles of 64 keys, of 3 in none.
+constexpr float kFaint = -22.0f, kNear = 9.0f;
 constexpr int kWholeMask = 4;        // mask words per node
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -74,7 +89,7 @@ struct Params {
   float* qscale;        // [n_seqs][n_kv][R]
   _Float16* qlimb;      // [n_seqs][n_kv][R][2][D]
   // partial results of a slot, KV head and tile of 32 query rows
-  float2* ml;           // [max_slots][n_kv][tiles][32] (maximum, sum)
+  float2* ml;           // [max_slots][n_kv][tiles][32] (reference, sum)
   float4* acc;          // [max_slots][n_kv][tiles][D / 8][64]: the registers of the lanes, as in the product
 };
 
@@ -415,16 +430,22 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     qh[j] = *reinterpret_cast<const half8*>(q);
     ql[j] = *reinterpret_cast<const half8*>(q + D);
   }
-  // scores are qs times s, in powers of 2; maxima are kept as s, so that the
-  // largest of a row is exactly 0 however large it is
-  const float qs = P.qscale[qrow], lazy = kLazyMax / qs;
+  // scores are qs times s, in powers of 2; the reference m is kept as s, so that
+  // the exponent of its key is exactly 0 however large it is
+  const float qs = P.qscale[qrow];
   uint32_t tm[kWholeMask] = {};
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  // A lane's place in a K tile (row l32, chunk h; of step j chunk 2 j + h) and in a V
+  // tile (row 4 h + kq, dims 16 dg + 4 dq ..; of 32 dims d chunk 4 d + ..).  The chunks'
+  // permutations turn bits of the address, so steps and dims do as well.
+  const int kq = (lane & 15) >> 2, dq = lane & 3, dg = (lane >> 4) & 1;
+  const uint32_t ko = l32 * 2 * D + 16 * (h ^ swz_k<D>(l32));
+  const uint32_t vo = (4 * h + kq) * 2 * D + 16 * ((2 * dg + (dq >> 1)) ^ swz_v<D>(kq)) + 8 * (dq & 1);
+  float m = -INFINITY, floor = -INFINITY, l = 0.f;
   bool odd = false;  // V holds infinities or NaN
   uint32_t* const cleaned = reinterpret_cast<uint32_t*>(lds + S::kFlag);
   if (RW > 1 && tid == 0) *cleaned = 0;  // seen by all from the first stage's barrier on
@@ -432,9 +453,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
   // N 32-key tiles, KW tiles apart.  kt, vt: LDS addresses of the first one's first
   // K and V row.  Edge (N = 1): the tile may reach beyond the cache into the nodes'
   // rows or past the last one.
-  auto tiles = [&](uint32_t base, uint32_t kt, uint32_t vt, auto edge, auto count) {
+  // Returns whether the tiles need a second turn, for the keys that the first left out.
+  auto turn_of = [&](uint32_t base, uint32_t kt, uint32_t vt, auto edge, auto count, auto second) __attribute__((always_inline)) {
     constexpr bool kEdge = decltype(edge)::value;
     constexpr int N = decltype(count)::value, kStep = KW * 32 * 2 * D;
+    constexpr bool kSecond = decltype(second)::value;
     f32x16 s[N];
 #pragma unroll
     for (int n = 0; n < N; n++)
@@ -446,7 +469,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     half8 kf[2][N];
     auto k_at = [&](int j, int n) {
       return *reinterpret_cast<const __attribute__((address_space(3))) half8*>(
-          (uintptr_t)(kt + n * kStep + l32 * 2 * D + 16 * ((2 * j + h) ^ swz_k<D>(l32))));
+          (uintptr_t)(((kt + ko) ^ (32 * j)) + n * kStep));
     };
     auto read_k = [&](int j) {
 #pragma unroll
@@ -493,14 +516,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
     }
     half8 vf[2][DT];
     auto read_v = [&](int ks) {
-      const int i16 = lane & 15, kq = i16 >> 2, dq = i16 & 3, dg = (lane >> 4) & 1;
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const int rr = 16 * (ks % 2) + 8 * u + 4 * h + kq;
-          const int c = 4 * d + 2 * dg + (dq >> 1);
-          const s16x4 x = read_tr(vt + ks / 2 * kStep + rr * 2 * D + 16 * (c ^ swz_v<D>(rr)) + 8 * (dq & 1));
+          const s16x4 x = read_tr(((vt + vo) ^ (64 * d)) + ks / 2 * kStep + (16 * (ks % 2) + 8 * u) * 2 * D);
           const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
 #pragma unroll
           for (int i = 0; i < 4; i++) vf[ks & 1][d][4 * u + i] = y[i];
@@ -508,11 +528,16 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       __builtin_amdgcn_sched_barrier(kNoLds);
     };
     read_v(0);
-    float mt = s[0][0];
+    // the largest score of each group of keys, and of the row
+    float top[2], mt;
+    auto tops = [&](auto larger) {
 #pragma unroll
-    for (int i = 1; i < 16 * N; i++) mt = __builtin_elementwise_maximum(mt, s[i / 16][i % 16]);
+      for (int i = 0; i < 16 * N; i++) top[i & 1] = i < 2 ? s[0][i] : larger(top[i & 1], s[i / 16][i % 16]);
+      mt = larger(top[0], top[1]);
+    };
+    tops([](float x, float y) { return __builtin_elementwise_maximum(x, y); });
     mt = swap_max_nan(mt);
-    if (__ballot(mt != mt)) {
+    if (__builtin_expect(__ballot(mt != mt) != 0, 0)) {
       // A score is NaN: the formula's, or made of an infinity in K that q's limbs meet
       // with both signs or as 0.  q's sign and size are the hi limb's: its product alone
       // says what an infinity makes of the score (an element of q below 2^-38 of its
@@ -533,21 +558,40 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
         for (int i = 0; i < 16; i++)
           if (s[n][i] != s[n][i]) s[n][i] = x[i];
       }
-      mt = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 16 * N; i++) mt = fmaxf(mt, s[i / 16][i % 16]);
+      tops([](float x, float y) { return fmaxf(x, y); });
       mt = swap_max(mt);
       read_v(0);  // so that its registers are free above
     }
-    if (__ballot(mt > m + lazy)) {
-      const float mn = fmaxf(m, mt);
-      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * qs);
+    if constexpr (kEdge) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) top[i] = top[i] == -INFINITY ? INFINITY : top[i];  // masked keys are not faint
+    }
+    float low = fminf(top[0], top[1]);  // of the lane's two groups, then of the row's four
+    const float far = (mt - m) * qs;
+    bool again = false;
+    if (kSecond || __ballot(far > kMoveUp || far < kMoveDown || (low - m) * qs < kFaint)) {
+      low = -swap_max(-low);
+      if (kSecond || __builtin_expect(__ballot((low - mt) * qs < kFaint) != 0, 0)) {
+        // first the keys near the tiles' maximum, then the others, with a reference of their own
+        const float split = mt - kNear * __builtin_amdgcn_rcpf(qs);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[n][i] = (s[n][i] < split) != kSecond ? -INFINITY : s[n][i];
+        tops([](float x, float y) { return fmaxf(x, y); });
+        mt = swap_max(mt);
+        again = !kSecond;
+      }
+      const float to = mt == -INFINITY ? m : fmaxf(mt, floor);  // -inf: the row sees nothing here
+      const float by = (to - m) * qs;
+      const bool moves = by > kMoveUp || by < ((low - m) * qs < kFaint ? -kMoveUp : kMoveDown);
+      const float al = moves ? __builtin_amdgcn_exp2f(-by) : 1.f;
       l *= al;
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] *= al;
-      m = mn;
+      if (moves) m = to, floor = fmaxf(floor, to - kLowest * __builtin_amdgcn_rcpf(qs));
     }
     const float mb = m == -INFINITY ? 0.f : m;
     float lt[4] = {0.f, 0.f, 0.f, 0.f};
@@ -571,6 +615,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
       for (int d = 0; d < DT; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[ks & 1][d], pl, acc[d], 0, 0, 0);
     }
     l += (lt[0] + lt[1]) + (lt[2] + lt[3]);  // one addition to the running sum
+    return again;
+  };
+
+  auto tiles = [&](uint32_t base, uint32_t kt, uint32_t vt, auto edge, auto count) {
+    if (__builtin_expect(turn_of(base, kt, vt, edge, count, std::false_type{}), 0))
+      turn_of(base, kt, vt, edge, count, std::true_type{});
   };
 
   // stages of cache rows only, then those that reach the nodes' rows or the chunk's end
@@ -767,7 +817,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const Params P, uint3
     float M = -INFINITY, L = 0.f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
     auto join = [&](float2 ml, float4 a) {
-      // a part without a maximum has no weight, but NaN of its scores stay
+      // a part without a reference has no weight, but NaN of its scores stay
       const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * qs);
       L = __builtin_fmaf(ml.y, ew, L);
       A.x = __builtin_fmaf(a.x, ew, A.x);
