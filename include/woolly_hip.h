@@ -505,8 +505,10 @@ WH_API int wh_embedding_lookup(int type, const void* table, size_t vocab, size_t
  *   out[t][h] = softmax(q k^T / sqrt(head_dim)) v
  * over cache rows 0 .. ctx_len - 1 and the rows of the node's ancestors and its
  * own.  Nodes that a row does not see never touch it, whatever they hold.  An
- * absent node's out row is zeros and its cache row stays as it was.  A sequence
- * with ctx_len + n_tree > max_ctx stores nothing, and its out rows are NaN.
+ * absent node's out row is zeros and its cache row stays as it was.  A tree takes
+ * n cache rows, up to its last node whose parent is -1 or an earlier node: absent
+ * nodes behind that need no room.  A sequence with ctx_len + n > max_ctx stores
+ * nothing, and its out rows are NaN.
  * head_dim 64 or 128, n_heads (at most 1024) a multiple of n_kv_heads, at most
  * 1024 sequences and 2^32 - 1 cache rows in all.  Caches and workspace are 16-byte aligned; the workspace holds
  * wh_attention_tree_workspace_bytes(..), 0 for shapes that are not taken; calls

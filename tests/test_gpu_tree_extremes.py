@@ -11,12 +11,12 @@ from woolly_amd.device import DeviceBuffer
 pytestmark = pytest.mark.gpu
 
 
-def exact(c):
-    """The case in 64 bits, with rows of weight 0 left out: (out, bound of the error), [n][t][h][..].  The bound is that
-    of _tree.attention over the keys that have a weight."""
+def exact(c, seqs=None):
+    """The case in 64 bits, with rows of weight 0 left out: (out, bound of the error), [n][t][h][..], of all sequences or
+    those given.  The bound is that of _tree.attention over the keys that have a weight."""
     q, k, v = c.views()
     out, bound = np.zeros((c.n, c.t, c.h, c.d)), np.zeros((c.n, c.t, c.h, 1))
-    for s in range(c.n):
+    for s in range(c.n) if seqs is None else seqs:
         kc, vc, g = c.kc[s].copy(), c.vc[s].copy(), c.h // c.kv
         ps = _tree.paths(c.parents[s])
         for i, p in enumerate(ps):
@@ -42,7 +42,7 @@ def exact(c):
                 mag = (np.abs(kk) @ np.abs(qr[h])).max() / np.sqrt(c.d)
                 e = mag * (2.0 ** -21 + 2 * c.d * 2.0 ** -24 + 2.0 ** -22) + 2.0 ** -20
                 bound[s, i, h] = (2 * e + 300 * 2.0 ** -24) * np.abs(vv).max()
-    return out, bound
+    return (out, bound) if seqs is None else (out[seqs], bound[seqs])
 
 
 # 16 heads per KV head: a tile of 32 query rows is two nodes.  Workgroups take the 24 tiles of a KV head by one up to 1920
@@ -196,3 +196,61 @@ def test_scores_far_apart(gpu, n_tree, heads, kv, d, ctx, spread):
     err, size = np.linalg.norm(got - want[:, :, None]), np.linalg.norm(np.broadcast_to(want[:, :, None], got.shape))
     print(f"[result] scores of spread {spread}: {err / size:.2e}, bar {weights_bar(top):.2e}", flush=True)
     assert err <= weights_bar(top) * size
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n_tree,there", [(2, 1), (8, 5), (33, 32), (64, 63), (65, 64), (100, 40), (128, 65), (128, 127), (128, 1)])
+def test_a_tree_that_just_fits(gpu, n_tree, there, d):
+    """Absent nodes behind a tree's last one need no room in the cache.  Five sequences: one with room, one
+    whose tree ends at the last row, one a row too long, one whose last node hangs below an absent one and takes a row all
+    the same, one without a tree on a full cache."""
+    c = Case(5, n_tree, 4, 2, d, [40] * 5, room=there - n_tree, shape="tree", seed=n_tree + there)
+    rows = c.max_ctx
+    assert rows == 40 + there
+    c.parents[:, there:] = -2
+    c.lens = [5, 40, 41, 40, rows]
+    c.parents[3, there] = there + 3   # absent
+    if there + 1 < n_tree:
+        c.parents[3, there + 1] = there
+    c.parents[4] = -2
+    orphan = there + 1 < n_tree       # row there + 1 is one too many
+    kc, vc = c.kc.copy(), c.vc.copy()
+    q, k, v = c.views()
+    want, bound = exact(c, [0, 1])
+    print(f"[case] {there} of {n_tree} nodes at the cache's end, d {d}", flush=True)
+    c.upload().launch()
+    out, gk, gv = c.results()
+    assert (np.abs(out[:2] - want) <= bound).all(), float(np.abs(out[:2] - want).max())
+    assert not out[:2, there:].any(), "absent nodes' rows"
+    assert np.isnan(out[2]).all()
+    assert np.isnan(out[3]).all() == orphan
+    assert not out[4].any()
+    for s in (0, 1):
+        for i, p in enumerate(_tree.paths(c.parents[s])):
+            if p is not None:
+                kc[s, c.lens[s] + i] = _tree.stored(_tree.rotate(k[s, i], c.lens[s] + len(p) - 1, c.inv))
+                vc[s, c.lens[s] + i] = _tree.stored(v[s, i].astype(np.float64))
+    keep = [0, 1, 2, 4] + ([3] if orphan else [])
+    assert np.array_equal(gk[keep].view(np.uint16), kc[keep].view(np.uint16))
+    assert np.array_equal(gv[keep].view(np.uint16), vc[keep].view(np.uint16))
+
+
+@pytest.mark.parametrize("n,n_tree", [(1, 1), (3, 17), (70, 5), (300, 2), (1024, 1), (37, 128), (257, 33)])
+def test_rows_of_many_trees(gpu, n, n_tree):
+    """Trees of every length in one batch, among them none at all, on caches that the shortest of them just fit."""
+    r = np.random.default_rng(n)
+    there = r.integers(0, n_tree + 1, n)
+    there[0] = n_tree
+    c = Case(n, n_tree, 2, 1, 64, [20] * n, room=0, seed=n)
+    for s in range(n):
+        c.parents[s, there[s]:] = r.choice([-2, -9, 200], n_tree - there[s])
+    c.lens = [int(c.max_ctx - t - (s % 3 == 0)) if t else 3 for s, t in enumerate(there)]
+    over = np.array([s % 5 == 4 and t > 0 for s, t in enumerate(there)])
+    c.lens = [int(c.max_ctx - t + 1) if o else n for n, t, o in zip(c.lens, there, over)]
+    some = [s for s in range(n) if not over[s]]
+    want, bound = exact(c, some)
+    print(f"[case] {n} trees of up to {n_tree}", flush=True)
+    c.upload().launch()
+    out, _, _ = c.results()
+    assert np.isnan(out[over]).all()
+    assert (np.abs(out[some] - want) <= bound).all(), float(np.abs(out[some] - want).max())

@@ -88,6 +88,11 @@ __device__ __forceinline__ TreeLanes tree_lanes(const int32_t* __restrict__ pare
   const int a = lane < n_tree ? parents[lane] : -2, b = lane + 64 < n_tree ? parents[lane + 64] : -2;
   return TreeLanes{a >= lane ? -2 : a, b >= lane + 64 ? -2 : b};
 }
+// Cache rows that a tree takes: up to its last node whose parent is -1 or an earlier one.
+__device__ __forceinline__ uint32_t tree_rows(const TreeLanes& tree) {
+  const unsigned long long lo = __ballot(tree.p0 >= -1), hi = __ballot(tree.p1 >= -1);
+  return hi ? 128 - __builtin_clzll(hi) : lo ? 64 - __builtin_clzll(lo) : 0;
+}
 __device__ __forceinline__ TreePath tree_path(const TreeLanes& tree, int t) {
   TreePath p{0, 0, -1};
   int at = t;

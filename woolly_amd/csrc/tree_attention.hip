@@ -83,7 +83,8 @@ struct Params {
   uint32_t n_seqs, n_tree, max_ctx, n_heads, n_kv, G, R, n_rg, max_slots, target, sparse, lone, unit, least, tiles;
   float scale;
   // workspace
-  uint4* slots;         // [max_slots] (sequence, first key, key behind the last, cache rows of the step); sequence n_seqs: none
+  uint4* slots;         // [max_slots] (sequence | rows of its tree << 16, first key, key behind the last, cache rows of the
+                        // step); sequence n_seqs: none
   uint32_t* first;      // [n_seqs + 1] first slot
   uint32_t* mask;       // [n_seqs][n_tree][4]
   float* qscale;        // [n_seqs][n_kv][R]
@@ -102,8 +103,9 @@ __device__ __forceinline__ _Float16 stored(double x) {
   return static_cast<_Float16>(f);
 }
 
-__device__ __forceinline__ bool seq_fits(const Params& P, uint32_t ctx) {
-  return ctx <= P.max_ctx && P.n_tree <= P.max_ctx - ctx;
+// n: the rows that the tree takes (tree_rows)
+__device__ __forceinline__ bool seq_fits(const Params& P, uint32_t ctx, uint32_t n) {
+  return ctx <= P.max_ctx && n <= P.max_ctx - ctx;
 }
 
 // Inclusive prefix sum over the workgroup's 256 threads, and their total; red: 4
@@ -131,21 +133,43 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32
 // partial results to write and to join.  (32 / 8 heads of 128, 26 nodes at 18000
 // and 25000 positions, lone = 1024 against 512 and then chunks of 512: 34.3 / 40.5,
 // 41.0 / 46.0 us; at 31000 53.0 / 53.1.)
-// Thread t plans sequences [t per, (t + 1) per); first: LDS [n_seqs + 1].  All rows
-// together number less than 2^32 (checked by the host).
+// Thread t plans sequences [t per, (t + 1) per); first, nodes, ends (cache rows of the
+// step, 0 for a sequence without work): LDS [n_seqs].  All rows together number less
+// than 2^32 (checked by the host).
 constexpr uint32_t kDeepChunk = 512;
-__device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
+__device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* nodes, uint32_t* ends, uint32_t* red) {
   const uint32_t t = threadIdx.x;
   const uint32_t per = (P.n_seqs + kPrepThreads - 1) / kPrepThreads;
   const uint32_t s0 = min(t * per, P.n_seqs), s1 = min(s0 + per, P.n_seqs);
+  const uint32_t ctx0 = s0 < s1 ? P.ctx_len[s0] : 0;  // asked for with the trees
+  // the trees' rows (tree_rows): a wave looks at 4 times 64 / g trees at once, a lane at
+  // one node of each (two where a tree has more than 64)
+  const uint32_t g = P.n_tree > 32 ? 64 : P.n_tree > 1 ? 1u << (32 - __builtin_clz(P.n_tree - 1)) : 1;
+  const uint32_t step = kPrepThreads / g;
+  const int i = t & (g - 1), n_tree = P.n_tree;
+  for (uint32_t s2 = __builtin_amdgcn_readfirstlane(t / 64) * (64 / g); s2 < P.n_seqs; s2 += 4 * step) {
+    int a[4], b[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const uint32_t s = s2 + u * step + (t & 63) / g;
+      const int32_t* parents = P.parents + static_cast<size_t>(s) * P.n_tree;
+      a[u] = s < P.n_seqs && i < n_tree ? parents[i] : -2;
+      b[u] = s < P.n_seqs && i + 64 < n_tree ? parents[i + 64] : -2;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const uint32_t s = s2 + u * step + (t & 63) / g;
+      const unsigned long long lo = __ballot(a[u] >= -1 && a[u] < i) >> (t & 63 & ~(g - 1)) & (~0ull >> (64 - g));
+      const unsigned long long hi = __ballot(b[u] >= -1 && b[u] < i + 64);  // g is 64 where there are any
+      if (i == 0 && s < P.n_seqs) nodes[s] = hi ? 128 - __builtin_clzll(hi) : lo ? 64 - __builtin_clzll(lo) : 0;
+    }
+  }
+  whd::lds_barrier();
   uint32_t mine = 0;
   for (uint32_t s = s0; s < s1; s++) {
-    const uint32_t ctx = P.ctx_len[s];
-    const int32_t* parents = P.parents + static_cast<size_t>(s) * P.n_tree;
-    bool any = parents[0] == -1;  // a sequence whose nodes are all absent has nothing to do
-    for (uint32_t i = 1; i < P.n_tree && !any; i++) any = parents[i] == -1;
-    const uint32_t n = any && seq_fits(P, ctx) ? ctx + P.n_tree : 0;
-    first[s] = n;
+    const uint32_t ctx = s == s0 ? ctx0 : P.ctx_len[s];
+    const uint32_t n = nodes[s] && seq_fits(P, ctx, nodes[s]) ? ctx + nodes[s] : 0;
+    ends[s] = n;
     mine += n;
   }
   uint32_t total, used;
@@ -155,10 +179,10 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
   even = lone <= P.lone ? lone : max(even, kDeepChunk);
   const uint32_t chunk = max((even + P.unit - 1) / P.unit * P.unit, P.least);
   uint32_t n = 0;
-  for (uint32_t s = s0; s < s1; s++) n += (first[s] + chunk - 1) / chunk;
+  for (uint32_t s = s0; s < s1; s++) n += (ends[s] + chunk - 1) / chunk;
   uint32_t at = block_scan(n, red, used) - n;
   for (uint32_t s = s0; s < s1; s++) {
-    const uint32_t c = (first[s] + chunk - 1) / chunk;
+    const uint32_t c = (ends[s] + chunk - 1) / chunk;
     first[s] = at;
     P.first[s] = at;
     at += c;
@@ -173,8 +197,8 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
     }
     uint4 slot = make_uint4(P.n_seqs, 0, 0, 0);
     if (y < used) {
-      const uint32_t rows = P.ctx_len[lo] + P.n_tree, c0 = (y - first[lo]) * chunk;
-      slot = make_uint4(lo, c0, min(c0 + chunk, rows), rows);
+      const uint32_t rows = ends[lo], c0 = (y - first[lo]) * chunk;
+      slot = make_uint4(lo | nodes[lo] << 16, c0, min(c0 + chunk, rows), rows);
     }
     P.slots[y] = slot;
   }
@@ -187,10 +211,10 @@ __device__ void plan_chunks(const Params& P, uint32_t* first, uint32_t* red) {
 // angles (22 sequences of 81 nodes, 80 + 16 heads: 68 -> 37 us).
 template <int D, int N>
 __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params P, uint32_t n_groups) {
-  __shared__ uint32_t first[wh::kMaxTreeSeqs + 1];
+  __shared__ uint32_t first[wh::kMaxTreeSeqs], nodes[wh::kMaxTreeSeqs], ends[wh::kMaxTreeSeqs];
   __shared__ uint32_t red[kPrepThreads / 64];
   if (blockIdx.x == P.n_seqs * P.n_tree * n_groups) {
-    plan_chunks(P, first, red);
+    plan_chunks(P, first, nodes, ends, red);
     return;
   }
   const uint32_t group = blockIdx.x % n_groups, row_id = blockIdx.x / n_groups;
@@ -219,7 +243,7 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
   const float inv = P.inv_freq[i];
   const uint32_t ctx = P.ctx_len[s];
   const whd::TreePath path = whd::tree_path(tree, t);
-  const bool present = path.present() && seq_fits(P, ctx);
+  const bool fits = seq_fits(P, ctx, whd::tree_rows(tree)), present = path.present() && fits;
   if (group == 0 && tid < kWholeMask) {
     const unsigned long long w = (tid < 2 ? path.lo : path.hi) >> (32 * (tid & 1));
     P.mask[row * kWholeMask + tid] = present ? static_cast<uint32_t>(w) : 0u;
@@ -238,7 +262,7 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
     if (hh < P.n_heads) {
       if (!present && lane < D / 2) {
         // an absent node's rows are zeros; those of a sequence that does not fit its cache are NaN
-        const float fill = seq_fits(P, ctx) ? 0.f : __builtin_nanf("");
+        const float fill = fits ? 0.f : __builtin_nanf("");
         float* o = P.out + row * P.n_heads * D + static_cast<size_t>(hh) * D;
         o[i] = fill;
         o[i + D / 2] = fill;
@@ -373,9 +397,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, RW == 1 && D == 128 ? 1 : 2) void 
   extern __shared__ __align__(256) unsigned char lds[];
   const uint32_t kvh = blockIdx.x % P.n_kv, rg = blockIdx.x / P.n_kv % P.n_rg, slot = blockIdx.x / (P.n_kv * P.n_rg);
   const uint4 sc = P.slots[slot];
-  if (sc.x >= P.n_seqs) return;
-  const uint32_t seq = sc.x, c0 = sc.y, c1 = sc.z, rows = sc.w;  // c0 < c1 <= rows
-  const uint32_t ctx = rows - P.n_tree;
+  const uint32_t seq = sc.x & 0xFFFFu, c0 = sc.y, c1 = sc.z, rows = sc.w;  // c0 < c1 <= rows
+  if (seq >= P.n_seqs) return;
+  const uint32_t ctx = rows - (sc.x >> 16);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = wave / KW, kw = wave % KW;
