@@ -379,6 +379,10 @@ extern "C" {
                           path: *mut u32, n_accepted: *mut u32, next_token: *mut u32, ctx_len: *const u32,
                           ctx_len_out: *mut u32, history: *mut u32, history_stride: usize,
                           stream: wh_stream_t) -> c_int;
+    pub fn wh_tree_accept_in_cache(tokens: *const u32, parents: *const i32, picked: *const u32, n_seqs: usize,
+                                   n_tree: usize, path: *mut u32, n_accepted: *mut u32, next_token: *mut u32,
+                                   ctx_len: *const u32, ctx_len_out: *mut u32, history: *mut u32,
+                                   history_stride: usize, max_ctx: usize, stream: wh_stream_t) -> c_int;
     pub fn wh_kv_cache_compact(k_caches: *mut *mut c_void, v_caches: *mut *mut c_void, n_layers: usize,
                                n_seqs: usize, max_ctx: usize, n_kv_heads: usize, head_dim: usize, path: *const u32,
                                n_tree: usize, n_accepted: *const u32, ctx_len: *const u32,

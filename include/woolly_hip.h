@@ -579,11 +579,21 @@ WH_API int wh_logits_process(const wh_logits_rules* rules, const float* logits, 
  * absent) and next_token the token picked at the last of them (0xFFFFFFFF for
  * none).  With ctx_len: ctx_len_out (may be null, or ctx_len itself) receives
  * ctx_len + n_accepted, and history (may be null) the accepted tokens at
- * ctx_len .. of its sequence's history_stride tokens, those that fit. */
+ * ctx_len .. of its sequence's history_stride tokens, those that fit.
+ * The walk knows no caches: a tree that did not fit its cache (wh_attention_tree
+ * stored nothing of it) still has node 0 accepted.  wh_tree_accept_in_cache, for
+ * caches of max_ctx rows, accepts nothing of such a tree: n_accepted 0, next_token
+ * 0xFFFFFFFF, length and history as they were.  A step that ends otherwise, for
+ * instance where a grammar lets no token follow, has n_accepted > 0. */
 WH_API int wh_tree_accept(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs,
                           size_t n_tree, uint32_t* path, uint32_t* n_accepted, uint32_t* next_token,
                           const uint32_t* ctx_len, uint32_t* ctx_len_out, uint32_t* history, size_t history_stride,
                           wh_stream_t stream);
+
+WH_API int wh_tree_accept_in_cache(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs,
+                                   size_t n_tree, uint32_t* path, uint32_t* n_accepted, uint32_t* next_token,
+                                   const uint32_t* ctx_len, uint32_t* ctx_len_out, uint32_t* history,
+                                   size_t history_stride, size_t max_ctx, wh_stream_t stream);
 
 /* Moves the accepted nodes' cache rows together in every layer: row first + i
  * takes row first + path[i] for i < n_accepted, first = ctx_len - n_accepted,

@@ -237,6 +237,7 @@ SIGNATURES = {
     "wh_logits_process_workspace_bytes": (_sz, [C.POINTER(wh_logits_rules), _sz, _sz]),
     "wh_logits_process": (_int, [C.POINTER(wh_logits_rules), _f32p, _sz, _sz, _sz, _f32p, _sz, _vp, _vp, _sz, _vp]),
     "wh_tree_accept": (_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "wh_tree_accept_in_cache": (_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp]),
     "wh_kv_cache_compact": (_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp]),
     "wh_gguf_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "wh_gguf_open_buffer": (_int, [_vp, _sz, C.POINTER(_vp)]),

@@ -24,11 +24,13 @@ struct AcceptParams {
   uint32_t* history;
   size_t history_stride;
   uint32_t n_tree;
+  uint32_t max_ctx;         // cache rows that hold the trees, 0: whatever
 };
 
 // One wave per sequence, lane l holding nodes l and l + 64.  From node 0 the
 // walk goes to the first child that carries the token picked at the node; all
-// children are compared at once.
+// children are compared at once.  A tree that its cache did not hold (by tree_rows'
+// measure) has nothing accepted: no row of it is there to keep.
 __global__ __launch_bounds__(64) void tree_accept_kernel(const AcceptParams P) {
   const uint32_t s = blockIdx.x, lane = threadIdx.x;
   const size_t row = static_cast<size_t>(s) * P.n_tree;
@@ -45,6 +47,11 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(const AcceptParams P) {
   const uint32_t ctx = P.ctx_len ? P.ctx_len[s] : 0;
   uint32_t n = 0, next = kNoToken;
   int at = __shfl(parent[0], 0, 64) == -1 ? 0 : -1;
+  if (P.max_ctx) {
+    const uint32_t rows = whd::tree_rows(whd::TreeLanes{parent[0] >= static_cast<int>(lane) ? -2 : parent[0],
+                                                        parent[1] >= static_cast<int>(lane) + 64 ? -2 : parent[1]});
+    if (ctx > P.max_ctx || rows > P.max_ctx - ctx) at = -1;
+  }
   while (at >= 0) {  // at grows with every step: at most n_tree steps
     if (lane == static_cast<uint32_t>(at & 63)) order[at >> 6] = n;
     n++;
@@ -117,26 +124,45 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(const CompactParams P) 
 
 }  // namespace
 
-WH_API int wh_tree_accept(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs,
-                          size_t n_tree, uint32_t* path, uint32_t* n_accepted, uint32_t* next_token,
-                          const uint32_t* ctx_len, uint32_t* ctx_len_out, uint32_t* history, size_t history_stride,
-                          wh_stream_t stream) {
+// max_ctx 0: the caches are not looked at.
+static int accept(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs, size_t n_tree,
+                  uint32_t* path, uint32_t* n_accepted, uint32_t* next_token, const uint32_t* ctx_len,
+                  uint32_t* ctx_len_out, uint32_t* history, size_t history_stride, size_t max_ctx, wh_stream_t stream) {
   if (n_tree > wh::kMaxTreeNodes || n_seqs >= (static_cast<size_t>(1) << 31))
     return wh::set_error(WH_ERR_INVALID_SHAPE, "tree_accept: %zu nodes of %zu sequences (at most %zu nodes)", n_tree,
                          n_seqs, wh::kMaxTreeNodes);
   if (n_seqs == 0 || n_tree == 0) return WH_OK;
   if (!tokens || !parents || !picked || !path || !n_accepted || !next_token)
     return wh::set_error(WH_ERR_INVALID_ARGUMENT, "tree_accept: null pointer");
-  if ((ctx_len_out || history) && !ctx_len)
-    return wh::set_error(WH_ERR_INVALID_ARGUMENT, "tree_accept: ctx_len_out and history need ctx_len");
+  if ((ctx_len_out || history || max_ctx) && !ctx_len)
+    return wh::set_error(WH_ERR_INVALID_ARGUMENT, "tree_accept: ctx_len_out, history and max_ctx need ctx_len");
   const void* ptrs[] = {tokens, parents, picked, path, n_accepted, next_token, ctx_len, ctx_len_out, history};
   for (const void* p : ptrs)
     if (!wh::aligned(p, 4)) return wh::set_error(WH_ERR_INVALID_ARGUMENT, "tree_accept: arrays must be 4-byte aligned");
   const AcceptParams P{tokens,  parents,     picked,  path,           n_accepted, next_token,
-                       ctx_len, ctx_len_out, history, history_stride, static_cast<uint32_t>(n_tree)};
+                       ctx_len, ctx_len_out, history, history_stride, static_cast<uint32_t>(n_tree),
+                       static_cast<uint32_t>(max_ctx)};
   tree_accept_kernel<<<static_cast<unsigned>(n_seqs), 64, 0, reinterpret_cast<hipStream_t>(stream)>>>(P);
   WH_LAUNCH_CHECK("tree accept launch");
   return WH_OK;
+}
+
+WH_API int wh_tree_accept(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs,
+                          size_t n_tree, uint32_t* path, uint32_t* n_accepted, uint32_t* next_token,
+                          const uint32_t* ctx_len, uint32_t* ctx_len_out, uint32_t* history, size_t history_stride,
+                          wh_stream_t stream) {
+  return accept(tokens, parents, picked, n_seqs, n_tree, path, n_accepted, next_token, ctx_len, ctx_len_out, history,
+                history_stride, 0, stream);
+}
+
+WH_API int wh_tree_accept_in_cache(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs,
+                                   size_t n_tree, uint32_t* path, uint32_t* n_accepted, uint32_t* next_token,
+                                   const uint32_t* ctx_len, uint32_t* ctx_len_out, uint32_t* history,
+                                   size_t history_stride, size_t max_ctx, wh_stream_t stream) {
+  if (max_ctx == 0 || max_ctx >> 31)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "tree_accept_in_cache: max_ctx = %zu out of range", max_ctx);
+  return accept(tokens, parents, picked, n_seqs, n_tree, path, n_accepted, next_token, ctx_len, ctx_len_out, history,
+                history_stride, max_ctx, stream);
 }
 
 WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, size_t n_layers, size_t n_seqs,

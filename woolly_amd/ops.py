@@ -302,11 +302,15 @@ def logits_process(rules: LogitsRules, logits, ld: int, n_rows: int, vocab: int,
 
 
 def tree_accept(tokens, parents, picked, n_seqs: int, n_tree: int, path, n_accepted, next_token, ctx_len=None,
-                ctx_len_out=None, history=None, history_stride: int = 0, stream: Stream | None = None) -> None:
-    """The walk from node 0 along the picked tokens (wh_tree_accept)."""
-    _lib.check(_lib.load().wh_tree_accept(_p(tokens), _p(parents), _p(picked), n_seqs, n_tree, _p(path), _p(n_accepted),
-                                          _p(next_token), _p(ctx_len) or None, _p(ctx_len_out) or None,
-                                          _p(history) or None, history_stride, _s(stream)))
+                ctx_len_out=None, history=None, history_stride: int = 0, stream: Stream | None = None,
+                max_ctx: int | None = None) -> None:
+    """The walk from node 0 along the picked tokens (wh_tree_accept).  With max_ctx, the rows of the caches that hold
+    the trees, nothing of a tree that did not fit is accepted (wh_tree_accept_in_cache)."""
+    args = (_p(tokens), _p(parents), _p(picked), n_seqs, n_tree, _p(path), _p(n_accepted), _p(next_token),
+            _p(ctx_len) or None, _p(ctx_len_out) or None, _p(history) or None, history_stride)
+    lib = _lib.load()
+    _lib.check(lib.wh_tree_accept(*args, _s(stream)) if max_ctx is None else
+               lib.wh_tree_accept_in_cache(*args, max_ctx, _s(stream)))
 
 
 class KvCaches:
