@@ -551,7 +551,7 @@ typedef struct wh_logits_rules {
   const uint32_t* bias_ids;     /* l + bias of its token, [sequences][bias_stride]; the last entry of a token counts */
   const float* bias;
   size_t n_bias;
-  size_t bias_stride;           /* 0: the same entries for every sequence */
+  size_t bias_stride;           /* n_bias or more; 0: the same entries for every sequence */
   const uint32_t* mask;         /* bit i of a row clear: token i is not allowed, [rows][mask_stride] words */
   size_t mask_stride;
 } wh_logits_rules;

@@ -1,5 +1,5 @@
 """More of what the calls for a tree of drafted tokens refuse, without a GPU: every check runs before a launch."""
-from tests.test_tree_abi import P
+from tests.test_tree_abi import P, logits
 from woolly_amd import _lib
 
 
@@ -20,3 +20,14 @@ def test_accept_in_cache_refusals():
         assert call(**{name: P + 1}) == _lib.WH_ERR_INVALID_ARGUMENT, name
     assert call(n_seqs=0, tokens=None) == _lib.WH_OK
     assert call(n_tree=0, tokens=None) == _lib.WH_OK
+
+
+def test_bias_stride_below_the_entries():
+    """Each sequence would take the next one's first entries, the last would read past the arrays."""
+    rules = dict(n_bias=30, bias_ids=P, bias=P)
+    for stride in (1, 29):
+        assert logits(dict(rules, bias_stride=stride)) == _lib.WH_ERR_INVALID_SHAPE
+        assert b"bias stride" in _lib.load().wh_last_error()
+    for stride in (0, 30, 64):
+        assert logits(dict(rules, bias_stride=stride), workspace_bytes=0) == _lib.WH_ERR_BUFFER_TOO_SMALL
+    assert logits(dict(bias_stride=5), workspace_bytes=0) == _lib.WH_ERR_BUFFER_TOO_SMALL  # no entries at all

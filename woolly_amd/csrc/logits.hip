@@ -311,6 +311,9 @@ WH_API int wh_logits_process(const wh_logits_rules* rules, const float* logits, 
                          "logits_process: the repetition penalty must be finite and above 0, the others finite");
   if (r.n_bias && (!r.bias_ids || !r.bias || r.n_bias >> 31))
     return wh::set_error(WH_ERR_INVALID_ARGUMENT, "logits_process: %zu bias entries without ids or values", r.n_bias);
+  if (r.n_bias && r.bias_stride && r.bias_stride < r.n_bias)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "logits_process: bias stride %zu below the %zu entries of a sequence",
+                         r.bias_stride, r.n_bias);
   if (n_rows == 0 || (!out && !token)) return WH_OK;
   if (!logits) return wh::set_error(WH_ERR_INVALID_ARGUMENT, "logits_process: null logits");
   if (out == logits && ld_out != ld)
