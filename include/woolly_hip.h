@@ -598,7 +598,8 @@ WH_API int wh_tree_accept_in_cache(const uint32_t* tokens, const int32_t* parent
 /* Moves the accepted nodes' cache rows together in every layer: row first + i
  * takes row first + path[i] for i < n_accepted, first = ctx_len - n_accepted,
  * where ctx_len is the length behind the walk (ctx_len_out).  The caches are
- * host arrays of n_layers device pointers, no cache named twice.  Paths ascend, as
+ * host arrays of n_layers device pointers, no cache named twice and none within
+ * another.  Paths ascend, as
  * wh_tree_accept writes them; entries that do not name a later row of the tree
  * move nothing, nor does a sequence whose numbers do not fit its cache. */
 WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, size_t n_layers, size_t n_seqs,

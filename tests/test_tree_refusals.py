@@ -1,5 +1,7 @@
 """More of what the calls for a tree of drafted tokens refuse, without a GPU: every check runs before a launch."""
-from tests.test_tree_abi import P, logits
+import pytest
+
+from tests.test_tree_abi import P, compact, logits
 from woolly_amd import _lib
 
 
@@ -31,3 +33,27 @@ def test_bias_stride_below_the_entries():
     for stride in (0, 30, 64):
         assert logits(dict(rules, bias_stride=stride), workspace_bytes=0) == _lib.WH_ERR_BUFFER_TOO_SMALL
     assert logits(dict(bias_stride=5), workspace_bytes=0) == _lib.WH_ERR_BUFFER_TOO_SMALL  # no entries at all
+
+
+SIZE = 2 * 100 * 8 * 128 * 2  # bytes of a cache of compact()
+
+
+@pytest.mark.parametrize("k, v", [((P, P + 2 * SIZE), (P + SIZE, P + 3 * SIZE - 16)),  # v[1] begins within k[1]
+                                  ((P + 16, P + 4 * SIZE), (P + 2 * SIZE, P)),         # k[0] begins within v[1]
+                                  ((P, P + SIZE // 2), (P + 2 * SIZE, P + 4 * SIZE))])
+def test_compact_refuses_caches_that_overlap(k, v):
+    assert compact(k=k, v=v) == _lib.WH_ERR_INVALID_ARGUMENT
+    assert b"within another" in _lib.load().wh_last_error()
+
+
+def test_compact_looks_at_every_cache():
+    k, v = [P + 2 * i * SIZE for i in range(300)], [P + (2 * i + 1) * SIZE for i in range(300)]
+    assert compact(k=k, v=v[:299] + [P + 16]) == _lib.WH_ERR_INVALID_ARGUMENT
+    assert b"within another" in _lib.load().wh_last_error()
+    assert compact(k=k, v=v[:299] + [k[7]]) == _lib.WH_ERR_INVALID_ARGUMENT
+    assert b"layer 299 is named twice" in _lib.load().wh_last_error()
+
+
+def test_compact_sizes_that_no_memory_holds():
+    assert compact(k=(P,), v=(P + 64,), n_seqs=65535, max_ctx=(1 << 31) - 1, n_kv_heads=1 << 10, head_dim=1 << 17) == \
+        _lib.WH_ERR_INVALID_SHAPE

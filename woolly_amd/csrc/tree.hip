@@ -6,6 +6,10 @@
 // step keeps a few rows of each layer.  Both are one launch whose latency is
 // that of its dependent loads: 2.3 us for one walk over 26 nodes, 3.8 for 256
 // over 64; 4.1 us for 7 rows in 32 layers, 4.2 for 16 sequences in 24.
+#include <algorithm>
+#include <memory>
+#include <new>
+
 #include "tree.hpp"
 
 namespace {
@@ -185,14 +189,34 @@ WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, siz
     if (!k_caches[l] || !v_caches[l] || !wh::aligned(k_caches[l], 16) || !wh::aligned(v_caches[l], 16))
       return wh::set_error(WH_ERR_INVALID_ARGUMENT,
                            "kv_cache_compact: layer %zu caches must be non-null and 16-byte aligned", l);
-  // rows of a cache named twice would be moved twice at once
+  // rows of a cache named twice, or shared by two, would be moved twice at once: in order of
+  // their addresses every cache ends before the next begins
+  size_t cache_bytes;
+  if (__builtin_mul_overflow(n_seqs * max_ctx, row_bytes, &cache_bytes))
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "kv_cache_compact: %zu x %zu rows of %zu bytes are no cache", n_seqs, max_ctx,
+                         row_bytes);
+  uintptr_t few[4 * kCompactLayers];
+  std::unique_ptr<uintptr_t[]> many;
+  const size_t n_caches = 2 * n_layers;
+  if (n_caches > 4 * kCompactLayers) many.reset(new (std::nothrow) uintptr_t[n_caches]);
+  uintptr_t* at = many ? many.get() : few;
+  if (n_caches > 4 * kCompactLayers && !many)
+    return wh::set_error(WH_ERR_OOM, "kv_cache_compact: no memory for %zu caches", n_caches);
   for (size_t l = 0; l < n_layers; l++) {
-    bool twice = k_caches[l] == v_caches[l];
-    for (size_t i = 0; i < l; i++)
-      twice |= k_caches[i] == k_caches[l] || k_caches[i] == v_caches[l] || v_caches[i] == k_caches[l] ||
-               v_caches[i] == v_caches[l];
-    if (twice) return wh::set_error(WH_ERR_INVALID_ARGUMENT, "kv_cache_compact: a cache of layer %zu is named twice", l);
+    at[2 * l] = reinterpret_cast<uintptr_t>(k_caches[l]);
+    at[2 * l + 1] = reinterpret_cast<uintptr_t>(v_caches[l]);
   }
+  std::sort(at, at + n_caches);
+  for (const size_t least : {static_cast<size_t>(1), cache_bytes})
+    for (size_t i = 0; i + 1 < n_caches; i++)
+      if (at[i + 1] - at[i] < least) {
+        size_t l = n_layers - 1;
+        while (reinterpret_cast<uintptr_t>(k_caches[l]) != at[i + 1] && reinterpret_cast<uintptr_t>(v_caches[l]) != at[i + 1]) l--;
+        return least == 1
+                   ? wh::set_error(WH_ERR_INVALID_ARGUMENT, "kv_cache_compact: a cache of layer %zu is named twice", l)
+                   : wh::set_error(WH_ERR_INVALID_ARGUMENT,
+                                   "kv_cache_compact: a cache of layer %zu begins within another (of %zu bytes)", l, cache_bytes);
+      }
   CompactParams P{};
   P.path = path;
   P.n_accepted = n_accepted;
