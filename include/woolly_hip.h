@@ -487,7 +487,8 @@ WH_API int wh_embedding_lookup(int type, const void* table, size_t vocab, size_t
  *   it follows that node; any other value: the node is absent, and so is every
  *   node below it (a tree with fewer nodes than n_tree, e.g. in a captured
  *   graph).  At most WH_MAX_TREE_NODES nodes per tree.
- * n_seqs sequences are stepped together; arrays are [n_seqs][n_tree], and
+ * n_seqs sequences (at most 1024 for the attention, 65535 for the cache rows, less
+ * than 2^26 for the walk) are stepped together; arrays are [n_seqs][n_tree], and
  * every sequence has its own caches, [n_seqs][max_ctx][n_kv_heads][head_dim] f16,
  * of which the first ctx_len[s] rows are filled.  Lengths, parents and tokens
  * are device memory, read when the call runs: a captured step follows them. */

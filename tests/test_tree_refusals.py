@@ -1,7 +1,7 @@
 """More of what the calls for a tree of drafted tokens refuse, without a GPU: every check runs before a launch."""
 import pytest
 
-from tests.test_tree_abi import P, compact, logits
+from tests.test_tree_abi import P, accept, compact, logits
 from woolly_amd import _lib
 
 
@@ -55,5 +55,13 @@ def test_compact_looks_at_every_cache():
 
 
 def test_compact_sizes_that_no_memory_holds():
-    assert compact(k=(P,), v=(P + 64,), n_seqs=65535, max_ctx=(1 << 31) - 1, n_kv_heads=1 << 10, head_dim=1 << 17) == \
+    assert compact(k=(P,), v=(P + 64,), n_seqs=65535, max_ctx=(1 << 31) - 1, n_kv_heads=1 << 10, head_dim=1 << 16) == \
         _lib.WH_ERR_INVALID_SHAPE
+    assert b"are no cache" in _lib.load().wh_last_error()
+
+
+def test_sizes_beyond_a_launch():
+    assert accept(n_seqs=1 << 26) == _lib.WH_ERR_INVALID_SHAPE
+    for heads, dim in ((1 << 10, 1 << 17), (1 << 40, 1 << 24), ((1 << 62) + 4, 2), (1 << 63, 16)):  # the last three wrap
+        assert compact(k=(P,), v=(P + 64,), n_kv_heads=heads, head_dim=dim) == _lib.WH_ERR_INVALID_SHAPE
+        assert b"whole 16-byte pieces" in _lib.load().wh_last_error()

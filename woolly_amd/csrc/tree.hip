@@ -132,9 +132,10 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(const CompactParams P) 
 static int accept(const uint32_t* tokens, const int32_t* parents, const uint32_t* picked, size_t n_seqs, size_t n_tree,
                   uint32_t* path, uint32_t* n_accepted, uint32_t* next_token, const uint32_t* ctx_len,
                   uint32_t* ctx_len_out, uint32_t* history, size_t history_stride, size_t max_ctx, wh_stream_t stream) {
-  if (n_tree > wh::kMaxTreeNodes || n_seqs >= (static_cast<size_t>(1) << 31))
-    return wh::set_error(WH_ERR_INVALID_SHAPE, "tree_accept: %zu nodes of %zu sequences (at most %zu nodes)", n_tree,
-                         n_seqs, wh::kMaxTreeNodes);
+  // a launch has less than 2^32 threads, 64 of them to a sequence
+  if (n_tree > wh::kMaxTreeNodes || n_seqs >> 26)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "tree_accept: %zu nodes (at most %zu) of %zu sequences (less than 2^26)", n_tree,
+                         wh::kMaxTreeNodes, n_seqs);
   if (n_seqs == 0 || n_tree == 0) return WH_OK;
   if (!tokens || !parents || !picked || !path || !n_accepted || !next_token)
     return wh::set_error(WH_ERR_INVALID_ARGUMENT, "tree_accept: null pointer");
@@ -172,9 +173,11 @@ WH_API int wh_tree_accept_in_cache(const uint32_t* tokens, const int32_t* parent
 WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, size_t n_layers, size_t n_seqs,
                                size_t max_ctx, size_t n_kv_heads, size_t head_dim, const uint32_t* path, size_t n_tree,
                                const uint32_t* n_accepted, const uint32_t* ctx_len, wh_stream_t stream) {
-  const size_t row_bytes = n_kv_heads * head_dim * 2;
-  if (row_bytes == 0 || row_bytes % 16 != 0 || row_bytes >> 31)
-    return wh::set_error(WH_ERR_INVALID_SHAPE, "kv_cache_compact: rows of %zu x %zu f16 must be whole 16-byte pieces",
+  // a row is at most 65535 workgroups of 256 pieces
+  size_t row_bytes;
+  if (__builtin_mul_overflow(n_kv_heads, head_dim, &row_bytes) || __builtin_mul_overflow(row_bytes, 2, &row_bytes) ||
+      row_bytes == 0 || row_bytes % 16 != 0 || row_bytes >> 28)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "kv_cache_compact: rows of %zu x %zu f16 must be whole 16-byte pieces, below 2^28 bytes",
                          n_kv_heads, head_dim);
   if (n_tree > wh::kMaxTreeNodes || n_seqs > 65535 || max_ctx == 0 || max_ctx >> 31)
     return wh::set_error(WH_ERR_INVALID_SHAPE,
