@@ -16,32 +16,36 @@ def exact(c, seqs=None):
     those given.  The bound is that of _tree.attention over the keys that have a weight."""
     q, k, v = c.views()
     out, bound = np.zeros((c.n, c.t, c.h, c.d)), np.zeros((c.n, c.t, c.h, 1))
+    c.top = 0.0  # the largest |score|
     for s in range(c.n) if seqs is None else seqs:
-        kc, vc, g = c.kc[s].copy(), c.vc[s].copy(), c.h // c.kv
+        kc, vc, g, ctx = c.kc[s].copy(), c.vc[s].copy(), c.h // c.kv, c.lens[s]
         ps = _tree.paths(c.parents[s])
-        for i, p in enumerate(ps):
-            if p is not None:
-                kc[c.lens[s] + i] = _tree.stored(_tree.rotate(k[s, i], c.lens[s] + len(p) - 1, c.inv))
-                vc[c.lens[s] + i] = _tree.stored(v[s, i].astype(np.float64))
-        for i, p in enumerate(ps):
-            if p is None:
-                continue
-            rows = np.concatenate([np.arange(c.lens[s]), c.lens[s] + np.array(p)]).astype(int)
-            qr = _tree.rotate(q[s, i], c.lens[s] + len(p) - 1, c.inv)
-            for h in range(c.h):
-                kk, vv = kc[rows, h // g].astype(np.float64), vc[rows, h // g].astype(np.float64)
-                with np.errstate(invalid="ignore"):
-                    sc = kk @ qr[h] / np.sqrt(c.d)
-                    if np.isnan(sc).any() or sc.max() == np.inf:
-                        out[s, i, h] = np.nan
-                        continue
-                    some = sc > -np.inf
-                    sc, kk, vv = sc[some], kk[some], vv[some]
-                    w = np.exp(sc - sc.max())
-                    out[s, i, h] = w @ vv / w.sum()
-                mag = (np.abs(kk) @ np.abs(qr[h])).max() / np.sqrt(c.d)
-                e = mag * (2.0 ** -21 + 2 * c.d * 2.0 ** -24 + 2.0 ** -22) + 2.0 ** -20
-                bound[s, i, h] = (2 * e + 300 * 2.0 ** -24) * np.abs(vv).max()
+        there = [t for t, p in enumerate(ps) if p is not None]
+        if not there:
+            continue
+        for t in there:
+            kc[ctx + t] = _tree.stored(_tree.rotate(k[s, t], ctx + len(ps[t]) - 1, c.inv))
+            vc[ctx + t] = _tree.stored(v[s, t].astype(np.float64))
+        rows = ctx + there[-1] + 1
+        for h in range(c.h):
+            kk, vv = kc[:rows, h // g].astype(np.float64), vc[:rows, h // g].astype(np.float64)
+            qr = np.stack([_tree.rotate(q[s, t, h], ctx + len(ps[t]) - 1, c.inv) for t in there])
+            with np.errstate(invalid="ignore"):
+                sc = qr @ kk.T / np.sqrt(c.d)
+                mag = np.abs(qr) @ np.abs(kk).T / np.sqrt(c.d)
+            for i, t in enumerate(there):
+                see = np.concatenate([np.arange(ctx), ctx + np.array(ps[t])]).astype(int)
+                x = sc[i, see]
+                if np.isnan(x).any() or x.max() == np.inf:
+                    out[s, t, h] = np.nan
+                    continue
+                some = x > -np.inf
+                x, vals = x[some], vv[see][some]
+                w = np.exp(x - x.max())
+                out[s, t, h] = w @ vals / w.sum()
+                c.top = max(c.top, float(np.abs(x).max()))
+                e = mag[i, see][some].max() * (2.0 ** -21 + 2 * c.d * 2.0 ** -24 + 2.0 ** -22) + 2.0 ** -20
+                bound[s, t, h] = (2 * e + 300 * 2.0 ** -24) * np.abs(vals).max()
     return (out, bound) if seqs is None else (out[seqs], bound[seqs])
 
 
@@ -254,3 +258,56 @@ def test_rows_of_many_trees(gpu, n, n_tree):
     out, _, _ = c.results()
     assert np.isnan(out[over]).all()
     assert (np.abs(out[some] - want) <= bound).all(), float(np.abs(out[some] - want).max())
+
+
+@pytest.mark.parametrize("heads,kv,d,n_tree,lens,room", [(8, 2, 128, 5, [300], 9), (8, 2, 64, 26, [1000], 9), (8, 2, 128, 26, [4070], 0),
+                                                         (32, 8, 128, 9, [700, 0, 33, 2500], 40), (8, 1, 64, 64, [3000], 4000),
+                                                         (16, 1, 128, 64, [2000], 50000), (8, 8, 64, 30, [100, 5000], 9)])
+def test_errors_are_those_of_f32(gpu, heads, kv, d, n_tree, lens, room):
+    """Over all rows together the roundings are random: far below the bound of a single one, which a lost limb of the
+    queries or the weights (2^-12) would keep."""
+    c = Case(len(lens), n_tree, heads, kv, d, lens, room=room, seed=d + n_tree)
+    want, _ = exact(c)
+    c.upload().launch()
+    got = c.results()[0]
+    rel = float(np.linalg.norm(got - want) / np.linalg.norm(want))
+    print(f"[result] {heads}/{kv}x{d} {n_tree} nodes at {lens}: rel-L2 {rel:.2e}, bar {weights_bar(c.top):.2e}", flush=True)
+    assert rel <= weights_bar(c.top)
+
+
+@pytest.mark.parametrize("d,kv,group", [(64, 2, 2), (128, 2, 2), (128, 1, 8), (64, 8, 1)])
+@pytest.mark.parametrize("n_tree,ctx,room", [(20, 0, 5), (128, 37, 0), (128, 500, 0), (128, 1000, 3000), (70, 4097, 0),
+                                             (33, 17500, 0), (33, 36000, 9)])
+def test_every_key_is_read(gpu, d, kv, group, n_tree, ctx, room):
+    """Without rotation, a query of three or eight times a key has all its weight there: each query row looks for a key of its own,
+    its node's, its parent's, or one at the end of a tile, a stage or a chunk; the row is that key's v."""
+    c = Case(1, n_tree, kv * group, kv, d, [ctx], room=room, shape="chain" if ctx % 2 else "forest", seed=ctx + d)
+    c.inv[:] = 0
+    q, k, v = c.views()
+    k[:] = c.rng.standard_normal(k.shape)
+    paths = _tree.paths(c.parents[0])
+    ends = [e + o for e in (0, 32, 64, 128, 256, 384, 512, 768, 1024, 2048, 4096, 8192, 16384, ctx) for o in (-2, -1, 0, 1)]
+    ends = [e for e in ends if 0 <= e < ctx] or [0]
+    goal = np.zeros((n_tree, kv * group), int)
+    for t in range(n_tree):
+        for h in range(kv * group):
+            pick = (t + 3 * h) % 4
+            if pick == 0 or ctx == 0:
+                goal[t, h] = ctx + paths[t][-1 - (t % 3 == 0 and len(paths[t]) > 1)]
+            elif pick == 1:
+                goal[t, h] = int(c.rng.integers(0, ctx))
+            else:
+                goal[t, h] = ends[(t * kv * group + h) % len(ends)]
+            g = goal[t, h]
+            key = c.kc[0, g, h // group] if g < ctx else k[0, g - ctx, h // group]
+            q[0, t, h] = np.float32(3 if d == 128 else 8) * key.astype(np.float32)
+    want, _ = exact(c)
+    vals = np.concatenate([c.vc[0, :ctx], v[0].astype(np.float16)]).astype(np.float64)
+    for t in range(n_tree):
+        for h in range(kv * group):  # that is what the formula says, too
+            assert np.abs(want[0, t, h] - vals[goal[t, h], h // group]).max() < 0.05
+    c.upload().launch()
+    got = c.results()[0]
+    err = np.linalg.norm(got - want, axis=-1) / np.linalg.norm(want, axis=-1)
+    print(f"[result] keys of {kv}x{group}x{d} at {ctx}: rel-L2 {err.max():.2e} a row, bar {weights_bar(c.top):.2e}", flush=True)
+    assert err.max() <= weights_bar(c.top)
