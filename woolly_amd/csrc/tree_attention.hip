@@ -17,13 +17,13 @@
 //
 // What bounds it.  Short and middle contexts: the launches' dependent loads and
 // their ends.  26 nodes at 4070 positions, 32 / 8 heads of 128 (17.8 MB: 3.7 us at
-// the 4.8 TB/s of a large copy): 4.3 + 14.2 + 4.1 us, of the partial kernel's 14.2
+// the 4.8 TB/s of a large copy): 4.2 + 14.2 + 4.0 us, of the partial kernel's 14.2
 // some 3 until the first data is there, 6 for 4 tiles a wave, 2 for writing 6.9 MB of
-// partial results.  8 sequences of 16 nodes up to 8100, 32 / 4 heads of 64: 5.0 + 13.1
-// + 4.3.  5 nodes at 300 of 312 rows: 3.6 + 10.4.  Long contexts: the matrix cores.  64
-// nodes at 131000: 275 GFLOP of limb products in 250 us, 1.1 PFLOP/s; a large f16
+// partial results.  8 sequences of 16 nodes up to 8100, 32 / 4 heads of 64: 4.9 + 12.9
+// + 4.2.  5 nodes at 300 of 312 rows: 3.6 + 10.7.  Long contexts: the matrix cores.  64
+// nodes at 131000: 275 GFLOP of limb products in 252 us, 1.1 PFLOP/s; a large f16
 // library product reaches 1.15 on this card, where the clock falls under such work
-// (460 k cycles, 57 % of them with a product under way).
+// (467 k cycles, 56 % of them with a product under way).
 //
 // The angle is formed and reduced in 64 bits: in 32 bits p_t * inv_freq is off
 // by up to p_t 2^-24 radians, 0.008 at position 131072.  k is rotated in
@@ -43,8 +43,8 @@
 // Beside one key with nearly all the weight (often the first, whose v is small, so
 // that the others make the output) they keep what f32 would leave them; in that key's own
 // tile they take a turn of their own.  Relative L2 with 90 to 99.9999 % of the weight on
-// one key, up to 130000 positions: 4e-7 to 4e-6, the decode step's 5e-7 to 4e-6 (with m
-// the running maximum alone 1e-5 to 4e-2).
+// one key, up to 130000 positions: 3e-7 to 4e-6, the decode step's 5e-7 to 3e-6 (with m
+// the running maximum alone 1e-5 to 0.2).
 #include <type_traits>
 
 #include "gemm_dev.hpp"
@@ -58,13 +58,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Weights are held in f16 as 2^12 e^{s - m}, hi + lo.  The reference m of a row stays
 // where it is while the weight of a tile's largest score is within [2^-13, 2^3] of it (at
 // most 2^15 in f16), else it moves there, up or down, but never 2^48 below its highest.
-// Scores of deviation 1.3 and 3 move some row's in 3 % and 8 % of the tiles.
+// Scores of deviation 1.3 move some row's in 3 % of the tiles, of 3 in 8 to 12 %: 64 nodes
+// at 131000 positions take 280 and 284 us a call.
 constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f, kMoveDown = -13.0f, kLowest = 48.0f;
 // A row's keys in a tile are four groups, by their parity and by the lane that holds
 // them.  Where the largest weight of a group is below 2^-22 of the reference's (2^-10 in
 // f16: off by 2^-15 of itself), the row moves to the tile's maximum, and where it is so
 // against that too, the tile takes two turns: the keys down to 2^-9 of its largest weight,
-// then the others.  Scores of deviation 5 do so in 3 % of the tiles of 64 keys, of 3 in none.
+// then the others.  Scores of deviation 3 never do, of 5 in 3 % of the tiles of 64 keys and in
+// 13 % of those of 32 (323 us).
 constexpr float kFaint = -22.0f, kNear = 9.0f;
 constexpr int kWholeMask = 4;        // mask words per node
 
@@ -916,7 +918,9 @@ size_t single_rows(int rw, size_t R, size_t D) { return rw > 1 ? 128 : D == 64 ?
 // positions (1 tile) 13.1 / 16.2, 17.0 / 17.4 us, at 4070, 8100 (2) 20.3 / 22.1, 24.6 /
 // 25.1, beyond at 16000 (2) 32.6 / 32.0; 64 nodes at 60 (1) 12.8 / 18.5, at 1000 (2)
 // 20.2 / 21.3, beyond at 16000 (2) 49.1 / 48.3 and at 131000 292 / 276; 4 sequences of
-// 40 nodes at 200, 4070 (1, 2) 16.2 / 19.6, 28.8 / 31.7.
+// 40 nodes at 200, 4070 (1, 2) 16.2 / 19.6, 28.8 / 31.7.  (These, and the figures of
+// single_rows and plan_chunks, were taken with m as the running maximum; a call of either
+// form has taken 0 to 0.5 us more since.)
 int row_tiles(size_t R, size_t D, size_t n_kv, size_t n_seqs, size_t max_ctx) {
   auto fits = [&](size_t rows, size_t keys) {
     const size_t chunks = n_seqs * ((max_ctx + keys - 1) / keys);
