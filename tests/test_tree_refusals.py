@@ -1,4 +1,7 @@
 """More of what the calls for a tree of drafted tokens refuse, without a GPU: every check runs before a launch."""
+import subprocess
+import sys
+
 import pytest
 
 from tests.test_tree_abi import P, accept, compact, logits
@@ -65,3 +68,10 @@ def test_sizes_beyond_a_launch():
     for heads, dim in ((1 << 10, 1 << 17), (1 << 40, 1 << 24), ((1 << 62) + 4, 2), (1 << 63, 16)):  # the last three wrap
         assert compact(k=(P,), v=(P + 64,), n_kv_heads=heads, head_dim=dim) == _lib.WH_ERR_INVALID_SHAPE
         assert b"whole 16-byte pieces" in _lib.load().wh_last_error()
+
+
+def test_a_cache_without_rows_needs_no_workspace():
+    """In a process of its own: the division by its rows would end this one."""
+    code = "from woolly_amd import ops; print(ops.attention_tree_workspace_bytes(1, 5, 32, 8, 128, 0))"
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "0", (run.returncode, run.stderr[-300:])

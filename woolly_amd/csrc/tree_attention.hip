@@ -1074,7 +1074,7 @@ int launch_tree_attention(const TreeAttnArgs& a, void* workspace, hipStream_t s)
 
 WH_API size_t wh_attention_tree_workspace_bytes(size_t n_seqs, size_t n_tree, size_t n_heads, size_t n_kv_heads,
                                                 size_t head_dim, size_t max_ctx) {
-  if (n_seqs == 0 || n_tree == 0 || n_seqs > wh::kMaxTreeSeqs || n_tree > wh::kMaxTreeNodes || max_ctx >> 31 ||
+  if (n_seqs == 0 || n_tree == 0 || max_ctx == 0 || n_seqs > wh::kMaxTreeSeqs || n_tree > wh::kMaxTreeNodes || max_ctx >> 31 ||
       n_seqs * max_ctx >> 32 ||
       !wh::tree_attention_shape_ok(n_heads, n_kv_heads, head_dim))
     return 0;
