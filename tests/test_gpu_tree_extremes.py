@@ -83,7 +83,8 @@ def test_infinite_v_under_rows_that_move_and_rows_that_do_not(gpu, rows, ctx, d)
 
 
 @pytest.mark.parametrize("d,heads,kv", [(64, 8, 2), (128, 8, 2), (128, 32, 2)])
-@pytest.mark.parametrize("rows,ctx", [(300, 45), (300, 200), (3000, 700), (9000, 333)])
+# 12 nodes of 32 heads on 2 KV heads: tiles by one, one, two and four to a workgroup, tiles of 32 keys and two at a time
+@pytest.mark.parametrize("rows,ctx", [(300, 45), (300, 200), (3000, 700), (9000, 333), (60000, 333), (60000, 5000)])
 def test_infinite_keys(gpu, d, heads, kv, rows, ctx):
     """A k of infinity has a score of infinity where q has its sign, and the row is NaN; of -inf where q has the other,
     and the key has weight 0; and NaN where q is 0.  In whole tiles of the cache, in its last rows and in nodes."""
