@@ -63,6 +63,13 @@ pub const WH_GEMV_STREAM: c_int = 1;
 // --------------------------------------------------------------------- limits
 pub const WH_LLAMA_DECODE_NOALLOC_MAX_BYTES: usize = 16 << 20;
 pub const WH_MAX_TREE_NODES: usize = 128;
+pub const WH_MAX_MEMBERS: usize = 4096;
+pub const WH_MAX_BEAMS: usize = 32;
+pub const WH_ROPE_PLAIN: c_int = 0;
+pub const WH_ROPE_LINEAR: c_int = 1;
+pub const WH_ROPE_BASE: c_int = 2;
+pub const WH_ROPE_BY_TURNS: c_int = 3;
+pub const WH_ROPE_BY_INDEX: c_int = 4;
 pub const WH_GGUF_MAX_DIMS: usize = 8;
 
 // ------------------------------------------ GGUF metadata value types (metadata.rs:13-42)
@@ -121,6 +128,36 @@ pub struct wh_ffn_weights {
     pub down: *const c_void,
     pub hidden: usize,
     pub n_ff: usize,
+}
+
+/// How queries and keys are turned by their position (`wh_qk_norm_rope`); device arrays.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct wh_rope_rules {
+    pub inv_freq: *const c_float,
+    pub rot_dim: usize,
+    pub interleaved: c_int,
+    pub magnitude: c_float,
+    pub q_norm: *const c_float,
+    pub k_norm: *const c_float,
+    pub norm_eps: c_float,
+}
+
+/// The rules of a beam search's choice (`wh_beam_select`); device arrays.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct wh_beam_rules {
+    pub n_beams: usize,
+    pub n_out: usize,
+    pub last_tokens: *const u32,
+    pub end_token: u32,
+    pub length_penalty: c_float,
+    pub counts: *const u32,
+    pub counts_out: *mut u32,
+    pub history: *mut u32,
+    pub history_stride: usize,
+    pub len: *const u32,
+    pub len_out: *mut u32,
 }
 
 /// What is done to logits before a token is chosen (`wh_logits_process`); device arrays.
@@ -387,6 +424,37 @@ extern "C" {
                                n_seqs: usize, max_ctx: usize, n_kv_heads: usize, head_dim: usize, path: *const u32,
                                n_tree: usize, n_accepted: *const u32, ctx_len: *const u32,
                                stream: wh_stream_t) -> c_int;
+
+    // several continuations of one prompt
+    pub fn wh_rope_scaled_inv_freq(kind: c_int, base: c_float, rot_dim: usize, factor: c_float, original_ctx: usize,
+                                   low: c_float, high: c_float, out_host: *mut c_float,
+                                   magnitude: *mut c_float) -> c_int;
+    pub fn wh_qk_norm_rope(rules: *const wh_rope_rules, q: *const c_float, k: *const c_float, v: *const c_float,
+                           ldq: usize, ldkv: usize, base_len: *const u32, len: *const u32, n_groups: usize,
+                           n_per: usize, n_new: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize,
+                           q_out: *mut c_float, ldq_out: usize, k_out: *mut c_float, ldk_out: usize,
+                           k_cache: *mut c_void, v_cache: *mut c_void, max_rows: usize, stream: wh_stream_t) -> c_int;
+    pub fn wh_attention_shared_workspace_bytes(n_groups: usize, n_per: usize, n_heads: usize, n_kv_heads: usize,
+                                               head_dim: usize, max_prefix: usize, max_own: usize) -> usize;
+    pub fn wh_attention_shared(q: *const c_float, ldq: usize, prefix_len: *const u32, own_len: *const u32,
+                               n_groups: usize, n_per: usize, k_prefix: *const c_void, v_prefix: *const c_void,
+                               max_prefix: usize, k_own: *const c_void, v_own: *const c_void, max_own: usize,
+                               n_heads: usize, n_kv_heads: usize, head_dim: usize, out: *mut c_float,
+                               workspace: *mut c_void, workspace_bytes: usize, stream: wh_stream_t) -> c_int;
+    pub fn wh_beam_select_workspace_bytes(rules: *const wh_beam_rules, n_seqs: usize, vocab: usize) -> usize;
+    pub fn wh_beam_select(rules: *const wh_beam_rules, logits: *const c_float, ld: usize, n_seqs: usize, vocab: usize,
+                          scores: *const c_float, scores_out: *mut c_float, tokens: *mut u32, parents: *mut u32,
+                          workspace: *mut c_void, workspace_bytes: usize, stream: wh_stream_t) -> c_int;
+    pub fn wh_beam_reorder(states: *mut *mut c_void, n_states: usize, n_seqs: usize, n_beams: usize, max_rows: usize,
+                           row_bytes: usize, parents: *const u32, len: *const u32, pending: usize,
+                           stream: wh_stream_t) -> c_int;
+    pub fn wh_llama_forward_members_workspace_bytes(model: *const wh_llama_model, n_members: usize,
+                                                    max_own: usize) -> usize;
+    pub fn wh_llama_forward_members(model: *const wh_llama_model, rules: *const wh_rope_rules, tokens: *const u32,
+                                    n_members: usize, prefix_len: *const u32, len: *const u32,
+                                    k_own: *mut *mut c_void, v_own: *mut *mut c_void, max_own: usize, x: *mut c_float,
+                                    logits: *mut c_float, workspace: *mut c_void, workspace_bytes: usize,
+                                    stream: wh_stream_t) -> c_int;
 
     // GGUF files (loader.rs:111-295, format.rs, metadata.rs, tensor_info.rs)
     pub fn wh_gguf_open(path: *const c_char, out: *mut *mut wh_gguf) -> c_int;

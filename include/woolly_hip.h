@@ -607,6 +607,161 @@ WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, siz
                                size_t max_ctx, size_t n_kv_heads, size_t head_dim, const uint32_t* path, size_t n_tree,
                                const uint32_t* n_accepted, const uint32_t* ctx_len, wh_stream_t stream);
 
+/* ------------------------------- several continuations of one prompt */
+/* The beams of a search, samples of one prompt, requests behind one system
+ * prompt: n_groups groups of n_per "members".  A group's members share the cache
+ * rows of its prompt (the prefix, [n_groups][max_prefix][n_kv_heads][head_dim]
+ * f16, filled by wh_llama_forward_token or wh_llama_forward_tree), and each has
+ * rows of its own behind them ([n_groups * n_per][max_own][n_kv_heads][head_dim]).
+ * No counterpart in the reference, which runs one sequence.  Lengths are device
+ * memory, read when the call runs: a captured step follows them.  A member's
+ * length counts its own tokens, those of the present step included. */
+
+/* How queries and keys are turned by their position. */
+typedef struct wh_rope_rules {
+  const float* inv_freq;   /* device [rot_dim / 2] (wh_rope_inv_freq, wh_rope_scaled_inv_freq) */
+  size_t rot_dim;          /* the first rot_dim elements of a head turn (even; 0: all), the others stay */
+  int interleaved;         /* pairs (2 i, 2 i + 1) instead of (i, i + rot_dim / 2) */
+  float magnitude;         /* factor of the turned elements (0 counts as 1) */
+  const float* q_norm;     /* device [head_dim]: RMS norm of every query head before it turns (null: none) */
+  const float* k_norm;
+  float norm_eps;
+} wh_rope_rules;
+
+/* Inverse frequencies for contexts longer than the model was trained on
+ * (original_ctx), and the magnitude that goes with them (may be null).  With
+ * f_i = 1 / base^(2i / rot_dim), evaluated in 64 bits:
+ *   WH_ROPE_LINEAR    f_i / factor
+ *   WH_ROPE_BASE      the same with base * factor^(rot_dim / (rot_dim - 2))
+ *   WH_ROPE_BY_TURNS  f_i (g_i + (1 - g_i) / factor), g_i the share of the way
+ *                     from `low` to `high` turns within original_ctx, clamped
+ *   WH_ROPE_BY_INDEX  the same with g_i going from 1 to 0 in equal steps of i,
+ *                     between the whole indices around those of high and low
+ *                     turns; the magnitude is 0.1 log(factor) + 1
+ * low and high only for the last two: 0 < low < high.  Host outputs. */
+enum { WH_ROPE_PLAIN = 0, WH_ROPE_LINEAR = 1, WH_ROPE_BASE = 2, WH_ROPE_BY_TURNS = 3, WH_ROPE_BY_INDEX = 4 };
+WH_API int wh_rope_scaled_inv_freq(int kind, float base, size_t rot_dim, float factor, size_t original_ctx, float low,
+                                   float high, float* out_host, float* magnitude);
+
+/* Norms and rotation of n_new tokens of every member, and their rows into the
+ * members' caches, in one pass.  q, k and v rows are [n_groups * n_per][n_new]
+ * rows of ldq (q) and ldkv (k, v) elements, as for wh_attention_tree.  Token t of
+ * member m is the member's token i = len[m] - n_new + t (the new tokens are its
+ * last ones; where i < 0 it is absent: a shorter prompt of a batch) at position
+ * base_len[group] + i.  Per head, each where its weights are given:
+ *   x = x / sqrt(sum x^2 / head_dim + norm_eps) * weight
+ * then the rotation (the angle in 64 bits), and q_out receives the query rows
+ * (ldq_out; null: nothing), k_out the key rows in f32 (ldk_out), cache row i of
+ * the member k and v rounded to f16.  q_out may be q and k_out k with the same
+ * strides, else they lie apart from all inputs.  An absent token's q_out and
+ * k_out rows are zeros and nothing of it is stored; a token whose row the cache
+ * does not hold (i >= max_rows) is not stored either and its q_out row is NaN.
+ * base_len may be null (0), len null (n_new), the caches null together.
+ * head_dim even and at most 256, fewer than 2^31 rows x heads. */
+WH_API int wh_qk_norm_rope(const wh_rope_rules* rules, const float* q, const float* k, const float* v, size_t ldq,
+                           size_t ldkv, const uint32_t* base_len, const uint32_t* len, size_t n_groups, size_t n_per,
+                           size_t n_new, size_t n_heads, size_t n_kv_heads, size_t head_dim, float* q_out, size_t ldq_out,
+                           float* k_out, size_t ldk_out, void* k_cache, void* v_cache, size_t max_rows,
+                           wh_stream_t stream);
+
+/* Grouped-query attention of one (turned) query per member over its group's
+ * prefix and its own rows:
+ *   out[m][h] = softmax([K_prefix; K_own] q / sqrt(head_dim)) [V_prefix; V_own]
+ * The prefix is read once for all members of a group.  q is [n_groups * n_per]
+ * rows of ldq elements, out [n_groups * n_per][n_heads * head_dim]; prefix_len
+ * [n_groups] and own_len [n_groups * n_per] count filled rows, rows behind them
+ * touch nothing, whatever they hold.  A member without any row has a row of
+ * zeros; one whose length is beyond max_prefix or max_own one of NaN.  max_prefix
+ * or max_own may be 0, its caches and lengths null.  head_dim 64 or 128, n_heads
+ * (at most 1024) a multiple of n_kv_heads, at most WH_MAX_MEMBERS members in
+ * all, out apart from q.  Caches and workspace are 16-byte aligned; the workspace
+ * holds wh_attention_shared_workspace_bytes(..), 0 for shapes that are not taken;
+ * calls that overlap on one workspace race. */
+#define WH_MAX_MEMBERS 4096
+WH_API size_t wh_attention_shared_workspace_bytes(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads,
+                                                  size_t head_dim, size_t max_prefix, size_t max_own);
+WH_API int wh_attention_shared(const float* q, size_t ldq, const uint32_t* prefix_len, const uint32_t* own_len,
+                               size_t n_groups, size_t n_per, const void* k_prefix, const void* v_prefix,
+                               size_t max_prefix, const void* k_own, const void* v_own, size_t max_own, size_t n_heads,
+                               size_t n_kv_heads, size_t head_dim, float* out, void* workspace, size_t workspace_bytes,
+                               wh_stream_t stream);
+
+/* The choice of a beam search.  Beam b of a sequence has score[b], the sum of its
+ * tokens' log-probabilities, and a row of logits l; its continuation by token i
+ * has
+ *   s = score[b] + l_i - log sum_j exp l_j
+ * and of all continuations of a sequence's n_beams beams the n_out with the
+ * highest s / count^length_penalty are chosen, count the continuation's tokens;
+ * of equal ones the lowest beam's, then (in the order of the logits, where the
+ * sums do not tell them apart) the lowest token.  A beam whose last token is
+ * end_token has ended: its one continuation is itself (token end_token, score
+ * and count as they are), and its logits are not read.  A beam whose score is -inf or NaN is not
+ * there (a search begins with one beam at 0, the others at -inf); logits of -inf
+ * or NaN are not allowed, and a row with +inf has no continuation.  Sums and
+ * comparisons are made in 64 bits. */
+#define WH_MAX_BEAMS 32
+typedef struct wh_beam_rules {
+  size_t n_beams;               /* at most WH_MAX_BEAMS */
+  size_t n_out;                 /* at most 2 WH_MAX_BEAMS; 0 counts as n_beams */
+  const uint32_t* last_tokens;  /* [n_seqs][n_beams] (null: none has ended) */
+  uint32_t end_token;
+  float length_penalty;
+  const uint32_t* counts;       /* tokens per beam, [n_seqs][n_beams] (null: 0 each) */
+  uint32_t* counts_out;         /* [n_seqs][n_out] (null: not wanted) */
+  uint32_t* history;            /* tokens of the beams, [n_seqs][n_beams][history_stride] (null: not kept); n_out = n_beams */
+  size_t history_stride;
+  const uint32_t* len;          /* how many of them, [n_seqs][n_beams]; needed by history and len_out */
+  uint32_t* len_out;            /* [n_seqs][n_beams] (null: not wanted); n_out = n_beams */
+} wh_beam_rules;
+
+/* Chooses for n_seqs sequences from [n_seqs * n_beams] rows of vocab logits
+ * (row r at logits + r * ld).  scores_out, tokens and parents are [n_seqs][n_out],
+ * best first; where there are fewer continuations the rest has score -inf, token
+ * 0xFFFFFFFF, count 0 and its own place as parent (at most n_beams - 1).  With a
+ * history, beam i's becomes its parent's first len[parent] tokens and the chosen
+ * one behind them, where they fit; len_out[i] = len[parent] + 1.  Each output may
+ * be its own input (scores_out and scores, counts_out and counts, len_out and len,
+ * tokens and last_tokens) if n_out = n_beams.  The workspace (16-byte aligned)
+ * holds wh_beam_select_workspace_bytes(..); calls that overlap on one workspace
+ * race. */
+WH_API size_t wh_beam_select_workspace_bytes(const wh_beam_rules* rules, size_t n_seqs, size_t vocab);
+WH_API int wh_beam_select(const wh_beam_rules* rules, const float* logits, size_t ld, size_t n_seqs, size_t vocab,
+                          const float* scores, float* scores_out, uint32_t* tokens, uint32_t* parents, void* workspace,
+                          size_t workspace_bytes, wh_stream_t stream);
+
+/* What belongs to the beams follows them: in every state, [n_seqs][n_beams]
+ * [max_rows] rows of row_bytes, beam i's first len[i] - pending rows become its
+ * parent's, in place; len (wh_beam_select's len_out) and parents are
+ * [n_seqs][n_beams].  pending counts the tokens that have no row yet: 1 for the
+ * caches behind a step, whose chosen tokens have theirs in the next.  Rows behind
+ * them stay as they were, and so does a beam whose parent is no beam or whose rows
+ * do not fit.  The states are a host array of n_states device pointers (a layer's
+ * k_own and v_own, ..), aligned to 16 bytes where row_bytes is a multiple of 16,
+ * else to 4; none is named twice, and none lies within another. */
+WH_API int wh_beam_reorder(void* const* states, size_t n_states, size_t n_seqs, size_t n_beams, size_t max_rows,
+                           size_t row_bytes, const uint32_t* parents, const uint32_t* len, size_t pending,
+                           wh_stream_t stream);
+
+/* One step of the model for n_members (at most WH_MAX_TREE_NODES) continuations of the
+ * prompt in its caches: x [n_members][hidden] receives the members' last hidden
+ * states (x = the embedding rows of tokens, then every layer with
+ * wh_qk_norm_rope and wh_attention_shared), logits [n_members][vocab] (may be
+ * null) the head's rows.  Member m's token is its own token len[m] - 1, at
+ * position *prefix_len + len[m] - 1; its k and v go to that row of k_own[layer]
+ * and v_own[layer], host arrays of n_layers device pointers, [n_members][max_own]
+ * [n_kv_heads][head_dim] f16 each.  The model's caches are only read.  rules may be null: the model's
+ * rope_inv_freq, half layout, no norms.  tokens, prefix_len (one number) and len
+ * [n_members] are device memory, x is 16-byte aligned, the model has a token_embd
+ * table; a member whose rows do not fit has NaN.  The workspace (256-byte
+ * aligned) holds wh_llama_forward_members_workspace_bytes(..), 0 for a model or
+ * number that is not taken; calls that overlap on one workspace race.  Launches
+ * only, as the decode step. */
+WH_API size_t wh_llama_forward_members_workspace_bytes(const wh_llama_model* model, size_t n_members, size_t max_own);
+WH_API int wh_llama_forward_members(const wh_llama_model* model, const wh_rope_rules* rules, const uint32_t* tokens,
+                                    size_t n_members, const uint32_t* prefix_len, const uint32_t* len,
+                                    void* const* k_own, void* const* v_own, size_t max_own, float* x, float* logits,
+                                    void* workspace, size_t workspace_bytes, wh_stream_t stream);
+
 /* --------------------------------------------------------------- GGUF files */
 /* A parsed GGUF file: header, metadata key/values and the tensor table of
  * woolly-gguf's GGUFLoader (crates/woolly-gguf/src/loader.rs:111-200), over a

@@ -32,6 +32,9 @@ WH_ERR_TYPE_MISMATCH = 13
 LLAMA_DECODE_NOALLOC_MAX_BYTES = 16 << 20
 # WH_MAX_TREE_NODES: nodes of one tree of drafted tokens
 MAX_TREE_NODES = 128
+# WH_MAX_MEMBERS, WH_MAX_BEAMS: continuations of one call, beams of a sequence
+MAX_MEMBERS = 4096
+MAX_BEAMS = 32
 
 STATUS_NAMES = {
     0: "WH_OK",
@@ -153,6 +156,34 @@ class wh_logits_rules(C.Structure):
     ]
 
 
+class wh_rope_rules(C.Structure):
+    _fields_ = [
+        ("inv_freq", C.c_void_p),
+        ("rot_dim", C.c_size_t),
+        ("interleaved", C.c_int),
+        ("magnitude", C.c_float),
+        ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p),
+        ("norm_eps", C.c_float),
+    ]
+
+
+class wh_beam_rules(C.Structure):
+    _fields_ = [
+        ("n_beams", C.c_size_t),
+        ("n_out", C.c_size_t),
+        ("last_tokens", C.c_void_p),
+        ("end_token", C.c_uint32),
+        ("length_penalty", C.c_float),
+        ("counts", C.c_void_p),
+        ("counts_out", C.c_void_p),
+        ("history", C.c_void_p),
+        ("history_stride", C.c_size_t),
+        ("len", C.c_void_p),
+        ("len_out", C.c_void_p),
+    ]
+
+
 _sz = C.c_size_t
 _vp = C.c_void_p
 _int = C.c_int
@@ -239,6 +270,18 @@ SIGNATURES = {
     "wh_tree_accept": (_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "wh_tree_accept_in_cache": (_int, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp]),
     "wh_kv_cache_compact": (_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp]),
+    "wh_rope_scaled_inv_freq": (_int, [_int, C.c_float, _sz, C.c_float, _sz, C.c_float, C.c_float, _vp, _vp]),
+    "wh_qk_norm_rope": (_int, [C.POINTER(wh_rope_rules), _f32p, _f32p, _f32p, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz,
+                               _sz, _f32p, _sz, _f32p, _sz, _vp, _vp, _sz, _vp]),
+    "wh_attention_shared_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "wh_attention_shared": (_int, [_f32p, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _f32p, _vp,
+                                   _sz, _vp]),
+    "wh_beam_select_workspace_bytes": (_sz, [C.POINTER(wh_beam_rules), _sz, _sz]),
+    "wh_beam_select": (_int, [C.POINTER(wh_beam_rules), _f32p, _sz, _sz, _sz, _f32p, _f32p, _vp, _vp, _vp, _sz, _vp]),
+    "wh_beam_reorder": (_int, [_vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _sz, _vp]),
+    "wh_llama_forward_members_workspace_bytes": (_sz, [C.POINTER(wh_llama_model), _sz, _sz]),
+    "wh_llama_forward_members": (_int, [C.POINTER(wh_llama_model), C.POINTER(wh_rope_rules), _vp, _sz, _vp, _vp, _vp, _vp, _sz,
+                                        _f32p, _f32p, _vp, _sz, _vp]),
     "wh_gguf_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "wh_gguf_open_buffer": (_int, [_vp, _sz, C.POINTER(_vp)]),
     "wh_gguf_close": (_int, [_vp]),

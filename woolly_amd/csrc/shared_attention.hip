@@ -1,0 +1,658 @@
+// shared_attention.hip -- grouped-query attention of one query per member over
+// cache rows that its group shares (the prefix) and rows of its own, on gfx950.
+//
+// With G = n_heads / n_kv_heads and n_per members to a group:
+//   s_j = (q . k_j) / sqrt(d) over the prefix's and the member's own rows
+//   out = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},  m = max_j s_j
+// The prefix's rows are read once for the n_per G query rows that a KV head has
+// in a group.  Two launches:
+//   1. partial: a workgroup per (KV head, 32 query rows, chunk of the prefix), and
+//      per (KV head, member, chunk of its own rows): maximum, sum and weighted
+//      sum of V of each row
+//   2. combine: a wave per 32 query rows and 8 dims joins their chunks
+// The chunks' number is the launch's, their length follows from the lengths on
+// the device.
+//
+// Products on the matrix cores (v_mfma_f32_32x32x16_f16), as tree_attention.hip
+// has them: S^T = K Q^T leaves a lane with 16 keys of one query row, in the order
+// in which the registers are the B operand of O^T = V^T P^T.  q, scaled by a power
+// of two, and the weights are split into two f16 limbs each, K and V are taken as
+// they are.  A weight is 2^12 e^{s - m} (m the running maximum, or up to 2^3 below
+// it), its low limb held times 2^11 and summed apart in each tile, so a weight
+// keeps 2^-22 of itself down to 2^-29 of the largest one, and 2^-51 of that below: what
+// a key with nearly all the weight (often the first one, whose v is small) leaves
+// to the others is as exact as in f32.
+//
+// A wave has its own tiles of 32 keys, its own LDS and no barriers until the
+// chunk's end: the next K tile is asked for when the scores are there, the next V
+// tile when the products are.
+#include <type_traits>
+
+#include "attn_dev.hpp"
+#include "members.hpp"
+#include "tree.hpp"
+
+namespace {
+
+using whd::f32x16, whd::f32x4u, whd::s16x4;
+using whd::read_tr, whd::swap_max, whd::swap_max_nan, whd::swap_sum, whd::swz_k, whd::swz_v;
+
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f;
+constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
+constexpr uint32_t kLeastChunk = 128;  // keys: a tile for every wave
+
+struct Params {
+  const float* q;
+  size_t ldq;
+  const uint32_t *prefix_len, *own_len;
+  const _Float16 *k_prefix, *v_prefix, *k_own, *v_own;
+  float* out;
+  uint32_t n_groups, n_per, max_prefix, max_own, n_heads, n_kv, G;
+  uint32_t R;            // query rows of a KV head in a group: n_per G
+  uint32_t tiles;        // of 32 of them
+  uint32_t own_tiles;    // of a member's G
+  uint32_t own_rows;     // rows of such a tile that are stored: min(G, 32)
+  uint32_t cp, co;       // chunks of a prefix, of a member's own rows
+  uint32_t n_prefix_wgs;
+  float scale;           // log2(e) / sqrt(d)
+  // workspace: partial results (largest score of the row in units of q . k, sum), registers
+  // of the lanes [D / 8][2][rows]
+  float2* ml_p;          // [n_groups][cp][n_kv][tiles][32]
+  float4* acc_p;
+  float2* ml_o;          // [members][co][n_kv][own_tiles][own_rows]
+  float4* acc_o;
+};
+
+// Cache rows of a group's prefix and of a member, 0 where they do not fit.
+__device__ __forceinline__ uint32_t rows_of(const uint32_t* len, uint32_t i, uint32_t most) {
+  const uint32_t n = len ? len[i] : 0;
+  return n <= most ? n : 0;
+}
+__device__ __forceinline__ uint32_t chunk_of(uint32_t rows, uint32_t chunks) {
+  const uint32_t even = (rows + chunks - 1) / chunks;
+  return max((even + 31) / 32 * 32, kLeastChunk);
+}
+
+// Two weights as f16 hi + lo 2^-11: elements i and i + 1 of the fragments.
+__device__ __forceinline__ void split2(float a, float b, half8& hi, half8& lo, int i) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const half2v h = __builtin_convertvector((f32x2{a, b}), half2v);
+  const uint32_t hw = __builtin_bit_cast(uint32_t, h);
+  float ra, rb;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hw), "v"(a));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hw), "v"(b));
+  const half2v r = __builtin_convertvector((f32x2{ra * kLowScale, rb * kLowScale}), half2v);
+  hi[i] = h[0], hi[i + 1] = h[1];
+  lo[i] = r[0], lo[i + 1] = r[1];
+}
+
+template <int D>
+struct Shape {
+  static constexpr int KS = D / 16, DT = D / 32, kQuads = D / 8;
+  static constexpr int kTile = 32 * D * 2;       // bytes of 32 rows of K or V
+  static constexpr int kCopies = kTile / 1024;   // copies of 1 KB per tile
+  static constexpr int kPer = 1024 / (2 * D);    // rows of a copy
+  static constexpr int kStage = kWaves * 2 * kTile;
+  static constexpr int kMerge = kWaves * 32 * (D + 2) * 4;
+  static constexpr int kLds = kStage > kMerge ? kStage : kMerge;
+};
+
+// The query rows of a wave and what it has summed over its keys.
+template <int D>
+struct Rows {
+  half8 qh[D / 16], ql[D / 16];
+  float qs;  // log2(e) / sqrt(d) of a product of scaled q and k
+  int e;     // q is scaled by 2^e
+  f32x16 acc[D / 32];
+  float m, l;
+};
+
+// q rows: lane l has row l % 32, elements 16 j + 8 (l / 32) .. of each step j.
+template <int D>
+__device__ __forceinline__ void load_rows(Rows<D>& w, const float* q, float scale, int h) {
+  constexpr int KS = D / 16;
+  float x[KS][8];
+#pragma unroll
+  for (int j = 0; j < KS; j++) {
+    const f32x4u a = *reinterpret_cast<const f32x4u*>(q + 16 * j + 8 * h), b = *reinterpret_cast<const f32x4u*>(q + 16 * j + 8 * h + 4);
+#pragma unroll
+    for (int u = 0; u < 4; u++) x[j][u] = a[u], x[j][4 + u] = b[u];
+  }
+  float mx = 0.f;
+#pragma unroll
+  for (int j = 0; j < KS; j++)
+#pragma unroll
+    for (int u = 0; u < 8; u++) mx = fmaxf(mx, fabsf(x[j][u]));
+  mx = swap_max(mx);
+  // the row's largest magnitude to [2^13, 2^14): hi + lo hold every element to 2^-22 of
+  // itself or 2^-38 of the largest
+  w.e = mx > 0.f && mx < INFINITY ? min(13 - ilogbf(mx), 100) : 0;
+#pragma unroll
+  for (int j = 0; j < KS; j++)
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float v = ldexpf(x[j][u], w.e);
+      const _Float16 hi = static_cast<_Float16>(v);
+      w.qh[j][u] = hi;
+      w.ql[j][u] = static_cast<_Float16>(v - static_cast<float>(hi));
+    }
+  w.qs = ldexpf(scale, -w.e);
+#pragma unroll
+  for (int d = 0; d < D / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) w.acc[d][i] = 0.f;
+  w.m = -INFINITY;
+  w.l = 0.f;
+}
+
+// Scores of the 32 keys of the K tile at kt (LDS), key 8 (i / 4) + 4 h + i % 4 in s[i].
+template <int D>
+__device__ __forceinline__ f32x16 scores(const Rows<D>& w, uint32_t kt, int l32, int h) {
+  constexpr int KS = D / 16;
+  const uint32_t ko = l32 * 2 * D + 16 * (h ^ swz_k<D>(l32));
+  auto k_at = [&](int j) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) half8*>((uintptr_t)((kt + ko) ^ (32 * j)));
+  };
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+  for (int j = 0; j < KS; j++) {
+    const half8 k = k_at(j);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, w.qh[j], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, w.ql[j], s, 0, 0, 0);
+  }
+  float bad = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) bad = __builtin_elementwise_maximum(bad, s[i]);
+  if (__builtin_expect(__ballot(bad != bad) != 0, 0)) {
+    // A score is NaN: the formula's, or made of an infinity in K that q's limbs meet with both
+    // signs or as 0.  q's sign and size are the hi limb's: its product alone says what an
+    // infinity makes of the score.
+    f32x16 x;
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < KS; j++) {
+      half8 q = w.qh[0];
+#pragma unroll
+      for (int u = 1; u < KS; u++) q = j == u ? w.qh[u] : q;
+      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(j), q, x, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (s[i] != s[i]) s[i] = x[i];
+  }
+  return s;
+}
+
+// The weights of 32 scores (as hi and lo limbs), with the sums so far brought to the row's
+// reference.
+template <int D>
+__device__ __forceinline__ void weigh(Rows<D>& w, f32x16& s, half8 (&ph)[2], half8 (&pl)[2]) {
+  float mt = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; i++) mt = __builtin_elementwise_maximum(mt, s[i]);
+  mt = swap_max_nan(mt);
+  const float by = (mt - w.m) * w.qs;
+  const bool moves = !(by <= kMoveUp) && mt != -INFINITY;  // NaN moves: the row is NaN
+  if (__ballot(moves)) {
+    const float al = moves ? __builtin_amdgcn_exp2f(-by) : 1.f;
+    w.l *= al;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) w.acc[d][i] *= al;
+    if (moves) w.m = mt;
+  }
+  const float mb = w.m == -INFINITY ? 0.f : w.m;
+  float lt[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      float p[2];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * ks + i + k] - mb, w.qs, kPScaleLog2));
+        lt[(i + k) & 3] += p[k];
+      }
+      split2(p[0], p[1], ph[ks], pl[ks], i);
+    }
+  w.l += (lt[0] + lt[1]) + (lt[2] + lt[3]);
+}
+
+// acc += V^T P^T of the V tile at vt.
+template <int D>
+__device__ __forceinline__ void add_values(Rows<D>& w, uint32_t vt, const half8 (&ph)[2], const half8 (&pl)[2], int lane) {
+  const int h = lane >> 5, kq = (lane & 15) >> 2, dq = lane & 3, dg = (lane >> 4) & 1;
+  const uint32_t vo = (4 * h + kq) * 2 * D + 16 * ((2 * dg + (dq >> 1)) ^ swz_v<D>(kq)) + 8 * (dq & 1);
+#pragma unroll
+  for (int d = 0; d < D / 32; d++) {
+    f32x16 t;
+#pragma unroll
+    for (int i = 0; i < 16; i++) t[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      half8 v;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const s16x4 x = read_tr(((vt + vo) ^ (64 * d)) + (16 * ks + 8 * u) * 2 * D);
+        const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[4 * u + i] = y[i];
+      }
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ks], w.acc[d], 0, 0, 0);
+      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ks], t, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) w.acc[d][i] = __builtin_fmaf(t[i], kLowUnscale, w.acc[d][i]);
+  }
+}
+
+// Infinities and NaN of V: limbs and a weight's 0 make NaN of them.  Every weight
+// is above 0, so such an element's sum is that of the infinities and NaN alone:
+// the rows are read again for them.  Keys c0 + 32 first .. in steps of `step` tiles.
+template <int D>
+__device__ __forceinline__ void mend_values(Rows<D>& w, const uint8_t* vbase, size_t RS, uint32_t c0, uint32_t c1, uint32_t first,
+                                            uint32_t step, int lane) {
+  float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int d = 0; d < D / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) zero[i & 3] = __builtin_fmaf(w.acc[d][i], 0.f, zero[i & 3]);
+  if (__builtin_expect(__ballot(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.f)) == 0, 1)) return;
+  const int h = lane >> 5;
+#pragma unroll
+  for (int d = 0; d < D / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (!(fabsf(w.acc[d][i]) < INFINITY)) w.acc[d][i] = 0.f;
+  for (uint32_t base = c0 + 32 * first; base < c1; base += 32 * step) {
+    const uint32_t look = min(base + lane / 2, c1 - 1);  // lane l looks through half of row l / 2
+    const uint4* half = reinterpret_cast<const uint4*>(vbase + look * RS + (lane & 1) * D);
+    bool bad = false;
+    for (int j = 0; j < D / 16; j++) {
+      const uint4 x4 = half[j];
+      for (const uint32_t x : {x4.x, x4.y, x4.z, x4.w}) bad |= (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u;
+    }
+    unsigned long long rows_bad = __ballot(bad);
+    rows_bad = (rows_bad | rows_bad >> 1) & 0x5555555555555555ull;  // bit 2 k: row k
+    while (rows_bad) {
+      const uint32_t key = base + __builtin_ctzll(rows_bad) / 2;
+      rows_bad &= rows_bad - 1;
+      if (key >= c1) break;  // the last row, looked at again
+      const _Float16* v = reinterpret_cast<const _Float16*>(vbase + key * RS);
+#pragma unroll
+      for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float x = static_cast<float>(v[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
+          if (!(fabsf(x) < INFINITY)) w.acc[d][i] += x;
+        }
+    }
+  }
+}
+
+// What a workgroup works on.
+struct Work {
+  const uint8_t *k, *v;   // row 0 of its KV head
+  uint32_t c0, c1;        // its keys
+  uint32_t member0;       // query row r: member member0 + r / G, head kvh G + r % G
+  uint32_t row0, n_rows;  // its first query row, and how many there are
+  float2* ml;             // [stored]
+  float4* acc;            // [D / 8][2][stored]
+  uint32_t stored;        // rows of a tile that are stored
+};
+
+// grid: the prefixes' workgroups, then the members' own rows'; KV head fastest
+// (with 8 KV heads a head's workgroups run on one XCD and share its L2).
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Params P) {
+  using S = Shape<D>;
+  extern __shared__ __align__(256) unsigned char lds[];
+  Work W;
+  uint32_t b = blockIdx.x, kvh;
+  if (b < P.n_prefix_wgs) {
+    kvh = b % P.n_kv;
+    b /= P.n_kv;
+    const uint32_t tile = b % P.tiles;
+    b /= P.tiles;
+    const uint32_t c = b % P.cp, g = b / P.cp;
+    const uint32_t rows = rows_of(P.prefix_len, g, P.max_prefix), chunk = chunk_of(rows, P.cp);
+    W.c0 = c * chunk;
+    W.c1 = min(W.c0 + chunk, rows);
+    const size_t at = (static_cast<size_t>(g) * P.max_prefix * P.n_kv + kvh) * D;
+    W.k = reinterpret_cast<const uint8_t*>(P.k_prefix + at);
+    W.v = reinterpret_cast<const uint8_t*>(P.v_prefix + at);
+    W.member0 = g * P.n_per;
+    W.row0 = tile * 32;
+    W.n_rows = P.R;
+    W.stored = 32;
+    const size_t part = ((static_cast<size_t>(g) * P.cp + c) * P.n_kv + kvh) * P.tiles + tile;
+    W.ml = P.ml_p + part * 32;
+    W.acc = P.acc_p + part * 32 * (D / 4);
+  } else {
+    b -= P.n_prefix_wgs;
+    kvh = b % P.n_kv;
+    b /= P.n_kv;
+    const uint32_t tile = b % P.own_tiles;
+    b /= P.own_tiles;
+    const uint32_t c = b % P.co, m = b / P.co;
+    const uint32_t rows = rows_of(P.own_len, m, P.max_own), chunk = chunk_of(rows, P.co);
+    W.c0 = c * chunk;
+    W.c1 = min(W.c0 + chunk, rows);
+    const size_t at = (static_cast<size_t>(m) * P.max_own * P.n_kv + kvh) * D;
+    W.k = reinterpret_cast<const uint8_t*>(P.k_own + at);
+    W.v = reinterpret_cast<const uint8_t*>(P.v_own + at);
+    W.member0 = m;
+    W.row0 = tile * 32;
+    W.n_rows = P.G;
+    W.stored = P.own_rows;
+    const size_t part = ((static_cast<size_t>(m) * P.co + c) * P.n_kv + kvh) * P.own_tiles + tile;
+    W.ml = P.ml_o + part * P.own_rows;
+    W.acc = P.acc_o + part * P.own_rows * (D / 4);
+  }
+  if (W.c0 >= W.c1) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const size_t RS = static_cast<size_t>(P.n_kv) * D * 2;  // bytes between cache rows
+
+  // A tile's rows go to LDS 1 KB at a time: lane l has chunk l % kChunks of row l / kChunks.
+  // The chunks' permutation of K alternates between copies, that of V does not.
+  constexpr int kChunks = D / 8;
+  const uint32_t kt = lds_addr(lds) + wave * 2 * S::kTile, vt = kt + S::kTile;
+  const uint32_t crow = lane / kChunks, cchunk = lane % kChunks;
+  const uint32_t crs = crow * static_cast<uint32_t>(RS);
+  const uint32_t ck = 16 * (cchunk ^ (D == 128 ? crow : crow >> 1)), cv = 16 * (cchunk ^ swz_v<D>(crow));
+  constexpr int kTurns = D == 128 ? 4 : 2;  // copies until K's permutation repeats
+  auto copy_tile = [&](const uint8_t* src, uint32_t base, uint32_t to, uint32_t chunk, bool is_k) {
+    const uint8_t* p = src + base * RS;
+    const uint32_t last = W.c1 - 1 - base;
+    if (last >= 31) {
+#pragma unroll
+      for (int j = 0; j < S::kCopies; j++) {
+        copy16_to_lds(p, crs + (is_k ? chunk ^ (64 * (j % kTurns)) : chunk), to + 1024 * j);
+        p += S::kPer * RS;
+      }
+    } else {  // rows behind the last one repeat it: their scores are masked, V's are cleared
+#pragma unroll
+      for (int j = 0; j < S::kCopies; j++) {
+        const uint32_t row = min(crow + S::kPer * j, last) * static_cast<uint32_t>(RS);
+        copy16_to_lds(p, row + (is_k ? chunk ^ (64 * (j % kTurns)) : chunk), to + 1024 * j);
+      }
+    }
+  };
+  uint32_t base = W.c0 + 32 * wave;
+  const bool any = base < W.c1;
+  if (any) {
+    copy_tile(W.k, base, kt, ck, true);
+    copy_tile(W.v, base, vt, cv, false);
+  }
+  Rows<D> w;
+  const uint32_t r0 = W.row0 + l32, r = min(r0, W.n_rows - 1);
+  load_rows(w, P.q + (W.member0 + r / P.G) * P.ldq + static_cast<size_t>(kvh * P.G + r % P.G) * D, P.scale, h);
+  if (any) {
+    wait_vmcnt<0>();
+    while (true) {
+      const uint32_t next = base + 32 * kWaves, left = W.c1 - base;
+      const bool more = next < W.c1;
+      f32x16 s = scores(w, kt, l32, h);
+      asm volatile("" ::: "memory");  // the tile's reads are done: the scores came of them
+      if (more) copy_tile(W.k, next, kt, ck, true);
+      if (left < 32) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 8 * (i >> 2) + 4 * h + (i & 3) < static_cast<int>(left) ? s[i] : -INFINITY;
+      }
+      half8 ph[2], pl[2];
+      weigh(w, s, ph, pl);
+      if (more) wait_vmcnt<S::kCopies>(); else wait_vmcnt<0>();  // V, not the next K
+      if (left < 32) {
+        for (uint32_t j = left / S::kPer; j < S::kCopies; j++)
+          if (crow + S::kPer * j >= left)
+            *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + 1024 * j + 16 * lane)) = u32x4{0, 0, 0, 0};
+      }
+      add_values(w, vt, ph, pl, lane);
+      if (!more) break;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      copy_tile(W.v, next, vt, cv, false);
+      wait_vmcnt<S::kCopies>();  // the next K
+      base = next;
+    }
+    mend_values(w, W.v, RS, W.c0, W.c1, wave, kWaves, lane);
+  }
+  w.l = swap_sum(w.l);
+
+  // the waves join in LDS, in fixed order, and store in the lanes' order
+  whd::lds_barrier();
+  constexpr int kQuads = S::kQuads;
+  float4* am = reinterpret_cast<float4*>(lds);                        // [4][D / 8][64]
+  float2* mm = reinterpret_cast<float2*>(am + kWaves * kQuads * 64);  // [4][32]
+#pragma unroll
+  for (int d = 0; d < S::DT; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      am[(wave * kQuads + 4 * d + i) * 64 + lane] =
+          make_float4(w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]);
+  if (h == 0) mm[wave * 32 + l32] = make_float2(w.m, w.l);
+  whd::lds_barrier();
+  float M = -INFINITY, L = 0.f, ew[kWaves];
+  float2 ml[kWaves];
+#pragma unroll
+  for (int u = 0; u < kWaves; u++) {
+    ml[u] = mm[u * 32 + l32];
+    M = __builtin_elementwise_maximum(M, ml[u].x);
+  }
+#pragma unroll
+  for (int u = 0; u < kWaves; u++) {
+    ew[u] = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - M) * w.qs);
+    L = __builtin_fmaf(ml[u].y, ew[u], L);
+  }
+  if (r0 >= W.n_rows) return;
+#pragma unroll
+  for (int q = 0; q < kQuads / kWaves; q++) {
+    const int quad = wave + kWaves * q;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kWaves; u++) {
+      const float4 a = am[(u * kQuads + quad) * 64 + lane];
+      A.x = __builtin_fmaf(a.x, ew[u], A.x);
+      A.y = __builtin_fmaf(a.y, ew[u], A.y);
+      A.z = __builtin_fmaf(a.z, ew[u], A.z);
+      A.w = __builtin_fmaf(a.w, ew[u], A.w);
+    }
+    W.acc[(quad * 2 + h) * W.stored + l32] = A;
+  }
+  if (wave == 0 && h == 0) W.ml[l32] = make_float2(ldexpf(M, -w.e), L);
+}
+
+// ------------------------------------------------------------------ combine
+// out = sum_c acc_c w_c / sum_c l_c w_c, w_c = e^{m_c - m}.  A wave has one register
+// quad of 32 query rows: lane l four dims of row l % 32, so a row's maximum and
+// sums stay in its lane.  Items: KV head fastest, as the partial kernel's
+// workgroups.
+template <int D>
+__global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uint32_t n_items) {
+  constexpr uint32_t kQuads = D / 8;
+  const uint32_t lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  uint32_t b = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (b >= n_items) return;
+  const uint32_t kvh = b % P.n_kv;
+  b /= P.n_kv;
+  const uint32_t quad = b % kQuads;
+  b /= kQuads;
+  const uint32_t tile = b % P.tiles, g = b / P.tiles;
+  const uint32_t r = tile * 32 + l32;
+  if (r >= P.R) return;
+  const uint32_t m = g * P.n_per + r / P.G, hg = r % P.G;
+  const uint32_t plen = P.prefix_len ? P.prefix_len[g] : 0, olen = P.own_len ? P.own_len[m] : 0;
+  float* const o = P.out + (static_cast<size_t>(m) * P.n_heads + kvh * P.G + hg) * D + 32 * (quad >> 2) + 8 * (quad & 3) + 4 * h;
+  if (plen > P.max_prefix || olen > P.max_own || (plen | olen) == 0) {
+    const float fill = (plen | olen) == 0 ? 0.f : __builtin_nanf("");
+    *reinterpret_cast<f32x4u*>(o) = f32x4u{fill, fill, fill, fill};
+    return;
+  }
+  float M = -INFINITY, L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto join = [&](float2 ml, float4 a) {
+    const float mx = __builtin_elementwise_maximum(M, ml.x);
+    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mx) * P.scale);
+    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - mx) * P.scale);
+    M = mx;
+    L = __builtin_fmaf(ml.y, ew, L * keep);
+    A.x = __builtin_fmaf(a.x, ew, A.x * keep);
+    A.y = __builtin_fmaf(a.y, ew, A.y * keep);
+    A.z = __builtin_fmaf(a.z, ew, A.z * keep);
+    A.w = __builtin_fmaf(a.w, ew, A.w * keep);
+  };
+  if (plen) {
+    const uint32_t chunk = chunk_of(plen, P.cp), n = (plen + chunk - 1) / chunk;
+    const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
+    const size_t at = (static_cast<size_t>(g) * P.cp * P.n_kv + kvh) * P.tiles + tile;
+    for (uint32_t c = 0; c < n; c++)
+      join(P.ml_p[(at + c * step) * 32 + l32], P.acc_p[(at + c * step) * 32 * (D / 4) + (quad * 2 + h) * 32 + l32]);
+  }
+  if (olen) {
+    const uint32_t chunk = chunk_of(olen, P.co), n = (olen + chunk - 1) / chunk;
+    const size_t step = static_cast<size_t>(P.n_kv) * P.own_tiles;
+    const size_t at = (static_cast<size_t>(m) * P.co * P.n_kv + kvh) * P.own_tiles + hg / 32;
+    for (uint32_t c = 0; c < n; c++)
+      join(P.ml_o[(at + c * step) * P.own_rows + hg % 32],
+           P.acc_o[(at + c * step) * P.own_rows * (D / 4) + (quad * 2 + h) * P.own_rows + hg % 32]);
+  }
+  // no key's score above -inf: 0 / 0, as the formula
+  *reinterpret_cast<f32x4u*>(o) = f32x4u{A.x, A.y, A.z, A.w} / L;
+}
+
+// ------------------------------------------------------------------ launching
+size_t al256(size_t v) { return (v + 255) / 256 * 256; }
+size_t div_up(size_t a, size_t b) { return (a + b - 1) / b; }
+size_t clamp(size_t v, size_t lo, size_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D, size_t max_prefix, size_t max_own) {
+  Params P{};
+  P.n_groups = static_cast<uint32_t>(n_groups);
+  P.n_per = static_cast<uint32_t>(n_per);
+  P.max_prefix = static_cast<uint32_t>(max_prefix);
+  P.max_own = static_cast<uint32_t>(max_own);
+  P.n_heads = static_cast<uint32_t>(n_heads);
+  P.n_kv = static_cast<uint32_t>(n_kv);
+  P.G = static_cast<uint32_t>(n_heads / n_kv);
+  P.R = static_cast<uint32_t>(n_per) * P.G;
+  P.tiles = (P.R + 31) / 32;
+  P.own_tiles = (P.G + 31) / 32;
+  P.own_rows = P.G < 32 ? P.G : 32;
+  P.scale = kLog2e / sqrtf(static_cast<float>(D));
+  const size_t members = n_groups * n_per, target = 2 * static_cast<size_t>(wh::cu_count());
+  const size_t own = members * n_kv * P.own_tiles, prefix = n_groups * n_kv * P.tiles;
+  P.co = max_own == 0 ? 0 : static_cast<uint32_t>(clamp(target / own, 1, div_up(max_own, 512)));
+  const size_t rest = target > own * P.co + prefix ? target - own * P.co : prefix;
+  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp(rest / prefix, 1, div_up(max_prefix, kLeastChunk)));
+  P.n_prefix_wgs = static_cast<uint32_t>(prefix * P.cp);
+  return P;
+}
+
+// Lays the workspace out (offsets only where base is null); returns its size.
+size_t layout(Params& P, size_t D, void* base) {
+  char* b = static_cast<char*>(base);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* r = b ? b + off : nullptr;
+    off += al256(bytes);
+    return r;
+  };
+  const size_t p = static_cast<size_t>(P.n_groups) * P.cp * P.n_kv * P.tiles * 32;
+  const size_t o = static_cast<size_t>(P.n_groups) * P.n_per * P.co * P.n_kv * P.own_tiles * P.own_rows;
+  P.ml_p = reinterpret_cast<float2*>(take(8 * p));
+  P.acc_p = reinterpret_cast<float4*>(take(4 * D * p));
+  P.ml_o = reinterpret_cast<float2*>(take(8 * o));
+  P.acc_o = reinterpret_cast<float4*>(take(4 * D * o));
+  return off;
+}
+
+template <int D>
+int launch_all(const Params& P, hipStream_t s) {
+  const size_t own = static_cast<size_t>(P.n_groups) * P.n_per * P.co * P.n_kv * P.own_tiles;
+  const size_t wgs = P.n_prefix_wgs + own;
+  if (wgs) {
+    WH_ENSURE_LDS(static_cast<size_t>(Shape<D>::kLds), &shared_partial_kernel<D>);
+    shared_partial_kernel<D><<<static_cast<unsigned>(wgs), 64 * kWaves, Shape<D>::kLds, s>>>(P);
+    WH_LAUNCH_CHECK("shared attention kernel launch");
+  }
+  const size_t items = static_cast<size_t>(P.n_groups) * P.n_kv * P.tiles * (D / 8);
+  shared_combine_kernel<D><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(P, static_cast<uint32_t>(items));
+  WH_LAUNCH_CHECK("shared attention combine launch");
+  return WH_OK;
+}
+
+}  // namespace
+
+namespace wh {
+
+bool shared_attention_shape_ok(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                               size_t max_prefix, size_t max_own) {
+  return (head_dim == 64 || head_dim == 128) && n_kv_heads > 0 && n_heads > 0 && n_heads <= 1024 && n_heads % n_kv_heads == 0 &&
+         n_groups <= kMaxMembers && n_per <= kMaxMembers && n_groups * n_per <= kMaxMembers && !(max_prefix >> 31) &&
+         !(max_own >> 31);
+}
+
+size_t shared_attention_workspace_bytes(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                                        size_t max_prefix, size_t max_own) {
+  Params P = plan(n_groups, n_per, n_heads, n_kv_heads, head_dim, max_prefix, max_own);
+  return layout(P, head_dim, nullptr);
+}
+
+int launch_shared_attention(const SharedAttnArgs& a, void* workspace, hipStream_t s) {
+  Params P = plan(a.n_groups, a.n_per, a.n_heads, a.n_kv_heads, a.head_dim, a.max_prefix, a.max_own);
+  layout(P, a.head_dim, workspace);
+  P.q = a.q, P.ldq = a.ldq;
+  P.prefix_len = a.max_prefix ? a.prefix_len : nullptr;
+  P.own_len = a.max_own ? a.own_len : nullptr;
+  P.k_prefix = static_cast<const _Float16*>(a.k_prefix), P.v_prefix = static_cast<const _Float16*>(a.v_prefix);
+  P.k_own = static_cast<const _Float16*>(a.k_own), P.v_own = static_cast<const _Float16*>(a.v_own);
+  P.out = a.out;
+  return a.head_dim == 128 ? launch_all<128>(P, s) : launch_all<64>(P, s);
+}
+
+}  // namespace wh
+
+WH_API size_t wh_attention_shared_workspace_bytes(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads,
+                                                  size_t head_dim, size_t max_prefix, size_t max_own) {
+  if (n_groups == 0 || n_per == 0 ||
+      !wh::shared_attention_shape_ok(n_groups, n_per, n_heads, n_kv_heads, head_dim, max_prefix, max_own))
+    return 0;
+  return wh::shared_attention_workspace_bytes(n_groups, n_per, n_heads, n_kv_heads, head_dim, max_prefix, max_own);
+}
+
+WH_API int wh_attention_shared(const float* q, size_t ldq, const uint32_t* prefix_len, const uint32_t* own_len,
+                               size_t n_groups, size_t n_per, const void* k_prefix, const void* v_prefix,
+                               size_t max_prefix, const void* k_own, const void* v_own, size_t max_own, size_t n_heads,
+                               size_t n_kv_heads, size_t head_dim, float* out, void* workspace, size_t workspace_bytes,
+                               wh_stream_t stream) {
+  const char* const fn = "attention_shared";
+  if (!wh::shared_attention_shape_ok(n_groups, n_per, n_heads, n_kv_heads, head_dim, max_prefix, max_own))
+    return wh::set_error(WH_ERR_INVALID_SHAPE,
+                         "%s: head_dim %zu, %zu heads, %zu KV heads, %zu x %zu members, %zu and %zu rows not supported", fn,
+                         head_dim, n_heads, n_kv_heads, n_groups, n_per, max_prefix, max_own);
+  if (ldq < n_heads * head_dim)
+    return wh::set_error(WH_ERR_INVALID_SHAPE, "%s: row stride %zu below the rows' %zu elements", fn, ldq, n_heads * head_dim);
+  if (n_groups == 0 || n_per == 0) return WH_OK;
+  if (!q || !out || (max_prefix && (!prefix_len || !k_prefix || !v_prefix)) || (max_own && (!own_len || !k_own || !v_own)))
+    return wh::set_error(WH_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  const void* caches[] = {k_prefix, v_prefix, k_own, v_own, workspace};
+  for (const void* p : caches)
+    if (!wh::aligned(p, 16))
+      return wh::set_error(WH_ERR_INVALID_ARGUMENT, "%s: caches and workspace must be 16-byte aligned", fn);
+  const void* ptrs[] = {q, out, prefix_len, own_len};
+  for (const void* p : ptrs)
+    if (!wh::aligned(p, 4)) return wh::set_error(WH_ERR_INVALID_ARGUMENT, "%s: arrays must be 4-byte aligned", fn);
+  const size_t need = wh::shared_attention_workspace_bytes(n_groups, n_per, n_heads, n_kv_heads, head_dim, max_prefix, max_own);
+  if (workspace_bytes < need || (need && !workspace))
+    return wh::set_error(WH_ERR_BUFFER_TOO_SMALL, "%s: workspace too small: needed %zu bytes, available %zu", fn, need,
+                         workspace ? workspace_bytes : static_cast<size_t>(0));
+  const wh::SharedAttnArgs a{q,     ldq,   prefix_len, own_len, n_groups,   n_per,    k_prefix, v_prefix, max_prefix,
+                             k_own, v_own, max_own,    n_heads, n_kv_heads, head_dim, out};
+  return wh::launch_shared_attention(a, workspace, reinterpret_cast<hipStream_t>(stream));
+}

@@ -47,10 +47,13 @@
 // the running maximum alone 1e-5 to 0.2).
 #include <type_traits>
 
-#include "gemm_dev.hpp"
+#include "attn_dev.hpp"
 #include "tree.hpp"
 
 namespace {
+
+using whd::f32x16, whd::f32x4u, whd::s16x4;
+using whd::read_tr, whd::swap_max, whd::swap_max_nan, whd::swap_sum, whd::swz_k, whd::swz_v;
 
 constexpr int kPrepThreads = 256;
 constexpr int kAttnWaves = 4;
@@ -69,10 +72,6 @@ constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f, kMoveDown = -13.0f, kLowest
 // 13 % of those of 32 (323 us).
 constexpr float kFaint = -22.0f, kNear = 9.0f;
 constexpr int kWholeMask = 4;        // mask words per node
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // four floats of the caller's output
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 struct Params {
   const float *q, *k, *v;
@@ -299,35 +298,6 @@ __global__ __launch_bounds__(kPrepThreads) void tree_prepare_kernel(const Params
 }
 
 // ------------------------------------------------------------------ partial
-// LDS rows of K and V are D f16 without padding (the copies write 16 lanes'
-// chunks in a row), so the 16-byte chunks of row r are permuted: chunk c lies
-// at c ^ swz(r).  K: a wave's operand read takes one chunk of 32 rows; V: a
-// transposing read takes four chunks of each of 4 rows.  With these every 16
-// (32) lanes reach all 64 banks once.
-template <int D>
-__device__ __forceinline__ int swz_k(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
-template <int D>
-__device__ __forceinline__ int swz_v(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
-
-__device__ __forceinline__ s16x4 read_tr(uint32_t lds) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)lds);
-}
-
-// The largest of this lane's and lane ^ 32's value: NaN passed over, or kept.
-__device__ __forceinline__ float swap_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
-}
-__device__ __forceinline__ float swap_max_nan(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  return __builtin_elementwise_maximum(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
-                                       __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
-}
-__device__ __forceinline__ float swap_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-  return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
-}
-
 // The f16 values of a fragment with infinities and NaN replaced by 0.
 __device__ __forceinline__ half8 finite_only(half8 x) {
   u32x4 w = __builtin_bit_cast(u32x4, x);

@@ -333,6 +333,107 @@ def kv_cache_compact(caches: KvCaches, n_seqs: int, max_ctx: int, n_kv_heads: in
                                                _p(ctx_len), _s(stream)))
 
 
+# ------------------------------- several continuations of one prompt
+MAX_MEMBERS, MAX_BEAMS = _lib.MAX_MEMBERS, _lib.MAX_BEAMS
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BY_TURNS, ROPE_BY_INDEX = range(5)
+
+
+def rope_scaled_inv_freq(kind: int, base: float, rot_dim: int, factor: float = 1.0, original_ctx: int = 0, low: float = 0.0,
+                         high: float = 0.0):
+    """Inverse frequencies for contexts longer than original_ctx (wh_rope_scaled_inv_freq): (host array of rot_dim / 2 f32,
+    the magnitude that goes with them)."""
+    import numpy as np
+
+    out, magnitude = np.zeros(rot_dim // 2, np.float32), C.c_float()
+    _lib.check(_lib.load().wh_rope_scaled_inv_freq(kind, base, rot_dim, factor, original_ctx, low, high, out.ctypes.data,
+                                                   C.addressof(magnitude)))
+    return out, float(magnitude.value)
+
+
+class RopeRules:
+    """How queries and keys are normed and turned by their position (wh_rope_rules).  Keeps the buffers that it is given."""
+
+    def __init__(self, inv_freq, rot_dim: int = 0, interleaved: bool = False, magnitude: float = 1.0, q_norm=None, k_norm=None,
+                 eps: float = 1e-5) -> None:
+        self._keep = (inv_freq, q_norm, k_norm)
+        self.rules = _lib.wh_rope_rules(_p(inv_freq) or None, rot_dim, int(interleaved), magnitude, _p(q_norm) or None,
+                                        _p(k_norm) or None, eps)
+        self._ref = C.byref(self.rules)
+
+
+def qk_norm_rope(rules: RopeRules, q, k, v, ldq: int, ldkv: int, base_len, len, n_groups: int, n_per: int, n_new: int,
+                 n_heads: int, n_kv_heads: int, head_dim: int, q_out, ldq_out: int, k_out, ldk_out: int, k_cache, v_cache,
+                 max_rows: int, stream: Stream | None = None) -> None:
+    """Norms of the query and key heads, their rotation by position and the new rows into the members' caches
+    (wh_qk_norm_rope); base_len, len, q_out, k_out and the caches may each be None."""
+    _lib.check(_lib.load().wh_qk_norm_rope(rules._ref, _p(q), _p(k), _p(v) or None, ldq, ldkv, _p(base_len) or None,
+                                           _p(len) or None, n_groups, n_per, n_new, n_heads, n_kv_heads, head_dim,
+                                           _p(q_out) or None, ldq_out, _p(k_out) or None, ldk_out, _p(k_cache) or None,
+                                           _p(v_cache) or None, max_rows, _s(stream)))
+
+
+def attention_shared_workspace_bytes(n_groups: int, n_per: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                                     max_prefix: int, max_own: int) -> int:
+    return int(_lib.load().wh_attention_shared_workspace_bytes(n_groups, n_per, n_heads, n_kv_heads, head_dim, max_prefix,
+                                                               max_own))
+
+
+def attention_shared(q, ldq: int, prefix_len, own_len, n_groups: int, n_per: int, k_prefix, v_prefix, max_prefix: int, k_own,
+                     v_own, max_own: int, n_heads: int, n_kv_heads: int, head_dim: int, out, workspace, workspace_bytes: int,
+                     stream: Stream | None = None) -> None:
+    """Attention of one query per member over its group's prefix, read once for all of them, and its own rows
+    (wh_attention_shared)."""
+    _lib.check(_lib.load().wh_attention_shared(_p(q), ldq, _p(prefix_len) or None, _p(own_len) or None, n_groups, n_per,
+                                               _p(k_prefix) or None, _p(v_prefix) or None, max_prefix, _p(k_own) or None,
+                                               _p(v_own) or None, max_own, n_heads, n_kv_heads, head_dim, _p(out),
+                                               _p(workspace) or None, workspace_bytes, _s(stream)))
+
+
+class BeamRules:
+    """The rules of a beam search's choice: the members of wh_beam_rules by name (sizes, device buffers or addresses).
+    Keeps the buffers that it is given."""
+
+    def __init__(self, n_beams: int, n_out: int = 0, end_token: int = NO_TOKEN, length_penalty: float = 0.0, **members) -> None:
+        r = _lib.wh_beam_rules()
+        r.n_beams, r.n_out, r.end_token, r.length_penalty = n_beams, n_out, end_token, length_penalty
+        known = {n: t for n, t in _lib.wh_beam_rules._fields_}
+        for name, value in members.items():
+            if name not in known:
+                raise TypeError(f"BeamRules has no member {name!r}")
+            setattr(r, name, (_p(value) or None) if known[name] is C.c_void_p else int(value))
+        self._keep = members
+        self.rules = r
+        self._ref = C.byref(r)
+
+
+def beam_select_workspace_bytes(rules: BeamRules, n_seqs: int, vocab: int) -> int:
+    return int(_lib.load().wh_beam_select_workspace_bytes(rules._ref, n_seqs, vocab))
+
+
+def beam_select(rules: BeamRules, logits, ld: int, n_seqs: int, vocab: int, scores, scores_out, tokens, parents, workspace,
+                workspace_bytes: int, stream: Stream | None = None) -> None:
+    """The best continuations of every sequence's beams, and the beams' histories (wh_beam_select)."""
+    _lib.check(_lib.load().wh_beam_select(rules._ref, _p(logits), ld, n_seqs, vocab, _p(scores), _p(scores_out), _p(tokens),
+                                          _p(parents), _p(workspace) or None, workspace_bytes, _s(stream)))
+
+
+class BeamStates:
+    """The arrays that beam_reorder moves, as it takes them."""
+
+    def __init__(self, states) -> None:
+        self._keep = states
+        self.n_states = len(states)
+        self.array = (C.c_void_p * self.n_states)(*[_p(b) or None for b in states])
+        self.address = C.addressof(self.array)
+
+
+def beam_reorder(states: BeamStates, n_seqs: int, n_beams: int, max_rows: int, row_bytes: int, parents, len, pending: int,
+                 stream: Stream | None = None) -> None:
+    """Every beam's rows become its parent's, in place, in all states (wh_beam_reorder)."""
+    _lib.check(_lib.load().wh_beam_reorder(states.address, states.n_states, n_seqs, n_beams, max_rows, row_bytes, _p(parents),
+                                           _p(len), pending, _s(stream)))
+
+
 class LlamaModel:
     """A Llama-shaped model on the device for the decode step: `layers` is a
     list of dicts of device buffers (attn_norm, wq, wk, wv, wo, ffn_norm,
@@ -524,6 +625,21 @@ class LlamaModel:
         _lib.check(_lib.load().wh_llama_forward_tree(C.byref(self.model), _p(tokens), _p(parents), n_tree, _p(ctx_len),
                                                      _p(x), _p(logits) or None, _p(workspace), workspace_bytes,
                                                      _s(stream)))
+
+    def members_workspace_bytes(self, n_members: int, max_own: int) -> int:
+        return int(_lib.load().wh_llama_forward_members_workspace_bytes(C.byref(self.model), n_members, max_own))
+
+    def forward_members(self, tokens, n_members: int, prefix_len, len, own: KvCaches, max_own: int, x, logits, workspace,
+                        workspace_bytes: int, rules: RopeRules | None = None, stream: Stream | None = None) -> None:
+        """One step for several continuations of the prompt in the model's caches (wh_llama_forward_members): x
+        [n_members][hidden] and logits [n_members][vocab] (may be None); the layers' caches in `own` take the tokens'
+        rows.  rules: None for the model's rotation."""
+        if own.n_layers != self.model.n_layers:
+            raise ValueError(f"own caches of {own.n_layers} layers, the model has {self.model.n_layers}")
+        _lib.check(_lib.load().wh_llama_forward_members(
+            C.byref(self.model), rules._ref if rules else None, _p(tokens), n_members, _p(prefix_len), _p(len),
+            C.addressof(own.k), C.addressof(own.v), max_own, _p(x), _p(logits) or None, _p(workspace), workspace_bytes,
+            _s(stream)))
 
     def kv_caches(self) -> KvCaches:
         """The layers' caches for kv_cache_compact."""
