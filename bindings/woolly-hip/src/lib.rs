@@ -111,6 +111,9 @@ pub struct wh_gguf {
     _private: [u8; 0],
 }
 /// A hipStream_t; null is the device's null stream.
+/// C's double, under the name that the header has for it.
+#[allow(non_camel_case_types)]
+pub type double = std::ffi::c_double;
 pub type wh_stream_t = *mut wh_stream_opaque;
 /// A hipEvent_t.
 pub type wh_event_t = *mut wh_event_opaque;
@@ -137,7 +140,7 @@ pub struct wh_rope_rules {
     pub inv_freq: *const c_float,
     pub rot_dim: usize,
     pub interleaved: c_int,
-    pub magnitude: c_float,
+    pub magnitude: double,
     pub q_norm: *const c_float,
     pub k_norm: *const c_float,
     pub norm_eps: c_float,
@@ -428,7 +431,7 @@ extern "C" {
     // several continuations of one prompt
     pub fn wh_rope_scaled_inv_freq(kind: c_int, base: c_float, rot_dim: usize, factor: c_float, original_ctx: usize,
                                    low: c_float, high: c_float, out_host: *mut c_float,
-                                   magnitude: *mut c_float) -> c_int;
+                                   magnitude: *mut double) -> c_int;
     pub fn wh_qk_norm_rope(rules: *const wh_rope_rules, q: *const c_float, k: *const c_float, v: *const c_float,
                            ldq: usize, ldkv: usize, base_len: *const u32, len: *const u32, n_groups: usize,
                            n_per: usize, n_new: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize,

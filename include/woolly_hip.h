@@ -622,7 +622,7 @@ typedef struct wh_rope_rules {
   const float* inv_freq;   /* device [rot_dim / 2] (wh_rope_inv_freq, wh_rope_scaled_inv_freq) */
   size_t rot_dim;          /* the first rot_dim elements of a head turn (even; 0: all), the others stay */
   int interleaved;         /* pairs (2 i, 2 i + 1) instead of (i, i + rot_dim / 2) */
-  float magnitude;         /* factor of the turned elements (0 counts as 1) */
+  double magnitude;        /* factor of the turned elements (0 counts as 1) */
   const float* q_norm;     /* device [head_dim]: RMS norm of every query head before it turns (null: none) */
   const float* k_norm;
   float norm_eps;
@@ -641,7 +641,7 @@ typedef struct wh_rope_rules {
  * low and high only for the last two: 0 < low < high.  Host outputs. */
 enum { WH_ROPE_PLAIN = 0, WH_ROPE_LINEAR = 1, WH_ROPE_BASE = 2, WH_ROPE_BY_TURNS = 3, WH_ROPE_BY_INDEX = 4 };
 WH_API int wh_rope_scaled_inv_freq(int kind, float base, size_t rot_dim, float factor, size_t original_ctx, float low,
-                                   float high, float* out_host, float* magnitude);
+                                   float high, float* out_host, double* magnitude);
 
 /* Norms and rotation of n_new tokens of every member, and their rows into the
  * members' caches, in one pass.  q, k and v rows are [n_groups * n_per][n_new]

@@ -161,7 +161,7 @@ class wh_rope_rules(C.Structure):
         ("inv_freq", C.c_void_p),
         ("rot_dim", C.c_size_t),
         ("interleaved", C.c_int),
-        ("magnitude", C.c_float),
+        ("magnitude", C.c_double),
         ("q_norm", C.c_void_p),
         ("k_norm", C.c_void_p),
         ("norm_eps", C.c_float),

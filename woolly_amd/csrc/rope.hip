@@ -211,7 +211,7 @@ int check_rope_rules(const char* fn, const wh_rope_rules& r, size_t head_dim) {
   if (!r.inv_freq) return set_error(WH_ERR_INVALID_ARGUMENT, "%s: null inv_freq", fn);
   if (!aligned(r.inv_freq, 4) || !aligned(r.q_norm, 4) || !aligned(r.k_norm, 4))
     return set_error(WH_ERR_INVALID_ARGUMENT, "%s: inverse frequencies and norm weights must be 4-byte aligned", fn);
-  if (!(r.magnitude - r.magnitude == 0.f)) return set_error(WH_ERR_INVALID_ARGUMENT, "%s: the magnitude must be finite", fn);
+  if (!(r.magnitude - r.magnitude == 0.0)) return set_error(WH_ERR_INVALID_ARGUMENT, "%s: the magnitude must be finite", fn);
   if ((r.q_norm || r.k_norm) && !(r.norm_eps >= 0.f && r.norm_eps <= 3.402823466e38f))
     return set_error(WH_ERR_INVALID_ARGUMENT, "%s: norm_eps must be finite and not below 0", fn);
   return WH_OK;
@@ -233,14 +233,14 @@ int launch_rope(const wh_rope_rules& r, const RopeArgs& a, hipStream_t s) {
   P.rows = static_cast<uint32_t>(a.n_members * a.n_new);
   P.interleaved = r.interleaved;
   P.eps = r.norm_eps;
-  P.magnitude = r.magnitude == 0.f ? 1.0 : static_cast<double>(r.magnitude);
+  P.magnitude = r.magnitude == 0.0 ? 1.0 : r.magnitude;
   return P.d <= 64 ? launch<32, 1>(P, s) : P.d <= 128 ? launch<64, 1>(P, s) : launch<64, 2>(P, s);
 }
 
 }  // namespace wh
 
 WH_API int wh_rope_scaled_inv_freq(int kind, float base, size_t rot_dim, float factor, size_t original_ctx, float low,
-                                   float high, float* out_host, float* magnitude) {
+                                   float high, float* out_host, double* magnitude) {
   const char* const fn = "rope_scaled_inv_freq";
   if (kind < WH_ROPE_PLAIN || kind > WH_ROPE_BY_INDEX)
     return wh::set_error(WH_ERR_INVALID_ARGUMENT, "%s: unknown kind %d", fn, kind);
@@ -275,7 +275,7 @@ WH_API int wh_rope_scaled_inv_freq(int kind, float base, size_t rot_dim, float f
     out_host[i] = static_cast<float>(f * (g + (1.0 - g) / by));
   }
   if (magnitude)
-    *magnitude = kind == WH_ROPE_BY_INDEX && factor > 1.f ? static_cast<float>(0.1 * log(static_cast<double>(factor)) + 1.0) : 1.f;
+    *magnitude = kind == WH_ROPE_BY_INDEX && factor > 1.f ? 0.1 * log(static_cast<double>(factor)) + 1.0 : 1.0;
   return WH_OK;
 }
 

@@ -344,7 +344,7 @@ def rope_scaled_inv_freq(kind: int, base: float, rot_dim: int, factor: float = 1
     the magnitude that goes with them)."""
     import numpy as np
 
-    out, magnitude = np.zeros(rot_dim // 2, np.float32), C.c_float()
+    out, magnitude = np.zeros(rot_dim // 2, np.float32), C.c_double()
     _lib.check(_lib.load().wh_rope_scaled_inv_freq(kind, base, rot_dim, factor, original_ctx, low, high, out.ctypes.data,
                                                    C.addressof(magnitude)))
     return out, float(magnitude.value)
