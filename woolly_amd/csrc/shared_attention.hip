@@ -42,6 +42,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f;
 constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
 constexpr uint32_t kLeastChunk = 128;  // keys: a tile for every wave
+constexpr uint32_t kStageKeys = 64;    // of a workgroup of 128 query rows
+// LDS reads run one step ahead of the matrix products that take them: neither moves
+// across this
+constexpr int kNoLds = 0x406;
 
 struct Params {
   const float* q;
@@ -56,6 +60,7 @@ struct Params {
   uint32_t own_rows;     // rows of such a tile that are stored: min(G, 32)
   uint32_t cp, co;       // chunks of a prefix, of a member's own rows
   uint32_t n_prefix_wgs;
+  uint32_t rw;           // tiles of a prefix's workgroup
   float scale;           // log2(e) / sqrt(d)
   // workspace: partial results (largest score of the row in units of q . k, sum), registers
   // of the lanes [D / 8][2][rows]
@@ -72,7 +77,7 @@ __device__ __forceinline__ uint32_t rows_of(const uint32_t* len, uint32_t i, uin
 }
 __device__ __forceinline__ uint32_t chunk_of(uint32_t rows, uint32_t chunks) {
   const uint32_t even = (rows + chunks - 1) / chunks;
-  return max((even + 31) / 32 * 32, kLeastChunk);
+  return max((even + kLeastChunk - 1) / kLeastChunk * kLeastChunk, kLeastChunk);
 }
 
 // Two weights as f16 hi + lo 2^-11: elements i and i + 1 of the fragments.
@@ -149,20 +154,23 @@ __device__ __forceinline__ void load_rows(Rows<D>& w, const float* q, float scal
 
 // Scores of the 32 keys of the K tile at kt (LDS), key 8 (i / 4) + 4 h + i % 4 in s[i].
 template <int D>
-__device__ __forceinline__ f32x16 scores(const Rows<D>& w, uint32_t kt, int l32, int h) {
+__device__ __forceinline__ void scores(const Rows<D>& w, uint32_t kt, int l32, int h, f32x16& s) {
   constexpr int KS = D / 16;
-  const uint32_t ko = l32 * 2 * D + 16 * (h ^ swz_k<D>(l32));
+  uint32_t ko = kt + l32 * 2 * D + 16 * (h ^ swz_k<D>(l32));
+  asm("" : "+v"(ko));  // the steps' addresses are made of it each time: they would take registers across the loop
   auto k_at = [&](int j) {
-    return *reinterpret_cast<const __attribute__((address_space(3))) half8*>((uintptr_t)((kt + ko) ^ (32 * j)));
+    return *reinterpret_cast<const __attribute__((address_space(3))) half8*>((uintptr_t)(ko ^ (32 * j)));
   };
-  f32x16 s;
 #pragma unroll
   for (int i = 0; i < 16; i++) s[i] = 0.f;
+  half8 k[2];
+  k[0] = k_at(0);
 #pragma unroll
   for (int j = 0; j < KS; j++) {
-    const half8 k = k_at(j);
-    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, w.qh[j], s, 0, 0, 0);
-    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, w.ql[j], s, 0, 0, 0);
+    if (j + 1 < KS) k[(j + 1) & 1] = k_at(j + 1);
+    __builtin_amdgcn_sched_barrier(kNoLds);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j & 1], w.qh[j], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j & 1], w.ql[j], s, 0, 0, 0);
   }
   float bad = 0.f;
 #pragma unroll
@@ -185,16 +193,17 @@ __device__ __forceinline__ f32x16 scores(const Rows<D>& w, uint32_t kt, int l32,
     for (int i = 0; i < 16; i++)
       if (s[i] != s[i]) s[i] = x[i];
   }
-  return s;
 }
 
-// The weights of 32 scores (as hi and lo limbs), with the sums so far brought to the row's
-// reference.
-template <int D>
-__device__ __forceinline__ void weigh(Rows<D>& w, f32x16& s, half8 (&ph)[2], half8 (&pl)[2]) {
+// The weights of the scores of N tiles (as hi and lo limbs), with the sums so far brought
+// to the row's reference.
+template <int D, int N>
+__device__ __forceinline__ void weigh(Rows<D>& w, const f32x16 (&s)[N], half8 (&ph)[2 * N], half8 (&pl)[2 * N]) {
   float mt = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 16; i++) mt = __builtin_elementwise_maximum(mt, s[i]);
+  for (int n = 0; n < N; n++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) mt = __builtin_elementwise_maximum(mt, s[n][i]);
   mt = swap_max_nan(mt);
   const float by = (mt - w.m) * w.qs;
   const bool moves = !(by <= kMoveUp) && mt != -INFINITY;  // NaN moves: the row is NaN
@@ -210,13 +219,13 @@ __device__ __forceinline__ void weigh(Rows<D>& w, f32x16& s, half8 (&ph)[2], hal
   const float mb = w.m == -INFINITY ? 0.f : w.m;
   float lt[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int ks = 0; ks < 2; ks++)
+  for (int ks = 0; ks < 2 * N; ks++)
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       float p[2];
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * ks + i + k] - mb, w.qs, kPScaleLog2));
+        p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][8 * (ks % 2) + i + k] - mb, w.qs, kPScaleLog2));
         lt[(i + k) & 3] += p[k];
       }
       split2(p[0], p[1], ph[ks], pl[ks], i);
@@ -224,32 +233,58 @@ __device__ __forceinline__ void weigh(Rows<D>& w, f32x16& s, half8 (&ph)[2], hal
   w.l += (lt[0] + lt[1]) + (lt[2] + lt[3]);
 }
 
-// acc += V^T P^T of the V tile at vt.
-template <int D>
-__device__ __forceinline__ void add_values(Rows<D>& w, uint32_t vt, const half8 (&ph)[2], const half8 (&pl)[2], int lane) {
+// acc += V^T P^T of N V tiles, one behind the other from vt on.
+template <int D, int N>
+__device__ __forceinline__ void add_values(Rows<D>& w, uint32_t vt, const half8 (&ph)[2 * N], const half8 (&pl)[2 * N], int lane) {
   const int h = lane >> 5, kq = (lane & 15) >> 2, dq = lane & 3, dg = (lane >> 4) & 1;
-  const uint32_t vo = (4 * h + kq) * 2 * D + 16 * ((2 * dg + (dq >> 1)) ^ swz_v<D>(kq)) + 8 * (dq & 1);
+  uint32_t vo = vt + (4 * h + kq) * 2 * D + 16 * ((2 * dg + (dq >> 1)) ^ swz_v<D>(kq)) + 8 * (dq & 1);
+  asm("" : "+v"(vo));
+  constexpr int kSteps = D / 32 * 2 * N;
+  auto v_at = [&](int step) {  // 32 dims step / (2 N), 16 keys step % (2 N)
+    const int d = step / (2 * N), ks = step % (2 * N);
+    half8 v;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const s16x4 x = read_tr((vo ^ (64 * d)) + (16 * ks + 8 * u) * 2 * D);
+      const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[4 * u + i] = y[i];
+    }
+    return v;
+  };
+  half8 v[2];
+  v[0] = v_at(0);
 #pragma unroll
   for (int d = 0; d < D / 32; d++) {
     f32x16 t;
 #pragma unroll
     for (int i = 0; i < 16; i++) t[i] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-      half8 v;
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const s16x4 x = read_tr(((vt + vo) ^ (64 * d)) + (16 * ks + 8 * u) * 2 * D);
-        const auto y = __builtin_bit_cast(_Float16 __attribute__((ext_vector_type(4))), x);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[4 * u + i] = y[i];
-      }
-      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ks], w.acc[d], 0, 0, 0);
-      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ks], t, 0, 0, 0);
+    for (int ks = 0; ks < 2 * N; ks++) {
+      const int step = d * 2 * N + ks;
+      if (step + 1 < kSteps) v[(step + 1) & 1] = v_at(step + 1);
+      __builtin_amdgcn_sched_barrier(kNoLds);
+      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[step & 1], pl[ks], t, 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[step & 1], ph[ks], w.acc[d], 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) w.acc[d][i] = __builtin_fmaf(t[i], kLowUnscale, w.acc[d][i]);
   }
+}
+
+// Keys from `left` on of a tile are not there: their scores are -inf, their rows of V
+// cleared (they repeat the last row, and 0 times an infinity would be NaN).
+__device__ __forceinline__ void mask_scores(f32x16& s, int left, int h) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) s[i] = 8 * (i >> 2) + 4 * h + (i & 3) < left ? s[i] : -INFINITY;
+}
+template <int D>
+__device__ __forceinline__ void clear_values(uint32_t vt, int left, int lane) {
+  constexpr int kPer = 1024 / (2 * D);
+  const int row = lane / (D / 8);
+  for (int j = max(left, 0) / kPer; j < 32 / kPer; j++)
+    if (row + kPer * j >= left)
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + 1024 * j + 16 * lane)) = u32x4{0, 0, 0, 0};
 }
 
 // Infinities and NaN of V: limbs and a weight's 0 make NaN of them.  Every weight
@@ -302,64 +337,28 @@ struct Work {
   uint32_t c0, c1;        // its keys
   uint32_t member0;       // query row r: member member0 + r / G, head kvh G + r % G
   uint32_t row0, n_rows;  // its first query row, and how many there are
+  uint32_t kvh;
   float2* ml;             // [stored]
   float4* acc;            // [D / 8][2][stored]
   uint32_t stored;        // rows of a tile that are stored
 };
 
-// grid: the prefixes' workgroups, then the members' own rows'; KV head fastest
-// (with 8 KV heads a head's workgroups run on one XCD and share its L2).
 template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Params P) {
+__device__ __forceinline__ void load_rows_of(Rows<D>& w, const Params& P, const Work& W, uint32_t r0, int h) {
+  const uint32_t r = min(r0, W.n_rows - 1);
+  load_rows(w, P.q + (W.member0 + r / P.G) * P.ldq + static_cast<size_t>(W.kvh * P.G + r % P.G) * D, P.scale, h);
+}
+
+// 32 query rows, four waves that share the keys: a wave has tiles wave, wave + 4, ..
+// of the chunk, LDS of its own for one K and one V tile, and no barriers until the
+// end: the next K tile is asked for when the scores are there, the next V tile when the
+// products are.
+template <int D>
+__device__ __forceinline__ void few_rows(const Params& P, const Work& W, unsigned char* lds) {
   using S = Shape<D>;
-  extern __shared__ __align__(256) unsigned char lds[];
-  Work W;
-  uint32_t b = blockIdx.x, kvh;
-  if (b < P.n_prefix_wgs) {
-    kvh = b % P.n_kv;
-    b /= P.n_kv;
-    const uint32_t tile = b % P.tiles;
-    b /= P.tiles;
-    const uint32_t c = b % P.cp, g = b / P.cp;
-    const uint32_t rows = rows_of(P.prefix_len, g, P.max_prefix), chunk = chunk_of(rows, P.cp);
-    W.c0 = c * chunk;
-    W.c1 = min(W.c0 + chunk, rows);
-    const size_t at = (static_cast<size_t>(g) * P.max_prefix * P.n_kv + kvh) * D;
-    W.k = reinterpret_cast<const uint8_t*>(P.k_prefix + at);
-    W.v = reinterpret_cast<const uint8_t*>(P.v_prefix + at);
-    W.member0 = g * P.n_per;
-    W.row0 = tile * 32;
-    W.n_rows = P.R;
-    W.stored = 32;
-    const size_t part = ((static_cast<size_t>(g) * P.cp + c) * P.n_kv + kvh) * P.tiles + tile;
-    W.ml = P.ml_p + part * 32;
-    W.acc = P.acc_p + part * 32 * (D / 4);
-  } else {
-    b -= P.n_prefix_wgs;
-    kvh = b % P.n_kv;
-    b /= P.n_kv;
-    const uint32_t tile = b % P.own_tiles;
-    b /= P.own_tiles;
-    const uint32_t c = b % P.co, m = b / P.co;
-    const uint32_t rows = rows_of(P.own_len, m, P.max_own), chunk = chunk_of(rows, P.co);
-    W.c0 = c * chunk;
-    W.c1 = min(W.c0 + chunk, rows);
-    const size_t at = (static_cast<size_t>(m) * P.max_own * P.n_kv + kvh) * D;
-    W.k = reinterpret_cast<const uint8_t*>(P.k_own + at);
-    W.v = reinterpret_cast<const uint8_t*>(P.v_own + at);
-    W.member0 = m;
-    W.row0 = tile * 32;
-    W.n_rows = P.G;
-    W.stored = P.own_rows;
-    const size_t part = ((static_cast<size_t>(m) * P.co + c) * P.n_kv + kvh) * P.own_tiles + tile;
-    W.ml = P.ml_o + part * P.own_rows;
-    W.acc = P.acc_o + part * P.own_rows * (D / 4);
-  }
-  if (W.c0 >= W.c1) return;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const size_t RS = static_cast<size_t>(P.n_kv) * D * 2;  // bytes between cache rows
-
   // A tile's rows go to LDS 1 KB at a time: lane l has chunk l % kChunks of row l / kChunks.
   // The chunks' permutation of K alternates between copies, that of V does not.
   constexpr int kChunks = D / 8;
@@ -371,17 +370,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Pa
   auto copy_tile = [&](const uint8_t* src, uint32_t base, uint32_t to, uint32_t chunk, bool is_k) {
     const uint8_t* p = src + base * RS;
     const uint32_t last = W.c1 - 1 - base;
+    asm("" : "+v"(chunk));  // made anew each time, as the rows below: across the loop they would take registers
     if (last >= 31) {
 #pragma unroll
       for (int j = 0; j < S::kCopies; j++) {
         copy16_to_lds(p, crs + (is_k ? chunk ^ (64 * (j % kTurns)) : chunk), to + 1024 * j);
         p += S::kPer * RS;
       }
-    } else {  // rows behind the last one repeat it: their scores are masked, V's are cleared
+    } else {  // rows behind the last one repeat it
+      uint32_t row = crow;
 #pragma unroll
       for (int j = 0; j < S::kCopies; j++) {
-        const uint32_t row = min(crow + S::kPer * j, last) * static_cast<uint32_t>(RS);
-        copy16_to_lds(p, row + (is_k ? chunk ^ (64 * (j % kTurns)) : chunk), to + 1024 * j);
+        asm("" : "+v"(row));
+        copy16_to_lds(p, min(row, last) * static_cast<uint32_t>(RS) + (is_k ? chunk ^ (64 * (j % kTurns)) : chunk), to + 1024 * j);
+        row += S::kPer;
       }
     }
   };
@@ -392,29 +394,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Pa
     copy_tile(W.v, base, vt, cv, false);
   }
   Rows<D> w;
-  const uint32_t r0 = W.row0 + l32, r = min(r0, W.n_rows - 1);
-  load_rows(w, P.q + (W.member0 + r / P.G) * P.ldq + static_cast<size_t>(kvh * P.G + r % P.G) * D, P.scale, h);
+  const uint32_t r0 = W.row0 + l32;
+  load_rows_of(w, P, W, r0, h);
   if (any) {
     wait_vmcnt<0>();
     while (true) {
       const uint32_t next = base + 32 * kWaves, left = W.c1 - base;
       const bool more = next < W.c1;
-      f32x16 s = scores(w, kt, l32, h);
-      asm volatile("" ::: "memory");  // the tile's reads are done: the scores came of them
+      f32x16 s[1];
+      scores(w, kt, l32, h, s[0]);  // asks what they are: the tile has been read
       if (more) copy_tile(W.k, next, kt, ck, true);
-      if (left < 32) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 8 * (i >> 2) + 4 * h + (i & 3) < static_cast<int>(left) ? s[i] : -INFINITY;
-      }
+      if (left < 32) mask_scores(s[0], left, h);
       half8 ph[2], pl[2];
-      weigh(w, s, ph, pl);
+      weigh<D, 1>(w, s, ph, pl);
       if (more) wait_vmcnt<S::kCopies>(); else wait_vmcnt<0>();  // V, not the next K
-      if (left < 32) {
-        for (uint32_t j = left / S::kPer; j < S::kCopies; j++)
-          if (crow + S::kPer * j >= left)
-            *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + 1024 * j + 16 * lane)) = u32x4{0, 0, 0, 0};
-      }
-      add_values(w, vt, ph, pl, lane);
+      if (left < 32) clear_values<D>(vt, left, lane);
+      add_values<D, 1>(w, vt, ph, pl, lane);
       if (!more) break;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       copy_tile(W.v, next, vt, cv, false);
@@ -468,62 +463,237 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Pa
   if (wave == 0 && h == 0) W.ml[l32] = make_float2(ldexpf(M, -w.e), L);
 }
 
-// ------------------------------------------------------------------ combine
-// out = sum_c acc_c w_c / sum_c l_c w_c, w_c = e^{m_c - m}.  A wave has one register
-// quad of 32 query rows: lane l four dims of row l % 32, so a row's maximum and
-// sums stay in its lane.  Items: KV head fastest, as the partial kernel's
-// workgroups.
+// 128 query rows, 32 to a wave, that share stages of 64 keys in LDS, two of them in
+// turn: K and V are read from memory once for all of them.
 template <int D>
+__device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsigned char* lds) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const size_t RS = static_cast<size_t>(P.n_kv) * D * 2;
+  constexpr int kChunks = D / 8, kRowsAll = S::kPer * kWaves, kCopies = kStageKeys / kRowsAll;  // the chunks' permutation repeats within kRowsAll rows
+  const uint32_t lds0 = lds_addr(lds);
+  const uint32_t crow = wave * S::kPer + lane / kChunks, cchunk = lane % kChunks;
+  const uint32_t ck = 16 * (cchunk ^ swz_k<D>(crow)), cv = 16 * (cchunk ^ swz_v<D>(crow));
+  const uint32_t crs = crow * static_cast<uint32_t>(RS);
+  auto issue = [&](uint32_t base, uint32_t buf) {
+    const uint8_t *kb = W.k + base * RS, *vb = W.v + base * RS;
+    uint32_t at = lds0 + buf * 4 * S::kTile + wave * 1024;
+    if (base + kStageKeys <= W.c1) {
+#pragma unroll
+      for (int j = 0; j < kCopies; j++) {
+        copy16_to_lds(kb, crs + ck, at);
+        copy16_to_lds(vb, crs + cv, at + 2 * S::kTile);
+        kb += kRowsAll * RS;
+        vb += kRowsAll * RS;
+        at += kWaves * 1024;
+      }
+    } else {  // rows behind the last one repeat it
+      const uint32_t last = W.c1 - 1 - base;
+      uint32_t row = crow;
+#pragma unroll
+      for (int j = 0; j < kCopies; j++) {
+        asm("" : "+v"(row));
+        const uint32_t at_row = min(row, last) * static_cast<uint32_t>(RS);
+        copy16_to_lds(kb, at_row + ck, at);
+        copy16_to_lds(vb, at_row + cv, at + 2 * S::kTile);
+        at += kWaves * 1024;
+        row += kRowsAll;
+      }
+    }
+  };
+  issue(W.c0, 0);
+  Rows<D> w;
+  const uint32_t r0 = W.row0 + 32 * wave + l32;
+  load_rows_of(w, P, W, r0, h);
+  uint32_t buf = 0;
+#pragma unroll 1
+  for (uint32_t base = W.c0; base < W.c1; base += kStageKeys, buf ^= 1) {
+    wait_vmcnt<0>();  // this wave's copies of the stage
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // everyone's; and everyone has read the stage before
+    asm volatile("" ::: "memory");
+    if (base + kStageKeys < W.c1) issue(base + kStageKeys, buf ^ 1);
+    const uint32_t kt = lds0 + buf * 4 * S::kTile, vt = kt + 2 * S::kTile;
+    const int left = W.c1 - base;
+    f32x16 s[2];
+    scores(w, kt, l32, h, s[0]);
+    scores(w, kt + S::kTile, l32, h, s[1]);
+    if (left < static_cast<int>(kStageKeys)) {
+      mask_scores(s[0], left, h);
+      mask_scores(s[1], left - 32, h);
+      clear_values<D>(vt, left, lane);  // the waves store the same, each before it reads the rows
+      clear_values<D>(vt + S::kTile, left - 32, lane);
+    }
+    half8 ph[4], pl[4];
+    weigh<D, 2>(w, s, ph, pl);
+    add_values<D, 2>(w, vt, ph, pl, lane);
+  }
+  mend_values(w, W.v, RS, W.c0, W.c1, 0, 1, lane);
+  w.l = swap_sum(w.l);
+  if (r0 >= W.n_rows) return;
+  float4* const acc = W.acc + wave * 32 * (D / 4);
+#pragma unroll
+  for (int d = 0; d < S::DT; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      acc[((4 * d + i) * 2 + h) * 32 + l32] =
+          make_float4(w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]);
+  if (h == 0) W.ml[wave * 32 + l32] = make_float2(ldexpf(w.m, -w.e), w.l);
+}
+
+// grid: the prefixes' workgroups, then the members' own rows'; KV head fastest
+// (with 8 KV heads a head's workgroups run on one XCD and share its L2).  RW: tiles of
+// 32 query rows that a prefix's workgroup takes, 1 or 4.
+template <int D, int RW>
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Params P) {
+  extern __shared__ __align__(256) unsigned char lds[];
+  Work W;
+  uint32_t b = blockIdx.x;
+  if (b < P.n_prefix_wgs) {
+    W.kvh = b % P.n_kv;
+    b /= P.n_kv;
+    const uint32_t n_rg = (P.tiles + RW - 1) / RW, rg = b % n_rg;
+    b /= n_rg;
+    const uint32_t c = b % P.cp, g = b / P.cp;
+    const uint32_t rows = rows_of(P.prefix_len, g, P.max_prefix), chunk = chunk_of(rows, P.cp);
+    W.c0 = c * chunk;
+    W.c1 = min(W.c0 + chunk, rows);
+    if (W.c0 >= W.c1) return;
+    const size_t at = (static_cast<size_t>(g) * P.max_prefix * P.n_kv + W.kvh) * D;
+    W.k = reinterpret_cast<const uint8_t*>(P.k_prefix + at);
+    W.v = reinterpret_cast<const uint8_t*>(P.v_prefix + at);
+    W.member0 = g * P.n_per;
+    W.row0 = rg * 32 * RW;
+    W.n_rows = P.R;
+    W.stored = 32;
+    const size_t part = ((static_cast<size_t>(g) * P.cp + c) * P.n_kv + W.kvh) * P.tiles + rg * RW;
+    W.ml = P.ml_p + part * 32;
+    W.acc = P.acc_p + part * 32 * (D / 4);
+    if constexpr (RW > 1) {
+      many_rows<D>(P, W, lds);
+      return;
+    }
+  } else {
+    b -= P.n_prefix_wgs;
+    W.kvh = b % P.n_kv;
+    b /= P.n_kv;
+    const uint32_t tile = b % P.own_tiles;
+    b /= P.own_tiles;
+    const uint32_t c = b % P.co, m = b / P.co;
+    const uint32_t rows = rows_of(P.own_len, m, P.max_own), chunk = chunk_of(rows, P.co);
+    W.c0 = c * chunk;
+    W.c1 = min(W.c0 + chunk, rows);
+    if (W.c0 >= W.c1) return;
+    const size_t at = (static_cast<size_t>(m) * P.max_own * P.n_kv + W.kvh) * D;
+    W.k = reinterpret_cast<const uint8_t*>(P.k_own + at);
+    W.v = reinterpret_cast<const uint8_t*>(P.v_own + at);
+    W.member0 = m;
+    W.row0 = tile * 32;
+    W.n_rows = P.G;
+    W.stored = P.own_rows;
+    const size_t part = ((static_cast<size_t>(m) * P.co + c) * P.n_kv + W.kvh) * P.own_tiles + tile;
+    W.ml = P.ml_o + part * P.own_rows;
+    W.acc = P.acc_o + part * P.own_rows * (D / 4);
+  }
+  few_rows<D>(P, W, lds);
+}
+
+// ------------------------------------------------------------------ combine
+// out = sum_c acc_c w_c / sum_c l_c w_c, w_c = e^{m_c - m}.  An item is one register
+// quad of 32 query rows: lane l has four dims of row l % 32, so a row's maximum and
+// sums stay in its lane, and a load of the prefix's results is 1 KB in a row.  W waves
+// take an item: wave w chunks w, w + W, .., kBatch loads in flight, then they join in
+// fixed order.  Items: KV head fastest, as the partial kernel's workgroups.
+template <int D, int W>
 __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uint32_t n_items) {
-  constexpr uint32_t kQuads = D / 8;
+  constexpr uint32_t kQuads = D / 8, kBatch = 8;
+  __shared__ float4 pa[4][64];
+  __shared__ float2 pm[4][64];
   const uint32_t lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
-  uint32_t b = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (b >= n_items) return;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
+  uint32_t b = blockIdx.x * (4 / W) + wave / W;
+  if (b >= n_items) return;  // with W = 4 a workgroup has one item
   const uint32_t kvh = b % P.n_kv;
   b /= P.n_kv;
   const uint32_t quad = b % kQuads;
   b /= kQuads;
   const uint32_t tile = b % P.tiles, g = b / P.tiles;
-  const uint32_t r = tile * 32 + l32;
-  if (r >= P.R) return;
+  const uint32_t r0 = tile * 32 + l32, r = min(r0, P.R - 1);
   const uint32_t m = g * P.n_per + r / P.G, hg = r % P.G;
   const uint32_t plen = P.prefix_len ? P.prefix_len[g] : 0, olen = P.own_len ? P.own_len[m] : 0;
-  float* const o = P.out + (static_cast<size_t>(m) * P.n_heads + kvh * P.G + hg) * D + 32 * (quad >> 2) + 8 * (quad & 3) + 4 * h;
-  if (plen > P.max_prefix || olen > P.max_own || (plen | olen) == 0) {
-    const float fill = (plen | olen) == 0 ? 0.f : __builtin_nanf("");
-    *reinterpret_cast<f32x4u*>(o) = f32x4u{fill, fill, fill, fill};
-    return;
-  }
+  const bool fits = plen <= P.max_prefix && olen <= P.max_own;
   float M = -INFINITY, L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
   auto join = [&](float2 ml, float4 a) {
-    const float mx = __builtin_elementwise_maximum(M, ml.x);
-    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - mx) * P.scale);
-    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - mx) * P.scale);
-    M = mx;
-    L = __builtin_fmaf(ml.y, ew, L * keep);
-    A.x = __builtin_fmaf(a.x, ew, A.x * keep);
-    A.y = __builtin_fmaf(a.y, ew, A.y * keep);
-    A.z = __builtin_fmaf(a.z, ew, A.z * keep);
-    A.w = __builtin_fmaf(a.w, ew, A.w * keep);
+    // a part without a reference has no weight, but NaN of its scores stay
+    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * P.scale);
+    L = __builtin_fmaf(ml.y, ew, L);
+    A.x = __builtin_fmaf(a.x, ew, A.x);
+    A.y = __builtin_fmaf(a.y, ew, A.y);
+    A.z = __builtin_fmaf(a.z, ew, A.z);
+    A.w = __builtin_fmaf(a.w, ew, A.w);
   };
-  if (plen) {
+  auto raise = [&](float to) {
+    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - to) * P.scale);
+    M = to;
+    if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
+  };
+  if (plen && plen <= P.max_prefix) {
     const uint32_t chunk = chunk_of(plen, P.cp), n = (plen + chunk - 1) / chunk;
     const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
     const size_t at = (static_cast<size_t>(g) * P.cp * P.n_kv + kvh) * P.tiles + tile;
-    for (uint32_t c = 0; c < n; c++)
-      join(P.ml_p[(at + c * step) * 32 + l32], P.acc_p[(at + c * step) * 32 * (D / 4) + (quad * 2 + h) * 32 + l32]);
+    for (uint32_t c = part; c < n; c += W * kBatch) {
+      float2 ml[kBatch];
+      float4 a[kBatch];
+      float mx = M;
+#pragma unroll
+      for (uint32_t j = 0; j < kBatch; j++) {
+        const size_t o = (at + min(c + W * j, n - 1) * step) * 32;
+        ml[j] = P.ml_p[o + l32];
+        a[j] = P.acc_p[o * (D / 4) + (quad * 2 + h) * 32 + l32];
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kBatch; j++)
+        if (c + W * j < n) mx = __builtin_elementwise_maximum(mx, ml[j].x);
+      raise(mx);
+#pragma unroll
+      for (uint32_t j = 0; j < kBatch; j++)
+        if (c + W * j < n) join(ml[j], a[j]);
+    }
   }
-  if (olen) {
+  if (olen && olen <= P.max_own) {
     const uint32_t chunk = chunk_of(olen, P.co), n = (olen + chunk - 1) / chunk;
     const size_t step = static_cast<size_t>(P.n_kv) * P.own_tiles;
     const size_t at = (static_cast<size_t>(m) * P.co * P.n_kv + kvh) * P.own_tiles + hg / 32;
-    for (uint32_t c = 0; c < n; c++)
-      join(P.ml_o[(at + c * step) * P.own_rows + hg % 32],
-           P.acc_o[(at + c * step) * P.own_rows * (D / 4) + (quad * 2 + h) * P.own_rows + hg % 32]);
+    for (uint32_t c = part; c < n; c += W) {
+      const size_t o = (at + c * step) * P.own_rows;
+      const float2 ml = P.ml_o[o + hg % 32];
+      const float4 a = P.acc_o[o * (D / 4) + (quad * 2 + h) * P.own_rows + hg % 32];
+      raise(__builtin_elementwise_maximum(M, ml.x));
+      join(ml, a);
+    }
   }
-  // no key's score above -inf: 0 / 0, as the formula
-  *reinterpret_cast<f32x4u*>(o) = f32x4u{A.x, A.y, A.z, A.w} / L;
+  if constexpr (W > 1) {
+    pa[wave][lane] = A;
+    pm[wave][lane] = make_float2(M, L);
+    whd::lds_barrier();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; w++) M = __builtin_elementwise_maximum(M, pm[w][lane].x);
+    L = 0.f;
+    A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; w++) join(pm[w][lane], pa[w][lane]);
+  }
+  if (r0 >= P.R) return;
+  f32x4u v = f32x4u{A.x, A.y, A.z, A.w} / L;  // no key's score above -inf: 0 / 0, as the formula
+  if (!fits || (plen | olen) == 0) {
+    const float fill = fits ? 0.f : __builtin_nanf("");
+    v = f32x4u{fill, fill, fill, fill};
+  }
+  *reinterpret_cast<f32x4u*>(P.out + (static_cast<size_t>(m) * P.n_heads + kvh * P.G + hg) * D + 32 * (quad >> 2) +
+                             8 * (quad & 3) + 4 * h) = v;
 }
 
 // ------------------------------------------------------------------ launching
@@ -545,12 +715,15 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   P.own_tiles = (P.G + 31) / 32;
   P.own_rows = P.G < 32 ? P.G : 32;
   P.scale = kLog2e / sqrtf(static_cast<float>(D));
-  const size_t members = n_groups * n_per, target = 2 * static_cast<size_t>(wh::cu_count());
-  const size_t own = members * n_kv * P.own_tiles, prefix = n_groups * n_kv * P.tiles;
-  P.co = max_own == 0 ? 0 : static_cast<uint32_t>(clamp(target / own, 1, div_up(max_own, 512)));
-  const size_t rest = target > own * P.co + prefix ? target - own * P.co : prefix;
-  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp(rest / prefix, 1, div_up(max_prefix, kLeastChunk)));
+  const size_t members = n_groups * n_per, slots = 2 * static_cast<size_t>(wh::cu_count());
+  P.rw = P.tiles >= 3 ? 4 : 1;
+  // prefix: chunks that fill the CUs' slots once
+  const size_t prefix = n_groups * n_kv * ((P.tiles + P.rw - 1) / P.rw);
+  const size_t least = P.rw == 1 ? kLeastChunk : 512;
+  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp(slots / prefix, 1, div_up(max_prefix, least)));
   P.n_prefix_wgs = static_cast<uint32_t>(prefix * P.cp);
+  const size_t own = members * n_kv * P.own_tiles;
+  P.co = max_own == 0 ? 0 : static_cast<uint32_t>(clamp(slots / own, 1, div_up(max_own, 512)));
   return P;
 }
 
@@ -572,17 +745,27 @@ size_t layout(Params& P, size_t D, void* base) {
   return off;
 }
 
+template <int D, int RW>
+int launch_partial(const Params& P, size_t wgs, hipStream_t s) {
+  WH_ENSURE_LDS(static_cast<size_t>(Shape<D>::kLds), &shared_partial_kernel<D, RW>);
+  shared_partial_kernel<D, RW><<<static_cast<unsigned>(wgs), 64 * kWaves, Shape<D>::kLds, s>>>(P);
+  WH_LAUNCH_CHECK("shared attention kernel launch");
+  return WH_OK;
+}
+
 template <int D>
 int launch_all(const Params& P, hipStream_t s) {
   const size_t own = static_cast<size_t>(P.n_groups) * P.n_per * P.co * P.n_kv * P.own_tiles;
   const size_t wgs = P.n_prefix_wgs + own;
   if (wgs) {
-    WH_ENSURE_LDS(static_cast<size_t>(Shape<D>::kLds), &shared_partial_kernel<D>);
-    shared_partial_kernel<D><<<static_cast<unsigned>(wgs), 64 * kWaves, Shape<D>::kLds, s>>>(P);
-    WH_LAUNCH_CHECK("shared attention kernel launch");
+    const int st = P.rw == 1 ? launch_partial<D, 1>(P, wgs, s) : launch_partial<D, 4>(P, wgs, s);
+    if (st) return st;
   }
   const size_t items = static_cast<size_t>(P.n_groups) * P.n_kv * P.tiles * (D / 8);
-  shared_combine_kernel<D><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(P, static_cast<uint32_t>(items));
+  if (items <= 8 * static_cast<size_t>(wh::cu_count()))
+    shared_combine_kernel<D, 4><<<static_cast<unsigned>(items), 256, 0, s>>>(P, static_cast<uint32_t>(items));
+  else
+    shared_combine_kernel<D, 1><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(P, static_cast<uint32_t>(items));
   WH_LAUNCH_CHECK("shared attention combine launch");
   return WH_OK;
 }
