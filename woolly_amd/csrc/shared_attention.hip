@@ -621,8 +621,6 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
   const uint32_t tile = b % P.tiles, g = b / P.tiles;
   const uint32_t r0 = tile * 32 + l32, r = min(r0, P.R - 1);
   const uint32_t m = g * P.n_per + r / P.G, hg = r % P.G;
-  const uint32_t plen = P.prefix_len ? P.prefix_len[g] : 0, olen = P.own_len ? P.own_len[m] : 0;
-  const bool fits = plen <= P.max_prefix && olen <= P.max_own;
   float M = -INFINITY, L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
   auto join = [&](float2 ml, float4 a) {
@@ -639,20 +637,34 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
     M = to;
     if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
   };
+  // the first loads are asked for with the lengths: what turns out not to be there is not joined
+  const size_t step_p = static_cast<size_t>(P.n_kv) * P.tiles, step_o = static_cast<size_t>(P.n_kv) * P.own_tiles;
+  const size_t at_p = (static_cast<size_t>(g) * P.cp * P.n_kv + kvh) * P.tiles + tile;
+  const size_t at_o = (static_cast<size_t>(m) * P.co * P.n_kv + kvh) * P.own_tiles + hg / 32;
+  float2 ml[kBatch], ml_o = make_float2(-INFINITY, 0.f);
+  float4 a[kBatch], a_o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto load = [&](uint32_t c, uint32_t last) {
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; j++) {
+      const size_t o = (at_p + min(c + W * j, last) * step_p) * 32;
+      ml[j] = P.ml_p[o + l32];
+      a[j] = P.acc_p[o * (D / 4) + (quad * 2 + h) * 32 + l32];
+    }
+  };
+  auto load_own = [&](uint32_t c) {
+    const size_t o = (at_o + c * step_o) * P.own_rows;
+    ml_o = P.ml_o[o + hg % 32];
+    a_o = P.acc_o[o * (D / 4) + (quad * 2 + h) * P.own_rows + hg % 32];
+  };
+  if (part < P.co) load_own(part);
+  if (part < P.cp) load(part, P.cp - 1);
+  const uint32_t plen = P.prefix_len ? P.prefix_len[g] : 0, olen = P.own_len ? P.own_len[m] : 0;
+  const bool fits = plen <= P.max_prefix && olen <= P.max_own;
   if (plen && plen <= P.max_prefix) {
     const uint32_t chunk = chunk_of(plen, P.cp), n = (plen + chunk - 1) / chunk;
-    const size_t step = static_cast<size_t>(P.n_kv) * P.tiles;
-    const size_t at = (static_cast<size_t>(g) * P.cp * P.n_kv + kvh) * P.tiles + tile;
     for (uint32_t c = part; c < n; c += W * kBatch) {
-      float2 ml[kBatch];
-      float4 a[kBatch];
+      if (c != part) load(c, n - 1);
       float mx = M;
-#pragma unroll
-      for (uint32_t j = 0; j < kBatch; j++) {
-        const size_t o = (at + min(c + W * j, n - 1) * step) * 32;
-        ml[j] = P.ml_p[o + l32];
-        a[j] = P.acc_p[o * (D / 4) + (quad * 2 + h) * 32 + l32];
-      }
 #pragma unroll
       for (uint32_t j = 0; j < kBatch; j++)
         if (c + W * j < n) mx = __builtin_elementwise_maximum(mx, ml[j].x);
@@ -664,14 +676,10 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
   }
   if (olen && olen <= P.max_own) {
     const uint32_t chunk = chunk_of(olen, P.co), n = (olen + chunk - 1) / chunk;
-    const size_t step = static_cast<size_t>(P.n_kv) * P.own_tiles;
-    const size_t at = (static_cast<size_t>(m) * P.co * P.n_kv + kvh) * P.own_tiles + hg / 32;
     for (uint32_t c = part; c < n; c += W) {
-      const size_t o = (at + c * step) * P.own_rows;
-      const float2 ml = P.ml_o[o + hg % 32];
-      const float4 a = P.acc_o[o * (D / 4) + (quad * 2 + h) * P.own_rows + hg % 32];
-      raise(__builtin_elementwise_maximum(M, ml.x));
-      join(ml, a);
+      if (c != part) load_own(c);
+      raise(__builtin_elementwise_maximum(M, ml_o.x));
+      join(ml_o, a_o);
     }
   }
   if constexpr (W > 1) {
@@ -715,15 +723,28 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   P.own_tiles = (P.G + 31) / 32;
   P.own_rows = P.G < 32 ? P.G : 32;
   P.scale = kLog2e / sqrtf(static_cast<float>(D));
-  const size_t members = n_groups * n_per, slots = 2 * static_cast<size_t>(wh::cu_count());
-  P.rw = P.tiles >= 3 ? 4 : 1;
-  // prefix: chunks that fill the CUs' slots once
+  const size_t members = n_groups * n_per, cus = static_cast<size_t>(wh::cu_count());
+  // Prefix.  Work: 128 keys of a tile per CU.  Little work, or one that memory bounds (up to
+  // 64 query rows): 32 query rows to a workgroup, one workgroup per CU, as few partial
+  // results.  More: two per CU, so that one's products run beside the other's exponentials,
+  // or 128 rows to a workgroup, whose stages then are read from the L2 once for all of them
+  // (where the rows fill it to 4/5).  A call, 32 / 8 heads of 128, 32 rows at 1 and 2
+  // workgroups per CU, 128 rows at 1 and 2: 32 members (128 rows) at 4000 keys (work 4) 18.6,
+  // 22.8, 21.7, 21.7 us, at 16000 (16) 36.2, 35.5, 33.2, 37.9, at 60000 (59) 105, 99, 94, 92;
+  // 128 members at 2000 (8) 34.9, 37.6, 34.3, 33.8, at 8000 (31) 60, 63, 53, 59, at 30000 (117)
+  // 189, 163, 152, 140; 16 members (64 rows) at 60000 (29) 65, 69; 48 (192 rows) at 60000 151,
+  // 129, 139, 135.  32 / 4 heads of 64: 32 members (256 rows) at 4000 (4) 13.6, 14.5, 15.6,
+  // 15.6, at 16000 (16) 25.1, 22.4, 23.7, 24.8, at 30000 (29) 39.1, 32.7, 35.1, 31.6.
+  const double work = static_cast<double>(n_groups * n_kv * P.tiles) * static_cast<double>(max_prefix) / (128.0 * static_cast<double>(cus));
+  const uint32_t of_four = (P.tiles + 3) / 4 * 4;
+  P.rw = 4 * of_four <= 5 * P.tiles && work >= (D == 128 ? 10.0 : 24.0) ? 4 : 1;
+  const bool two = P.rw == 4 ? D == 64 || work >= 56.0 : P.tiles >= 3 && work >= (D == 128 ? 20.0 : 7.0);
   const size_t prefix = n_groups * n_kv * ((P.tiles + P.rw - 1) / P.rw);
-  const size_t least = P.rw == 1 ? kLeastChunk : 512;
-  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp(slots / prefix, 1, div_up(max_prefix, least)));
+  const size_t least = P.rw == 1 ? kLeastChunk : 256;
+  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp((two ? 2 : 1) * cus / prefix, 1, div_up(max_prefix, least)));
   P.n_prefix_wgs = static_cast<uint32_t>(prefix * P.cp);
   const size_t own = members * n_kv * P.own_tiles;
-  P.co = max_own == 0 ? 0 : static_cast<uint32_t>(clamp(slots / own, 1, div_up(max_own, 512)));
+  P.co = max_own == 0 ? 0 : static_cast<uint32_t>(clamp(cus / own, 1, div_up(max_own, kLeastChunk)));
   return P;
 }
 
