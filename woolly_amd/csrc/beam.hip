@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <memory>
 #include <new>
+#include <type_traits>
 
 #include "members.hpp"
 #include "tree.hpp"
@@ -49,11 +50,17 @@ __device__ __forceinline__ unsigned long long order64(double v) {
   const unsigned long long u = __builtin_bit_cast(unsigned long long, v + 0.0);
   return u >> 63 ? ~u : u | 1ull << 63;
 }
-// The n-th largest of the lanes' numbers, 0 where fewer than n lanes have one above 0.
+__device__ __forceinline__ double value64(unsigned long long o) {
+  return __builtin_bit_cast(double, o >> 63 ? o & ~(1ull << 63) : ~o);
+}
+
+// A bound that at least n of the lanes' numbers reach, 0 where fewer than n lanes have
+// one above 0: the n-th largest of them, cut to its upper kBits bits.
+template <int kBits>
 __device__ __forceinline__ uint32_t nth_largest(uint32_t v, uint32_t n) {
   uint32_t t = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; bit--) {
+  for (int bit = 31; bit >= 32 - kBits; bit--) {
     const uint32_t with = t | 1u << bit;
     if (static_cast<uint32_t>(__builtin_popcountll(__ballot(v >= with))) >= n) t = with;
   }
@@ -70,10 +77,24 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
   }
   return v;
 }
+// Sum over the wave's 64 lanes, in every lane: swaps within rows of 16 lanes, then of
+// rows and halves (as wave_join, tree.hpp).
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  auto lo = [](double x) { return static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, x)); };
+  auto hi = [](double x) { return static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, x) >> 32); };
+  auto make = [](uint32_t l, uint32_t h) { return __builtin_bit_cast(double, static_cast<unsigned long long>(h) << 32 | l); };
+  auto dpp = [](uint32_t x, auto ctrl) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  auto step = [&](auto ctrl) { v += make(dpp(lo(v), ctrl), dpp(hi(v), ctrl)); };
+  step(std::integral_constant<int, 0xB1>{});
+  step(std::integral_constant<int, 0x4E>{});
+  step(std::integral_constant<int, 0x141>{});
+  step(std::integral_constant<int, 0x140>{});
+  const auto l16 = __builtin_amdgcn_permlane16_swap(lo(v), lo(v), false, false), h16 = __builtin_amdgcn_permlane16_swap(hi(v), hi(v), false, false);
+  v = make(l16[0], h16[0]) + make(l16[1], h16[1]);
+  const auto l32 = __builtin_amdgcn_permlane32_swap(lo(v), lo(v), false, false), h32 = __builtin_amdgcn_permlane32_swap(hi(v), hi(v), false, false);
+  return make(l32[0], h32[0]) + make(l32[1], h32[1]);
 }
 
 struct Params {
@@ -102,14 +123,15 @@ __device__ __forceinline__ int state_of(const Params& P, uint32_t row) {
   return P.last && P.last[row] == P.end_token ? kEnded : kOpen;
 }
 
-// grid: (n_chunks, rows).  Thread t has logits 4 t .. 4 t + 3 of each 2048 (VEC:
-// rows 16-byte aligned) or t, t + 512, ..
+// grid: (n_chunks, rows).  Thread t has logits 4 t .. 4 t + 3 of each 4 kThreads
+// (VEC: rows 16-byte aligned) or t, t + kThreads, ..
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
+  constexpr int kWaves = kThreads / 64;
   __shared__ unsigned long long list[kList];
-  __shared__ uint32_t red[kThreads / 64][2];
-  __shared__ unsigned long long red64[kThreads / 64];
-  __shared__ double redd[kThreads / 64];
+  __shared__ uint32_t tops[kWaves], bounds[kWaves], counts[kWaves];
+  __shared__ unsigned long long red64[kWaves];
+  __shared__ double rests[kWaves], terms[kList];
   __shared__ uint32_t n_list;
   const uint32_t row = blockIdx.y, t = threadIdx.x, lane = t & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -117,38 +139,37 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
   const uint32_t i0 = blockIdx.x * kChunk, n = min(P.vocab - i0, static_cast<uint32_t>(kChunk));
   auto at = [&](int j) -> uint32_t { return VEC ? 4 * t + (j & 3) + 4 * kThreads * (j >> 2) : t + kThreads * j; };
   const float* p = P.logits + row * P.ld + i0;
-  uint32_t key[kPer];  // 0: not allowed, or not there
-  {
-    float x[kPer];
-    if constexpr (VEC) {
+  float x[kPer];  // -inf: not allowed, or not there
+  if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < kPer; j += 4) {
-        const uint32_t a = at(j);
-        if (a + 4 <= n) {
-          const float4 v = *reinterpret_cast<const float4*>(p + a);
-          x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
-        } else {
+    for (int j = 0; j < kPer; j += 4) {
+      const uint32_t a = at(j);
+      if (a + 4 <= n) {
+        const float4 v = *reinterpret_cast<const float4*>(p + a);
+        x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
+      } else {
 #pragma unroll
-          for (int k = 0; k < 4; k++) x[j + k] = a + k < n ? p[a + k] : -INFINITY;
-        }
+        for (int k = 0; k < 4; k++) x[j + k] = a + k < n ? p[a + k] : -INFINITY;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; j++) x[j] = at(j) < n ? p[at(j)] : -INFINITY;
     }
+  } else {
 #pragma unroll
-    for (int j = 0; j < kPer; j++) key[j] = x[j] > -INFINITY ? order32(x[j]) : 0u;  // false for NaN
+    for (int j = 0; j < kPer; j++) x[j] = at(j) < n ? p[at(j)] : -INFINITY;
   }
-  uint32_t top = 0;
+  float top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kPer; j++) top = max(top, key[j]);
+  for (int j = 0; j < kPer; j++) {
+    x[j] = fmaxf(x[j], -INFINITY);  // NaN: -inf
+    top = fmaxf(top, x[j]);
+  }
   if (t == 0) n_list = 0;
-  const uint32_t bound = nth_largest(top, P.n_out), wave_top = wave_max_u32(top);
-  if (lane == 0) red[wave][0] = wave_top, red[wave][1] = bound;
+  const uint32_t key = top > -INFINITY ? order32(top) : 0u;
+  const uint32_t bound = nth_largest<20>(key, P.n_out), wave_top = wave_max_u32(key);
+  if (lane == 0) tops[wave] = wave_top, bounds[wave] = bound;
   __syncthreads();
-  uint32_t most = 0, least = 1;
+  uint32_t most = 0, least = order32(-3.402823466e38f);
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; w++) most = max(most, red[w][0]), least = max(least, red[w][1]);
+  for (int w = 0; w < kWaves; w++) most = max(most, tops[w]), least = max(least, bounds[w]);
   const size_t chunk = static_cast<size_t>(row) * P.n_chunks + blockIdx.x;
   uint2* const out = P.lists + chunk * P.n_out;
   if (most == 0) {
@@ -157,70 +178,107 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
     return;
   }
   const float m = value32(most);
-  // logits that reach the bound, counted by all threads together (two barriers)
-  auto count = [&](uint32_t from) {
+  auto key_of = [&](int j) { return static_cast<unsigned long long>(order32(x[j])) << 32 | (0xFFFFFFFFu - (i0 + at(j))); };
+  // what reaches the bound into the list
+  auto gather = [&](float from) __attribute__((always_inline)) {
     uint32_t mine = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; j++) mine += __builtin_popcountll(__ballot(key[j] >= from));
-    if (lane == 0) red[wave][0] = mine;
-    __syncthreads();
-    uint32_t all = 0;
+    for (int j = 0; j < kPer; j++) mine += x[j] >= from;
+    if (mine == 0) return;
+    uint32_t place = atomicAdd(&n_list, mine);
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) all += red[w][0];
-    __syncthreads();
-    return all;
+    for (int j = 0; j < kPer; j++)
+      if (x[j] >= from) {
+        if (place < kList) list[place] = key_of(j);
+        place++;
+      }
   };
-  __syncthreads();
-  uint32_t c = count(least);
-  for (uint32_t up = most; c > kList && up - least > 1;) {  // at `least` n_out or more, above `up` fewer
-    const uint32_t mid = least + (up - least) / 2, n_mid = count(mid);
-    if (n_mid >= P.n_out) least = mid, c = n_mid; else up = mid;
-  }
-  // the largest logits into the list, the others' exponentials summed
-  float rest = 0.f;
+  float from = value32(least);
+  gather(from);
+  auto rest_below = [&](float to) __attribute__((always_inline)) {
+    float rest = 0.f;
 #pragma unroll
-  for (int j = 0; j < kPer; j++)
-    if (key[j] && key[j] < least) rest += __builtin_amdgcn_exp2f((value32(key[j]) - m) * 1.4426950408889634f);
-  double sum = rest;
-#pragma unroll
-  for (int j = 0; j < kPer; j++) {
-    if (key[j] < least) continue;
-    const uint32_t place = atomicAdd(&n_list, 1u);
-    if (place < kList) list[place] = static_cast<unsigned long long>(key[j]) << 32 | (0xFFFFFFFFu - (i0 + at(j)));
-    sum += exp(static_cast<double>(value32(key[j])) - static_cast<double>(m));
-  }
-  sum = wave_sum_f64(sum);
-  if (lane == 0) redd[wave] = sum;
+    for (int j = 0; j < kPer; j++) {
+      const float e = __builtin_amdgcn_exp2f((x[j] - m) * 1.4426950408889634f);
+      rest += x[j] < to ? e : 0.f;
+    }
+    const double sum = wave_sum_f64(rest);
+    if (lane == 0) rests[wave] = sum;
+  };
+  rest_below(from);
   __syncthreads();
-  if (t == 0) {
-    double s = 0.0;
-    for (int w = 0; w < kThreads / 64; w++) s += redd[w];
-    P.sums[chunk] = s;
+  uint32_t c = n_list;
+  if (__builtin_expect(c > kList, 0)) {
+    // the bound halved on: at `least` n_out or more, above `up` fewer (or all the same)
+    auto count = [&](float f) __attribute__((always_inline)) {
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) mine += __builtin_popcountll(__ballot(x[j] >= f));
+      __syncthreads();
+      if (lane == 0) counts[wave] = mine;
+      __syncthreads();
+      uint32_t all = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) all += counts[w];
+      return all;
+    };
+    for (uint32_t up = most; c > kList && up - least > 1;) {
+      const uint32_t mid = least + (up - least) / 2, n_mid = count(value32(mid));
+      if (n_mid >= P.n_out) least = mid, c = n_mid; else up = mid;
+    }
+    from = value32(least);
+    __syncthreads();
+    if (t == 0) n_list = 0;
+    __syncthreads();
+    if (c <= kList) gather(from);
+    rest_below(c <= kList ? from : INFINITY);
+    __syncthreads();
   }
   if (c <= kList) {
-    if (t >= c && t < P.n_out) out[t] = make_uint2(0, kNoToken);
-    if (t < c) {
-      const unsigned long long k = list[t];
-      uint32_t before = 0;
-      for (uint32_t j = 0; j < c; j++) before += list[j] > k;
-      if (before < P.n_out) out[before] = make_uint2(static_cast<uint32_t>(k >> 32), 0xFFFFFFFFu - static_cast<uint32_t>(k));
+    // a thread's place is the number of those before it; the sum is made in their order (the
+    // list's own is whichever came first)
+    if (t < kList) {
+      if (t >= c && t < P.n_out) out[t] = make_uint2(0, kNoToken);
+      if (t < c) {
+        const unsigned long long k = list[t];
+        uint32_t before = 0;
+        for (uint32_t j = 0; j < c; j++) before += list[j] > k;
+        if (before < P.n_out) out[before] = make_uint2(static_cast<uint32_t>(k >> 32), 0xFFFFFFFFu - static_cast<uint32_t>(k));
+        terms[before] = exp(static_cast<double>(value32(static_cast<uint32_t>(k >> 32))) - static_cast<double>(m));
+      }
+    }
+    __syncthreads();
+    if (wave == 0) {
+      double sum = 0.0;
+#pragma unroll
+      for (uint32_t i = lane; i < kList; i += 64)
+        if (i < c) sum += terms[i];
+      sum = wave_sum_f64(sum);
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) sum += rests[w];
+      if (lane == 0) P.sums[chunk] = sum;
     }
     return;
   }
   // too many that are equal: the highest below the last one, n_out times
+  if (t == 0) {
+    double sum = 0.0;
+    for (int w = 0; w < kWaves; w++) sum += rests[w];
+    P.sums[chunk] = sum;
+  }
   unsigned long long last = ~0ull;
   for (uint32_t i = 0; i < P.n_out; i++) {
     unsigned long long best = 0;
 #pragma unroll
     for (int j = 0; j < kPer; j++) {
-      const unsigned long long k = static_cast<unsigned long long>(key[j]) << 32 | (0xFFFFFFFFu - (i0 + at(j)));
-      if (key[j] && k < last && k > best) best = k;
+      const unsigned long long k = key_of(j);
+      if (x[j] > -INFINITY && k < last && k > best) best = k;
     }
     best = wave_max_u64(best);
     if (lane == 0) red64[wave] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) best = red64[w] > best ? red64[w] : best;
+    for (int w = 0; w < kWaves; w++) best = red64[w] > best ? red64[w] : best;
     __syncthreads();
     last = best;
     if (t == 0) out[i] = make_uint2(static_cast<uint32_t>(best >> 32), 0xFFFFFFFFu - static_cast<uint32_t>(best));
@@ -244,10 +302,12 @@ __device__ __forceinline__ unsigned long long rank_of(double s, double norm, flo
   return order64(alpha == 0.f ? s : s / norm);
 }
 
-// grid: n_seqs.
+// grid: n_seqs.  A thread has one of the sequence's lists, or several.
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const Params P) {
+  constexpr uint32_t kHead = 4;  // entries of a list that are asked for at once
   __shared__ double lse[wh::kMaxBeams], score[wh::kMaxBeams], norm[wh::kMaxBeams];
   __shared__ int state[wh::kMaxBeams];
+  __shared__ uint32_t tops[wh::kMaxBeams];
   __shared__ uint32_t red[kPickThreads / 64];
   __shared__ Cand best[kPickThreads / 64];
   __shared__ Cand list[kPickList];
@@ -256,65 +316,98 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const Params P)
   __shared__ uint32_t n_list;
   const uint32_t s = blockIdx.x, t = threadIdx.x, lane = t & 63, row0 = s * P.n_beams;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  if (t == 0) n_list = 0;
-  if (t < 2 * wh::kMaxBeams) chosen[t] = Cand{0, 0, 0, kNoToken};
-  for (uint32_t b = wave; b < P.n_beams; b += kPickThreads / 64) {
-    const uint32_t row = row0 + b;
-    int st = state_of(P, row);
-    double l = 0.0;
-    if (st == kOpen) {
-      const size_t c0 = static_cast<size_t>(row) * P.n_chunks;
-      uint32_t most = 0;
-      for (uint32_t c = lane; c < P.n_chunks; c += 64) most = max(most, P.lists[(c0 + c) * P.n_out].x);
-      most = wave_max_u32(most);
-      const double m = value32(most);
-      double sum = 0.0;
-      for (uint32_t c = lane; c < P.n_chunks; c += 64) {
-        const uint32_t x = P.lists[(c0 + c) * P.n_out].x;
-        if (x) sum += P.sums[c0 + c] * exp(static_cast<double>(value32(x)) - m);
-      }
-      sum = wave_sum_f64(sum);
-      l = m + log(sum);
-      if (most == 0 || !(l < INFINITY)) st = kGone;  // no token is allowed, or one at +inf
-    }
-    if (lane == 0) {
-      const uint32_t count = (P.counts ? P.counts[row] : 0u) + (st == kOpen);
-      lse[b] = l;
-      score[b] = P.scores[row];
-      norm[b] = P.alpha == 0.f ? 1.0 : pow(static_cast<double>(max(count, 1u)), static_cast<double>(P.alpha));
-      state[b] = st;
-    }
-  }
-  __syncthreads();
   const uint32_t n_lists = P.n_beams * P.n_chunks, total = n_lists * P.n_out;
   const uint2* const lists = P.lists + static_cast<size_t>(row0) * P.n_chunks * P.n_out;
+  const double* const sums = P.sums + static_cast<size_t>(row0) * P.n_chunks;
+  // asked for before it is known which of it counts (a beam that has ended wrote none)
+  uint2 head[kHead];
+  double sum0 = 0.0;
+  if (t < n_lists) {
+    sum0 = sums[t];
+#pragma unroll
+    for (uint32_t j = 0; j < kHead; j++) head[j] = j < P.n_out ? lists[static_cast<size_t>(t) * P.n_out + j] : make_uint2(0, kNoToken);
+  }
+  if (t == 0) n_list = 0;
+  if (t < 2 * wh::kMaxBeams) chosen[t] = Cand{0, 0, 0, kNoToken};
+  if (t < P.n_beams) {
+    const uint32_t row = row0 + t;
+    const int st = state_of(P, row);
+    const uint32_t count = (P.counts ? P.counts[row] : 0u) + (st == kOpen);
+    tops[t] = 0;
+    state[t] = st;
+    score[t] = P.scores[row];
+    norm[t] = P.alpha == 0.f ? 1.0 : pow(static_cast<double>(max(count, 1u)), static_cast<double>(P.alpha));
+  }
+  __syncthreads();
+  // the beams' largest logits, then lse = log of the sum of the chunks' sums
+  for (uint32_t i = t; i < n_lists; i += kPickThreads) {
+    const uint32_t b = i / P.n_chunks;
+    if (state[b] == kOpen) atomicMax(&tops[b], i == t ? head[0].x : lists[static_cast<size_t>(i) * P.n_out].x);
+  }
+  __syncthreads();
+  double* const terms = reinterpret_cast<double*>(list);  // [kPickThreads], a list's part of its beam's sum
+  for (uint32_t i0 = 0; i0 < n_lists; i0 += kPickThreads) {
+    const uint32_t i = i0 + t, b = i < n_lists ? i / P.n_chunks : 0;
+    double term = 0.0;
+    if (i < n_lists && state[b] == kOpen) {
+      const uint32_t x = i0 == 0 ? head[0].x : lists[static_cast<size_t>(i) * P.n_out].x;
+      if (x) term = (i0 == 0 ? sum0 : sums[i]) * exp(static_cast<double>(value32(x)) - static_cast<double>(value32(tops[b])));
+    }
+    terms[t] = term;
+    __syncthreads();
+    for (uint32_t b2 = wave; b2 < P.n_beams; b2 += kPickThreads / 64) {  // in fixed order
+      const uint32_t lo = max(b2 * P.n_chunks, i0), hi = min((b2 + 1) * P.n_chunks, min(i0 + kPickThreads, n_lists));
+      if (lo >= hi) continue;
+      double part = 0.0;
+      for (uint32_t e = lo + lane; e < hi; e += 64) part += terms[e - i0];
+      part = wave_sum_f64(part);
+      if (lane == 0) lse[b2] = lo == b2 * P.n_chunks ? part : lse[b2] + part;
+    }
+    __syncthreads();
+  }
+  if (t < P.n_beams && state[t] == kOpen) {
+    const double l = static_cast<double>(value32(tops[t])) + log(lse[t]);
+    if (tops[t] == 0 || !(l < INFINITY)) state[t] = kGone;  // no token is allowed, or one at +inf
+    lse[t] = l;
+  }
+  __syncthreads();
   // entry j of the sequence's list i
-  auto entry = [&](uint32_t i, uint32_t j) {
+  auto cand = [&](uint32_t i, uint32_t j, auto load) {
     const uint32_t b = i / P.n_chunks;
     if (state[b] == kEnded)  // itself, once
       return i % P.n_chunks + j == 0 ? Cand{rank_of(score[b], norm[b], P.alpha), b, 0, P.end_token} : Cand{0, 0, 0, kNoToken};
     if (state[b] == kGone) return Cand{0, 0, 0, kNoToken};
-    const uint2 x = lists[static_cast<size_t>(i) * P.n_out + j];
+    const uint2 x = load();
     if (x.x == 0) return Cand{0, 0, 0, kNoToken};
     return Cand{rank_of(score[b] + (static_cast<double>(value32(x.x)) - lse[b]), norm[b], P.alpha), b, x.x, x.y};
   };
-  // the lists' first entries give a bound that n_out of them reach (on the upper half of the
-  // rank's bits); what reaches it stands at the front of its list
+  auto entry = [&](uint32_t i, uint32_t j) { return cand(i, j, [&] { return lists[static_cast<size_t>(i) * P.n_out + j]; }); };
+  // the lists' first entries give a bound that n_out of them reach (on ranks rounded to 32
+  // bits); what reaches it stands at the front of its list
+  auto coarse = [](const Cand& k) { return k.rank ? order32(static_cast<float>(value64(k.rank))) : 0u; };
   uint32_t top = 0;
-  for (uint32_t i = t; i < n_lists; i += kPickThreads) top = max(top, static_cast<uint32_t>(entry(i, 0).rank >> 32));
-  const uint32_t bound = nth_largest(top, P.n_out);
+  for (uint32_t i = t; i < n_lists; i += kPickThreads) top = max(top, coarse(i == t ? cand(i, 0, [&] { return head[0]; }) : entry(i, 0)));
+  const uint32_t bound = nth_largest<24>(top, P.n_out);
   if (lane == 0) red[wave] = bound;
   __syncthreads();
   uint32_t least = 1;
 #pragma unroll
   for (int w = 0; w < kPickThreads / 64; w++) least = max(least, red[w]);
-  for (uint32_t i = t; i < n_lists; i += kPickThreads)
-    for (uint32_t j = 0; j < P.n_out; j++) {
-      const Cand k = entry(i, j);
-      if (static_cast<uint32_t>(k.rank >> 32) < least) break;
+  for (uint32_t i = t; i < n_lists; i += kPickThreads) {
+    auto put = [&](const Cand& k) {
+      if (coarse(k) < least) return false;
       const uint32_t place = atomicAdd(&n_list, 1u);
       if (place < kPickList) list[place] = k;
+      return true;
+    };
+    bool on = true;
+    uint32_t j = 0;
+    if (i == t) {
+#pragma unroll
+      for (j = 0; j < kHead; j++) on = on && j < P.n_out && put(cand(i, j, [&] { return head[j]; }));
     }
+    for (; on && j < P.n_out; j++) on = put(entry(i, j));
+  }
   __syncthreads();
   const uint32_t c = n_list;
   if (c <= kPickList) {
