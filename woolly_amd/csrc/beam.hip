@@ -34,9 +34,11 @@ constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 constexpr int kThreads = 512;                 // of the first launch
 constexpr int kPer = 16;                      // logits per thread
 constexpr int kChunk = kThreads * kPer;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kList = 128;               // logits of a chunk that are ranked, 2 n_out or more
-constexpr int kPickThreads = 1024;
-constexpr uint32_t kPickList = 1024;
+constexpr size_t kPickWaves = 16;             // of the second launch, at most
+constexpr uint32_t kPickList = 1024;          // continuations that are ranked at once
+constexpr uint32_t kPickFew = 160;            // more than so many are worth a closer bound
 
 // The order of floats as that of unsigned numbers; nothing for what is not allowed.
 __device__ __forceinline__ uint32_t order32(float v) {
@@ -50,21 +52,29 @@ __device__ __forceinline__ unsigned long long order64(double v) {
   const unsigned long long u = __builtin_bit_cast(unsigned long long, v + 0.0);
   return u >> 63 ? ~u : u | 1ull << 63;
 }
-__device__ __forceinline__ double value64(unsigned long long o) {
-  return __builtin_bit_cast(double, o >> 63 ? o & ~(1ull << 63) : ~o);
-}
-
-// A bound that at least n of the lanes' numbers reach, 0 where fewer than n lanes have
-// one above 0: the n-th largest of them, cut to its upper kBits bits.
-template <int kBits>
-__device__ __forceinline__ uint32_t nth_largest(uint32_t v, uint32_t n) {
-  uint32_t t = 0;
+// A bound that at least n of the lanes' numbers reach, N of them to a lane and `most` the
+// largest; 0 where fewer than n are above 0.  The n-th largest lies somewhere below `most`:
+// the power of two of that distance is found by halving (5 counts), then two more of its
+// bits, so that some more than n may reach the bound.
+template <int N>
+__device__ __forceinline__ uint32_t near_top(const uint32_t (&v)[N], uint32_t most, uint32_t n) {
+  auto count = [&](uint32_t from) __attribute__((always_inline)) {
+    uint32_t c = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 32 - kBits; bit--) {
-    const uint32_t with = t | 1u << bit;
-    if (static_cast<uint32_t>(__builtin_popcountll(__ballot(v >= with))) >= n) t = with;
-  }
-  return t;
+    for (int j = 0; j < N; j++) c += __builtin_popcountll(__ballot(v[j] >= from));
+    return c;
+  };
+  auto below = [&](uint32_t by) __attribute__((always_inline)) { return most > by ? most - by : 1u; };
+  if (count(1) < n) return 0;
+  int bits = 0;  // a distance of 2^bits - 1 is enough, one bit less is not
+#pragma unroll
+  for (int step = 16; step >= 1; step >>= 1)
+    if (count(below((1u << (bits + step - 1)) - 1u)) < n) bits += step;
+  uint32_t by = bits < 31 ? (1u << bits) - 1u : 0xFFFFFFFFu;  // of 31 bits none was counted: all
+#pragma unroll
+  for (int b = 2; b <= 3; b++)
+    if (bits >= b && count(below(by - (1u << (bits - b)))) >= n) by -= 1u << (bits - b);
+  return below(by);
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   return whd::wave_join(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
@@ -103,6 +113,7 @@ struct Params {
   uint32_t vocab, n_seqs, n_beams, n_out, n_chunks;
   const float* scores;
   const uint32_t* last;    // null: none has ended
+  bool eager;              // logits are asked for before it is known whether they count
   uint32_t end_token;
   float alpha;
   const uint32_t* counts;
@@ -135,36 +146,41 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
   __shared__ uint32_t n_list;
   const uint32_t row = blockIdx.y, t = threadIdx.x, lane = t & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  if (state_of(P, row) != kOpen) return;
+  if (!P.eager && state_of(P, row) != kOpen) return;
   const uint32_t i0 = blockIdx.x * kChunk, n = min(P.vocab - i0, static_cast<uint32_t>(kChunk));
   auto at = [&](int j) -> uint32_t { return VEC ? 4 * t + (j & 3) + 4 * kThreads * (j >> 2) : t + kThreads * j; };
   const float* p = P.logits + row * P.ld + i0;
-  float x[kPer];  // -inf: not allowed, or not there
-  if constexpr (VEC) {
+  float x[kPer], top;  // -inf: not allowed, or not there
+  auto load = [&]() __attribute__((always_inline)) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int j = 0; j < kPer; j += 4) {
-      const uint32_t a = at(j);
-      if (a + 4 <= n) {
-        const float4 v = *reinterpret_cast<const float4*>(p + a);
-        x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
-      } else {
+      for (int j = 0; j < kPer; j += 4) {
+        const uint32_t a = at(j);
+        if (a + 4 <= n) {
+          const float4 v = *reinterpret_cast<const float4*>(p + a);
+          x[j] = v.x, x[j + 1] = v.y, x[j + 2] = v.z, x[j + 3] = v.w;
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) x[j + k] = a + k < n ? p[a + k] : -INFINITY;
+          for (int k = 0; k < 4; k++) x[j + k] = a + k < n ? p[a + k] : -INFINITY;
+        }
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; j++) x[j] = at(j) < n ? p[at(j)] : -INFINITY;
     }
-  } else {
+    top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kPer; j++) x[j] = at(j) < n ? p[at(j)] : -INFINITY;
-  }
-  float top = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < kPer; j++) {
-    x[j] = fmaxf(x[j], -INFINITY);  // NaN: -inf
-    top = fmaxf(top, x[j]);
-  }
+    for (int j = 0; j < kPer; j++) {
+      x[j] = fmaxf(x[j], -INFINITY);  // NaN: -inf
+      top = fmaxf(top, x[j]);
+    }
+  };
+  load();
+  if (P.eager && state_of(P, row) != kOpen) return;
   if (t == 0) n_list = 0;
+  if (t < kList) list[t] = 0;
   const uint32_t key = top > -INFINITY ? order32(top) : 0u;
-  const uint32_t bound = nth_largest<20>(key, P.n_out), wave_top = wave_max_u32(key);
+  const uint32_t wave_top = wave_max_u32(key), keys[1] = {key}, bound = near_top(keys, wave_top, P.n_out);
   if (lane == 0) tops[wave] = wave_top, bounds[wave] = bound;
   __syncthreads();
   uint32_t most = 0, least = order32(-3.402823466e38f);
@@ -179,37 +195,34 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
   }
   const float m = value32(most);
   auto key_of = [&](int j) { return static_cast<unsigned long long>(order32(x[j])) << 32 | (0xFFFFFFFFu - (i0 + at(j))); };
-  // what reaches the bound into the list
+  // what reaches the bound goes into the list, and out of x
   auto gather = [&](float from) __attribute__((always_inline)) {
-    uint32_t mine = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; j++) mine += x[j] >= from;
-    if (mine == 0) return;
-    uint32_t place = atomicAdd(&n_list, mine);
+    if (!(top >= from)) return;
 #pragma unroll
     for (int j = 0; j < kPer; j++)
       if (x[j] >= from) {
+        const uint32_t place = atomicAdd(&n_list, 1u);
         if (place < kList) list[place] = key_of(j);
-        place++;
+        x[j] = -INFINITY;
       }
   };
-  float from = value32(least);
-  gather(from);
-  auto rest_below = [&](float to) __attribute__((always_inline)) {
-    float rest = 0.f;
+  // The exponentials of the rest.  m log2(e) is rounded once for all of them: what that
+  // leaves is a factor of their sum.
+  const float ml = m * kLog2e;
+  auto add_rest = [&]() __attribute__((always_inline)) {
+    float rest[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      const float e = __builtin_amdgcn_exp2f((x[j] - m) * 1.4426950408889634f);
-      rest += x[j] < to ? e : 0.f;
-    }
-    const double sum = wave_sum_f64(rest);
+    for (int j = 0; j < kPer; j++) rest[j & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], kLog2e, -ml));
+    const double sum = wave_sum_f64(rest[0] + rest[1]) * static_cast<double>(__builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -ml)));
     if (lane == 0) rests[wave] = sum;
   };
-  rest_below(from);
+  gather(value32(least));
+  add_rest();
   __syncthreads();
   uint32_t c = n_list;
   if (__builtin_expect(c > kList, 0)) {
     // the bound halved on: at `least` n_out or more, above `up` fewer (or all the same)
+    load();
     auto count = [&](float f) __attribute__((always_inline)) {
       uint32_t mine = 0;
 #pragma unroll
@@ -226,12 +239,12 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
       const uint32_t mid = least + (up - least) / 2, n_mid = count(value32(mid));
       if (n_mid >= P.n_out) least = mid, c = n_mid; else up = mid;
     }
-    from = value32(least);
     __syncthreads();
     if (t == 0) n_list = 0;
+    if (t < kList) list[t] = 0;
     __syncthreads();
-    if (c <= kList) gather(from);
-    rest_below(c <= kList ? from : INFINITY);
+    if (c <= kList) gather(value32(least));
+    add_rest();
     __syncthreads();
   }
   if (c <= kList) {
@@ -242,7 +255,9 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
       if (t < c) {
         const unsigned long long k = list[t];
         uint32_t before = 0;
-        for (uint32_t j = 0; j < c; j++) before += list[j] > k;
+        for (uint32_t j = 0; j < c; j += 8)
+#pragma unroll
+          for (uint32_t u = 0; u < 8; u++) before += list[j + u] > k;  // 0 behind the last
         if (before < P.n_out) out[before] = make_uint2(static_cast<uint32_t>(k >> 32), 0xFFFFFFFFu - static_cast<uint32_t>(k));
         terms[before] = exp(static_cast<double>(value32(static_cast<uint32_t>(k >> 32))) - static_cast<double>(m));
       }
@@ -298,184 +313,228 @@ __device__ __forceinline__ bool before(Cand a, Cand b) {
   return a.token < b.token;
 }
 
-__device__ __forceinline__ unsigned long long rank_of(double s, double norm, float alpha) {
-  return order64(alpha == 0.f ? s : s / norm);
-}
-
-// grid: n_seqs.  A thread has one of the sequence's lists, or several.
-__global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const Params P) {
+// grid: n_seqs, a wave per beam (or several), a lane per chunk's list (or several).
+__global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(const Params P) {
   constexpr uint32_t kHead = 4;  // entries of a list that are asked for at once
-  __shared__ double lse[wh::kMaxBeams], score[wh::kMaxBeams], norm[wh::kMaxBeams];
+  __shared__ double lse[wh::kMaxBeams], score[wh::kMaxBeams], per_token[wh::kMaxBeams];
   __shared__ int state[wh::kMaxBeams];
-  __shared__ uint32_t tops[wh::kMaxBeams];
-  __shared__ uint32_t red[kPickThreads / 64];
-  __shared__ Cand best[kPickThreads / 64];
-  __shared__ Cand list[kPickList];
+  __shared__ uint32_t count_in[wh::kMaxBeams], len_in[wh::kMaxBeams];
+  __shared__ uint32_t red[kPickWaves];
+  __shared__ Cand best[kPickWaves];
+  __shared__ unsigned long long ranks[kPickList + 8];
+  __shared__ uint3 rest[kPickList];  // beam, logit, token
   __shared__ Cand chosen[2 * wh::kMaxBeams];
   __shared__ uint32_t from[wh::kMaxBeams], have[wh::kMaxBeams];
   __shared__ uint32_t n_list;
-  const uint32_t s = blockIdx.x, t = threadIdx.x, lane = t & 63, row0 = s * P.n_beams;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const uint32_t n_lists = P.n_beams * P.n_chunks, total = n_lists * P.n_out;
-  const uint2* const lists = P.lists + static_cast<size_t>(row0) * P.n_chunks * P.n_out;
-  const double* const sums = P.sums + static_cast<size_t>(row0) * P.n_chunks;
-  // asked for before it is known which of it counts (a beam that has ended wrote none)
-  uint2 head[kHead];
-  double sum0 = 0.0;
-  if (t < n_lists) {
-    sum0 = sums[t];
+  const uint32_t s = blockIdx.x, t = threadIdx.x, lane = t & 63, row0 = s * P.n_beams, threads = blockDim.x;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6), n_waves = threads / 64;
+  const uint32_t per_beam = P.n_chunks * P.n_out;
+  const uint2* const lists = P.lists + static_cast<size_t>(row0) * per_beam;
+  auto load_heads = [&](uint32_t b, uint2 (&head)[kHead]) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t j = 0; j < kHead; j++) head[j] = j < P.n_out ? lists[static_cast<size_t>(t) * P.n_out + j] : make_uint2(0, kNoToken);
-  }
+    for (uint32_t j = 0; j < kHead; j++)
+      head[j] = lane < P.n_chunks && j < P.n_out ? lists[static_cast<size_t>(b) * per_beam + lane * P.n_out + j] : make_uint2(0, kNoToken);
+  };
+  // what an entry of a list is compared by
+  auto rank_of = [&](uint32_t b, uint32_t x) __attribute__((always_inline)) {
+    const double v = state[b] == kEnded ? score[b] : score[b] + (static_cast<double>(value32(x)) - lse[b]);
+    return v * per_token[b];
+  };
   if (t == 0) n_list = 0;
   if (t < 2 * wh::kMaxBeams) chosen[t] = Cand{0, 0, 0, kNoToken};
-  if (t < P.n_beams) {
-    const uint32_t row = row0 + t;
-    const int st = state_of(P, row);
-    const uint32_t count = (P.counts ? P.counts[row] : 0u) + (st == kOpen);
-    tops[t] = 0;
-    state[t] = st;
-    score[t] = P.scores[row];
-    norm[t] = P.alpha == 0.f ? 1.0 : pow(static_cast<double>(max(count, 1u)), static_cast<double>(P.alpha));
-  }
-  __syncthreads();
-  // the beams' largest logits, then lse = log of the sum of the chunks' sums
-  for (uint32_t i = t; i < n_lists; i += kPickThreads) {
-    const uint32_t b = i / P.n_chunks;
-    if (state[b] == kOpen) atomicMax(&tops[b], i == t ? head[0].x : lists[static_cast<size_t>(i) * P.n_out].x);
-  }
-  __syncthreads();
-  double* const terms = reinterpret_cast<double*>(list);  // [kPickThreads], a list's part of its beam's sum
-  for (uint32_t i0 = 0; i0 < n_lists; i0 += kPickThreads) {
-    const uint32_t i = i0 + t, b = i < n_lists ? i / P.n_chunks : 0;
-    double term = 0.0;
-    if (i < n_lists && state[b] == kOpen) {
-      const uint32_t x = i0 == 0 ? head[0].x : lists[static_cast<size_t>(i) * P.n_out].x;
-      if (x) term = (i0 == 0 ? sum0 : sums[i]) * exp(static_cast<double>(value32(x)) - static_cast<double>(value32(tops[b])));
+  for (uint32_t i = t; i < kPickList + 8; i += threads) ranks[i] = 0;
+  // Every beam's lse, and a bound that n_out of its continuations reach: the n_out-th of its
+  // lists' first few.
+  uint2 mine[kHead];
+  uint32_t my_first[kHead] = {0, 0, 0, 0}, least = 1;
+  double my_value[kHead];
+  for (uint32_t b = wave; b < P.n_beams; b += n_waves) {
+    const uint32_t row = row0 + b;
+    const double* const sums = P.sums + static_cast<size_t>(row) * P.n_chunks;
+    // asked for before it is known whether it counts (a beam that has ended wrote nothing)
+    uint2 head[kHead];
+    load_heads(b, head);
+    double sum = lane < P.n_chunks ? sums[lane] : 0.0;
+    int st = state_of(P, row);
+    const float sc = P.scores[row];
+    const uint32_t count = P.counts ? P.counts[row] : 0u, len = P.len ? P.len[row] : 0u;
+    double l = 0.0;
+    if (st == kOpen) {
+      uint32_t most = head[0].x;
+      for (uint32_t c = lane + 64; c < P.n_chunks; c += 64) most = max(most, lists[static_cast<size_t>(b) * per_beam + c * P.n_out].x);
+      most = wave_max_u32(most);
+      const double m = value32(most);
+      sum = head[0].x ? sum * exp(static_cast<double>(value32(head[0].x)) - m) : 0.0;
+      for (uint32_t c = lane + 64; c < P.n_chunks; c += 64) {
+        const uint32_t x = lists[static_cast<size_t>(b) * per_beam + c * P.n_out].x;
+        if (x) sum += sums[c] * exp(static_cast<double>(value32(x)) - m);
+      }
+      l = m + log(wave_sum_f64(sum));
+      if (most == 0 || !(l < INFINITY)) st = kGone;  // no token is allowed, or one at +inf
     }
-    terms[t] = term;
-    __syncthreads();
-    for (uint32_t b2 = wave; b2 < P.n_beams; b2 += kPickThreads / 64) {  // in fixed order
-      const uint32_t lo = max(b2 * P.n_chunks, i0), hi = min((b2 + 1) * P.n_chunks, min(i0 + kPickThreads, n_lists));
-      if (lo >= hi) continue;
-      double part = 0.0;
-      for (uint32_t e = lo + lane; e < hi; e += 64) part += terms[e - i0];
-      part = wave_sum_f64(part);
-      if (lane == 0) lse[b2] = lo == b2 * P.n_chunks ? part : lse[b2] + part;
-    }
-    __syncthreads();
-  }
-  if (t < P.n_beams && state[t] == kOpen) {
-    const double l = static_cast<double>(value32(tops[t])) + log(lse[t]);
-    if (tops[t] == 0 || !(l < INFINITY)) state[t] = kGone;  // no token is allowed, or one at +inf
-    lse[t] = l;
-  }
-  __syncthreads();
-  // entry j of the sequence's list i
-  auto cand = [&](uint32_t i, uint32_t j, auto load) {
-    const uint32_t b = i / P.n_chunks;
-    if (state[b] == kEnded)  // itself, once
-      return i % P.n_chunks + j == 0 ? Cand{rank_of(score[b], norm[b], P.alpha), b, 0, P.end_token} : Cand{0, 0, 0, kNoToken};
-    if (state[b] == kGone) return Cand{0, 0, 0, kNoToken};
-    const uint2 x = load();
-    if (x.x == 0) return Cand{0, 0, 0, kNoToken};
-    return Cand{rank_of(score[b] + (static_cast<double>(value32(x.x)) - lse[b]), norm[b], P.alpha), b, x.x, x.y};
-  };
-  auto entry = [&](uint32_t i, uint32_t j) { return cand(i, j, [&] { return lists[static_cast<size_t>(i) * P.n_out + j]; }); };
-  // the lists' first entries give a bound that n_out of them reach (on ranks rounded to 32
-  // bits); what reaches it stands at the front of its list
-  auto coarse = [](const Cand& k) { return k.rank ? order32(static_cast<float>(value64(k.rank))) : 0u; };
-  uint32_t top = 0;
-  for (uint32_t i = t; i < n_lists; i += kPickThreads) top = max(top, coarse(i == t ? cand(i, 0, [&] { return head[0]; }) : entry(i, 0)));
-  const uint32_t bound = nth_largest<24>(top, P.n_out);
-  if (lane == 0) red[wave] = bound;
-  __syncthreads();
-  uint32_t least = 1;
+    if (st != kOpen) {
 #pragma unroll
-  for (int w = 0; w < kPickThreads / 64; w++) least = max(least, red[w]);
-  for (uint32_t i = t; i < n_lists; i += kPickThreads) {
-    auto put = [&](const Cand& k) {
-      if (coarse(k) < least) return false;
-      const uint32_t place = atomicAdd(&n_list, 1u);
-      if (place < kPickList) list[place] = k;
-      return true;
+      for (uint32_t j = 0; j < kHead; j++) head[j] = make_uint2(0, kNoToken);
+      if (st == kEnded && lane == 0) head[0] = make_uint2(1, P.end_token);  // itself, once
+    }
+    if (lane == 0) {
+      const uint32_t tokens = max(count + (st == kOpen), 1u);
+      per_token[b] = P.alpha == 0.f ? 1.0 : exp(-static_cast<double>(P.alpha) * log(static_cast<double>(tokens)));
+      lse[b] = l;
+      score[b] = sc;
+      count_in[b] = count;
+      len_in[b] = len;
+      state[b] = st;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the beam's numbers, for the other lanes
+    uint32_t first[kHead];
+    double value[kHead];
+#pragma unroll
+    for (uint32_t j = 0; j < kHead; j++) {
+      value[j] = rank_of(b, head[j].x);
+      first[j] = head[j].x ? order32(static_cast<float>(value[j])) : 0u;
+    }
+    least = max(least, near_top(first, wave_max_u32(first[0]), P.n_out));
+    if (b == wave) {
+#pragma unroll
+      for (uint32_t j = 0; j < kHead; j++) mine[j] = head[j], my_first[j] = first[j], my_value[j] = value[j];
+    }
+  }
+  if (lane == 0) red[wave] = least;
+  __syncthreads();
+  for (uint32_t w = 0; w < n_waves; w++) least = max(least, red[w]);
+  // what reaches the highest bound; it stands at the front of its list
+  auto gather = [&]() __attribute__((always_inline)) {
+    auto put = [&](uint32_t place, uint32_t b, uint2 x, double v) __attribute__((always_inline)) {
+      if (place < kPickList) ranks[place] = order64(v), rest[place] = make_uint3(b, x.x, x.y);
     };
-    bool on = true;
-    uint32_t j = 0;
-    if (i == t) {
+    // entries j .. of list c of beam b, until one is below the bound
+    auto follow = [&](uint32_t b, uint32_t c, uint32_t j) __attribute__((always_inline)) {
+      for (; j < P.n_out; j++) {
+        const uint2 x = lists[static_cast<size_t>(b) * per_beam + c * P.n_out + j];
+        const double v = rank_of(b, x.x);
+        if (x.x == 0 || order32(static_cast<float>(v)) < least) break;
+        put(atomicAdd(&n_list, 1u), b, x, v);
+      }
+    };
+    uint32_t n = 0;
 #pragma unroll
-      for (j = 0; j < kHead; j++) on = on && j < P.n_out && put(cand(i, j, [&] { return head[j]; }));
+    for (uint32_t j = 0; j < kHead; j++) n += my_first[j] >= least;
+    if (n) {
+      const uint32_t place = atomicAdd(&n_list, n);
+#pragma unroll
+      for (uint32_t j = 0; j < kHead; j++)
+        if (j < n) put(place + j, wave, mine[j], my_value[j]);
+      if (n == kHead && state[wave] == kOpen) follow(wave, lane, kHead);
     }
-    for (; on && j < P.n_out; j++) on = put(entry(i, j));
+    for (uint32_t b = wave; b < P.n_beams; b += n_waves) {  // lists behind a lane's first one
+      if (state[b] == kEnded && b != wave && lane == 0) {
+        const double v = rank_of(b, 1);
+        if (order32(static_cast<float>(v)) >= least) put(atomicAdd(&n_list, 1u), b, make_uint2(1, P.end_token), v);
+      }
+      if (state[b] != kOpen) continue;
+      for (uint32_t c = lane + (b == wave ? 64 : 0); c < P.n_chunks; c += 64) follow(b, c, 0);
+    }
+    __syncthreads();
+  };
+  gather();
+  if (n_list > kPickFew) {
+    // a closer bound, halved on by counting each lane's first few entries
+    uint32_t up = 0xFFFFFFFFu, n_least = 0xFFFFFFFFu;
+    while (n_least > P.n_out + P.n_out / 2 && up - least > 1) {
+      const uint32_t mid = least + (up - least) / 2;
+      uint32_t n = 0;
+#pragma unroll
+      for (uint32_t j = 0; j < kHead; j++) n += __builtin_popcountll(__ballot(my_first[j] >= mid));
+      __syncthreads();
+      if (lane == 0) red[wave] = n;
+      __syncthreads();
+      n = 0;
+      for (uint32_t w = 0; w < n_waves; w++) n += red[w];
+      if (n >= P.n_out) least = mid, n_least = n; else up = mid;
+    }
+    __syncthreads();
+    for (uint32_t i = t; i < kPickList + 8; i += threads) ranks[i] = 0;
+    if (t == 0) n_list = 0;
+    __syncthreads();
+    gather();
   }
-  __syncthreads();
   const uint32_t c = n_list;
-  if (c <= kPickList) {
-    for (uint32_t i = t; i < c; i += kPickThreads) {
-      const Cand k = list[i];
-      uint32_t place = 0;
-      for (uint32_t j = 0; j < c; j++) place += before(list[j], k);
+  if (c <= kPickList) {  // the place of each is the number of those before it
+    for (uint32_t i = t; i < c; i += threads) {
+      const unsigned long long r = ranks[i];
+      const uint3 y = rest[i];
+      const Cand k{r, y.x, y.y, y.z};
+      uint32_t place = 0, same = 0;
+      for (uint32_t j = 0; j < c; j += 8)
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++) {
+          const unsigned long long o = ranks[j + u];  // 0 behind the last
+          place += o > r;
+          same += o == r;
+        }
+      if (same > 1)
+        for (uint32_t j = 0; j < c; j++) {
+          const uint3 z = rest[j];
+          if (ranks[j] == r) place += before(Cand{r, z.x, z.y, z.z}, k);
+        }
       if (place < P.n_out) chosen[place] = k;
     }
-  } else {  // the first one behind the last, n_out times
+  } else {  // too many that are equal, or nearly: the first one behind the last, n_out times
     Cand last{~0ull, 0, 0, 0};
     for (uint32_t i = 0; i < P.n_out; i++) {
-      Cand mine{0, 0, 0, kNoToken};
-      for (uint32_t e = t; e < total; e += kPickThreads) {
-        const Cand k = entry(e / P.n_out, e % P.n_out);
-        if (k.rank && before(last, k) && (mine.rank == 0 || before(k, mine))) mine = k;
+      Cand first{0, 0, 0, kNoToken};
+      for (uint32_t e = t; e < P.n_beams * per_beam; e += threads) {
+        const uint32_t b = e / per_beam;
+        if (state[b] == kGone || (state[b] == kEnded && e % per_beam != 0)) continue;
+        const uint2 x = state[b] == kEnded ? make_uint2(1, P.end_token) : lists[e];
+        if (x.x == 0) continue;
+        const Cand k{order64(rank_of(b, x.x)), b, x.x, x.y};
+        if (before(last, k) && (first.rank == 0 || before(k, first))) first = k;
       }
 #pragma unroll
       for (int off = 32; off >= 1; off >>= 1) {
-        const Cand o{__shfl_xor(mine.rank, off, 64), __shfl_xor(mine.beam, off, 64), __shfl_xor(mine.logit, off, 64),
-                     __shfl_xor(mine.token, off, 64)};
-        if (o.rank && (mine.rank == 0 || before(o, mine))) mine = o;
+        const Cand o{__shfl_xor(first.rank, off, 64), __shfl_xor(first.beam, off, 64), __shfl_xor(first.logit, off, 64),
+                     __shfl_xor(first.token, off, 64)};
+        if (o.rank && (first.rank == 0 || before(o, first))) first = o;
       }
-      if (lane == 0) best[wave] = mine;
+      if (lane == 0) best[wave] = first;
       __syncthreads();
-      for (int w = 0; w < kPickThreads / 64; w++) {
+      for (uint32_t w = 0; w < n_waves; w++) {
         const Cand o = best[w];
-        if (o.rank && (mine.rank == 0 || before(o, mine))) mine = o;
+        if (o.rank && (first.rank == 0 || before(o, first))) first = o;
       }
       __syncthreads();
-      if (t == 0) chosen[i] = mine;
-      last = mine;
-      if (mine.rank == 0) break;
+      if (t == 0) chosen[i] = first;
+      last = first;
+      if (first.rank == 0) break;
     }
   }
   __syncthreads();
-  // what an output may overwrite is read before any of them is written
-  const uint32_t o = s * P.n_out + t;
-  uint32_t parent = 0, count = 0, len = 0;
-  if (t < P.n_out) {
+  if (t < P.n_out) {  // all that an output may overwrite has been read
     const Cand k = chosen[t];
-    parent = k.rank ? k.beam : min(t, P.n_beams - 1);
-    if (k.rank) count = (P.counts ? P.counts[row0 + parent] : 0u) + (state[parent] == kOpen);
-    if (P.len) len = P.len[row0 + parent];
-    if (t < wh::kMaxBeams) from[t] = parent, have[t] = len;
-  }
-  __syncthreads();
-  if (t < P.n_out) {
-    const Cand k = chosen[t];
+    const uint32_t o = s * P.n_out + t, b = k.rank ? k.beam : min(t, P.n_beams - 1);
     float v = -INFINITY;
-    if (k.rank) v = static_cast<float>(state[parent] == kEnded ? score[parent] : score[parent] + (static_cast<double>(value32(k.logit)) - lse[parent]));
+    if (k.rank) v = static_cast<float>(state[b] == kEnded ? score[b] : score[b] + (static_cast<double>(value32(k.logit)) - lse[b]));
     P.scores_out[o] = v;
     P.tokens[o] = k.token;
-    P.parents[o] = parent;
-    if (P.counts_out) P.counts_out[o] = count;
-    if (P.len_out) P.len_out[o] = len + 1;
+    P.parents[o] = b;
+    if (P.counts_out) P.counts_out[o] = k.rank ? count_in[b] + (state[b] == kOpen) : 0u;
+    if (P.len_out) P.len_out[o] = len_in[b] + 1;
+    if (t < wh::kMaxBeams) from[t] = b, have[t] = len_in[b];
   }
   if (!P.history) return;
   // some columns of the histories at a time: what the beams take of them is read before any is written
+  __syncthreads();
   uint32_t most = 0;
   for (uint32_t i = 0; i < P.n_beams; i++) most = max(most, have[i]);
   const size_t end = min(static_cast<size_t>(most) + 1, P.history_stride);
   uint32_t* const h = P.history + static_cast<size_t>(row0) * P.history_stride;
-  uint32_t* const tile = reinterpret_cast<uint32_t*>(list);
-  const uint32_t columns = sizeof(list) / 4 / P.n_beams;
+  uint32_t* const tile = reinterpret_cast<uint32_t*>(ranks);
+  const uint32_t columns = kPickList * 2 / P.n_beams;
   for (size_t p0 = 0; p0 < end; p0 += columns) {
     const uint32_t n = static_cast<uint32_t>(min(end - p0, static_cast<size_t>(columns)));
-    for (uint32_t e = t; e < n * P.n_beams; e += kPickThreads) {
+    for (uint32_t e = t; e < n * P.n_beams; e += threads) {
       const uint32_t i = e / n;
       const size_t p = p0 + e % n;
       uint32_t v = chosen[i].token;
@@ -484,7 +543,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(const Params P)
       tile[e] = v;
     }
     __syncthreads();
-    for (uint32_t e = t; e < n * P.n_beams; e += kPickThreads) {
+    for (uint32_t e = t; e < n * P.n_beams; e += threads) {
       const uint32_t i = e / n;
       const size_t p = p0 + e % n;
       if (p <= have[i] && (p == have[i] || from[i] != i)) h[i * P.history_stride + p] = tile[e];
@@ -592,11 +651,13 @@ WH_API int wh_beam_select(const wh_beam_rules* rules, const float* logits, size_
   P.sums = static_cast<double*>(workspace);
   P.lists = reinterpret_cast<uint2*>(static_cast<char*>(workspace) + al256(rows * P.n_chunks * sizeof(double)));
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  P.eager = rows * P.n_chunks <= 2 * static_cast<size_t>(wh::cu_count());
   const dim3 grid(P.n_chunks, static_cast<unsigned>(rows));
   if (wh::aligned(logits, 16) && ld % 4 == 0) beam_chunk_kernel<true><<<grid, kThreads, 0, s>>>(P);
   else beam_chunk_kernel<false><<<grid, kThreads, 0, s>>>(P);
   WH_LAUNCH_CHECK("beam selection launch");
-  beam_pick_kernel<<<static_cast<unsigned>(n_seqs), kPickThreads, 0, s>>>(P);
+  const size_t waves = r.n_beams < 4 ? 4 : r.n_beams < kPickWaves ? r.n_beams : kPickWaves;
+  beam_pick_kernel<<<static_cast<unsigned>(n_seqs), static_cast<unsigned>(64 * waves), 0, s>>>(P);
   WH_LAUNCH_CHECK("beam choice launch");
   return WH_OK;
 }
