@@ -4,7 +4,7 @@
 // Selection.  Beam b continued by token i has s = score_b + l_i - lse_b,
 // lse_b = log sum_j exp l_j; of a sequence's continuations the n_out with the
 // highest s / count^alpha are wanted, in order.  Two launches:
-//   1. a workgroup per 8192 logits of a beam: the sum of their exponentials
+//   1. a workgroup per 4096 logits of a beam: the sum of their exponentials
 //      relative to the largest, and the n_out highest logits
 //   2. a workgroup per sequence: the beams' lse, the n_out best of all chunks'
 //      lists, and the histories
@@ -31,7 +31,7 @@
 namespace {
 
 constexpr uint32_t kNoToken = 0xFFFFFFFFu;
-constexpr int kThreads = 512;                 // of the first launch
+constexpr int kThreads = 256;                 // of the first launch
 constexpr int kPer = 16;                      // logits per thread
 constexpr int kChunk = kThreads * kPer;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -113,7 +113,6 @@ struct Params {
   uint32_t vocab, n_seqs, n_beams, n_out, n_chunks;
   const float* scores;
   const uint32_t* last;    // null: none has ended
-  bool eager;              // logits are asked for before it is known whether they count
   uint32_t end_token;
   float alpha;
   const uint32_t* counts;
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
   __shared__ uint32_t n_list;
   const uint32_t row = blockIdx.y, t = threadIdx.x, lane = t & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  if (!P.eager && state_of(P, row) != kOpen) return;
+  if (state_of(P, row) != kOpen) return;
   const uint32_t i0 = blockIdx.x * kChunk, n = min(P.vocab - i0, static_cast<uint32_t>(kChunk));
   auto at = [&](int j) -> uint32_t { return VEC ? 4 * t + (j & 3) + 4 * kThreads * (j >> 2) : t + kThreads * j; };
   const float* p = P.logits + row * P.ld + i0;
@@ -176,7 +175,6 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
     }
   };
   load();
-  if (P.eager && state_of(P, row) != kOpen) return;
   if (t == 0) n_list = 0;
   if (t < kList) list[t] = 0;
   const uint32_t key = top > -INFINITY ? order32(top) : 0u;
@@ -206,14 +204,11 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
         x[j] = -INFINITY;
       }
   };
-  // The exponentials of the rest.  m log2(e) is rounded once for all of them: what that
-  // leaves is a factor of their sum.
-  const float ml = m * kLog2e;
   auto add_rest = [&]() __attribute__((always_inline)) {
     float rest[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kPer; j++) rest[j & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], kLog2e, -ml));
-    const double sum = wave_sum_f64(rest[0] + rest[1]) * static_cast<double>(__builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -ml)));
+    for (int j = 0; j < kPer; j++) rest[j & 1] += __builtin_amdgcn_exp2f((x[j] - m) * kLog2e);
+    const double sum = wave_sum_f64(rest[0] + rest[1]);
     if (lane == 0) rests[wave] = sum;
   };
   gather(value32(least));
@@ -651,7 +646,6 @@ WH_API int wh_beam_select(const wh_beam_rules* rules, const float* logits, size_
   P.sums = static_cast<double*>(workspace);
   P.lists = reinterpret_cast<uint2*>(static_cast<char*>(workspace) + al256(rows * P.n_chunks * sizeof(double)));
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  P.eager = rows * P.n_chunks <= 2 * static_cast<size_t>(wh::cu_count());
   const dim3 grid(P.n_chunks, static_cast<unsigned>(rows));
   if (wh::aligned(logits, 16) && ld % 4 == 0) beam_chunk_kernel<true><<<grid, kThreads, 0, s>>>(P);
   else beam_chunk_kernel<false><<<grid, kThreads, 0, s>>>(P);
