@@ -21,7 +21,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr size_t kManyHeads = 32768;  // heads of all rows from which on a wave takes eight turns
+constexpr size_t kManyHeads = 32768;  // heads of all rows from which on a wave takes more turns
 struct Params {
   const float *q, *k, *v;
   size_t ldq, ldkv, ldq_out, ldk_out, max_rows;
@@ -31,7 +31,7 @@ struct Params {
   _Float16 *k_cache, *v_cache;
   uint32_t n_per, n_new, n_heads, n_kv, d, half, groups, rows;  // half: turned pairs
   int interleaved;
-  float eps;
+  float eps, per_d;      // 1 / d
   double magnitude;
 };
 
@@ -141,7 +141,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const Params P) {
       for (int u = 0; u < PP; u++)
         if (in[u]) sum = __builtin_fmaf(x[n][u], x[n][u], __builtin_fmaf(y[n][u], y[n][u], sum));
       sum = lanes_sum<L>(sum);
-      const float r = 1.0f / sqrtf(sum / static_cast<float>(P.d) + P.eps);
+      const float mean = __builtin_fmaf(sum, P.per_d, P.eps);
+      float r = __builtin_amdgcn_rsqf(mean);         // off by a unit of f32 at most
+      if (mean < 0x1p-126f) r = 1.0f / sqrtf(mean);  // which it flushes
 #pragma unroll
       for (int u = 0; u < PP; u++) {
         x[n][u] = x[n][u] * r * (is_q ? qw[u][0] : kw[u][0]);
@@ -187,14 +189,18 @@ int launch(const Params& P, hipStream_t s) {
   const uint32_t slots = P.n_heads + P.n_kv;
   Params A = P;
   // few rows: the launch is as long as its dependent loads, and takes as many waves as there are
-  // heads; many rows: a wave's heads share the angles
+  // heads; many rows: a wave's heads share the angles (4000 rows of 32 / 8 heads of 128 with 4,
+  // 5, 8 and 10 heads 38.4, 37.1, 36.2, 36.3 us, normed 41.7, 41.0, 40.6, 42.1; 16 / 4 heads of
+  // 256 47.3, 45.2, 49.6, 45.8; 16 x 300 of 32 / 4 heads of 64 in neighbouring pairs, two heads
+  // at a time, 22.2, 21.7, 23.0, 23.3)
+  constexpr int kMany = L == 64 && PP == 1 ? 8 : 5;
   const bool few = static_cast<size_t>(P.rows) * slots < kManyHeads;
-  const uint32_t per = 64 / L * (few ? 2 : 8);
+  const uint32_t per = 64 / L * (few ? 2 : kMany);
   A.groups = (slots + per - 1) / per;
   const size_t items = static_cast<size_t>(P.rows) * A.groups;
   const unsigned grid = static_cast<unsigned>((items + kThreads / 64 - 1) / (kThreads / 64));
   if (few) rope_kernel<L, PP, 2><<<grid, kThreads, 0, s>>>(A);
-  else rope_kernel<L, PP, 8><<<grid, kThreads, 0, s>>>(A);
+  else rope_kernel<L, PP, kMany><<<grid, kThreads, 0, s>>>(A);
   WH_LAUNCH_CHECK("norm and rotation launch");
   return WH_OK;
 }
@@ -233,6 +239,7 @@ int launch_rope(const wh_rope_rules& r, const RopeArgs& a, hipStream_t s) {
   P.rows = static_cast<uint32_t>(a.n_members * a.n_new);
   P.interleaved = r.interleaved;
   P.eps = r.norm_eps;
+  P.per_d = 1.0f / static_cast<float>(a.head_dim);
   P.magnitude = r.magnitude == 0.0 ? 1.0 : r.magnitude;
   return P.d <= 64 ? launch<32, 1>(P, s) : P.d <= 128 ? launch<64, 1>(P, s) : launch<64, 2>(P, s);
 }
