@@ -19,7 +19,9 @@
 //
 // Reordering.  A thread holds one 16-byte column of a state's rows for all beams:
 // it loads what its moved beams take before it stores any of it, so rows move in
-// place, whatever the parents are.
+// place, whatever the parents are.  Bound by memory: each moved row is read and
+// written once (4 of 8 beams x 500 rows of 2 KB x 64 states, 524 MB: 105 us, 5.0 TB/s;
+// 2 of 4 x 60 rows 6.4 us, 4.9 TB/s).
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -578,12 +580,14 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const ReorderParams P
   for (int i = 0; i < NB; i++) most = n[i] > most ? n[i] : most;
   for (size_t c = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; c < most; c += static_cast<size_t>(gridDim.x) * 256) {
     Piece v[NB];
+    asm volatile("" ::: "memory");  // the table stays in LDS: in registers it would cost waves
 #pragma unroll
     for (int i = 0; i < NB; i++)
       if (c < n[i]) v[i] = base[from[i] + c];
 #pragma unroll
     for (int i = 0; i < NB; i++)
-      if (c < n[i]) base[i * beam + c] = v[i];
+      if (c < n[i])  // past the caches: 115 -> 105 us for 524 MB, 7.3 -> 6.4 for 31
+        __builtin_nontemporal_store(v[i], &base[i * beam + c]);
   }
 }
 
