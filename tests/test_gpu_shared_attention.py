@@ -113,6 +113,46 @@ def test_long(gpu, heads, kv, d):
     c.check([0, 17, 39])
 
 
+# heads, kv, d, members, max_prefix, max_own: workgroups of 64 and of 128 query rows, one and two to a CU, the last one's rows
+# not all there, and (5 tiles of 32) workgroups of 32 rows, two to a CU
+WIDE = [(4, 1, 128, 43, 60000, 400), (4, 1, 128, 43, 96000, 20), (4, 1, 128, 52, 50000, 60), (8, 2, 128, 60, 120000, 30),
+        (4, 1, 128, 39, 140000, 20), (8, 1, 64, 52, 64000, 30), (8, 1, 64, 23, 50000, 20)]
+
+
+@pytest.mark.parametrize("heads, kv, d, per, max_prefix, max_own", WIDE)
+def test_many_rows(gpu, heads, kv, d, per, max_prefix, max_own):
+    """Members whose query rows share the prefix's stages, at lengths that end anywhere in a stage, none and one."""
+    print(f"[case] shared many rows {heads} {kv} {d} {per} {max_prefix}", flush=True)
+    r = np.random.default_rng(per)
+    for n in (0, 1, 64, 95, 2111, max_prefix):
+        own = [int(v) for v in r.integers(0, 20, per)]
+        own[0] = 0
+        c = Case(heads, kv, d, per, [n], own, max_prefix=max_prefix, max_own=max_own, seed=n).upload()
+        c.call()
+        c.check([0, 8, 19, per - 1] if n > 3000 else None)
+
+
+@pytest.mark.parametrize("heads, kv, d, per, max_prefix, max_own", WIDE)
+def test_infinities_of_many_rows(gpu, heads, kv, d, per, max_prefix, max_own):
+    for n in (75, 1000):
+        c = Case(heads, kv, d, per, [n], [2] * per, max_prefix=max_prefix, max_own=max_own)
+        c.vp[0, 5, 0, 3] = np.inf
+        c.vp[0, 40, 0, 9] = -np.inf
+        c.vp[0, n - 1, 0, 11] = np.nan
+        c.kp[0, 37, 0] = np.where(c.q[1, :d] > 0, -np.inf, np.inf)  # member 1, head 0: score -inf; any other row's is NaN
+        c.upload().call()
+        got = c.out()
+        assert got[1, 0, 3] == np.inf and np.isneginf(got[1, 0, 9]) and np.isnan(got[1, 0, 11])
+        g = heads // kv
+        others = [(m, h) for m in range(per) for h in range(g) if (m, h) != (1, 0)]
+        assert all(np.isnan(got[m, h]).all() for m, h in others)
+        rest = [i for i in range(d) if i not in (3, 9, 11)]
+        keep = np.delete(np.arange(n), 37)
+        want, bound = _members.attention(c.q[1, :d][None], np.concatenate([c.kp[0, keep, :1], c.ko[1, :2, :1]]),
+                                         np.concatenate([c.vp[0, keep, :1], c.vo[1, :2, :1]]))
+        assert (np.abs(got[1, 0] - want[0])[rest] <= bound[0, rest]).all()
+
+
 def test_prefix_or_own_rows_alone(gpu):
     for d in (64, 128):
         c = Case(8, 2, d, 3, [200], [0, 0, 0]).upload()

@@ -6,10 +6,10 @@
 //   out = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m},  m = max_j s_j
 // The prefix's rows are read once for the n_per G query rows that a KV head has
 // in a group.  Two launches:
-//   1. partial: a workgroup per (KV head, 32 query rows, chunk of the prefix), and
-//      per (KV head, member, chunk of its own rows): maximum, sum and weighted
-//      sum of V of each row
-//   2. combine: a wave per 32 query rows and 8 dims joins their chunks
+//   1. partial: a workgroup per (KV head, 32, 64 or 128 query rows, chunk of the
+//      prefix), and per (KV head, member, chunk of its own rows): maximum, sum and
+//      weighted sum of V of each row
+//   2. combine: a wave, or four, per 32 query rows and 8 dims join their chunks
 // The chunks' number is the launch's, their length follows from the lengths on
 // the device.
 //
@@ -23,9 +23,13 @@
 // a key with nearly all the weight (often the first one, whose v is small) leaves
 // to the others is as exact as in f32.
 //
-// A wave has its own tiles of 32 keys, its own LDS and no barriers until the
-// chunk's end: the next K tile is asked for when the scores are there, the next V
-// tile when the products are.
+// Few query rows: a wave has its own tiles of 32 keys, its own LDS and no barriers
+// until the chunk's end; memory bounds it (8 members at 30000 + 250 rows, 131 MB,
+// 33.5 us with both launches).  Many: the waves share stages of 64 keys; the matrix
+// cores bound it, whose clock falls under such work (48 members at 131000 + 400 rows,
+// 206 GFLOP of limbs, 260 us, 64 members 295 us, 0.93 PFLOP/s; vector and matrix
+// instructions take about as many cycles, and which of two waves goes first makes no
+// difference).
 #include <type_traits>
 
 #include "attn_dev.hpp"
@@ -349,6 +353,55 @@ __device__ __forceinline__ void load_rows_of(Rows<D>& w, const Params& P, const 
   load_rows(w, P.q + (W.member0 + r / P.G) * P.ldq + static_cast<size_t>(W.kvh * P.G + r % P.G) * D, P.scale, h);
 }
 
+// Waves whose query rows are the same and that have taken keys apart, N of them with
+// kWaves / N tiles, join in LDS, in fixed order, and store in the lanes' order.
+template <int D, int N>
+__device__ __forceinline__ void join_waves(const Rows<D>& w, const Work& W, unsigned char* lds, uint32_t wave, int lane) {
+  constexpr int kQuads = D / 8, kApart = kWaves / N;
+  const int l32 = lane & 31, h = lane >> 5;
+  const uint32_t tile = wave % kApart, part = wave / kApart;
+  whd::lds_barrier();
+  float4* am = reinterpret_cast<float4*>(lds);                        // [4][D / 8][64]
+  float2* mm = reinterpret_cast<float2*>(am + kWaves * kQuads * 64);  // [4][32]
+#pragma unroll
+  for (int d = 0; d < D / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      am[(wave * kQuads + 4 * d + i) * 64 + lane] =
+          make_float4(w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]);
+  if (h == 0) mm[wave * 32 + l32] = make_float2(w.m, w.l);
+  whd::lds_barrier();
+  float M = -INFINITY, L = 0.f, ew[N];
+  float2 ml[N];
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    ml[u] = mm[(u * kApart + tile) * 32 + l32];
+    M = __builtin_elementwise_maximum(M, ml[u].x);
+  }
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    ew[u] = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - M) * w.qs);
+    L = __builtin_fmaf(ml[u].y, ew[u], L);
+  }
+  if (W.row0 + 32 * tile + l32 >= W.n_rows) return;
+  float4* const acc = W.acc + tile * 32 * (D / 4);
+#pragma unroll
+  for (int q = 0; q < kQuads / N; q++) {
+    const int quad = part + N * q;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const float4 a = am[((u * kApart + tile) * kQuads + quad) * 64 + lane];
+      A.x = __builtin_fmaf(a.x, ew[u], A.x);
+      A.y = __builtin_fmaf(a.y, ew[u], A.y);
+      A.z = __builtin_fmaf(a.z, ew[u], A.z);
+      A.w = __builtin_fmaf(a.w, ew[u], A.w);
+    }
+    acc[(quad * 2 + h) * W.stored + l32] = A;
+  }
+  if (part == 0 && h == 0) W.ml[tile * 32 + l32] = make_float2(ldexpf(M, -w.e), L);
+}
+
 // 32 query rows, four waves that share the keys: a wave has tiles wave, wave + 4, ..
 // of the chunk, LDS of its own for one K and one V tile, and no barriers until the
 // end: the next K tile is asked for when the scores are there, the next V tile when the
@@ -394,8 +447,7 @@ __device__ __forceinline__ void few_rows(const Params& P, const Work& W, unsigne
     copy_tile(W.v, base, vt, cv, false);
   }
   Rows<D> w;
-  const uint32_t r0 = W.row0 + l32;
-  load_rows_of(w, P, W, r0, h);
+  load_rows_of(w, P, W, W.row0 + l32, h);
   if (any) {
     wait_vmcnt<0>();
     while (true) {
@@ -420,52 +472,13 @@ __device__ __forceinline__ void few_rows(const Params& P, const Work& W, unsigne
   }
   w.l = swap_sum(w.l);
 
-  // the waves join in LDS, in fixed order, and store in the lanes' order
-  whd::lds_barrier();
-  constexpr int kQuads = S::kQuads;
-  float4* am = reinterpret_cast<float4*>(lds);                        // [4][D / 8][64]
-  float2* mm = reinterpret_cast<float2*>(am + kWaves * kQuads * 64);  // [4][32]
-#pragma unroll
-  for (int d = 0; d < S::DT; d++)
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      am[(wave * kQuads + 4 * d + i) * 64 + lane] =
-          make_float4(w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]);
-  if (h == 0) mm[wave * 32 + l32] = make_float2(w.m, w.l);
-  whd::lds_barrier();
-  float M = -INFINITY, L = 0.f, ew[kWaves];
-  float2 ml[kWaves];
-#pragma unroll
-  for (int u = 0; u < kWaves; u++) {
-    ml[u] = mm[u * 32 + l32];
-    M = __builtin_elementwise_maximum(M, ml[u].x);
-  }
-#pragma unroll
-  for (int u = 0; u < kWaves; u++) {
-    ew[u] = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - M) * w.qs);
-    L = __builtin_fmaf(ml[u].y, ew[u], L);
-  }
-  if (r0 >= W.n_rows) return;
-#pragma unroll
-  for (int q = 0; q < kQuads / kWaves; q++) {
-    const int quad = wave + kWaves * q;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < kWaves; u++) {
-      const float4 a = am[(u * kQuads + quad) * 64 + lane];
-      A.x = __builtin_fmaf(a.x, ew[u], A.x);
-      A.y = __builtin_fmaf(a.y, ew[u], A.y);
-      A.z = __builtin_fmaf(a.z, ew[u], A.z);
-      A.w = __builtin_fmaf(a.w, ew[u], A.w);
-    }
-    W.acc[(quad * 2 + h) * W.stored + l32] = A;
-  }
-  if (wave == 0 && h == 0) W.ml[l32] = make_float2(ldexpf(M, -w.e), L);
+  join_waves<D, kWaves>(w, W, lds, wave, lane);
 }
 
-// 128 query rows, 32 to a wave, that share stages of 64 keys in LDS, two of them in
-// turn: K and V are read from memory once for all of them.
-template <int D>
+// 32 RW query rows, 64 or 128, that share stages of 64 keys in LDS, two of them in
+// turn: K and V are read from memory once for all of them.  A wave has 32 rows, of a
+// stage all keys or, with 64 rows, half of them.
+template <int D, int RW>
 __device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsigned char* lds) {
   using S = Shape<D>;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
@@ -504,7 +517,8 @@ __device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsign
   };
   issue(W.c0, 0);
   Rows<D> w;
-  const uint32_t r0 = W.row0 + 32 * wave + l32;
+  constexpr int kTiles = 2 * RW / kWaves;  // of 32 keys, of a stage, for a wave
+  const uint32_t r0 = W.row0 + 32 * (wave % RW) + l32, first = kTiles == 1 ? wave / RW : 0;
   load_rows_of(w, P, W, r0, h);
   uint32_t buf = 0;
 #pragma unroll 1
@@ -514,23 +528,28 @@ __device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsign
     __builtin_amdgcn_s_barrier();  // everyone's; and everyone has read the stage before
     asm volatile("" ::: "memory");
     if (base + kStageKeys < W.c1) issue(base + kStageKeys, buf ^ 1);
-    const uint32_t kt = lds0 + buf * 4 * S::kTile, vt = kt + 2 * S::kTile;
-    const int left = W.c1 - base;
-    f32x16 s[2];
-    scores(w, kt, l32, h, s[0]);
-    scores(w, kt + S::kTile, l32, h, s[1]);
-    if (left < static_cast<int>(kStageKeys)) {
-      mask_scores(s[0], left, h);
-      mask_scores(s[1], left - 32, h);
-      clear_values<D>(vt, left, lane);  // the waves store the same, each before it reads the rows
-      clear_values<D>(vt + S::kTile, left - 32, lane);
+    const uint32_t kt = lds0 + buf * 4 * S::kTile + first * S::kTile, vt = kt + 2 * S::kTile;
+    const int left = W.c1 - base - 32 * first;
+    f32x16 s[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; n++) scores(w, kt + n * S::kTile, l32, h, s[n]);
+    if (left < 32 * kTiles) {
+#pragma unroll
+      for (int n = 0; n < kTiles; n++) {
+        mask_scores(s[n], left - 32 * n, h);
+        clear_values<D>(vt + n * S::kTile, left - 32 * n, lane);  // the waves store the same, each before it reads the rows
+      }
     }
-    half8 ph[4], pl[4];
-    weigh<D, 2>(w, s, ph, pl);
-    add_values<D, 2>(w, vt, ph, pl, lane);
+    half8 ph[2 * kTiles], pl[2 * kTiles];
+    weigh<D, kTiles>(w, s, ph, pl);
+    add_values<D, kTiles>(w, vt, ph, pl, lane);
   }
-  mend_values(w, W.v, RS, W.c0, W.c1, 0, 1, lane);
+  mend_values(w, W.v, RS, W.c0, W.c1, first, kTiles == 1 ? 2 : 1, lane);
   w.l = swap_sum(w.l);
+  if constexpr (kTiles == 1) {
+    join_waves<D, 2>(w, W, lds, wave, lane);
+    return;
+  }
   if (r0 >= W.n_rows) return;
   float4* const acc = W.acc + wave * 32 * (D / 4);
 #pragma unroll
@@ -544,7 +563,7 @@ __device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsign
 
 // grid: the prefixes' workgroups, then the members' own rows'; KV head fastest
 // (with 8 KV heads a head's workgroups run on one XCD and share its L2).  RW: tiles of
-// 32 query rows that a prefix's workgroup takes, 1 or 4.
+// 32 query rows that a prefix's workgroup takes, 1, 2 or 4.
 template <int D, int RW>
 __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Params P) {
   extern __shared__ __align__(256) unsigned char lds[];
@@ -571,7 +590,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Pa
     W.ml = P.ml_p + part * 32;
     W.acc = P.acc_p + part * 32 * (D / 4);
     if constexpr (RW > 1) {
-      many_rows<D>(P, W, lds);
+      many_rows<D, RW>(P, W, lds);
       return;
     }
   } else {
@@ -724,21 +743,37 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   P.own_rows = P.G < 32 ? P.G : 32;
   P.scale = kLog2e / sqrtf(static_cast<float>(D));
   const size_t members = n_groups * n_per, cus = static_cast<size_t>(wh::cu_count());
-  // Prefix.  Work: 128 keys of a tile per CU.  Little work, or one that memory bounds (up to
-  // 64 query rows): 32 query rows to a workgroup, one workgroup per CU, as few partial
-  // results.  More: two per CU, so that one's products run beside the other's exponentials,
-  // or 128 rows to a workgroup, whose stages then are read from the L2 once for all of them
-  // (where the rows fill it to 4/5).  A call, 32 / 8 heads of 128, 32 rows at 1 and 2
-  // workgroups per CU, 128 rows at 1 and 2: 32 members (128 rows) at 4000 keys (work 4) 18.6,
-  // 22.8, 21.7, 21.7 us, at 16000 (16) 36.2, 35.5, 33.2, 37.9, at 60000 (59) 105, 99, 94, 92;
-  // 128 members at 2000 (8) 34.9, 37.6, 34.3, 33.8, at 8000 (31) 60, 63, 53, 59, at 30000 (117)
-  // 189, 163, 152, 140; 16 members (64 rows) at 60000 (29) 65, 69; 48 (192 rows) at 60000 151,
-  // 129, 139, 135.  32 / 4 heads of 64: 32 members (256 rows) at 4000 (4) 13.6, 14.5, 15.6,
-  // 15.6, at 16000 (16) 25.1, 22.4, 23.7, 24.8, at 30000 (29) 39.1, 32.7, 35.1, 31.6.
-  const double work = static_cast<double>(n_groups * n_kv * P.tiles) * static_cast<double>(max_prefix) / (128.0 * static_cast<double>(cus));
-  const uint32_t of_four = (P.tiles + 3) / 4 * 4;
-  P.rw = 4 * of_four <= 5 * P.tiles && work >= (D == 128 ? 10.0 : 24.0) ? 4 : 1;
-  const bool two = P.rw == 4 ? D == 64 || work >= 56.0 : P.tiles >= 3 && work >= (D == 128 ? 20.0 : 7.0);
+  // Prefix.  Work: 128 keys of a tile per CU.  Little work: 32 query rows to a workgroup, one
+  // workgroup per CU, as few partial results.  More: 64 or 128 rows to a workgroup, whose
+  // stages are read from the L2 once for all of them (where the rows fill it), then two
+  // workgroups per CU, so that one's products run beside the other's exponentials, unless the
+  // members' own rows, which memory bounds, need the second place.  A call in us, 32 / 8 heads
+  // of 128, with 32, 64 and 128 rows at one / at two workgroups per CU:
+  //   members  prefix  own  work       32           64          128
+  //        32    4000    0     4  17.3 / 18.6  18.0 / 17.8  20.6 / 20.6
+  //        64    6000    0    12  31.0 / 29.6  30.4 / 29.5  28.9 / 32.0
+  //        64    6000  350    12  42.6 / 47.9  40.8 / 47.7  44.4 / 46.4
+  //        48   12000    0    18  37.5 / 35.7  37.5 / 35.4  38.0 / 38.2
+  //        64   20000  350    39  85.0 / 82.8  78.9 / 81.8  69.9 / 79.1
+  //        48   60000  350    88  152 / 133    140 / 125    151 / 137
+  //        64   40000  350    78  145 / 131    134 / 121    123 / 118
+  //        16   60000   50    29  63.5 / 65.6  61.0 / 59.1  82.7 / 76.4
+  //        48  131000  400   192  323 / 273    293 / 258    319 / 285
+  //        40   60000    0    73  129 / 115    134 / 119    145 / 132  (5 tiles)
+  // 32 / 4 heads of 64, whose rows are half as long:
+  //        16    4000    0     2  10.6 / 11.8  12.0 / 12.2  13.0 / 13.1
+  //        32   16000  100    16  24.2 / 21.8  24.1 / 23.8  22.9 / 25.1
+  //        24   60000  100    44  53.5 / 43.2  51.9 / 44.7  55.7 / 49.8
+  //        32   60000  400    59  64.5 / 54.3  62.2 / 51.1  54.6 / 49.6
+  auto work_of = [&](size_t rows_of_32, size_t keys) {
+    return static_cast<double>(rows_of_32) * static_cast<double>(keys) / (128.0 * static_cast<double>(cus));
+  };
+  const double work = work_of(n_groups * n_kv * P.tiles, max_prefix), work_own = work_of(members * n_kv * P.own_tiles, max_own);
+  const uint32_t of_four = (P.tiles + 3) / 4 * 4, of_two = (P.tiles + 1) / 2 * 2;
+  if (D == 128) P.rw = work < 10.0 ? 1 : 4 * of_four <= 5 * P.tiles && 4.0 * work_own <= work ? 4 : 8 * of_two <= 9 * P.tiles ? 2 : 1;
+  else P.rw = 4 * of_four <= 5 * P.tiles && work >= 24.0 ? 4 : 1;
+  const double two_from = D == 64 ? P.rw == 4 ? 0.0 : 7.0 : P.rw == 4 ? 56.0 : P.rw == 2 ? 16.0 : 20.0;
+  const bool two = (P.rw > 1 || P.tiles >= 3) && work >= two_from && 10.0 * work_own <= work;
   const size_t prefix = n_groups * n_kv * ((P.tiles + P.rw - 1) / P.rw);
   const size_t least = P.rw == 1 ? kLeastChunk : 256;
   P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp((two ? 2 : 1) * cus / prefix, 1, div_up(max_prefix, least)));
@@ -779,7 +814,10 @@ int launch_all(const Params& P, hipStream_t s) {
   const size_t own = static_cast<size_t>(P.n_groups) * P.n_per * P.co * P.n_kv * P.own_tiles;
   const size_t wgs = P.n_prefix_wgs + own;
   if (wgs) {
-    const int st = P.rw == 1 ? launch_partial<D, 1>(P, wgs, s) : launch_partial<D, 4>(P, wgs, s);
+    int st;
+    if (P.rw == 1) st = launch_partial<D, 1>(P, wgs, s);
+    else if (D == 64 || P.rw == 4) st = launch_partial<D, 4>(P, wgs, s);
+    else if constexpr (D == 128) st = launch_partial<D, 2>(P, wgs, s);
     if (st) return st;
   }
   const size_t items = static_cast<size_t>(P.n_groups) * P.n_kv * P.tiles * (D / 8);
