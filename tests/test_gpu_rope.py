@@ -70,7 +70,7 @@ def case(groups=1, per=3, new=1, heads=8, kv=2, d=128, rot=0, inter=False, magni
             expect[1, m, i] = vals[row].astype(np.float16).view(np.uint16)
             err = np.abs(have[0][m, i].astype(np.float64) - want_k[row])
             assert (err <= bound_k[row] + np.abs(want_k[row]) * 2.0 ** -11 * (1 + 2.0 ** -10) + 2.0 ** -25).all(), (row, err.max())
-            if not k_norm and pos.max() < 10 ** 6:  # in 64 bits: the row is the formula's
+            if pos.max() < 10 ** 6:  # in 64 bits, the norm too: the row is the formula's
                 far = have[0][m, i] != _members.stored(want_k[row])
                 assert far.mean() <= 2.0 ** -9, far.mean()  # but for sums that lie on the border of two f32
             expect[0, m, i] = have[0][m, i].view(np.uint16)

@@ -25,7 +25,6 @@
 #include <algorithm>
 #include <memory>
 #include <new>
-#include <type_traits>
 
 #include "members.hpp"
 #include "tree.hpp"
@@ -89,26 +88,6 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
   }
   return v;
 }
-// Sum over the wave's 64 lanes, in every lane: swaps within rows of 16 lanes, then of
-// rows and halves (as wave_join, tree.hpp).
-__device__ __forceinline__ double wave_sum_f64(double v) {
-  auto lo = [](double x) { return static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, x)); };
-  auto hi = [](double x) { return static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, x) >> 32); };
-  auto make = [](uint32_t l, uint32_t h) { return __builtin_bit_cast(double, static_cast<unsigned long long>(h) << 32 | l); };
-  auto dpp = [](uint32_t x, auto ctrl) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xF, 0xF, false));
-  };
-  auto step = [&](auto ctrl) { v += make(dpp(lo(v), ctrl), dpp(hi(v), ctrl)); };
-  step(std::integral_constant<int, 0xB1>{});
-  step(std::integral_constant<int, 0x4E>{});
-  step(std::integral_constant<int, 0x141>{});
-  step(std::integral_constant<int, 0x140>{});
-  const auto l16 = __builtin_amdgcn_permlane16_swap(lo(v), lo(v), false, false), h16 = __builtin_amdgcn_permlane16_swap(hi(v), hi(v), false, false);
-  v = make(l16[0], h16[0]) + make(l16[1], h16[1]);
-  const auto l32 = __builtin_amdgcn_permlane32_swap(lo(v), lo(v), false, false), h32 = __builtin_amdgcn_permlane32_swap(hi(v), hi(v), false, false);
-  return make(l32[0], h32[0]) + make(l32[1], h32[1]);
-}
-
 struct Params {
   const float* logits;
   size_t ld;
@@ -210,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
     float rest[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kPer; j++) rest[j & 1] += __builtin_amdgcn_exp2f((x[j] - m) * kLog2e);
-    const double sum = wave_sum_f64(rest[0] + rest[1]);
+    const double sum = whd::lanes_sum_f64<64>(rest[0] + rest[1]);
     if (lane == 0) rests[wave] = sum;
   };
   gather(value32(least));
@@ -265,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const Params P) {
 #pragma unroll
       for (uint32_t i = lane; i < kList; i += 64)
         if (i < c) sum += terms[i];
-      sum = wave_sum_f64(sum);
+      sum = whd::lanes_sum_f64<64>(sum);
 #pragma unroll
       for (int w = 0; w < kWaves; w++) sum += rests[w];
       if (lane == 0) P.sums[chunk] = sum;
@@ -366,7 +345,7 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(const Params
         const uint32_t x = lists[static_cast<size_t>(b) * per_beam + c * P.n_out].x;
         if (x) sum += sums[c] * exp(static_cast<double>(value32(x)) - m);
       }
-      l = m + log(wave_sum_f64(sum));
+      l = m + log(whd::lanes_sum_f64<64>(sum));
       if (most == 0 || !(l < INFINITY)) st = kGone;  // no token is allowed, or one at +inf
     }
     if (st != kOpen) {

@@ -4,6 +4,8 @@
 // kernels and launch them.
 #pragma once
 
+#include <type_traits>
+
 #include "wh_common.hpp"
 
 namespace wh {
@@ -47,3 +49,31 @@ size_t shared_attention_workspace_bytes(size_t n_groups, size_t n_per, size_t n_
 int launch_shared_attention(const SharedAttnArgs& a, void* workspace, hipStream_t stream);
 
 }  // namespace wh
+
+namespace whd {
+
+// Sum over the L lanes (32 or 64) that work together, in every one of them: swaps within rows of
+// 16 lanes, then of rows and halves (as wave_join, tree.hpp).
+template <int L>
+__device__ __forceinline__ double lanes_sum_f64(double v) {
+  auto lo = [](double x) { return static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, x)); };
+  auto hi = [](double x) { return static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, x) >> 32); };
+  auto make = [](uint32_t l, uint32_t h) { return __builtin_bit_cast(double, static_cast<unsigned long long>(h) << 32 | l); };
+  auto dpp = [](uint32_t x, auto ctrl) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  auto step = [&](auto ctrl) { v += make(dpp(lo(v), ctrl), dpp(hi(v), ctrl)); };
+  step(std::integral_constant<int, 0xB1>{});
+  step(std::integral_constant<int, 0x4E>{});
+  step(std::integral_constant<int, 0x141>{});
+  step(std::integral_constant<int, 0x140>{});
+  const auto l16 = __builtin_amdgcn_permlane16_swap(lo(v), lo(v), false, false), h16 = __builtin_amdgcn_permlane16_swap(hi(v), hi(v), false, false);
+  v = make(l16[0], h16[0]) + make(l16[1], h16[1]);
+  if constexpr (L == 64) {
+    const auto l32 = __builtin_amdgcn_permlane32_swap(lo(v), lo(v), false, false), h32 = __builtin_amdgcn_permlane32_swap(hi(v), hi(v), false, false);
+    v = make(l32[0], h32[0]) + make(l32[1], h32[1]);
+  }
+  return v;
+}
+
+}  // namespace whd

@@ -10,9 +10,9 @@
 //
 // The angle is formed in 64 bits, as turns, of which only the part behind the
 // point is kept: in 32 bits p * inv_freq would be off by p 2^-24 radians.  Its
-// sine and cosine are of that part, in 64 bits; k is turned in 64 bits and
-// rounded to f32, then to f16, so a cache row is what the formula gives (and what
-// wh_attention_tree stores), q in 32.
+// sine and cosine are of that part, in 64 bits; k is normed and turned in 64 bits
+// and rounded to f32, then to f16, so a cache row is what the formula gives (and
+// what wh_attention_tree stores), q in 32.
 #include <type_traits>
 
 #include "members.hpp"
@@ -31,8 +31,8 @@ struct Params {
   _Float16 *k_cache, *v_cache;
   uint32_t n_per, n_new, n_heads, n_kv, d, half, groups, rows;  // half: turned pairs
   int interleaved;
-  float eps, per_d;      // 1 / d
-  double magnitude;
+  float eps;
+  double per_d, magnitude;  // 1 / d
 };
 
 // A 64-bit value as the cache holds it: rounded to f32, then to f16.  (The
@@ -135,19 +135,37 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const Params P) {
   for (int n = 0; n < N; n++) {
     const uint32_t h = h0 + n * (64 / L);
     const bool is_q = h < P.n_heads;
-    if ((is_q ? P.q_norm : P.k_norm) != nullptr) {
-      float sum = 0.f;
+    double kx[PP], ky[PP];  // of a key head
+    if (is_q) {
+      if (P.q_norm) {
+        float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < PP; u++)
-        if (in[u]) sum = __builtin_fmaf(x[n][u], x[n][u], __builtin_fmaf(y[n][u], y[n][u], sum));
-      sum = lanes_sum<L>(sum);
-      const float mean = __builtin_fmaf(sum, P.per_d, P.eps);
-      float r = __builtin_amdgcn_rsqf(mean);         // off by a unit of f32 at most
-      if (mean < 0x1p-126f) r = 1.0f / sqrtf(mean);  // which it flushes
+        for (int u = 0; u < PP; u++)
+          if (in[u]) sum = __builtin_fmaf(x[n][u], x[n][u], __builtin_fmaf(y[n][u], y[n][u], sum));
+        const float mean = __builtin_fmaf(lanes_sum<L>(sum), static_cast<float>(P.per_d), P.eps);
+        float r = __builtin_amdgcn_rsqf(mean);         // off by a unit of f32 at most
+        if (mean < 0x1p-126f) r = 1.0f / sqrtf(mean);  // which it flushes
+#pragma unroll
+        for (int u = 0; u < PP; u++) x[n][u] = x[n][u] * r * qw[u][0], y[n][u] = y[n][u] * r * qw[u][1];
+      }
+    } else {
+      double r = 1.0;
+      if (P.k_norm) {
+        double sum = 0.0;
+#pragma unroll
+        for (int u = 0; u < PP; u++) {
+          const double dx = in[u] ? x[n][u] : 0.f, dy = in[u] ? y[n][u] : 0.f;
+          sum = __builtin_fma(dx, dx, __builtin_fma(dy, dy, sum));
+        }
+        const double mean = __builtin_fma(whd::lanes_sum_f64<L>(sum), P.per_d, static_cast<double>(P.eps));
+        r = __builtin_amdgcn_rsq(mean);                                             // to 2^-22 or so, and Newton's step
+        if (mean < INFINITY) r *= __builtin_fma(-0.5 * mean * r, r, 1.5);
+      }
 #pragma unroll
       for (int u = 0; u < PP; u++) {
-        x[n][u] = x[n][u] * r * (is_q ? qw[u][0] : kw[u][0]);
-        y[n][u] = y[n][u] * r * (is_q ? qw[u][1] : kw[u][1]);
+        const double nx = x[n][u] * r * kw[u][0], ny = y[n][u] * r * kw[u][1];
+        kx[u] = turned[u] ? nx * cs[u] - ny * sn[u] : nx;
+        ky[u] = turned[u] ? nx * sn[u] + ny * cs[u] : ny;
       }
     }
     if (h >= n_slots) continue;
@@ -164,18 +182,16 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const Params P) {
           o[b[u]] = present && fits ? oy : other;
         }
       } else {
-        const double kx = turned[u] ? x[n][u] * cs[u] - y[n][u] * sn[u] : x[n][u];
-        const double ky = turned[u] ? x[n][u] * sn[u] + y[n][u] * cs[u] : y[n][u];
         const uint32_t kh = h - P.n_heads;
         if (P.k_out) {
           float* o = P.k_out + row * P.ldk_out + static_cast<size_t>(kh) * P.d;
-          o[a[u]] = present ? static_cast<float>(kx) : 0.f;
-          o[b[u]] = present ? static_cast<float>(ky) : 0.f;
+          o[a[u]] = present ? static_cast<float>(kx[u]) : 0.f;
+          o[b[u]] = present ? static_cast<float>(ky[u]) : 0.f;
         }
         if (P.k_cache && present && fits) {
           const size_t at = ((m * P.max_rows + static_cast<size_t>(i)) * P.n_kv + kh) * P.d;
-          P.k_cache[at + a[u]] = stored(kx);
-          P.k_cache[at + b[u]] = stored(ky);
+          P.k_cache[at + a[u]] = stored(kx[u]);
+          P.k_cache[at + b[u]] = stored(ky[u]);
           P.v_cache[at + a[u]] = static_cast<_Float16>(vx[n][u]);
           P.v_cache[at + b[u]] = static_cast<_Float16>(vy[n][u]);
         }
@@ -190,10 +206,10 @@ int launch(const Params& P, hipStream_t s) {
   Params A = P;
   // few rows: the launch is as long as its dependent loads, and takes as many waves as there are
   // heads; many rows: a wave's heads share the angles (4000 rows of 32 / 8 heads of 128 with 4,
-  // 5, 8 and 10 heads 38.4, 37.1, 36.2, 36.3 us, normed 41.7, 41.0, 40.6, 42.1; 16 / 4 heads of
-  // 256 47.3, 45.2, 49.6, 45.8; 16 x 300 of 32 / 4 heads of 64 in neighbouring pairs, two heads
-  // at a time, 22.2, 21.7, 23.0, 23.3)
-  constexpr int kMany = L == 64 && PP == 1 ? 8 : 5;
+  // 5, 8 and 10 heads 35.5, 35.9, 35.5, 35.2 us, in neighbouring pairs 37.3, 40.8, 38.4, 38.1,
+  // normed 41.7, 42.0, 41.2, 41.1; 16 / 4 heads of 256, normed, 50.8, 47.2, 52.8, 51.0; 16 x 300
+  // of 32 / 4 heads of 64, two heads at a time, 21.9, 21.4, 22.0, 22.2)
+  constexpr int kMany = PP == 1 ? 4 : 5;
   const bool few = static_cast<size_t>(P.rows) * slots < kManyHeads;
   const uint32_t per = 64 / L * (few ? 2 : kMany);
   A.groups = (slots + per - 1) / per;
@@ -239,7 +255,7 @@ int launch_rope(const wh_rope_rules& r, const RopeArgs& a, hipStream_t s) {
   P.rows = static_cast<uint32_t>(a.n_members * a.n_new);
   P.interleaved = r.interleaved;
   P.eps = r.norm_eps;
-  P.per_d = 1.0f / static_cast<float>(a.head_dim);
+  P.per_d = 1.0 / static_cast<double>(a.head_dim);
   P.magnitude = r.magnitude == 0.0 ? 1.0 : r.magnitude;
   return P.d <= 64 ? launch<32, 1>(P, s) : P.d <= 128 ? launch<64, 1>(P, s) : launch<64, 2>(P, s);
 }
