@@ -494,7 +494,10 @@ KERNEL_SOURCE_GROUPS["decode"] = tuple(sorted(set(sum(KERNEL_SOURCE_GROUPS.value
                                               {_C + "decode.hip", _C + "embed.hip"}))
 # verifying a tree of drafted tokens: attention, logits, acceptance and cache rows
 KERNEL_SOURCE_GROUPS["tree"] = (_C + "tree_attention.hip", _C + "tree_step.hip", _C + "tree.hip", _C + "logits.hip", _C + "tree.hpp",
-                                _C + "gemm_dev.hpp") + _COMMON
+                                _C + "gemm_dev.hpp", _C + "attn_dev.hpp", _C + "llama_step.hpp") + _COMMON
+# several continuations of one prompt: norms and rotation, attention, beam selection and reordering
+KERNEL_SOURCE_GROUPS["members"] = (_C + "rope.hip", _C + "shared_attention.hip", _C + "beam.hip", _C + "members_step.hip", _C + "members.hpp",
+                                   _C + "tree.hpp", _C + "gemm_dev.hpp", _C + "attn_dev.hpp", _C + "llama_step.hpp") + _COMMON
 GEMV_KERNEL_SOURCES = KERNEL_SOURCE_GROUPS["gemv"]
 PMC_PROFILE = ROOT / "profiles" / "gemv_q4_0_14336x4096_pmc.txt"
 

@@ -765,6 +765,10 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   //        32   16000  100    16  24.2 / 21.8  24.1 / 23.8  22.9 / 25.1
   //        24   60000  100    44  53.5 / 43.2  51.9 / 44.7  55.7 / 49.8
   //        32   60000  400    59  64.5 / 54.3  62.2 / 51.1  54.6 / 49.6
+  // Several prompts are seldom of one length, and two shorter chunks per CU even that out (64
+  // dims: 6 x 5 members up to 12000 keys 28.8 -> 24.7 us, of equal lengths 30.6 -> 31.5; 16 x 1
+  // up to 6000 33.7 -> 27.9, equal 44.1 -> 47.1; of 128 dims it takes more than it gives: 6 x 5
+  // up to 12000 53.7 -> 51.2, equal 65.4 -> 71.3).
   auto work_of = [&](size_t rows_of_32, size_t keys) {
     return static_cast<double>(rows_of_32) * static_cast<double>(keys) / (128.0 * static_cast<double>(cus));
   };
@@ -773,7 +777,8 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   if (D == 128) P.rw = work < 10.0 ? 1 : 4 * of_four <= 5 * P.tiles && 4.0 * work_own <= work ? 4 : 8 * of_two <= 9 * P.tiles ? 2 : 1;
   else P.rw = 4 * of_four <= 5 * P.tiles && work >= 24.0 ? 4 : 1;
   const double two_from = D == 64 ? P.rw == 4 ? 0.0 : 7.0 : P.rw == 4 ? 56.0 : P.rw == 2 ? 16.0 : 20.0;
-  const bool two = (P.rw > 1 || P.tiles >= 3) && work >= two_from && 10.0 * work_own <= work;
+  const bool uneven = D == 64 && n_groups > 1 && work >= 16.0;
+  const bool two = (((P.rw > 1 || P.tiles >= 3) && work >= two_from) || uneven) && 10.0 * work_own <= work;
   const size_t prefix = n_groups * n_kv * ((P.tiles + P.rw - 1) / P.rw);
   const size_t least = P.rw == 1 ? kLeastChunk : 256;
   P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp((two ? 2 : 1) * cus / prefix, 1, div_up(max_prefix, least)));
