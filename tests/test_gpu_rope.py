@@ -135,3 +135,27 @@ def test_values_apart(gpu):
     k = down(caches[0], np.float16, kv * d).reshape(kv, d)
     assert not np.isfinite(k[0, 3]) and np.isfinite(np.delete(k[0], [3, 11])).all()
     assert (down(caches[1], np.float16, kv * d) == 1).all()
+
+
+def test_norms_of_tiny_heads(gpu):
+    """Heads whose mean square is no normal f32 number, and heads of zeros, without an epsilon.
+
+    Squares of 1e-19 are off by 2^-150, 7e-8 of them, as is each of the sum's steps in f32: with the other roundings of the
+    norm and the turn under 2^-19 of the pair.  Keys are normed in 64 bits."""
+    d, heads, kv = 64, 3, 2
+    x = np.full((1, (heads + 2 * kv) * d), 1e-19, np.float32) * np.tile([1, -1], (heads + 2 * kv) * d // 2).astype(np.float32)
+    x[0, d:2 * d] = 0            # query head 1
+    x[0, heads * d:heads * d + d] = 0  # key head 0
+    inv, w = np.linspace(0.1, 0.7, d // 2).astype(np.float32), np.linspace(0.5, 1.5, d).astype(np.float32)
+    xb, invb, wb, out, kout = up(x)[0], up(inv)[0], up(w)[0], DeviceBuffer(4 * heads * d), DeviceBuffer(4 * kv * d)
+    for eps in (0.0, 1e-6):
+        rules = ops.RopeRules(invb, 0, False, 1.0, wb, wb, eps)
+        ops.qk_norm_rope(rules, xb, xb.ptr + 4 * heads * d, xb.ptr + 4 * (heads + kv) * d, x.shape[1], x.shape[1], None, None, 1, 1, 1,
+                         heads, kv, d, out, heads * d, kout, kv * d, None, None, 0)
+        with np.errstate(invalid="ignore"):
+            want_q, _ = _members.rope(x[:, :heads * d].reshape(1, heads, d), np.array([0]), inv, d, False, 1.0, w, eps)
+            want_k, _ = _members.rope(x[:, heads * d:(heads + kv) * d].reshape(1, kv, d), np.array([0]), inv, d, False, 1.0, w, eps)
+        q, k = down(out, np.float32, heads * d).reshape(heads, d), down(kout, np.float32, kv * d).reshape(kv, d)
+        for got, want, bar in ((q, want_q[0], 2.0 ** -19), (k, want_k[0], 2.0 ** -23)):
+            assert np.array_equal(np.isnan(got), np.isnan(want)), eps
+            assert (np.abs(got - want) <= bar * np.abs(want))[~np.isnan(want)].all(), eps

@@ -16,6 +16,9 @@
 // are equal for that they are taken one maximum at a time.
 // lse in 64 bits: the few highest terms, which make the sum, are exponentials in
 // 64 bits, the others in 32 bits summed in 64.
+// The first launch is bound by memory (16 x 8 beams of 128256 logits, 65.7 MB, in 16.6
+// us, 4.0 TB/s; 4 of 32000 in 5), the second by its steps that wait for each other,
+// however few beams there are (9 and 6 us).
 //
 // Reordering.  A thread holds one 16-byte column of a state's rows for all beams:
 // it loads what its moved beams take before it stores any of it, so rows move in

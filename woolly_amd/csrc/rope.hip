@@ -13,6 +13,10 @@
 // sine and cosine are of that part, in 64 bits; k is normed and turned in 64 bits
 // and rounded to f32, then to f16, so a cache row is what the formula gives (and
 // what wh_attention_tree stores), q in 32.
+//
+// Many rows are bound by memory: 4000 of 32 / 8 heads of 128, 180 MB read and
+// written, 35.5 us, normed 41 (5.1 and 4.4 TB/s); few by the launch and two loads
+// one behind the other: 8 rows 3.1 us in a graph.
 #include <type_traits>
 
 #include "members.hpp"
@@ -21,7 +25,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr size_t kManyHeads = 32768;  // heads of all rows from which on a wave takes more turns
+constexpr size_t kManyHeads = 8192;  // heads of all rows from which on a wave takes more turns
 struct Params {
   const float *q, *k, *v;
   size_t ldq, ldkv, ldq_out, ldk_out, max_rows;
@@ -204,19 +208,24 @@ template <int L, int PP>
 int launch(const Params& P, hipStream_t s) {
   const uint32_t slots = P.n_heads + P.n_kv;
   Params A = P;
-  // few rows: the launch is as long as its dependent loads, and takes as many waves as there are
-  // heads; many rows: a wave's heads share the angles (4000 rows of 32 / 8 heads of 128 with 4,
-  // 5, 8 and 10 heads 35.5, 35.9, 35.5, 35.2 us, in neighbouring pairs 37.3, 40.8, 38.4, 38.1,
-  // normed 41.7, 42.0, 41.2, 41.1; 16 / 4 heads of 256, normed, 50.8, 47.2, 52.8, 51.0; 16 x 300
-  // of 32 / 4 heads of 64, two heads at a time, 21.9, 21.4, 22.0, 22.2)
-  constexpr int kMany = PP == 1 ? 4 : 5;
-  const bool few = static_cast<size_t>(P.rows) * slots < kManyHeads;
-  const uint32_t per = 64 / L * (few ? 2 : kMany);
+  // Few rows: the launch is as long as its dependent loads, and takes as many waves as there are
+  // pairs of heads; many rows: a wave's heads share the angles.  Rows of 32 / 8 heads of 128 with
+  // 2 and 4 heads to a wave: 60 rows 3.4, 3.6 us, 150 4.2, 4.2, 300 6.1, 5.6, 1200 14.6, 11.8; 4000
+  // with 4, 5, 8 and 10 heads 35.5, 35.9, 35.5, 35.2, in neighbouring pairs 37.3, 40.8, 38.4, 38.1,
+  // normed 41.7, 42.0, 41.2, 41.1.  Wider heads gain nothing from it (16 / 4 heads of 256 with 2, 3,
+  // 4 and 5: 2000 rows 24.6, 25.0, 27.0, 25.6, 4000 42.4, 41.7, 45.1, 43.7; 32 / 8 of 160, 4000
+  // rows: 65.9, 65.5, 64.6, 71.2).
+  const bool many = PP == 1 && static_cast<size_t>(P.rows) * slots >= kManyHeads;
+  const uint32_t per = 64 / L * (many ? 4 : 2);
   A.groups = (slots + per - 1) / per;
   const size_t items = static_cast<size_t>(P.rows) * A.groups;
   const unsigned grid = static_cast<unsigned>((items + kThreads / 64 - 1) / (kThreads / 64));
-  if (few) rope_kernel<L, PP, 2><<<grid, kThreads, 0, s>>>(A);
-  else rope_kernel<L, PP, kMany><<<grid, kThreads, 0, s>>>(A);
+  if constexpr (PP == 1) {
+    if (many) rope_kernel<L, PP, 4><<<grid, kThreads, 0, s>>>(A);
+    else rope_kernel<L, PP, 2><<<grid, kThreads, 0, s>>>(A);
+  } else {
+    rope_kernel<L, PP, 2><<<grid, kThreads, 0, s>>>(A);
+  }
   WH_LAUNCH_CHECK("norm and rotation launch");
   return WH_OK;
 }
