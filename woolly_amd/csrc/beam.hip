@@ -18,7 +18,8 @@
 // 64 bits, the others in 32 bits summed in 64.
 // The first launch is bound by memory (16 x 8 beams of 128256 logits, 65.7 MB, in 16.6
 // us, 4.0 TB/s; 4 of 32000 in 5), the second by its steps that wait for each other,
-// however few beams there are (9 and 6 us).
+// however few beams there are (8 beams 7.5 us, 4 beams 5.5: 3 until the bound is there,
+// 2 for the ranks and outputs, 1 for the histories).
 //
 // Reordering.  A thread holds one 16-byte column of a state's rows for all beams:
 // it loads what its moved beams take before it stores any of it, so rows move in
@@ -503,31 +504,35 @@ __global__ __launch_bounds__(64 * kPickWaves) void beam_pick_kernel(const Params
     if (t < wh::kMaxBeams) from[t] = b, have[t] = len_in[b];
   }
   if (!P.history) return;
-  // some columns of the histories at a time: what the beams take of them is read before any is written
+  // A wave has a beam (or two), and 256 columns of the histories at a time: what the beams take
+  // of them is read before any of it is written.
+  constexpr uint32_t kColumns = 4, kBeams = (wh::kMaxBeams + kPickWaves - 1) / kPickWaves;
   __syncthreads();
   uint32_t most = 0;
   for (uint32_t i = 0; i < P.n_beams; i++) most = max(most, have[i]);
   const size_t end = min(static_cast<size_t>(most) + 1, P.history_stride);
   uint32_t* const h = P.history + static_cast<size_t>(row0) * P.history_stride;
-  uint32_t* const tile = reinterpret_cast<uint32_t*>(ranks);
-  const uint32_t columns = kPickList * 2 / P.n_beams;
-  for (size_t p0 = 0; p0 < end; p0 += columns) {
-    const uint32_t n = static_cast<uint32_t>(min(end - p0, static_cast<size_t>(columns)));
-    for (uint32_t e = t; e < n * P.n_beams; e += threads) {
-      const uint32_t i = e / n;
-      const size_t p = p0 + e % n;
-      uint32_t v = chosen[i].token;
-      asm("" : "+v"(v));  // not one load from either place
-      if (p < have[i]) v = h[from[i] * P.history_stride + p];
-      tile[e] = v;
+  for (size_t p0 = 0; p0 < end; p0 += 64 * kColumns) {
+    uint32_t v[kBeams][kColumns];
+    bool moves[kBeams][kColumns];
+#pragma unroll
+    for (uint32_t u = 0; u < kBeams; u++) {
+      const uint32_t i = min(wave + u * n_waves, P.n_beams - 1), parent = from[i], n = have[i], token = chosen[i].token;
+#pragma unroll
+      for (uint32_t j = 0; j < kColumns; j++) {
+        const size_t p = p0 + 64 * j + lane;
+        moves[u][j] = wave + u * n_waves < P.n_beams && p < end && (p == n || (p < n && parent != i));
+        uint32_t old = 0;
+        if (moves[u][j] && p < n) old = h[parent * P.history_stride + p];
+        v[u][j] = p == n ? token : old;
+      }
     }
     __syncthreads();
-    for (uint32_t e = t; e < n * P.n_beams; e += threads) {
-      const uint32_t i = e / n;
-      const size_t p = p0 + e % n;
-      if (p <= have[i] && (p == have[i] || from[i] != i)) h[i * P.history_stride + p] = tile[e];
-    }
-    __syncthreads();
+#pragma unroll
+    for (uint32_t u = 0; u < kBeams; u++)
+#pragma unroll
+      for (uint32_t j = 0; j < kColumns; j++)
+        if (moves[u][j]) h[static_cast<size_t>(wave + u * n_waves) * P.history_stride + p0 + 64 * j + lane] = v[u][j];
   }
 }
 
