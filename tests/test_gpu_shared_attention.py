@@ -153,6 +153,35 @@ def test_infinities_of_many_rows(gpu, heads, kv, d, per, max_prefix, max_own):
         assert (np.abs(got[1, 0] - want[0])[rest] <= bound[0, rest]).all()
 
 
+# heads, kv, d, groups, members each, max_prefix: chunks shared by the lengths, in workgroups of 32, 64 and 128 query rows,
+# more groups than chunks per group, as many groups as a wave has lanes, and one more
+GROUPS = [(8, 2, 64, 7, 3, 24000), (4, 1, 128, 2, 16, 84000), (4, 1, 128, 3, 31, 28000), (8, 1, 64, 33, 2, 10000), (6, 1, 128, 64, 1, 5200),
+          (6, 1, 128, 65, 1, 5200), (16, 16, 64, 12, 1, 2000)]
+
+
+@pytest.mark.parametrize("heads, kv, d, groups, per, max_prefix", GROUPS)
+def test_groups_of_any_length(gpu, heads, kv, d, groups, per, max_prefix):
+    """Prefixes of equal lengths, of lengths far apart, empty ones among them, and of lengths that do not fit."""
+    print(f"[case] shared groups {heads} {kv} {d} {groups} {per} {max_prefix}", flush=True)
+    r = np.random.default_rng(groups)
+    own = [int(v) for v in r.integers(0, 9, groups * per)]
+    c = Case(heads, kv, d, per, [max_prefix] * groups, own, max_prefix=max_prefix).upload()
+    some = sorted({0, 1, groups // 2, groups - 1})
+    falling = [int(v) for v in np.exp(np.linspace(np.log(max_prefix), 0, groups))]
+    for lens in ([300] * groups, falling, falling[::-1], [int(v) for v in r.integers(0, 2000, groups)], [0] * groups,
+                 [0] * (groups - 1) + [max_prefix], [max_prefix] + [128] * (groups - 1)):
+        lens = [min(l, max_prefix) for l in lens]
+        c.prefix = lens
+        c.lens[0].upload(u32(lens))
+        c.call()
+        c.check(sorted({g * per + m for g in some for m in {0, per - 1}}))
+    lens[groups // 2] = max_prefix + 1
+    c.lens[0].upload(u32(lens))
+    c.call()
+    assert np.isnan(c.out()[groups // 2 * per:(groups // 2 + 1) * per]).all()
+    c.check([m for m in (0, groups * per - 1) if m // per != groups // 2])
+
+
 def test_prefix_or_own_rows_alone(gpu):
     for d in (64, 128):
         c = Case(8, 2, d, 3, [200], [0, 0, 0]).upload()

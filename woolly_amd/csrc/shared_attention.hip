@@ -46,6 +46,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f;
 constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
 constexpr uint32_t kLeastChunk = 128;  // keys: a tile for every wave
+constexpr double kShareFrom = 10.0;    // work (plan)
 constexpr uint32_t kStageKeys = 64;    // of a workgroup of 128 query rows
 // LDS reads run one step ahead of the matrix products that take them: neither moves
 // across this
@@ -63,12 +64,14 @@ struct Params {
   uint32_t own_tiles;    // of a member's G
   uint32_t own_rows;     // rows of such a tile that are stored: min(G, 32)
   uint32_t cp, co;       // chunks of a prefix, of a member's own rows
+  uint32_t slots;        // chunks of all prefixes: cp each, or (shared) as the lengths are
+  int shared;
   uint32_t n_prefix_wgs;
   uint32_t rw;           // tiles of a prefix's workgroup
   float scale;           // log2(e) / sqrt(d)
   // workspace: partial results (largest score of the row in units of q . k, sum), registers
   // of the lanes [D / 8][2][rows]
-  float2* ml_p;          // [n_groups][cp][n_kv][tiles][32]
+  float2* ml_p;          // [slots][n_kv][tiles][32]
   float4* acc_p;
   float2* ml_o;          // [members][co][n_kv][own_tiles][own_rows]
   float4* acc_o;
@@ -82,6 +85,51 @@ __device__ __forceinline__ uint32_t rows_of(const uint32_t* len, uint32_t i, uin
 __device__ __forceinline__ uint32_t chunk_of(uint32_t rows, uint32_t chunks) {
   const uint32_t even = (rows + chunks - 1) / chunks;
   return max((even + kLeastChunk - 1) / kLeastChunk * kLeastChunk, kLeastChunk);
+}
+
+// Groups whose prefixes differ in length share the slots: about the shortest chunks that fit
+// into them.  Lane l has group l.  With n = ceil(units / per) in
+// f32: a quotient is off by 2^-22 of itself and, below 2^20 units, an integer or at least 2^-20
+// of itself above one.
+struct Shares {
+  uint32_t rows, n, upto;  // of the lane's group: cache rows, chunks, chunks up to its last one
+  uint32_t chunk;
+};
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t lane) {
+  return __builtin_amdgcn_readlane(v, __builtin_amdgcn_readfirstlane(lane));
+}
+__device__ __forceinline__ Shares shares_of(const Params& P, uint32_t lane) {
+  Shares a;
+  a.rows = lane < P.n_groups ? rows_of(P.prefix_len, lane, P.max_prefix) : 0;
+  const uint32_t units = (a.rows + kLeastChunk - 1) / kLeastChunk;
+  const uint32_t all = whd::wave_join(units, [](uint32_t x, uint32_t y) { return x + y; });
+  auto quotient = [](uint32_t u, uint32_t by) {
+    return ceilf(static_cast<float>(u) * (__builtin_amdgcn_rcpf(static_cast<float>(by)) * (1.f - 0x1p-21f)));
+  };
+  // of chunks of `least` units there may be too many, of `most` there are not: each group rounds up once
+  uint32_t least = max((all + P.slots - 1) / P.slots, 1u), most = max((all + P.slots - P.n_groups - 1) / (P.slots - P.n_groups), 1u);
+  auto fits = [&](uint32_t per) {
+    return whd::wave_join(static_cast<uint32_t>(quotient(units, per)), [](uint32_t x, uint32_t y) { return x + y; }) <= P.slots;
+  };
+  if (fits(least)) most = least;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t mid = least + (most - least) / 2;
+    if (fits(mid)) most = mid; else least = mid;
+  }
+  const uint32_t per = __builtin_amdgcn_readfirstlane(most);
+  a.chunk = per * kLeastChunk;
+  a.n = static_cast<uint32_t>(quotient(units, per));
+  // sums over the lanes up to this one: within rows of 16, then the rows before
+  uint32_t v = a.n;
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x111, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x112, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x114, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x118, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xA, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xC, 0xF, false));
+  a.upto = v;
+  return a;
 }
 
 // Two weights as f16 hi + lo 2^-11: elements i and i + 1 of the fragments.
@@ -574,8 +622,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Pa
     b /= P.n_kv;
     const uint32_t n_rg = (P.tiles + RW - 1) / RW, rg = b % n_rg;
     b /= n_rg;
-    const uint32_t c = b % P.cp, g = b / P.cp;
-    const uint32_t rows = rows_of(P.prefix_len, g, P.max_prefix), chunk = chunk_of(rows, P.cp);
+    const uint32_t slot = b;
+    uint32_t g, c, rows, chunk;
+    if (!P.shared) {
+      g = slot / P.cp, c = slot % P.cp;
+      rows = rows_of(P.prefix_len, g, P.max_prefix);
+      chunk = chunk_of(rows, P.cp);
+    } else {
+      const Shares a = shares_of(P, threadIdx.x & 63);
+      g = __builtin_popcountll(__ballot(a.upto <= slot));
+      if (g >= P.n_groups) return;
+      c = slot - lane_of(a.upto - a.n, g);
+      rows = lane_of(a.rows, g);
+      chunk = a.chunk;
+    }
     W.c0 = c * chunk;
     W.c1 = min(W.c0 + chunk, rows);
     if (W.c0 >= W.c1) return;
@@ -586,7 +646,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_partial_kernel(const Pa
     W.row0 = rg * 32 * RW;
     W.n_rows = P.R;
     W.stored = 32;
-    const size_t part = ((static_cast<size_t>(g) * P.cp + c) * P.n_kv + W.kvh) * P.tiles + rg * RW;
+    const size_t part = (static_cast<size_t>(slot) * P.n_kv + W.kvh) * P.tiles + rg * RW;
     W.ml = P.ml_p + part * 32;
     W.acc = P.acc_p + part * 32 * (D / 4);
     if constexpr (RW > 1) {
@@ -658,7 +718,7 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
   };
   // the first loads are asked for with the lengths: what turns out not to be there is not joined
   const size_t step_p = static_cast<size_t>(P.n_kv) * P.tiles, step_o = static_cast<size_t>(P.n_kv) * P.own_tiles;
-  const size_t at_p = (static_cast<size_t>(g) * P.cp * P.n_kv + kvh) * P.tiles + tile;
+  size_t at_p = (static_cast<size_t>(g) * P.cp * P.n_kv + kvh) * P.tiles + tile;
   const size_t at_o = (static_cast<size_t>(m) * P.co * P.n_kv + kvh) * P.own_tiles + hg / 32;
   float2 ml[kBatch], ml_o = make_float2(-INFINITY, 0.f);
   float4 a[kBatch], a_o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -676,13 +736,21 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
     a_o = P.acc_o[o * (D / 4) + (quad * 2 + h) * P.own_rows + hg % 32];
   };
   if (part < P.co) load_own(part);
-  if (part < P.cp) load(part, P.cp - 1);
+  if (part < P.cp) load(part, P.cp - 1);  // cp is 0 where the chunks are shared
   const uint32_t plen = P.prefix_len ? P.prefix_len[g] : 0, olen = P.own_len ? P.own_len[m] : 0;
   const bool fits = plen <= P.max_prefix && olen <= P.max_own;
   if (plen && plen <= P.max_prefix) {
-    const uint32_t chunk = chunk_of(plen, P.cp), n = (plen + chunk - 1) / chunk;
+    uint32_t n;
+    if (!P.shared) {
+      const uint32_t chunk = chunk_of(plen, P.cp);
+      n = (plen + chunk - 1) / chunk;
+    } else {
+      const Shares sh = shares_of(P, lane);
+      n = lane_of(sh.n, g);
+      at_p += lane_of(sh.upto - sh.n, g) * step_p;
+    }
     for (uint32_t c = part; c < n; c += W * kBatch) {
-      if (c != part) load(c, n - 1);
+      if (c != part || P.shared) load(c, n - 1);
       float mx = M;
 #pragma unroll
       for (uint32_t j = 0; j < kBatch; j++)
@@ -765,10 +833,6 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   //        32   16000  100    16  24.2 / 21.8  24.1 / 23.8  22.9 / 25.1
   //        24   60000  100    44  53.5 / 43.2  51.9 / 44.7  55.7 / 49.8
   //        32   60000  400    59  64.5 / 54.3  62.2 / 51.1  54.6 / 49.6
-  // Several prompts are seldom of one length, and two shorter chunks per CU even that out (64
-  // dims: 6 x 5 members up to 12000 keys 28.8 -> 24.7 us, of equal lengths 30.6 -> 31.5; 16 x 1
-  // up to 6000 33.7 -> 27.9, equal 44.1 -> 47.1; of 128 dims it takes more than it gives: 6 x 5
-  // up to 12000 53.7 -> 51.2, equal 65.4 -> 71.3).
   auto work_of = [&](size_t rows_of_32, size_t keys) {
     return static_cast<double>(rows_of_32) * static_cast<double>(keys) / (128.0 * static_cast<double>(cus));
   };
@@ -777,12 +841,27 @@ Params plan(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv, size_t D
   if (D == 128) P.rw = work < 10.0 ? 1 : 4 * of_four <= 5 * P.tiles && 4.0 * work_own <= work ? 4 : 8 * of_two <= 9 * P.tiles ? 2 : 1;
   else P.rw = 4 * of_four <= 5 * P.tiles && work >= 24.0 ? 4 : 1;
   const double two_from = D == 64 ? P.rw == 4 ? 0.0 : 7.0 : P.rw == 4 ? 56.0 : P.rw == 2 ? 16.0 : 20.0;
-  const bool uneven = D == 64 && n_groups > 1 && work >= 16.0;
-  const bool two = (((P.rw > 1 || P.tiles >= 3) && work >= two_from) || uneven) && 10.0 * work_own <= work;
-  const size_t prefix = n_groups * n_kv * ((P.tiles + P.rw - 1) / P.rw);
+  const bool two = (P.rw > 1 || P.tiles >= 3) && work >= two_from && 10.0 * work_own <= work;
+  const size_t each = n_kv * ((P.tiles + P.rw - 1) / P.rw), wanted = (two ? 2 : 1) * cus / each;
   const size_t least = P.rw == 1 ? kLeastChunk : 256;
-  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp((two ? 2 : 1) * cus / prefix, 1, div_up(max_prefix, least)));
-  P.n_prefix_wgs = static_cast<uint32_t>(prefix * P.cp);
+  P.cp = max_prefix == 0 ? 0 : static_cast<uint32_t>(clamp(wanted / n_groups, 1, div_up(max_prefix, least)));
+  P.slots = static_cast<uint32_t>(n_groups) * P.cp;
+  // Several prompts are seldom of one length.  Chunks planned from the lengths cost each workgroup
+  // 1 us of looking at all of them, so they need some work.  In us, cp chunks each / shared, of
+  // equal lengths, of any up to the longest, of lengths that fall by a factor:
+  //   6 groups x 5 members, 12000, 64 dims    32.1 / 32.6   28.8 / 25.1   24.0 / 15.4
+  //   6 x 5, 12000, 128 dims                  67.7 / 68.0   54.2 / 49.1   38.6 / 21.9
+  //   16 x 4, 4000, 128 dims                  63.9 / 67.3   46.5 / 45.4   36.2 / 29.4
+  //   32 x 1, 6000, 128 dims                  144 / 147     109 / 104     76.2 / 34.3
+  //   3 x 4, 1100, 128 dims (work 1)          15.4 / 16.0   13.7 / 14.3   11.5 / 13.8
+  //   8 x 8, 4000, 64 dims (work 4)           16.5 / 17.4   15.6 / 16.3   14.7 / 15.7
+  const size_t shared = wanted >= 2 * n_groups ? wanted : 2 * wanted;
+  if (n_groups > 1 && n_groups <= 64 && shared >= 2 * n_groups && work >= kShareFrom && max_prefix < 1u << 27) {
+    P.shared = 1;
+    P.cp = 0;
+    P.slots = static_cast<uint32_t>(shared);
+  }
+  P.n_prefix_wgs = static_cast<uint32_t>(each * P.slots);
   const size_t own = members * n_kv * P.own_tiles;
   P.co = max_own == 0 ? 0 : static_cast<uint32_t>(clamp(cus / own, 1, div_up(max_own, kLeastChunk)));
   return P;
@@ -797,7 +876,7 @@ size_t layout(Params& P, size_t D, void* base) {
     off += al256(bytes);
     return r;
   };
-  const size_t p = static_cast<size_t>(P.n_groups) * P.cp * P.n_kv * P.tiles * 32;
+  const size_t p = static_cast<size_t>(P.slots) * P.n_kv * P.tiles * 32;
   const size_t o = static_cast<size_t>(P.n_groups) * P.n_per * P.co * P.n_kv * P.own_tiles * P.own_rows;
   P.ml_p = reinterpret_cast<float2*>(take(8 * p));
   P.acc_p = reinterpret_cast<float4*>(take(4 * D * p));
