@@ -182,6 +182,24 @@ def test_groups_of_any_length(gpu, heads, kv, d, groups, per, max_prefix):
     c.check([m for m in (0, groups * per - 1) if m // per != groups // 2])
 
 
+@pytest.mark.parametrize("heads, kv, d, groups, per", [(8, 4, 64, 1, 64), (16, 8, 128, 3, 11), (16, 8, 128, 1, 32), (32, 8, 64, 5, 13)])
+def test_own_rows_of_any_length(gpu, heads, kv, d, groups, per):
+    """As many members as are taken by the length of their own rows, and one more: rows of one number, none, one, too many."""
+    print(f"[case] shared own rows {heads} {kv} {d} {groups} {per}", flush=True)
+    r, n, most = np.random.default_rng(per), groups * per, 700
+    c = Case(heads, kv, d, per, [70] * groups, [most] * n).upload()
+    far = np.zeros(n, int)
+    far[n // 3] = most
+    for own in (np.full(n, 129), np.zeros(n, int), np.ones(n, int), far, r.integers(0, most + 1, n), np.arange(n) * most // n,
+                np.arange(n)[::-1] * most // n, np.where(np.arange(n) == n - 1, most + 1, 33)):
+        c.own = [int(v) for v in own]
+        c.lens[1].upload(u32(c.own))
+        c.call()
+        if max(c.own) > most:
+            assert np.isnan(c.out()[-1]).all()
+        c.check([m for m in (0, 1, n // 3, n // 2, n - 2, n - 1) if c.own[m] <= most])
+
+
 def test_prefix_or_own_rows_alone(gpu):
     for d in (64, 128):
         c = Case(8, 2, d, 3, [200], [0, 0, 0]).upload()
