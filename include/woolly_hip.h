@@ -695,10 +695,10 @@ WH_API int wh_attention_shared(const float* q, size_t ldq, const uint32_t* prefi
  * of equal ones the lowest beam's, then (in the order of the logits, where the
  * sums do not tell them apart) the lowest token.  A beam whose last token is
  * end_token has ended: its one continuation is itself (token end_token, score
- * and count as they are), and its logits are not read.  A beam whose score is -inf or NaN is not
- * there (a search begins with one beam at 0, the others at -inf); logits of -inf
- * or NaN are not allowed, and a row with +inf has no continuation.  Sums and
- * comparisons are made in 64 bits. */
+ * and count as they are), and its logits are not read.  A beam whose score is
+ * infinite or NaN is not there (a search begins with one beam at 0, the others at
+ * -inf); logits of -inf or NaN are not allowed, and a row with +inf has no
+ * continuation.  Sums and comparisons are made in 64 bits. */
 #define WH_MAX_BEAMS 32
 typedef struct wh_beam_rules {
   size_t n_beams;               /* at most WH_MAX_BEAMS */
@@ -749,13 +749,14 @@ WH_API int wh_beam_reorder(void* const* states, size_t n_states, size_t n_seqs, 
  * null) the head's rows.  Member m's token is its own token len[m] - 1, at
  * position *prefix_len + len[m] - 1; its k and v go to that row of k_own[layer]
  * and v_own[layer], host arrays of n_layers device pointers, [n_members][max_own]
- * [n_kv_heads][head_dim] f16 each.  The model's caches are only read.  rules may be null: the model's
- * rope_inv_freq, half layout, no norms.  tokens, prefix_len (one number) and len
- * [n_members] are device memory, x is 16-byte aligned, the model has a token_embd
- * table; a member whose rows do not fit has NaN.  The workspace (256-byte
- * aligned) holds wh_llama_forward_members_workspace_bytes(..), 0 for a model or
- * number that is not taken; calls that overlap on one workspace race.  Launches
- * only, as the decode step. */
+ * [n_kv_heads][head_dim] f16 each.  The model's caches are only read.  rules may
+ * be null: the model's rope_inv_freq, half layout, no norms.  tokens, prefix_len
+ * (one number) and len [n_members] are device memory, x is 16-byte aligned, the
+ * model has a token_embd table.  A member whose rows do not fit has NaN; one with
+ * len 0 is not there: nothing of it is stored and its rows mean nothing.  The
+ * workspace (256-byte aligned) holds wh_llama_forward_members_workspace_bytes(..),
+ * 0 for a model or number that is not taken; calls that overlap on one workspace
+ * race.  Launches only, as the decode step. */
 WH_API size_t wh_llama_forward_members_workspace_bytes(const wh_llama_model* model, size_t n_members, size_t max_own);
 WH_API int wh_llama_forward_members(const wh_llama_model* model, const wh_rope_rules* rules, const uint32_t* tokens,
                                     size_t n_members, const uint32_t* prefix_len, const uint32_t* len,

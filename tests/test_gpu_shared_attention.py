@@ -305,3 +305,40 @@ def test_graph_follows_the_lengths(gpu):
     first = c.out()
     c.call()
     assert np.array_equal(first, c.out()), "the same call twice, the same bits"
+
+
+def test_captured_groups_of_other_lengths(gpu):
+    """Chunks and the members' order follow the lengths of each replay."""
+    c = Case(16, 4, 64, 13, [9000] * 5, [90] * 65, max_prefix=9000, max_own=90).upload()  # the groups share chunks
+    d = Case(16, 8, 128, 16, [500] * 3, [300] * 48).upload()                             # longest own rows first
+    s = Stream()
+    with Graph.capture(s) as g:
+        c.call(s)
+        d.call(s)
+    r = np.random.default_rng(3)
+    for prefix in ([9000, 1, 700, 0, 130], [0] * 5, [9000] * 5):
+        for case, most in ((c, 90), (d, 300)):
+            case.prefix = [min(v, case.max_prefix) for v in prefix[:case.groups]]
+            case.own = [int(v) for v in r.integers(0, most + 1, case.n)]
+            case.lens[0].upload(u32(case.prefix))
+            case.lens[1].upload(u32(case.own))
+        g.launch(s)
+        s.synchronize()
+        c.check([0, 14, 27, 51, 64])
+        d.check([0, 15, 16, 47])
+        first = c.out(), d.out()
+        c.call()
+        d.call()
+        assert np.array_equal(first[0], c.out()) and np.array_equal(first[1], d.out())
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that overlap, each with its own workspace."""
+    cases = [Case(16, 4, 128, 9, [4000, 50], [700] * 18, seed=i).upload() for i in range(2)]
+    streams = [Stream(), Stream()]
+    for _ in range(20):
+        for c, s in zip(cases, streams):
+            c.call(s)
+    for c, s in zip(cases, streams):
+        s.synchronize()
+        c.check([0, 8, 17])
