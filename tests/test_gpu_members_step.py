@@ -113,6 +113,24 @@ def test_members_logits_are_the_paths_logits(gpu, orc, name):
             assert rel_l2(got[i], want) <= 1e-4, (step, i, rel_l2(got[i], want))
 
 
+def test_step_without_logits(gpu):
+    """The hidden states are the same, the logits not touched; a member with no token of its own stores nothing."""
+    m = Model(*MODELS["q4_0"], layers=2, vocab=300, ctx=32, seed=4)
+    prompt_into(m, [1, 2, 3])
+    out = []
+    for with_logits in (True, False):
+        bufs, own = own_caches(m, 3, 4)
+        wsz = m.tree.members_workspace_bytes(3, 4)
+        x, lg, ws = DeviceBuffer(4 * 3 * m.hidden), DeviceBuffer(4 * 3 * m.vocab), DeviceBuffer(wsz)
+        lg.fill(0xEE)
+        m.tree.forward_members(up(u32([5, 6, 7]))[0], 3, up(u32([3]))[0], up(u32([1, 0, 1]))[0], own, 4, x, lg if with_logits else None, ws, wsz)
+        out.append(down(x, np.float32, 3 * m.hidden).reshape(3, -1))
+        assert with_logits or (down(lg, np.uint8, 4 * 3 * m.vocab) == 0xEE).all()
+        rows = [down(b, np.uint16, 3 * 4 * m.kv * m.d).reshape(3, 4, -1) for b in bufs[0] + bufs[1]]
+        assert all((r[1] == 0xFFFF).all() and (r[[0, 2], 1:] == 0xFFFF).all() and (r[[0, 2], 0] != 0xFFFF).all() for r in rows)
+    assert np.array_equal(out[0][[0, 2]], out[1][[0, 2]])
+
+
 def test_rules_of_the_model(gpu):
     """The model's own rotation given as rules is the default, bit for bit; others are not."""
     m = Model(*MODELS["q4_0"], layers=2, vocab=400, ctx=32, seed=8)

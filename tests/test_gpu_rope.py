@@ -159,3 +159,32 @@ def test_norms_of_tiny_heads(gpu):
         for got, want, bar in ((q, want_q[0], 2.0 ** -19), (k, want_k[0], 2.0 ** -23)):
             assert np.array_equal(np.isnan(got), np.isnan(want)), eps
             assert (np.abs(got - want) <= bar * np.abs(want))[~np.isnan(want)].all(), eps
+
+
+def test_outputs_that_are_not_wanted(gpu):
+    """Each output by itself is what it is beside the others."""
+    heads, kv, d, n, room = 6, 2, 96, 5, 4
+    width = (heads + 2 * kv) * d
+    x = np.random.default_rng(0).standard_normal((n, width)).astype(np.float32)
+    xb, inv = up(x)[0], up(np.linspace(0.1, 0.9, d // 2).astype(np.float32))[0]
+    base, lens = up(u32([7]))[0], up(u32([1, 4, 2, 5, 0]))[0]  # one that does not fit, one that is absent
+    sizes = (4 * n * heads * d, 4 * n * kv * d, 2 * n * room * kv * d, 2 * n * room * kv * d)
+
+    def call(q, k, cache):
+        bufs = [DeviceBuffer(s) for s in sizes]
+        for b in bufs:
+            b.fill(0xEE)
+        ops.qk_norm_rope(ops.RopeRules(inv), xb, xb.ptr + 4 * heads * d, xb.ptr + 4 * (heads + kv) * d, width, width, base, lens, 1, n, 1,
+                         heads, kv, d, bufs[0] if q else None, heads * d, bufs[1] if k else None, kv * d, bufs[2] if cache else None,
+                         bufs[3] if cache else None, room if cache else 0)
+        return [down(b, np.uint8, s) for b, s in zip(bufs, sizes)]
+
+    every, without = call(True, True, True), call(True, True, False)
+    untouched = [np.full(s, 0xEE, np.uint8) for s in sizes]
+    for want in (dict(q=True, k=False, cache=True), dict(q=False, k=True, cache=True), dict(q=False, k=False, cache=True),
+                 dict(q=True, k=False, cache=False), dict(q=False, k=True, cache=False), dict(q=False, k=False, cache=False)):
+        got = call(**want)
+        have = (want["q"], want["k"], want["cache"], want["cache"])
+        full = every if want["cache"] else without
+        for g, f, u, h in zip(got, full, untouched, have):
+            assert np.array_equal(g, f if h else u), want
