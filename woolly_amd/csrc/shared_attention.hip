@@ -17,11 +17,15 @@
 // has them: S^T = K Q^T leaves a lane with 16 keys of one query row, in the order
 // in which the registers are the B operand of O^T = V^T P^T.  q, scaled by a power
 // of two, and the weights are split into two f16 limbs each, K and V are taken as
-// they are.  A weight is 2^12 e^{s - m} (m the running maximum, or up to 2^3 below
-// it), its low limb held times 2^11 and summed apart in each tile, so a weight
-// keeps 2^-22 of itself down to 2^-29 of the largest one, and 2^-51 of that below: what
-// a key with nearly all the weight (often the first one, whose v is small) leaves
-// to the others is as exact as in f32.
+// they are.  A weight is 2^12 e^{s - m}, m a reference that follows the tiles' largest
+// scores up and down, its low limb held times 2^11 and summed apart in each tile: it
+// keeps 2^-22 of itself down to 2^-26 of the reference's, and 2^-48 of that below.
+// Beside one key with nearly all the weight (often the first one, whose v is small) the
+// others make the output, and keep what f32 would leave them: m moves down to them, and
+// that key's own tile takes two turns.  Relative L2 with 90 to 99.9999999 % on one key of
+// 60000: 2e-7 to 4e-6 (with m the running maximum alone up to 2e-2).  That costs the calls
+// 0 to 3 %: 48 members at 131000 253 -> 254 us, 64 at 20000 63.3 -> 63.0, 32 at 60000 of 64 dims
+// 48.7 -> 49.3, 8 at 30000 33.6 -> 33.8.
 //
 // Few query rows: a wave has its own tiles of 32 keys, its own LDS and no barriers
 // until the chunk's end; memory bounds it (8 members at 30000 + 250 rows, 131 MB,
@@ -43,7 +47,14 @@ using whd::read_tr, whd::swap_max, whd::swap_max_nan, whd::swap_sum, whd::swz_k,
 
 constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f;
+// Weights are held in f16 as 2^12 e^{s - m}.  The reference m of a row moves to a tile's largest
+// score where that is above 2^3 (at most 2^15 in f16), and down to it, but never 2^48 below its
+// highest, where keys are faint: a row's keys in a tile are four groups, by their parity and by the
+// lane that holds them, and a group is faint whose largest weight is below 2^-26 of the reference's
+// (2^-14 in f16, below which the low limb is off by more than 2^-22 of it).  Where it is so against
+// the tile's largest too, the tile takes two turns: the keys down to 2^-9 of that one, then the others.
+constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f, kLowest = 48.0f;
+constexpr float kFaint = -26.0f, kNear = 9.0f;
 constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
 constexpr uint32_t kLeastChunk = 128;  // keys: a tile for every wave
 constexpr double kShareFrom = 10.0;    // work (plan)
@@ -180,6 +191,7 @@ struct Rows {
   int e;     // q is scaled by 2^e
   f32x16 acc[D / 32];
   float m, l;
+  float floor;  // m goes no lower
 };
 
 // q rows: lane l has row l % 32, elements 16 j + 8 (l / 32) .. of each step j.
@@ -216,74 +228,110 @@ __device__ __forceinline__ void load_rows(Rows<D>& w, const float* q, float scal
   for (int d = 0; d < D / 32; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) w.acc[d][i] = 0.f;
-  w.m = -INFINITY;
+  w.m = w.floor = -INFINITY;
   w.l = 0.f;
 }
 
-// Scores of the 32 keys of the K tile at kt (LDS), key 8 (i / 4) + 4 h + i % 4 in s[i].
+// The operands of the 32 keys of the K tile at kt (LDS), 16 elements of their rows to a step.
 template <int D>
-__device__ __forceinline__ void scores(const Rows<D>& w, uint32_t kt, int l32, int h, f32x16& s) {
+struct Keys {
+  uint32_t at;
+  __device__ __forceinline__ Keys(uint32_t kt, int l32, int h) : at(kt + l32 * 2 * D + 16 * (h ^ swz_k<D>(l32))) {
+    asm("" : "+v"(at));  // the steps' addresses are made of it each time: they would take registers across the loop
+  }
+  __device__ __forceinline__ half8 step(int j) const {
+    return *reinterpret_cast<const __attribute__((address_space(3))) half8*>((uintptr_t)(at ^ (32 * j)));
+  }
+};
+
+// Scores of the keys, key 8 (i / 4) + 4 h + i % 4 in s[i].
+template <int D>
+__device__ __forceinline__ void scores(const Rows<D>& w, const Keys<D>& keys, f32x16& s) {
   constexpr int KS = D / 16;
-  uint32_t ko = kt + l32 * 2 * D + 16 * (h ^ swz_k<D>(l32));
-  asm("" : "+v"(ko));  // the steps' addresses are made of it each time: they would take registers across the loop
-  auto k_at = [&](int j) {
-    return *reinterpret_cast<const __attribute__((address_space(3))) half8*>((uintptr_t)(ko ^ (32 * j)));
-  };
 #pragma unroll
   for (int i = 0; i < 16; i++) s[i] = 0.f;
   half8 k[2];
-  k[0] = k_at(0);
+  k[0] = keys.step(0);
 #pragma unroll
   for (int j = 0; j < KS; j++) {
-    if (j + 1 < KS) k[(j + 1) & 1] = k_at(j + 1);
+    if (j + 1 < KS) k[(j + 1) & 1] = keys.step(j + 1);
     __builtin_amdgcn_sched_barrier(kNoLds);
     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j & 1], w.qh[j], s, 0, 0, 0);
     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j & 1], w.ql[j], s, 0, 0, 0);
   }
-  float bad = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; i++) bad = __builtin_elementwise_maximum(bad, s[i]);
-  if (__builtin_expect(__ballot(bad != bad) != 0, 0)) {
-    // A score is NaN: the formula's, or made of an infinity in K that q's limbs meet with both
-    // signs or as 0.  q's sign and size are the hi limb's: its product alone says what an
-    // infinity makes of the score.
-    f32x16 x;
-#pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = 0.f;
-#pragma unroll 1
-    for (int j = 0; j < KS; j++) {
-      half8 q = w.qh[0];
-#pragma unroll
-      for (int u = 1; u < KS; u++) q = j == u ? w.qh[u] : q;
-      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(j), q, x, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (s[i] != s[i]) s[i] = x[i];
-  }
 }
 
-// The weights of the scores of N tiles (as hi and lo limbs), with the sums so far brought
-// to the row's reference.
+// A score that is NaN: the formula's, or made of an infinity in K that q's limbs meet with
+// both signs or as 0.  q's sign and size are the hi limb's: its product alone says what an
+// infinity makes of the score.
+template <int D>
+__device__ __forceinline__ void mend_scores(const Rows<D>& w, const Keys<D>& keys, f32x16& s) {
+  constexpr int KS = D / 16;
+  f32x16 x;
+#pragma unroll
+  for (int i = 0; i < 16; i++) x[i] = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < KS; j++) {
+    half8 q = w.qh[0];
+#pragma unroll
+    for (int u = 1; u < KS; u++) q = j == u ? w.qh[u] : q;
+    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys.step(j), q, x, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    if (s[i] != s[i]) s[i] = x[i];
+}
+
+// Brings the row's reference, and with it the sums so far, to the scores of N tiles.  Returns
+// whether the tiles need a second turn, for the keys that it has left out of this one.
+// mend: mend_scores of the tiles.
+template <int D, int N, bool SECOND, typename Mend>
+__device__ __forceinline__ bool settle(Rows<D>& w, f32x16 (&s)[N], std::bool_constant<SECOND>, const Mend& mend) {
+  float top[2], mt;  // the largest score of the lane's groups of keys, and of the row
+  auto tops = [&](auto larger) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 16 * N; i++) top[i & 1] = i < 2 ? s[0][i] : larger(top[i & 1], s[i / 16][i % 16]);
+    mt = larger(top[0], top[1]);
+  };
+  auto largest = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };  // NaN if there is one
+  tops(largest);
+  mt = swap_max_nan(mt);
+  // NaN goes on
+  if (!SECOND && __ballot(!((mt - w.m) * w.qs <= kMoveUp) || (fminf(top[0], top[1]) - w.m) * w.qs < kFaint) == 0) return false;
+  if (__builtin_expect(__ballot(mt != mt) != 0, 0)) {
+    mend();
+    tops(largest);
+    mt = swap_max_nan(mt);  // NaN still: the row is NaN
+  }
+  bool again = false;
+#pragma unroll
+  for (int i = 0; i < 2; i++) top[i] = top[i] == -INFINITY ? INFINITY : top[i];  // keys of weight 0 are not faint
+  const float low = -swap_max(-fminf(top[0], top[1]));
+  if (SECOND || __builtin_expect(__ballot((low - mt) * w.qs < kFaint) != 0, 0)) {
+    const float split = mt - kNear * __builtin_amdgcn_rcpf(w.qs);
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[n][i] = (s[n][i] < split) != SECOND ? -INFINITY : s[n][i];
+    tops([](float a, float b) { return fmaxf(a, b); });
+    mt = swap_max(mt);
+    again = !SECOND;
+  }
+  const float to = __builtin_elementwise_maximum(mt, w.floor), by = (to - w.m) * w.qs;
+  const bool moves = mt != -INFINITY && (!(by <= kMoveUp) || (by < -kMoveUp && (low - w.m) * w.qs < kFaint));
+  const float al = moves ? __builtin_amdgcn_exp2f(-by) : 1.f;
+  w.l *= al;
+#pragma unroll
+  for (int d = 0; d < D / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) w.acc[d][i] *= al;
+  if (moves) w.m = to, w.floor = fmaxf(w.floor, to - kLowest * __builtin_amdgcn_rcpf(w.qs));
+  return again;
+}
+
+// The weights of the scores of N tiles, as hi and lo limbs.
 template <int D, int N>
 __device__ __forceinline__ void weigh(Rows<D>& w, const f32x16 (&s)[N], half8 (&ph)[2 * N], half8 (&pl)[2 * N]) {
-  float mt = -INFINITY;
-#pragma unroll
-  for (int n = 0; n < N; n++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) mt = __builtin_elementwise_maximum(mt, s[n][i]);
-  mt = swap_max_nan(mt);
-  const float by = (mt - w.m) * w.qs;
-  const bool moves = !(by <= kMoveUp) && mt != -INFINITY;  // NaN moves: the row is NaN
-  if (__ballot(moves)) {
-    const float al = moves ? __builtin_amdgcn_exp2f(-by) : 1.f;
-    w.l *= al;
-#pragma unroll
-    for (int d = 0; d < D / 32; d++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) w.acc[d][i] *= al;
-    if (moves) w.m = mt;
-  }
   const float mb = w.m == -INFINITY ? 0.f : w.m;
   float lt[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -517,15 +565,21 @@ __device__ __forceinline__ void few_rows(const Params& P, const Work& W, unsigne
     while (true) {
       const uint32_t next = base + 32 * kWaves, left = W.c1 - base;
       const bool more = next < W.c1;
-      f32x16 s[1];
-      scores(w, kt, l32, h, s[0]);  // asks what they are: the tile has been read
-      if (more) copy_tile(W.k, next, kt, ck, true);
-      if (left < 32) mask_scores(s[0], left, h);
-      half8 ph[2], pl[2];
-      weigh<D, 1>(w, s, ph, pl);
-      if (more) wait_vmcnt<S::kCopies>(); else wait_vmcnt<0>();  // V, not the next K
-      if (left < 32) clear_values<D>(vt, left, lane);
-      add_values<D, 1>(w, vt, ph, pl, lane);
+      auto turn = [&](auto second) __attribute__((always_inline)) {
+        f32x16 s[1];
+        const Keys<D> keys(kt, l32, h);
+        scores(w, keys, s[0]);
+        if (left < 32) mask_scores(s[0], left, h);
+        const bool again = settle(w, s, second, [&] { mend_scores(w, keys, s[0]); });  // asks what they are: the tile has been read
+        if (more && !again) copy_tile(W.k, next, kt, ck, true);
+        half8 ph[2], pl[2];
+        weigh<D, 1>(w, s, ph, pl);
+        if (more && !again) wait_vmcnt<S::kCopies>(); else wait_vmcnt<0>();  // V, not the next K
+        if (left < 32) clear_values<D>(vt, left, lane);
+        add_values<D, 1>(w, vt, ph, pl, lane);
+        return again;
+      };
+      if (__builtin_expect(turn(std::false_type{}), 0)) turn(std::true_type{});
       if (!more) break;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       copy_tile(W.v, next, vt, cv, false);
@@ -594,19 +648,27 @@ __device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsign
     if (base + kStageKeys < W.c1) issue(base + kStageKeys, buf ^ 1);
     const uint32_t kt = lds0 + buf * 4 * S::kTile + first * S::kTile, vt = kt + 2 * S::kTile;
     const int left = W.c1 - base - 32 * first;
-    f32x16 s[kTiles];
+    auto turn = [&](auto second) __attribute__((always_inline)) {
+      f32x16 s[kTiles];
 #pragma unroll
-    for (int n = 0; n < kTiles; n++) scores(w, kt + n * S::kTile, l32, h, s[n]);
-    if (left < 32 * kTiles) {
+      for (int n = 0; n < kTiles; n++) scores(w, Keys<D>(kt + n * S::kTile, l32, h), s[n]);
+      if (left < 32 * kTiles) {
 #pragma unroll
-      for (int n = 0; n < kTiles; n++) {
-        mask_scores(s[n], left - 32 * n, h);
-        clear_values<D>(vt + n * S::kTile, left - 32 * n, lane);  // the waves store the same, each before it reads the rows
+        for (int n = 0; n < kTiles; n++) {
+          mask_scores(s[n], left - 32 * n, h);
+          clear_values<D>(vt + n * S::kTile, left - 32 * n, lane);  // the waves store the same, each before it reads the rows
+        }
       }
-    }
-    half8 ph[2 * kTiles], pl[2 * kTiles];
-    weigh<D, kTiles>(w, s, ph, pl);
-    add_values<D, kTiles>(w, vt, ph, pl, lane);
+      const bool again = settle(w, s, second, [&] {
+#pragma unroll
+        for (int n = 0; n < kTiles; n++) mend_scores(w, Keys<D>(kt + n * S::kTile, l32, h), s[n]);
+      });
+      half8 ph[2 * kTiles], pl[2 * kTiles];
+      weigh<D, kTiles>(w, s, ph, pl);
+      add_values<D, kTiles>(w, vt, ph, pl, lane);
+      return again;
+    };
+    if (__builtin_expect(turn(std::false_type{}), 0)) turn(std::true_type{});
   }
   mend_values(w, W.v, RS, W.c0, W.c1, first, kTiles == 1 ? 2 : 1, lane);
   w.l = swap_sum(w.l);
