@@ -403,12 +403,13 @@ __device__ __forceinline__ void clear_values(uint32_t vt, int left, int lane) {
       *reinterpret_cast<__attribute__((address_space(3))) u32x4*>((uintptr_t)(vt + 1024 * j + 16 * lane)) = u32x4{0, 0, 0, 0};
 }
 
-// Infinities and NaN of V: limbs and a weight's 0 make NaN of them.  Every weight
-// is above 0, so such an element's sum is that of the infinities and NaN alone:
-// the rows are read again for them.  Keys c0 + 32 first .. in steps of `step` tiles.
+// Infinities and NaN of V: limbs and a weight's 0 make NaN of them.  A weight is above 0,
+// however small, but for a score of -inf, so such an element's sum is that of the infinities
+// and NaN alone, or NaN (0 times infinity): the rows are read again for them.  Keys
+// c0 + 32 first .. in steps of `step` tiles.
 template <int D>
-__device__ __forceinline__ void mend_values(Rows<D>& w, const uint8_t* vbase, size_t RS, uint32_t c0, uint32_t c1, uint32_t first,
-                                            uint32_t step, int lane) {
+__device__ __forceinline__ void mend_values(Rows<D>& w, const uint8_t* kbase, const uint8_t* vbase, size_t RS, uint32_t c0, uint32_t c1,
+                                            uint32_t first, uint32_t step, int lane) {
   float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int d = 0; d < D / 32; d++)
@@ -435,13 +436,23 @@ __device__ __forceinline__ void mend_values(Rows<D>& w, const uint8_t* vbase, si
       const uint32_t key = base + __builtin_ctzll(rows_bad) / 2;
       rows_bad &= rows_bad - 1;
       if (key >= c1) break;  // the last row, looked at again
-      const _Float16* v = reinterpret_cast<const _Float16*>(vbase + key * RS);
+      const _Float16 *k = reinterpret_cast<const _Float16*>(kbase + key * RS), *v = reinterpret_cast<const _Float16*>(vbase + key * RS);
+      float score = 0.f;  // -inf as mend_scores has it
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) {
+        u32x4 q = __builtin_bit_cast(u32x4, w.qh[j]);
+        asm volatile("" : "+v"(q)::"memory");  // a step at a time: this is rare, and short of registers
+        const half8 a = *reinterpret_cast<const half8*>(k + 16 * j + 8 * h), b = __builtin_bit_cast(half8, q);
+#pragma unroll
+        for (int u = 0; u < 8; u++) score = __builtin_fmaf(static_cast<float>(a[u]), static_cast<float>(b[u]), score);
+      }
+      const bool none = swap_sum(score) == -INFINITY;
 #pragma unroll
       for (int d = 0; d < D / 32; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const float x = static_cast<float>(v[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
-          if (!(fabsf(x) < INFINITY)) w.acc[d][i] += x;
+          if (!(fabsf(x) < INFINITY)) w.acc[d][i] += none ? __builtin_nanf("") : x;
         }
     }
   }
@@ -464,6 +475,9 @@ __device__ __forceinline__ void load_rows_of(Rows<D>& w, const Params& P, const 
   const uint32_t r = min(r0, W.n_rows - 1);
   load_rows(w, P.q + (W.member0 + r / P.G) * P.ldq + static_cast<size_t>(W.kvh * P.G + r % P.G) * D, P.scale, h);
 }
+
+// The factor that brings sums to a reference `by` powers of two higher.  Not 0: an infinity stays one.
+__device__ __forceinline__ float factor_of(float by) { return __builtin_elementwise_maximum(__builtin_amdgcn_exp2f(by), 0x1p-126f); }
 
 // Waves whose query rows are the same and that have taken keys apart, N of them with
 // kWaves / N tiles, join in LDS, in fixed order, and store in the lanes' order.
@@ -492,7 +506,7 @@ __device__ __forceinline__ void join_waves(const Rows<D>& w, const Work& W, unsi
   }
 #pragma unroll
   for (int u = 0; u < N; u++) {
-    ew[u] = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[u].x - M) * w.qs);
+    ew[u] = ml[u].x == -INFINITY ? 0.f : factor_of((ml[u].x - M) * w.qs);
     L = __builtin_fmaf(ml[u].y, ew[u], L);
   }
   if (W.row0 + 32 * tile + l32 >= W.n_rows) return;
@@ -586,7 +600,7 @@ __device__ __forceinline__ void few_rows(const Params& P, const Work& W, unsigne
       wait_vmcnt<S::kCopies>();  // the next K
       base = next;
     }
-    mend_values(w, W.v, RS, W.c0, W.c1, wave, kWaves, lane);
+    mend_values(w, W.k, W.v, RS, W.c0, W.c1, wave, kWaves, lane);
   }
   w.l = swap_sum(w.l);
 
@@ -670,7 +684,7 @@ __device__ __forceinline__ void many_rows(const Params& P, const Work& W, unsign
     };
     if (__builtin_expect(turn(std::false_type{}), 0)) turn(std::true_type{});
   }
-  mend_values(w, W.v, RS, W.c0, W.c1, first, kTiles == 1 ? 2 : 1, lane);
+  mend_values(w, W.k, W.v, RS, W.c0, W.c1, first, kTiles == 1 ? 2 : 1, lane);
   w.l = swap_sum(w.l);
   if constexpr (kTiles == 1) {
     join_waves<D, 2>(w, W, lds, wave, lane);
@@ -781,8 +795,8 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
   float M = -INFINITY, L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
   auto join = [&](float2 ml, float4 a) {
-    // a part without a reference has no weight, but NaN of its scores stay
-    const float ew = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - M) * P.scale);
+    // a part without a reference has no weight, but its NaN stay
+    const float ew = ml.x == -INFINITY ? 0.f : factor_of((ml.x - M) * P.scale);
     L = __builtin_fmaf(ml.y, ew, L);
     A.x = __builtin_fmaf(a.x, ew, A.x);
     A.y = __builtin_fmaf(a.y, ew, A.y);
@@ -790,7 +804,7 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const Params P, uin
     A.w = __builtin_fmaf(a.w, ew, A.w);
   };
   auto raise = [&](float to) {
-    const float keep = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - to) * P.scale);
+    const float keep = M == -INFINITY ? 0.f : factor_of((M - to) * P.scale);
     M = to;
     if (keep != 1.f) L *= keep, A.x *= keep, A.y *= keep, A.z *= keep, A.w *= keep;
   };
