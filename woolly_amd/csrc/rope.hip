@@ -12,7 +12,8 @@
 // point is kept: in 32 bits p * inv_freq would be off by p 2^-24 radians.  Its
 // sine and cosine are of that part, in 64 bits; k is normed and turned in 64 bits
 // and rounded to f32, then to f16, so a cache row is what the formula gives (and
-// what wh_attention_tree stores), q in 32.
+// what wh_attention_tree stores), q in 32 (its norm in 64 where the mean square is
+// no normal f32 number).
 //
 // Many rows are bound by memory: 4000 of 32 / 8 heads of 128, 180 MB read and
 // written, 35.5 us, normed 41 (5.1 and 4.4 TB/s); few by the launch and two loads
@@ -140,6 +141,17 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const Params P) {
     const uint32_t h = h0 + n * (64 / L);
     const bool is_q = h < P.n_heads;
     double kx[PP], ky[PP];  // of a key head
+    auto root64 = [&]() __attribute__((always_inline)) {  // 1 / sqrt(mean square + eps)
+      double sum = 0.0;
+#pragma unroll
+      for (int u = 0; u < PP; u++) {
+        const double dx = in[u] ? x[n][u] : 0.f, dy = in[u] ? y[n][u] : 0.f;
+        sum = __builtin_fma(dx, dx, __builtin_fma(dy, dy, sum));
+      }
+      const double mean = __builtin_fma(whd::lanes_sum_f64<L>(sum), P.per_d, static_cast<double>(P.eps));
+      const double r = __builtin_amdgcn_rsq(mean);  // to 2^-22 or so, and Newton's step
+      return mean < INFINITY ? r * __builtin_fma(-0.5 * mean * r, r, 1.5) : r;
+    };
     if (is_q) {
       if (P.q_norm) {
         float sum = 0.f;
@@ -147,24 +159,20 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const Params P) {
         for (int u = 0; u < PP; u++)
           if (in[u]) sum = __builtin_fmaf(x[n][u], x[n][u], __builtin_fmaf(y[n][u], y[n][u], sum));
         const float mean = __builtin_fmaf(lanes_sum<L>(sum), static_cast<float>(P.per_d), P.eps);
-        float r = __builtin_amdgcn_rsqf(mean);         // off by a unit of f32 at most
-        if (mean < 0x1p-126f) r = 1.0f / sqrtf(mean);  // which it flushes
+        const bool apart = !(mean >= 0x1p-126f && mean < INFINITY);  // not f32's: values beyond 2^-63 .. 2^63
+        if (__builtin_expect(__ballot(apart) == 0, 1)) {
+          const float r = __builtin_amdgcn_rsqf(mean);  // off by a unit of f32 at most
 #pragma unroll
-        for (int u = 0; u < PP; u++) x[n][u] = x[n][u] * r * qw[u][0], y[n][u] = y[n][u] * r * qw[u][1];
+          for (int u = 0; u < PP; u++) x[n][u] = x[n][u] * r * qw[u][0], y[n][u] = y[n][u] * r * qw[u][1];
+        } else {
+          const double r = root64();
+#pragma unroll
+          for (int u = 0; u < PP; u++)
+            x[n][u] = static_cast<float>(x[n][u] * r * qw[u][0]), y[n][u] = static_cast<float>(y[n][u] * r * qw[u][1]);
+        }
       }
     } else {
-      double r = 1.0;
-      if (P.k_norm) {
-        double sum = 0.0;
-#pragma unroll
-        for (int u = 0; u < PP; u++) {
-          const double dx = in[u] ? x[n][u] : 0.f, dy = in[u] ? y[n][u] : 0.f;
-          sum = __builtin_fma(dx, dx, __builtin_fma(dy, dy, sum));
-        }
-        const double mean = __builtin_fma(whd::lanes_sum_f64<L>(sum), P.per_d, static_cast<double>(P.eps));
-        r = __builtin_amdgcn_rsq(mean);                                             // to 2^-22 or so, and Newton's step
-        if (mean < INFINITY) r *= __builtin_fma(-0.5 * mean * r, r, 1.5);
-      }
+      const double r = P.k_norm ? root64() : 1.0;
 #pragma unroll
       for (int u = 0; u < PP; u++) {
         const double nx = x[n][u] * r * kw[u][0], ny = y[n][u] * r * kw[u][1];
