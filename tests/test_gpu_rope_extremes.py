@@ -51,3 +51,21 @@ def test_infinities_and_nan_of_a_normed_head(gpu):
         assert np.isnan(got[i]) and not np.delete(got, pair(i)).any()
     assert np.isnan(q[1]).all()
     assert (np.abs(q[2] - 1) <= 2.0 ** -20).all()
+
+
+def test_more_rows_than_a_launch_dimension_takes(gpu):
+    """2^26 rows and some of two heads of two elements: 64 threads to a row are more than 2^32 in all."""
+    rows, period = (1 << 26) + 37, 4099
+    r = np.random.default_rng(0)
+    pattern = r.standard_normal((period, 6)).astype(np.float32)
+    x = DeviceBuffer.from_array(np.tile(pattern, (-(-rows // period), 1))[:rows])
+    inv = np.array([0.37], np.float32)
+    out = DeviceBuffer(8 * rows)
+    out.fill(0xEE)
+    print(f"[case] rope of {rows} rows", flush=True)
+    ops.qk_norm_rope(ops.RopeRules(up(inv)[0]), x, x.ptr + 8, x.ptr + 16, 6, 6, None, None, 1, 1, rows, 1, 1, 2, out, 2, None, 0, None, None, 0)
+    got = down(out, np.float32, 2 * rows).reshape(rows, 1, 2)
+    some = np.unique(np.concatenate([np.arange(0, rows, 997), np.arange(300), np.arange(rows - 300, rows), (1 << 24) + np.arange(-300, 300)]))
+    want, bound = _members.rope(pattern[some % period, None, :2], some, inv, 2, False)
+    assert (np.abs(got[some] - want) <= bound).all()
+    assert not (got.view(np.uint32) == 0xEEEEEEEE).any()

@@ -26,6 +26,7 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr size_t kGridWidth = 1 << 22;  // a launch has fewer than 2^32 threads in a dimension
 constexpr size_t kManyHeads = 8192;  // heads of all rows from which on a wave takes more turns
 struct Params {
   const float *q, *k, *v;
@@ -70,13 +71,13 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // A wave takes N turns of 64 / L heads of one row, the query heads first, then
 // the key heads with their values.  A lane has PP pairs of its head: pair
 // l + L u, turned ones first, then (in two halves) the rest of the head.
-// grid: rows * groups of heads.
+// grid: rows * groups of heads, in rows of kGridWidth workgroups.
 template <int L, int PP, int N>
 __global__ __launch_bounds__(kThreads) void rope_kernel(const Params P) {
   constexpr uint32_t kHeads = 64 / L * N;
   const uint32_t lane = threadIdx.x & 63, l = lane % L;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t item = blockIdx.x * (kThreads / 64) + wave;
+  const uint32_t item = (blockIdx.y * gridDim.x + blockIdx.x) * (kThreads / 64) + wave;
   const uint32_t row = item / P.groups, group = item % P.groups;  // row: member * n_new + token
   const uint32_t n_slots = P.n_heads + P.n_kv;
   const uint32_t h0 = group * kHeads + (L == 32 ? lane / 32 : 0);
@@ -227,7 +228,8 @@ int launch(const Params& P, hipStream_t s) {
   const uint32_t per = 64 / L * (many ? 4 : 2);
   A.groups = (slots + per - 1) / per;
   const size_t items = static_cast<size_t>(P.rows) * A.groups;
-  const unsigned grid = static_cast<unsigned>((items + kThreads / 64 - 1) / (kThreads / 64));
+  const size_t workgroups = (items + kThreads / 64 - 1) / (kThreads / 64), x = workgroups < kGridWidth ? workgroups : kGridWidth;
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>((workgroups + x - 1) / x));  // items below 2^31: at most 2^7 rows
   if constexpr (PP == 1) {
     if (many) rope_kernel<L, PP, 4><<<grid, kThreads, 0, s>>>(A);
     else rope_kernel<L, PP, 2><<<grid, kThreads, 0, s>>>(A);
