@@ -674,7 +674,7 @@ WH_API int wh_qk_norm_rope(const wh_rope_rules* rules, const float* q, const flo
  * zeros; one whose length is beyond max_prefix or max_own one of NaN.  max_prefix
  * or max_own may be 0, its caches and lengths null.  head_dim 64 or 128, n_heads
  * (at most 1024) a multiple of n_kv_heads, at most WH_MAX_MEMBERS members in
- * all, out apart from q.  Caches and workspace are 16-byte aligned; the workspace
+ * all (fewer than 4096 groups of one with 1024 KV heads of 128), out apart from q.  Caches and workspace are 16-byte aligned; the workspace
  * holds wh_attention_shared_workspace_bytes(..), 0 for shapes that are not taken;
  * calls that overlap on one workspace race. */
 #define WH_MAX_MEMBERS 4096

@@ -1016,9 +1016,12 @@ namespace wh {
 
 bool shared_attention_shape_ok(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                                size_t max_prefix, size_t max_own) {
-  return (head_dim == 64 || head_dim == 128) && n_kv_heads > 0 && n_heads > 0 && n_heads <= 1024 && n_heads % n_kv_heads == 0 &&
-         n_groups <= kMaxMembers && n_per <= kMaxMembers && n_groups * n_per <= kMaxMembers && !(max_prefix >> 31) &&
-         !(max_own >> 31);
+  if ((head_dim != 64 && head_dim != 128) || n_kv_heads == 0 || n_heads == 0 || n_heads > 1024 || n_heads % n_kv_heads != 0 ||
+      n_groups > kMaxMembers || n_per > kMaxMembers || n_groups * n_per > kMaxMembers || max_prefix >> 31 || max_own >> 31)
+    return false;
+  // the join's launch: a wave per item, fewer than 2^32 threads
+  const size_t tiles = div_up(n_per * (n_heads / n_kv_heads), 32);
+  return !(n_groups * n_kv_heads * tiles * (head_dim / 8) * 64 >> 32);
 }
 
 size_t shared_attention_workspace_bytes(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads, size_t head_dim,
