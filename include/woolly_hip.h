@@ -611,8 +611,8 @@ WH_API int wh_kv_cache_compact(void* const* k_caches, void* const* v_caches, siz
 /* The beams of a search, samples of one prompt, requests behind one system
  * prompt: n_groups groups of n_per "members".  A group's members share the cache
  * rows of its prompt (the prefix, [n_groups][max_prefix][n_kv_heads][head_dim]
- * f16, filled by wh_llama_forward_token or wh_llama_forward_tree), and each has
- * rows of its own behind them ([n_groups * n_per][max_own][n_kv_heads][head_dim]).
+ * f16, filled by wh_llama_forward_token or wh_llama_forward_tree where the rotation is
+ * the model's own, see wh_llama_forward_members), and each has rows of its own behind them ([n_groups * n_per][max_own][n_kv_heads][head_dim]).
  * No counterpart in the reference, which runs one sequence.  Lengths are device
  * memory, read when the call runs: a captured step follows them.  A member's
  * length counts its own tokens, those of the present step included. */
@@ -750,7 +750,14 @@ WH_API int wh_beam_reorder(void* const* states, size_t n_states, size_t n_seqs, 
  * position *prefix_len + len[m] - 1; its k and v go to that row of k_own[layer]
  * and v_own[layer], host arrays of n_layers device pointers, [n_members][max_own]
  * [n_kv_heads][head_dim] f16 each.  The model's caches are only read.  rules may
- * be null: the model's rope_inv_freq, half layout, no norms.  tokens, prefix_len
+ * be null: the model's rope_inv_freq, half layout, no norms.  The prefix's rows have to
+ * be made by the same rules, which the call cannot see: wh_llama_forward_token and
+ * wh_llama_forward_tree make those of the default only.  For others the caller makes
+ * them, layer by layer: wh_qk_norm_rope over the prompt's q and k in place (no
+ * caches), then wh_attention_tree (a chain of up to 128 tokens at a time) with inverse
+ * frequencies of 0, which turns nothing more and stores the rows.  One set of norm
+ * weights serves all layers; a model with one for each layer runs these operators by
+ * themselves in its step, too.  tokens, prefix_len
  * (one number) and len [n_members] are device memory, x is 16-byte aligned, the
  * model has a token_embd table.  A member whose rows do not fit has NaN; one with
  * len 0 is not there: nothing of it is stored and its rows mean nothing.  The

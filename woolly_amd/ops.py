@@ -633,7 +633,7 @@ class LlamaModel:
                         workspace_bytes: int, rules: RopeRules | None = None, stream: Stream | None = None) -> None:
         """One step for several continuations of the prompt in the model's caches (wh_llama_forward_members): x
         [n_members][hidden] and logits [n_members][vocab] (may be None); the layers' caches in `own` take the tokens'
-        rows.  rules: None for the model's rotation."""
+        rows.  rules: None for the model's rotation; others need a prompt whose rows were made by the same."""
         if own.n_layers != self.model.n_layers:
             raise ValueError(f"own caches of {own.n_layers} layers, the model has {self.model.n_layers}")
         _lib.check(_lib.load().wh_llama_forward_members(
