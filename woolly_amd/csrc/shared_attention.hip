@@ -23,9 +23,10 @@
 // Beside one key with nearly all the weight (often the first one, whose v is small) the
 // others make the output, and keep what f32 would leave them: m moves down to them, and
 // that key's own tile takes two turns.  Relative L2 with 90 to 99.9999999 % on one key of
-// 60000: 2e-7 to 4e-6 (with m the running maximum alone up to 2e-2).  That costs the calls
-// 0 to 3 %: 48 members at 131000 253 -> 254 us, 64 at 20000 63.3 -> 63.0, 32 at 60000 of 64 dims
-// 48.7 -> 49.3, 8 at 30000 33.6 -> 33.8.
+// 60000: 2e-7 to 4e-6 (with m the running maximum alone up to 2e-2).  The calls take what they
+// took: 48 members at 131000 252 -> 253 us, 64 at 20000 62.8 -> 62.0, 32 at 60000 of 64 dims 49.2 ->
+// 48.6, 8 at 30000 33.8 -> 33.8, 4 at 900 10.2 -> 10.5; moving up, which the first tiles do, and down
+// in one block cost another 1 to 3 %.
 //
 // Few query rows: a wave has its own tiles of 32 keys, its own LDS and no barriers
 // until the chunk's end; memory bounds it (8 members at 30000 + 250 rows, 131 MB,
@@ -191,7 +192,7 @@ struct Rows {
   int e;     // q is scaled by 2^e
   f32x16 acc[D / 32];
   float m, l;
-  float floor;  // m goes no lower
+  float peak;  // m before it last went down, or the highest of those
 };
 
 // q rows: lane l has row l % 32, elements 16 j + 8 (l / 32) .. of each step j.
@@ -228,7 +229,7 @@ __device__ __forceinline__ void load_rows(Rows<D>& w, const float* q, float scal
   for (int d = 0; d < D / 32; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) w.acc[d][i] = 0.f;
-  w.m = w.floor = -INFINITY;
+  w.m = w.peak = -INFINITY;
   w.l = 0.f;
 }
 
@@ -296,19 +297,38 @@ __device__ __forceinline__ bool settle(Rows<D>& w, f32x16 (&s)[N], std::bool_con
   auto largest = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };  // NaN if there is one
   tops(largest);
   mt = swap_max_nan(mt);
-  // NaN goes on
-  if (!SECOND && __ballot(!((mt - w.m) * w.qs <= kMoveUp) || (fminf(top[0], top[1]) - w.m) * w.qs < kFaint) == 0) return false;
-  if (__builtin_expect(__ballot(mt != mt) != 0, 0)) {
+  auto move = [&](bool moves, float to) __attribute__((always_inline)) {
+    const float al = moves ? __builtin_amdgcn_exp2f((w.m - to) * w.qs) : 1.f;
+    w.l *= al;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) w.acc[d][i] *= al;
+    if (moves) w.m = to;
+  };
+  auto mend_nan = [&]() __attribute__((always_inline)) {
+    if (__builtin_expect(__ballot(mt != mt) == 0, 1)) return;
     mend();
     tops(largest);
     mt = swap_max_nan(mt);  // NaN still: the row is NaN
+  };
+  if constexpr (SECOND) {
+    mend_nan();
+  } else {
+    if (__ballot(!((mt - w.m) * w.qs <= kMoveUp))) {  // NaN comes here
+      mend_nan();
+      move(!((mt - w.m) * w.qs <= kMoveUp) && mt != -INFINITY, mt);
+    }
+    if (__builtin_expect(__ballot((fminf(top[0], top[1]) - w.m) * w.qs < kFaint) == 0, 1)) return false;
   }
+  // keys are faint
   bool again = false;
+  const float unit = __builtin_amdgcn_rcpf(w.qs);
 #pragma unroll
-  for (int i = 0; i < 2; i++) top[i] = top[i] == -INFINITY ? INFINITY : top[i];  // keys of weight 0 are not faint
+  for (int i = 0; i < 2; i++) top[i] = top[i] == -INFINITY ? INFINITY : top[i];  // but those of weight 0 are not
   const float low = -swap_max(-fminf(top[0], top[1]));
-  if (SECOND || __builtin_expect(__ballot((low - mt) * w.qs < kFaint) != 0, 0)) {
-    const float split = mt - kNear * __builtin_amdgcn_rcpf(w.qs);
+  if (SECOND || __ballot((low - mt) * w.qs < kFaint)) {
+    const float split = mt - kNear * unit;
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
@@ -317,15 +337,9 @@ __device__ __forceinline__ bool settle(Rows<D>& w, f32x16 (&s)[N], std::bool_con
     mt = swap_max(mt);
     again = !SECOND;
   }
-  const float to = __builtin_elementwise_maximum(mt, w.floor), by = (to - w.m) * w.qs;
-  const bool moves = mt != -INFINITY && (!(by <= kMoveUp) || (by < -kMoveUp && (low - w.m) * w.qs < kFaint));
-  const float al = moves ? __builtin_amdgcn_exp2f(-by) : 1.f;
-  w.l *= al;
-#pragma unroll
-  for (int d = 0; d < D / 32; d++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) w.acc[d][i] *= al;
-  if (moves) w.m = to, w.floor = fmaxf(w.floor, to - kLowest * __builtin_amdgcn_rcpf(w.qs));
+  w.peak = fmaxf(w.peak, w.m);
+  const float to = fmaxf(mt, w.peak - kLowest * unit);
+  move(mt != -INFINITY && (to - w.m) * w.qs < -kMoveUp && (low - w.m) * w.qs < kFaint, to);
   return again;
 }
 
