@@ -637,7 +637,8 @@ typedef struct wh_rope_rules {
  *                     from `low` to `high` turns within original_ctx, clamped
  *   WH_ROPE_BY_INDEX  the same with g_i going from 1 to 0 in equal steps of i,
  *                     between the whole indices around those of high and low
- *                     turns; the magnitude is 0.1 log(factor) + 1
+ *                     turns; the magnitude is 0.1 log(factor) + 1 (the published
+ *                     YaRN method, with its bounds 0 and rot_dim - 1 of the indices)
  * low and high only for the last two: 0 < low < high.  Host outputs. */
 enum { WH_ROPE_PLAIN = 0, WH_ROPE_LINEAR = 1, WH_ROPE_BASE = 2, WH_ROPE_BY_TURNS = 3, WH_ROPE_BY_INDEX = 4 };
 WH_API int wh_rope_scaled_inv_freq(int kind, float base, size_t rot_dim, float factor, size_t original_ctx, float low,
@@ -676,7 +677,8 @@ WH_API int wh_qk_norm_rope(const wh_rope_rules* rules, const float* q, const flo
  * (at most 1024) a multiple of n_kv_heads, at most WH_MAX_MEMBERS members in
  * all (fewer than 4096 groups of one with 1024 KV heads of 128), out apart from q.  Caches and workspace are 16-byte aligned; the workspace
  * holds wh_attention_shared_workspace_bytes(..), 0 for shapes that are not taken;
- * calls that overlap on one workspace race. */
+ * calls that overlap on one workspace race.  The split into workgroups is made for
+ * max_prefix and max_own, not the lengths: far larger caches cost up to a fifth. */
 #define WH_MAX_MEMBERS 4096
 WH_API size_t wh_attention_shared_workspace_bytes(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads,
                                                   size_t head_dim, size_t max_prefix, size_t max_own);
@@ -698,7 +700,9 @@ WH_API int wh_attention_shared(const float* q, size_t ldq, const uint32_t* prefi
  * and count as they are), and its logits are not read.  A beam whose score is
  * infinite or NaN is not there (a search begins with one beam at 0, the others at
  * -inf); logits of -inf or NaN are not allowed, and a row with +inf has no
- * continuation.  Sums and comparisons are made in 64 bits. */
+ * continuation.  Comparisons and sums are made in 64 bits, but of a row's exponentials
+ * only the highest few; the others are f32's, which puts log sum exp off by some 2^-25
+ * and by at most 2^-22 (log vocab + 1) + 2^-21. */
 #define WH_MAX_BEAMS 32
 typedef struct wh_beam_rules {
   size_t n_beams;               /* at most WH_MAX_BEAMS */

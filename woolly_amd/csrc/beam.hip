@@ -14,18 +14,23 @@
 // place of each is the number of those before it.  Logits that are equal come in
 // the order of their tokens: the keys that are compared hold both.  Where too many
 // are equal for that they are taken one maximum at a time.
-// lse in 64 bits: the few highest terms, which make the sum, are exponentials in
-// 64 bits, the others in 32 bits summed in 64.
-// The first launch is bound by memory (16 x 8 beams of 128256 logits, 65.7 MB, in 16.6
-// us, 4.0 TB/s; 4 of 32000 in 5), the second by its steps that wait for each other,
+// lse: the few highest terms, which make the sum where it is uneven, are exponentials in
+// 64 bits, the others f32's (a 64-bit one is a few dozen instructions), 8 to a thread's f32
+// sum, the threads' sums in 64.  A distance d to the top is off by 2^-24 d, its product with
+// log2 e by as much: lse is off by 3e-8 for usual logits, less than half the last place of an
+// f32 score above 1.
+// The first launch asks for its 4096 logits once and ranks them with nothing in flight (16 x 8
+// beams of 128256 logits, of which 51.2 MB are read and those of ended beams are not, in 17
+// us, 3.0 TB/s; 4 of 32000 in 5), the second is bound by its steps that wait for each other,
 // however few beams there are (8 beams 7.5 us, 4 beams 5.5: 3 until the bound is there,
 // 2 for the ranks and outputs, 1 for the histories).
 //
 // Reordering.  A thread holds one 16-byte column of a state's rows for all beams:
 // it loads what its moved beams take before it stores any of it, so rows move in
-// place, whatever the parents are.  Bound by memory: each moved row is read and
-// written once (4 of 8 beams x 500 rows of 2 KB x 64 states, 524 MB: 105 us, 5.0 TB/s;
-// 2 of 4 x 60 rows 6.4 us, 4.9 TB/s).
+// place, whatever the parents are.  Bound by memory: a row is written for each beam that
+// moves, and read once for those that share a parent (4 of 8 beams x 500 rows of 2 KB x 64
+// states: 262 MB written, 137 MB read past the Infinity Cache, 75 to 79 us, 5.1 TB/s; as calls
+// 90; 2 of 4 x 60 rows 5.3 us).
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -573,7 +578,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const ReorderParams P
       if (c < n[i]) v[i] = base[from[i] + c];
 #pragma unroll
     for (int i = 0; i < NB; i++)
-      if (c < n[i])  // past the caches: 115 -> 105 us for 524 MB, 7.3 -> 6.4 for 31
+      if (c < n[i])  // past the caches: 115 -> 105 us a call for 262 MB in a graph, 7.3 -> 6.4 for 16
         __builtin_nontemporal_store(v[i], &base[i * beam + c]);
   }
 }

@@ -16,7 +16,7 @@
 // no normal f32 number).
 //
 // Many rows are bound by memory: 4000 of 32 / 8 heads of 128, 180 MB read and
-// written, 35.5 us, normed 41 (5.1 and 4.4 TB/s); few by the launch and two loads
+// written, 35.5 us, normed 42 (5.1 and 4.3 TB/s); few by the launch and two loads
 // one behind the other: 8 rows 3.1 us in a graph.
 #include <type_traits>
 
@@ -302,7 +302,7 @@ WH_API int wh_rope_scaled_inv_freq(int kind, float base, size_t rot_dim, float f
   // the index whose frequency makes `turns` turns within the context
   auto index_of = [&](double turns) { return d * log(ctx / (turns * two_pi)) / (2.0 * log(b)); };
   double first = 0.0, last = 0.0;
-  if (kind == WH_ROPE_BY_INDEX) {
+  if (kind == WH_ROPE_BY_INDEX) {  // bounds and step of the published YaRN method, by which models are trained
     first = fmax(floor(index_of(high)), 0.0);
     last = fmin(ceil(index_of(low)), d - 1.0);
     if (!(last > first)) last = first + 0.001;  // a step
