@@ -51,24 +51,26 @@ def _split(x, scale):
 
 def emulate(q, k, v, tile=32, q_limbs=2, p_limbs=2, falls=True):
     """One query row over one chunk: q and the weights in f16 limbs, all else in 64 bits.  falls: the reference follows the
-    tiles down, and tiles whose keys lie far apart take two turns."""
+    tiles down to where they are faint, and tiles with one of the highest keys beside a faint half take two turns."""
     x = np.ldexp(q, 13 - int(np.floor(np.log2(np.abs(q).max())))).astype(np.float32)
     hi, lo = _split(x, 1.0)
     s = k.astype(np.float64) @ (hi + (lo if q_limbs == 2 else 0)) * (np.abs(q).max() / np.abs(x).max()) / np.sqrt(len(q)) / np.log(2)
-    m = floor = -np.inf
+    m = peak = -np.inf
     l, acc = 0.0, np.zeros(v.shape[1])
     for b in range(0, len(s), tile):
-        t, vt, group = s[b:b + tile], v[b:b + tile].astype(np.float64), (np.arange(b, min(b + tile, len(s))) % 8) // 4 * 2
-        group = group + np.arange(len(t)) % 2
-        low = min(t[group == g].max() for g in set(group))
+        t, vt, half = s[b:b + tile], v[b:b + tile].astype(np.float64), np.arange(b, min(b + tile, len(s))) % 8 // 4
+        if t.max() - m > 3:
+            l, acc, m = l * 2.0 ** (m - t.max()), acc * 2.0 ** (m - t.max()), t.max()
+        peak = max(peak, m)
+        low = min(t[half == g].max() for g in set(half))
+        counts = lambda x, ref: falls and peak - 78 <= x < ref - 30
         near = t >= t.max() - 9
-        for keep in ([near, ~near] if falls and low - t.max() < -26 else [near | True]):
+        for keep in [near, ~near] if t.max() >= peak - 10 and counts(low, t.max()) else [near | True]:
             if not keep.any():
                 continue
-            to = max(t[keep].max(), floor)
-            if to - m > 3 or (falls and low - m < -26 and to - m < -3):
+            to = max(t[keep].max(), peak - 48)
+            if counts(t[keep].max(), m):
                 l, acc, m = l * 2.0 ** (m - to), acc * 2.0 ** (m - to), to
-                floor = max(floor, m - 48)
             p = np.exp2(t[keep] - m + 12).astype(np.float32)
             hi, lo = _split(p, 2048.0)
             l += p.astype(np.float64).sum()

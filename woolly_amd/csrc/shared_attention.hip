@@ -23,10 +23,11 @@
 // Beside one key with nearly all the weight (often the first one, whose v is small) the
 // others make the output, and keep what f32 would leave them: m moves down to them, and
 // that key's own tile takes two turns.  Relative L2 with 90 to 99.9999999 % on one key of
-// 60000: 2e-7 to 4e-6 (with m the running maximum alone up to 2e-2).  The calls take what they
-// took: 48 members at 131000 252 -> 253 us, 64 at 20000 62.8 -> 62.0, 32 at 60000 of 64 dims 49.2 ->
-// 48.6, 8 at 30000 33.8 -> 33.8, 4 at 900 10.2 -> 10.5; moving up, which the first tiles do, and down
-// in one block cost another 1 to 3 %.
+// 60000: 2e-7 to 4e-6 (with m the running maximum alone up to 2e-2).  Calls whose scores have a
+// deviation up to 5 take what they took with that: 48 members at 131000 253 -> 251 us, 64 at 20000
+// 63 -> 62, 32 at 60000 of 64 dims 49.5 -> 48.5, 8 at 30000 33.7 -> 33.8, 4 at 900 10.2 -> 10.5; with 8
+// the first takes 300, with 16 435, where most tiles have keys far apart.  Moving up, which the
+// first tiles do, in one block with the rest cost another 1 to 3 %.
 //
 // Few query rows: a wave has its own tiles of 32 keys, its own LDS and no barriers
 // until the chunk's end; memory bounds it (8 members at 30000 + 250 rows, 131 MB,
@@ -50,14 +51,17 @@ using whd::read_tr, whd::swap_max, whd::swap_max_nan, whd::swap_sum, whd::swz_k,
 
 constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are held in f16 as 2^12 e^{s - m}.  The reference m of a row moves to a tile's largest
-// score where that is above 2^3 (at most 2^15 in f16), and down to it, but never 2^48 below its
-// highest, where keys are faint: a row's keys in a tile are four groups, by their parity and by the
-// lane that holds them, and a group is faint whose largest weight is below 2^-26 of the reference's
-// (2^-14 in f16, below which the low limb is off by more than 2^-22 of it).  Where it is so against
-// the tile's largest too, the tile takes two turns: the keys down to 2^-9 of that one, then the others.
+// Weights are held in f16 as 2^12 e^{s - m}.  The reference m of a row moves up to a tile's largest
+// score where that is above 2^3 of it (at most 2^15 in f16), and down to it, but never 2^48 below its
+// highest, where it is faint: below 2^-30 (2^-18 in f16, where the low limb is off by 2^-18 of it).
+// A tile with a key far above its neighbours takes two turns: the keys down to 2^-9 of it, then the
+// others.  Half of a row's keys in a tile are one lane's, and such a key is told by the other half,
+// faint against it, and by being within 2^-10 of the row's highest.  (Such keys in both halves
+// hide the rest of their tile.)  Of 32 rows with scores of deviation 1.3, 3 and 5 some row's m moves
+// up in 10, 12 and 16 % of the tiles, none down; with 8 it is 50 % and 9 %, and 2 % take two turns; with
+// 16 all, 83 and 50 %.
 constexpr float kPScaleLog2 = 12.0f, kMoveUp = 3.0f, kLowest = 48.0f;
-constexpr float kFaint = -26.0f, kNear = 9.0f;
+constexpr float kFaint = -30.0f, kNear = -9.0f, kHigh = -10.0f;
 constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
 constexpr uint32_t kLeastChunk = 128;  // keys: a tile for every wave
 constexpr double kShareFrom = 10.0;    // work (plan)
@@ -290,15 +294,14 @@ __device__ __forceinline__ void mend_scores(const Rows<D>& w, const Keys<D>& key
 // mend: mend_scores of the tiles.
 template <int D, int N, bool SECOND, typename Mend>
 __device__ __forceinline__ bool settle(Rows<D>& w, f32x16 (&s)[N], std::bool_constant<SECOND>, const Mend& mend) {
-  float top[2], mt;  // the largest score of the lane's groups of keys, and of the row
-  auto tops = [&](auto larger) __attribute__((always_inline)) {
+  float top, mt;  // the largest score of the lane's half, and of the row; NaN if there is one
+  auto largest = [&]() __attribute__((always_inline)) {
+    top = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 16 * N; i++) top[i & 1] = i < 2 ? s[0][i] : larger(top[i & 1], s[i / 16][i % 16]);
-    mt = larger(top[0], top[1]);
+    for (int i = 1; i < 16 * N; i++) top = __builtin_elementwise_maximum(top, s[i / 16][i % 16]);
+    mt = swap_max_nan(top);
   };
-  auto largest = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };  // NaN if there is one
-  tops(largest);
-  mt = swap_max_nan(mt);
+  largest();
   auto move = [&](bool moves, float to) __attribute__((always_inline)) {
     const float al = moves ? __builtin_amdgcn_exp2f((w.m - to) * w.qs) : 1.f;
     w.l *= al;
@@ -311,8 +314,7 @@ __device__ __forceinline__ bool settle(Rows<D>& w, f32x16 (&s)[N], std::bool_con
   auto mend_nan = [&]() __attribute__((always_inline)) {
     if (__builtin_expect(__ballot(mt != mt) == 0, 1)) return;
     mend();
-    tops(largest);
-    mt = swap_max_nan(mt);  // NaN still: the row is NaN
+    largest();  // NaN still: the row is NaN
   };
   if constexpr (SECOND) {
     mend_nan();
@@ -321,27 +323,26 @@ __device__ __forceinline__ bool settle(Rows<D>& w, f32x16 (&s)[N], std::bool_con
       mend_nan();
       move(!((mt - w.m) * w.qs <= kMoveUp) && mt != -INFINITY, mt);
     }
-    if (__builtin_expect(__ballot((fminf(top[0], top[1]) - w.m) * w.qs < kFaint) == 0, 1)) return false;
+    if (__builtin_expect(__ballot((top - w.m) * w.qs < kFaint) == 0, 1)) return false;
   }
-  // keys are faint
-  bool again = false;
+  // What is faint counts down to 2^-78 of the row's highest, where m cannot follow.
   const float unit = __builtin_amdgcn_rcpf(w.qs);
-#pragma unroll
-  for (int i = 0; i < 2; i++) top[i] = top[i] == -INFINITY ? INFINITY : top[i];  // but those of weight 0 are not
-  const float low = -swap_max(-fminf(top[0], top[1]));
-  if (SECOND || __ballot((low - mt) * w.qs < kFaint)) {
-    const float split = mt - kNear * unit;
+  w.peak = fmaxf(w.peak, w.m);
+  auto counts = [&](float score, float ref) { return (score - ref) * w.qs < kFaint && (score - w.peak) * w.qs >= kFaint - kLowest; };
+  bool again = false;
+  if (SECOND || __ballot((mt - w.peak) * w.qs >= kHigh && counts(top, mt))) {
+    const float split = __builtin_fmaf(kNear, unit, mt);
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
       for (int i = 0; i < 16; i++) s[n][i] = (s[n][i] < split) != SECOND ? -INFINITY : s[n][i];
-    tops([](float a, float b) { return fmaxf(a, b); });
-    mt = swap_max(mt);
+    float most = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16 * N; i++) most = fmaxf(most, s[i / 16][i % 16]);
+    mt = swap_max(most);
     again = !SECOND;
   }
-  w.peak = fmaxf(w.peak, w.m);
-  const float to = fmaxf(mt, w.peak - kLowest * unit);
-  move(mt != -INFINITY && (to - w.m) * w.qs < -kMoveUp && (low - w.m) * w.qs < kFaint, to);
+  move(counts(mt, w.m), fmaxf(mt, w.peak - kLowest * unit));
   return again;
 }
 
