@@ -678,7 +678,7 @@ WH_API int wh_qk_norm_rope(const wh_rope_rules* rules, const float* q, const flo
  * all (fewer than 4096 groups of one with 1024 KV heads of 128), out apart from q.  Caches and workspace are 16-byte aligned; the workspace
  * holds wh_attention_shared_workspace_bytes(..), 0 for shapes that are not taken;
  * calls that overlap on one workspace race.  The split into workgroups is made for
- * max_prefix and max_own, not the lengths: far larger caches cost up to a fifth. */
+ * max_prefix and max_own, not the lengths: far larger caches cost up to a quarter. */
 #define WH_MAX_MEMBERS 4096
 WH_API size_t wh_attention_shared_workspace_bytes(size_t n_groups, size_t n_per, size_t n_heads, size_t n_kv_heads,
                                                   size_t head_dim, size_t max_prefix, size_t max_own);
